@@ -643,6 +643,96 @@ int32_t mg_photometric_loss_backward(const float *x, const float *y,
                                      int32_t W, float ssim_weight, float *d_x,
                                      mg_stream_t stream);
 
+/* ------------------------------------------------- operators over tokens */
+
+/* What a network that predicts or refines splats from image patches needs
+ * beside matrix products. No counterpart in the reference. Element types are
+ * MG_F32, MG_BF16 or MG_F16; everything is computed in float32 and rounded once
+ * where it is stored. Strides count elements; the last dimension of every
+ * input is contiguous, and outputs are contiguous. */
+enum { MG_F32 = 0, MG_BF16 = 1, MG_F16 = 2 };
+
+/* Layer norm of `rows` rows of `width` elements, x_stride elements apart:
+ * y = (x - mean) * rstd * weight + bias with rstd = 1 / sqrt(var + eps). weight
+ * and bias may be NULL (1 and 0) and are float32 or of x's type. mean and rstd
+ * (rows, float32) may both be NULL when no backward pass follows. */
+int32_t mg_layer_norm_forward(int64_t rows, int64_t width, int32_t dtype,
+                              const void *x, int64_t x_stride,
+                              int32_t weight_dtype, const void *weight,
+                              const void *bias, float eps, void *y, float *mean,
+                              float *rstd, mg_stream_t stream);
+/* dx (contiguous), dweight and dbias (of the weights' type), each of which may
+ * be NULL. Sums over rows are formed in a fixed order, so that equal calls give
+ * equal bits. */
+int64_t mg_layer_norm_backward_workspace_bytes(int64_t rows, int64_t width);
+int32_t mg_layer_norm_backward(int64_t rows, int64_t width, int32_t dtype,
+                               const void *x, int64_t x_stride, const void *dy,
+                               int64_t dy_stride, int32_t weight_dtype,
+                               const void *weight, const float *mean,
+                               const float *rstd, void *dx, void *dweight,
+                               void *dbias, void *workspace,
+                               int64_t workspace_bytes, mg_stream_t stream);
+
+/* Rotary positions of q (tokens, q_heads, dim) and k (tokens, k_heads, dim;
+ * k_heads 0: none). Pair i of the first 2 * pairs elements of a head, which is
+ * (i, pairs + i) or, interleaved, (2i, 2i + 1), is turned by position *
+ * frequencies[i] radians (inverse: by its negative, the adjoint); the others are
+ * copied. positions (tokens, axes) are int32, or int64 with positions_64; pair i
+ * goes by axis i / (pairs / axes). frequencies: float64, on the device. */
+int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q,
+                  int64_t q_token_stride, int64_t q_head_stride,
+                  int32_t q_heads, const void *k, int64_t k_token_stride,
+                  int64_t k_head_stride, int32_t k_heads, int32_t dim,
+                  const void *positions, int32_t positions_64, int32_t axes,
+                  const double *frequencies, int32_t pairs, int32_t interleaved,
+                  int32_t inverse, void *q_out, void *k_out,
+                  mg_stream_t stream);
+
+/* Attention over packed sequences: q (q_tokens, q_heads, dim), k and v
+ * (k_tokens, k_heads, dim), bfloat16 or float16, dim a multiple of 8 up to 128,
+ * q_heads a multiple of k_heads (a key head serves as many query heads, in
+ * order), rows 16-byte aligned. Sequence s has query tokens q_offsets[s] ..
+ * q_offsets[s + 1] - 1 and key tokens by k_offsets (device, sequences + 1 each;
+ * both NULL: one sequence of all tokens). Offsets are held to the tensors and
+ * made to rise; tokens outside every sequence get zeros. A query sees its
+ * sequence's keys, causal those that stand at or before it, the last query
+ * standing at the last key; a query that sees none gets zeros. softmax(scale *
+ * q k) v, scale >= 0. What a query does not see may hold anything in k; in v
+ * too, as long as it is finite.
+ *
+ * lse (q_heads, q_tokens, float32; NULL: not kept) is the base 2 logarithm of a
+ * row's sum of exponentials, +inf for a row that sees nothing: the backward
+ * pass needs it. The workspace holds partial sums where few rows attend to
+ * many keys; its size depends on the arguments of the query alone. */
+int64_t mg_attention_forward_workspace_bytes(int64_t q_tokens, int64_t k_tokens,
+                                             int32_t q_heads, int32_t k_heads,
+                                             int32_t dim, int32_t sequences);
+int32_t mg_attention_forward(
+    int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+    int32_t k_heads, int32_t dim, const void *q, int64_t q_token_stride,
+    int64_t q_head_stride, const void *k, int64_t k_token_stride,
+    int64_t k_head_stride, const void *v, int64_t v_token_stride,
+    int64_t v_head_stride, const int32_t *q_offsets, const int32_t *k_offsets,
+    int32_t sequences, int32_t causal, float scale, void *out, float *lse,
+    void *workspace, int64_t workspace_bytes, mg_stream_t stream);
+/* Gradients of the above from its out and lse and the gradient dout of out
+ * (strided as q): dq, dk, dv (contiguous; dk and dv may both be NULL). Heads
+ * that share keys have their gradients summed in float32. Equal calls give
+ * equal bits. */
+int64_t mg_attention_backward_workspace_bytes(int64_t q_tokens, int64_t k_tokens,
+                                              int32_t q_heads, int32_t k_heads,
+                                              int32_t dim, int32_t sequences);
+int32_t mg_attention_backward(
+    int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+    int32_t k_heads, int32_t dim, const void *q, int64_t q_token_stride,
+    int64_t q_head_stride, const void *k, int64_t k_token_stride,
+    int64_t k_head_stride, const void *v, int64_t v_token_stride,
+    int64_t v_head_stride, const int32_t *q_offsets, const int32_t *k_offsets,
+    int32_t sequences, int32_t causal, float scale, const void *out,
+    const float *lse, const void *dout, int64_t dout_token_stride,
+    int64_t dout_head_stride, void *dq, void *dk, void *dv, void *workspace,
+    int64_t workspace_bytes, mg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,13 @@ Public surface (names of the reference's modules):
     io                     Splats, load_ply, save_ply, export_ply
     ext                    the reference's native-extension functions (backend._load())
     ListCapacity           tile-list sizing without a host read (render(list_capacity=))
+
+Operators of networks over image patches that predict or refine splats (no
+counterpart in the reference):
+    layer_norm             layer norm and its gradients
+    rotary, rotary_frequencies
+                           rotary positions of queries and keys
+    attention              attention over packed sequences and its gradients
 """
 
 from .api import BACKENDS, render  # noqa: F401
@@ -22,6 +29,9 @@ from .selective_adam import SelectiveAdam  # noqa: F401
 from .ssim import gaussian_kernel, photometric_loss, ssim  # noqa: F401
 from .mipfilter import apply_3d_filter, compute_3d_filter  # noqa: F401
 from .backend import ListCapacity  # noqa: F401
+from .norm import layer_norm  # noqa: F401
+from .rotary import rotary, rotary_frequencies  # noqa: F401
+from .attention import attention  # noqa: F401
 from . import backend, ext  # noqa: F401
 
 __version__ = "0.1.0"

@@ -121,6 +121,21 @@ _SIGNATURES = {
                                                    _vp]),
     "mg_photometric_loss_backward": (_i32, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _f32, _vp,
                                             _vp]),
+    "mg_layer_norm_forward": (_i32, [_i64, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _f32, _vp,
+                                     _vp, _vp, _vp]),
+    "mg_layer_norm_backward_workspace_bytes": (_i64, [_i64, _i64]),
+    "mg_layer_norm_backward": (_i32, [_i64, _i64, _i32, _vp, _i64, _vp, _i64, _i32, _vp, _vp,
+                                      _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mg_rotary": (_i32, [_i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32, _i32, _vp,
+                         _i32, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "mg_attention_forward_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "mg_attention_forward": (_i32, [_i32, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _vp,
+                                    _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _f32,
+                                    _vp, _vp, _vp, _i64, _vp]),
+    "mg_attention_backward_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "mg_attention_backward": (_i32, [_i32, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _vp,
+                                     _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _f32,
+                                     _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
 }
 
 EXPORTS = tuple(_SIGNATURES)
@@ -178,6 +193,30 @@ def dev_tensor(t: torch.Tensor, what: str, dtype: torch.dtype | None = torch.flo
     if dtype is not None and t.dtype != dtype:
         raise RuntimeError(f"{what} must be {dtype}, got {t.dtype}")
     return t.data_ptr()
+
+
+#: Type codes of the token operators (MG_F32, MG_BF16, MG_F16).
+TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def launch(fn, t: torch.Tensor, *args) -> None:
+    """fn(*args, stream) on the device of ``t`` and that device's current stream."""
+    index = t.device.index
+    if index != torch.cuda.current_device():
+        with torch.cuda.device(index):
+            check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+
+
+def type_code(t: torch.Tensor, what: str) -> int:
+    """The type code of a tensor that a token operator takes."""
+    code = TYPE_CODES.get(t.dtype)
+    if code is None:
+        raise RuntimeError(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
+    if not t.is_cuda:
+        raise RuntimeError(f"{what} must be a HIP (ROCm) tensor, got device '{t.device}'")
+    return code
 
 
 class AdamEpilogue(ctypes.Structure):

@@ -1,0 +1,271 @@
+// Shared by the attention kernels' two files. Internal header.
+#pragma once
+
+#include "attention_tiles.h"
+#include "mg_types.h"
+
+namespace mg {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) char lds_char;
+typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+
+template <typename T>
+using vec8 = T __attribute__((ext_vector_type(8)));
+template <typename T>
+using vec4 = T __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x16 mfma32(vec8<bf16_t> a, vec8<bf16_t> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mfma32(vec8<f16_t> a, vec8<f16_t> b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Keys (or, in the keys' gradient, queries) of one LDS tile.
+constexpr int kTileRows = 64;
+template <int DK>
+constexpr int kTileBytes = kTileRows * tile_chunks<DK>() * 16;
+// Loads of 64 chunks that fill a tile.
+template <int DK>
+constexpr int kTileLoads = kTileRows * tile_chunks<DK>() / 64;
+
+struct AttnTensor {
+    const void *p;
+    int64_t tok_stride, head_stride;     // elements
+};
+
+struct AttnArgs {
+    AttnTensor q, k, v, dout;            // dout: the backward pass only
+    const int32_t *q_off, *k_off;        // NULL: one sequence of all tokens
+    int32_t n_seq;
+    int32_t q_tokens, k_tokens;
+    int32_t k_heads, group, dim;         // q_heads = k_heads * group
+    int32_t causal;
+    float scale, scale_log2;             // scale, scale * log2(e)
+    void *out;                           // (q_tokens, q_heads, dim)
+    float *lse;                          // (q_heads, q_tokens), in powers of 2; NULL: not kept
+    // Split over the keys: chunks of split_keys, joined from `partial`, which has
+    // room for `items` of each key head.
+    int32_t split_keys, items;
+    float *partial;
+    // Backward.
+    const float *delta;                  // (q_heads, q_tokens)
+    const float *grad_scale;             // {c, 1 / c}: see attention_bwd.hip
+    void *dq, *dk, *dv;
+};
+
+// ---------------------------------------------------------------- sequences
+// A work item's sequence. Tokens before the first offset and past the last
+// belong to no sequence: they are given out as sequences of queries without
+// keys (kByKeys: of keys without queries), so that their outputs and gradients
+// are zeros and no row stays unwritten.
+struct SeqItem {
+    int q_lo, q_len, k_lo, k_len;
+    int within;        // the item's number within its sequence
+    int before;        // sum of the second count over the sequences before
+    bool found;
+};
+
+__device__ __forceinline__ int clamp_to(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+// Tokens of pseudo sequence s of n + 2 (0: before the first, n + 1: past the
+// last). Offsets are held to [0, tokens] and made to rise, so that no value of
+// theirs leads out of the tensors.
+__device__ __forceinline__ void seq_bounds(const int32_t *off, int n, int tokens, int s, int &lo,
+                                           int &len) {
+    if (!off) {
+        lo = 0;
+        len = s == 1 ? tokens : 0;
+        return;
+    }
+    lo = s == 0 ? 0 : clamp_to(off[s - 1], 0, tokens);
+    len = (s > n ? tokens : clamp_to(off[s], lo, tokens)) - lo;
+}
+
+__device__ __forceinline__ int wave_inclusive_sum(int v) {
+    const int lane = lane_id();
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(v, o, 64);
+        v += lane >= o ? up : 0;
+    }
+    return v;
+}
+
+// The sequence that has `item` when a sequence has count(q_len, k_len) items;
+// `before` sums second(q_len, k_len). Every lane of a wave calls with the same
+// item and gets the same answer; where no sequence has the item, found is false.
+template <bool kByKeys, typename Count, typename Second>
+__device__ __forceinline__ SeqItem find_item(const AttnArgs &a, int item, Count count,
+                                             Second second) {
+    SeqItem r{};
+    int base = 0, base2 = 0;
+    for (int s0 = 0; s0 < a.n_seq + 2; s0 += 64) {
+        const int s = s0 + lane_id();
+        int q_lo = 0, q_len = 0, k_lo = 0, k_len = 0, n = 0, n2 = 0;
+        if (s < a.n_seq + 2) {
+            seq_bounds(a.q_off, a.n_seq, a.q_tokens, s, q_lo, q_len);
+            seq_bounds(a.k_off, a.n_seq, a.k_tokens, s, k_lo, k_len);
+            if (s == 0 || s > a.n_seq) (kByKeys ? q_len : k_len) = 0;
+            n = count(q_len, k_len);
+            n2 = second(q_len, k_len);
+        }
+        const int upto = wave_inclusive_sum(n), upto2 = wave_inclusive_sum(n2);
+        const uint64_t past = ballot(base + upto > item);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            r.q_lo = get(q_lo), r.q_len = get(q_len), r.k_lo = get(k_lo), r.k_len = get(k_len);
+            r.within = clamp_to(item - (base + get(upto) - get(n)), 0, get(n) - 1);
+            r.before = base2 + get(upto2) - get(n2);
+            r.found = true;
+            return r;
+        }
+        base += __builtin_amdgcn_readlane(upto, 63);
+        base2 += __builtin_amdgcn_readlane(upto2, 63);
+    }
+    return r;
+}
+
+// ------------------------------------------------------------- filling tiles
+// A value that is the same in all lanes, where the compiler cannot tell.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Descriptor of `bytes` bytes from a wave-uniform address; accesses past them
+// do not reach memory.
+__device__ __forceinline__ i32x4 buffer_of(const void *base, uint32_t bytes) {
+    const uint64_t at = (uintptr_t)base;
+    return i32x4{uniform((int)(uint32_t)at), uniform((int)(uint32_t)(at >> 32) & 0xffff),
+                 uniform((int)bytes), 0x00020000};
+}
+
+// Asks for rows row0 .. row0 + 63 (of n_rows; past the last, the last row again,
+// whose products the masks leave out) of one head into an LDS tile, straight
+// from memory: nothing passes through registers, and the wave goes on at once.
+// tiles_ready() waits. Wave `wave` of kWaves makes every kWaves-th load.
+//
+// The loads are written in assembly because the compiler, which cannot tell
+// one LDS buffer from the other, would wait for them before the next LDS read.
+template <int DK, int kWaves>
+struct TileFill {
+    static constexpr int kLoads = kTileLoads<DK> / kWaves;
+    static_assert(kTileLoads<DK> % kWaves == 0, "whole loads a wave");
+    uint32_t off[kLoads];          // bytes from row0's, of a whole tile
+
+    __device__ __forceinline__ void init(int64_t tok_stride, int dim, int wave) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) off[i] = offset(i, tok_stride, dim, wave, kTileRows);
+    }
+
+    // Columns past the head's dimension read column 0 .. 7: the products beside
+    // them are with zeros or are dropped.
+    static __device__ __forceinline__ uint32_t offset(int i, int64_t tok_stride, int dim, int wave,
+                                                      int rows) {
+        const int lane = lane_id(), load = i * kWaves + wave;
+        const int r = min(fill_row<DK>(load, lane), rows - 1), c = fill_chunk<DK>(load, lane);
+        return (uint32_t)r * (uint32_t)(tok_stride * 2) + (c * 8 < dim ? c * 16 : 0);
+    }
+
+    __device__ __forceinline__ void ask(const char *head, int64_t tok_stride, int dim, int row0,
+                                        int n_rows, int wave, uint32_t lds) const {
+        const int rows = min(n_rows - row0, kTileRows);
+        const char *base = head + (int64_t)row0 * tok_stride * 2;
+        const uint32_t bytes = (uint32_t)(rows - 1) * (uint32_t)(tok_stride * 2) + dim * 2;
+        const i32x4 rsrc = buffer_of(base, bytes);
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const uint32_t at =
+                rows == kTileRows ? off[i] : offset(i, tok_stride, dim, wave, rows);
+            const int to = uniform((int)lds + (i * kWaves + wave) * 1024);
+            asm volatile("s_mov_b32 m0, %0\n\t"
+                         "s_nop 0\n\t"
+                         "buffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :
+                         : "s"(to), "v"(at), "s"(rsrc)
+                         : "memory");
+        }
+    }
+};
+
+// The tiles asked for are there, for every wave, and no wave reads from what is
+// asked for next.
+__device__ __forceinline__ void tiles_ready() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_address(const char *p) {
+    return (uint32_t)(uintptr_t)(const lds_char *)p;
+}
+
+// ------------------------------------------------------------------ operands
+template <typename T, int DK>
+__device__ __forceinline__ vec8<T> row_operand(const char *tile, int row0, int step) {
+    return *reinterpret_cast<const vec8<T> *>(tile + row_operand_byte<DK>(lane_id(), row0, step));
+}
+
+// Rows row0 .. row0 + 15 in the order a C leaves its rows, columns 32 block ...
+template <typename T, int DK>
+__device__ __forceinline__ vec8<T> column_operand(const char *tile, int row0, int block) {
+    const auto read = [&](int r) {
+        return __builtin_bit_cast(
+            vec4<T>, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                         (lds_s16x4 *)(tile + column_operand_byte<DK>(lane_id(), r, block))));
+    };
+    return __builtin_shufflevector(read(row0), read(row0 + 8), 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
+// Eight elements of row `row` from column `at` in memory, zeros if !ok.
+template <typename T>
+__device__ __forceinline__ vec8<T> memory_operand(const T *row, int at, bool ok) {
+    vec8<T> v = {};
+    if (ok) v = *reinterpret_cast<const vec8<T> *>(row + at);
+    return v;
+}
+
+// Max and sum over the two halves of a wave, lane l and l + 32.
+__device__ __forceinline__ float halves_max(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]),
+                 __builtin_bit_cast(float, (uint32_t)r[1]));
+}
+__device__ __forceinline__ float halves_sum(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __builtin_bit_cast(float, (uint32_t)r[0]) + __builtin_bit_cast(float, (uint32_t)r[1]);
+}
+
+// Host: f<T, DK>() for the element type and the head dimension's tile.
+template <typename F>
+static void attn_form(int32_t dtype, int dim, F f) {
+    const auto with = [&](auto t) {
+        using std::integral_constant;
+        if (dim <= 32)
+            f(t, integral_constant<int, 32>{});
+        else if (dim <= 64)
+            f(t, integral_constant<int, 64>{});
+        else if (dim <= 96)
+            f(t, integral_constant<int, 96>{});
+        else
+            f(t, integral_constant<int, 128>{});
+    };
+    if (dtype == MG_BF16)
+        with(bf16_t{});
+    else
+        with(f16_t{});
+}
+
+// scale * log2(e). A scale of 0 (all seen keys alike) keeps a trace, by which
+// the -inf of an unseen key stays what it is.
+inline float scale_to_log2(float scale) {
+    const float s = scale * 1.44269504088896340736f;
+    return s < 1e-30f ? 1e-30f : s;
+}
+
+int32_t attn_check(const char *who, const AttnArgs &a, int32_t dtype);
+
+}  // namespace mg

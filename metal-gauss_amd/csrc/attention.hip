@@ -1,0 +1,391 @@
+// Attention over packed sequences, forward:
+//
+//   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i k_j - lse_i)
+//
+// over the keys j of query i's own sequence, causal: those that stand at or
+// before it, a sequence's last query standing at its last key. Queries that see
+// no key give zeros.
+//
+// A work item is a tile of rows of one key head, a row being a query token
+// together with one of the `group` query heads that share the head: a single
+// token's heads fill a tile together, and keys and values are read once for
+// all of them. Its waves hold 32 rows each; keys and values pass through LDS in
+// tiles of 64, double buffered. With S^T = K Q^T a lane of the product holds
+// scores of one row only, so the running maximum and sum of its softmax are a
+// lane's own registers (and its partner's, 32 lanes on), and the scores are
+// already where the product O^T = V^T P^T wants them.
+//
+// The running maximum lags: the accumulators are rescaled only when a score
+// passes the maximum they go by by more than 2^8, which leaves every sum exact
+// to its 24 bits and skips nearly all rescaling.
+#include "attention.h"
+
+namespace mg {
+
+constexpr float kMaxLag = 8.f;                   // powers of 2
+constexpr int kWideWaves = 4, kNarrowWaves = 1;
+constexpr int64_t kSplitSlots = 1024;            // work items that keep the GPU busy
+
+// Keys that the last row of a tile sees bound its loop.
+__device__ __forceinline__ int keys_seen(const SeqItem &s, int token, int causal) {
+    if (!causal) return s.k_len;
+    return clamp_to(token + 1 + s.k_len - s.q_len, 0, s.k_len);
+}
+
+// One work item: false if there is none of this number.
+template <typename T, int DK, int kWaves, bool kSplit>
+__device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
+    constexpr int kRows = 32 * kWaves, kSteps = DK / 16, kBlocks = DK / 32;
+    __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK>];
+    const int lane = lane_id(), half = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int kh = work % a.k_heads, item = work / a.k_heads, G = a.group;
+    const auto tiles_of = [&](int ql, int) { return (ql * G + kRows - 1) / kRows; };
+    const auto chunks_of = [&](int, int kl) {
+        return kSplit ? max(1, (kl + a.split_keys - 1) / a.split_keys) : 1;
+    };
+    const SeqItem s = find_item<false>(
+        a, item, [&](int ql, int kl) { return tiles_of(ql, kl) * chunks_of(ql, kl); },
+        [](int, int) { return 0; });
+    if (!s.found || (kSplit && item >= a.items)) return false;
+    const int chunks = chunks_of(s.q_len, s.k_len);
+    const int tile = tiles_of(s.q_len, 0) - 1 - s.within / chunks, chunk = s.within % chunks;
+
+    // This lane's row.
+    const int row0 = tile * kRows + wave * 32;
+    const int row = row0 + lane % 32;
+    const int token = row / G, head = kh * G + row % G;
+    const bool row_ok = token < s.q_len;
+    const int see = row_ok ? keys_seen(s, token, a.causal) : 0;
+    // The keys of its wave's first and last row, and of the tile's last.
+    const int last_token = min((tile * kRows + kRows - 1) / G, s.q_len - 1);
+    const int see_first = keys_seen(s, min(row0 / G, s.q_len - 1), a.causal);
+    const int see_last = keys_seen(s, min((row0 + 31) / G, s.q_len - 1), a.causal);
+    int k_from = 0, k_to = keys_seen(s, last_token, a.causal);
+    if (kSplit) {
+        k_from = min(chunk * a.split_keys, k_to);
+        k_to = min(k_from + a.split_keys, k_to);
+    }
+
+    vec8<T> q[kSteps];
+    {
+        const T *qr = static_cast<const T *>(a.q.p) + (int64_t)(s.q_lo + token) * a.q.tok_stride +
+                      (int64_t)head * a.q.head_stride;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int at = 16 * i + 8 * half;
+            q[i] = memory_operand<T>(qr, at, row_ok && at < a.dim);
+        }
+    }
+    const char *kp = reinterpret_cast<const char *>(static_cast<const T *>(a.k.p) +
+                                                    (int64_t)s.k_lo * a.k.tok_stride +
+                                                    (int64_t)kh * a.k.head_stride);
+    const char *vp = reinterpret_cast<const char *>(static_cast<const T *>(a.v.p) +
+                                                    (int64_t)s.k_lo * a.v.tok_stride +
+                                                    (int64_t)kh * a.v.head_stride);
+    TileFill<DK, kWaves> fill_k, fill_v;
+    fill_k.init(a.k.tok_stride, a.dim, wave);
+    fill_v.init(a.v.tok_stride, a.dim, wave);
+    const auto ask = [&](int key0, int buf) {
+        fill_k.ask(kp, a.k.tok_stride, a.dim, key0, s.k_len, wave, lds_address(s_tile[buf][0]));
+        fill_v.ask(vp, a.v.tok_stride, a.dim, key0, s.k_len, wave, lds_address(s_tile[buf][1]));
+    };
+
+    f32x16 o[kBlocks] = {};
+    float top = -INFINITY, sum = 0.f;     // top: in powers of 2, what p goes by
+    int buf = 0;
+    if (k_from < k_to) ask(k_from, 0);
+    for (int key0 = k_from; key0 < k_to; key0 += kTileRows, buf ^= 1) {
+        tiles_ready();
+        if (key0 + kTileRows < k_to) ask(key0 + kTileRows, buf ^ 1);
+        if (key0 >= see_last) continue;   // the wave's rows see none of these keys
+        const char *kt = s_tile[buf][0], *vt = s_tile[buf][1];
+        f32x16 sc[2] = {};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            sc[0] = mfma32(row_operand<T, DK>(kt, 0, i), q[i], sc[0]);
+            sc[1] = mfma32(row_operand<T, DK>(kt, 32, i), q[i], sc[1]);
+        }
+        if (key0 + kTileRows > see_first) {
+            // Selected, not added to: a NaN of a key that is not seen goes too.
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (key0 + 32 * b + c_row(e, half) >= see) sc[b][e] = -INFINITY;
+        }
+        float most = fmaxf(sc[0][0], sc[1][0]);
+#pragma unroll
+        for (int e = 1; e < 16; ++e) most = fmaxf(most, fmaxf(sc[0][e], sc[1][e]));
+        most = halves_max(most) * a.scale_log2;
+        if (ballot(most > top + kMaxLag)) {
+            const float next = fmaxf(top, most);
+            // A row that has seen no finite score yet keeps zeros.
+            const float shrink = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
+            top = next;
+            sum *= shrink;
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) o[b] *= shrink;
+        }
+        const float by = top == -INFINITY ? 0.f : top;
+        vec8<T> p[4];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(sc[b][e], a.scale_log2, -by));
+                sum += x;
+                // Rounded to the type of the values for the product, after
+                // the sum has its full digits: half an ulp of each p at most.
+                p[2 * b + e / 8][e % 8] = (T)x;
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+                o[b] = mfma32(column_operand<T, DK>(vt, 16 * i, b), p[i], o[b]);
+    }
+    lds_reads_done();
+    sum = halves_sum(sum);
+
+    if constexpr (kSplit) {
+        const int64_t slot = (int64_t)work * kRows + wave * 32 + lane % 32;
+        float *po = a.partial + slot * (DK + 2);
+        if (!row_ok) return true;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) po[2 + 32 * b + c_row(e, half)] = o[b][e];
+        if (half == 0) {
+            po[0] = top;
+            po[1] = sum;
+        }
+        return true;
+    }
+    if (!row_ok) return true;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    T *out = static_cast<T *>(a.out) +
+             ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int at = 32 * b + c_row(e, half);
+            vec4<T> w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (T)(o[b][e + i] * inv);
+            if (at < a.dim) *reinterpret_cast<vec4<T> *>(out + at) = w;
+        }
+    if (a.lse && half == 0)
+        a.lse[(int64_t)head * a.q_tokens + s.q_lo + token] =
+            sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+    return true;
+}
+
+// How many items the chunks make is known on the device alone: as many
+// workgroups as fill the GPU take them in turn.
+template <typename T, int DK, int kWaves, bool kSplit>
+__global__ __launch_bounds__(64 * kWaves) void attn_fwd_kernel(AttnArgs a) {
+    if constexpr (!kSplit) {
+        attn_fwd_item<T, DK, kWaves, kSplit>(a, blockIdx.x);
+    } else {
+        for (int work = blockIdx.x; attn_fwd_item<T, DK, kWaves, kSplit>(a, work);
+             work += gridDim.x)
+            tiles_ready();
+    }
+}
+
+// Joins the chunks of a tile's rows: o = sum 2^(top_c - top) o_c / sum of the
+// same of sum_c.
+template <typename T, int DK, int kWaves>
+__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
+    constexpr int kRows = 32 * kWaves;
+    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads, G = a.group;
+    const auto tiles_of = [&](int ql, int) { return (ql * G + kRows - 1) / kRows; };
+    const auto chunks_of = [&](int kl) { return max(1, (kl + a.split_keys - 1) / a.split_keys); };
+    const SeqItem s = find_item<false>(a, item, tiles_of, [&](int ql, int kl) {
+        return tiles_of(ql, kl) * chunks_of(kl);
+    });
+    // Offsets that fall again could make more items than there are.
+    if (!s.found || s.before + (s.within + 1) * chunks_of(s.k_len) > a.items) return;
+    const int chunks = chunks_of(s.k_len), tile = tiles_of(s.q_len, 0) - 1 - s.within;
+    for (int i = threadIdx.x; i < kRows * (DK / 4); i += 256) {
+        const int r = i / (DK / 4), at = i % (DK / 4) * 4;
+        const int row = tile * kRows + r, token = row / G, head = kh * G + row % G;
+        if (token >= s.q_len || at >= a.dim) continue;
+        const auto part = [&](int c) {
+            const int64_t split_item = s.before + s.within * chunks + c;
+            return a.partial + ((split_item * a.k_heads + kh) * kRows + r) * (DK + 2);
+        };
+        float top = -INFINITY;
+        for (int c = 0; c < chunks; ++c) top = fmaxf(top, part(c)[0]);
+        float sum = 0.f, o[4] = {};
+        for (int c = 0; c < chunks; ++c) {
+            const float *p = part(c);
+            const float w = p[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[0] - top);
+            sum = fmaf(p[1], w, sum);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = fmaf(p[2 + at + k], w, o[k]);
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        T *out = static_cast<T *>(a.out) +
+                 ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim + at;
+        vec4<T> w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = (T)(o[k] * inv);
+        *reinterpret_cast<vec4<T> *>(out) = w;
+        if (a.lse && at == 0)
+            a.lse[(int64_t)head * a.q_tokens + s.q_lo + token] =
+                sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+    }
+}
+
+// -------------------------------------------------------------------- host
+int32_t attn_check(const char *who, const AttnArgs &a, int32_t dtype) {
+    MG_REQUIRE(dtype == MG_BF16 || dtype == MG_F16, "%s: bfloat16 or float16 needed", who);
+    MG_REQUIRE(a.dim >= 8 && a.dim <= 128 && a.dim % 8 == 0,
+               "%s: heads of %d elements; multiples of 8 up to 128 are taken", who, a.dim);
+    MG_REQUIRE(a.k_heads >= 1 && a.group >= 1 && (int64_t)a.k_heads * a.group <= 65536,
+               "%s: the query heads must be a multiple of the key heads", who);
+    MG_REQUIRE(a.n_seq >= 1 && a.n_seq < (1 << 30), "%s: %d sequences", who, a.n_seq);
+    MG_REQUIRE(a.q_off || a.k_off || a.n_seq == 1, "%s: %d sequences without offsets", who,
+               a.n_seq);
+    MG_REQUIRE((a.q_off == nullptr) == (a.k_off == nullptr),
+               "%s: offsets of queries and keys go together", who);
+    MG_REQUIRE(a.scale >= 0.f && a.scale < INFINITY, "%s: scale %g", who, (double)a.scale);
+    for (const AttnTensor *t : {&a.q, &a.k, &a.v, &a.dout}) {
+        MG_REQUIRE(((uintptr_t)t->p & 15) == 0 && t->tok_stride % 8 == 0 &&
+                       t->head_stride % 8 == 0,
+                   "%s: rows must be 16-byte aligned", who);
+        MG_REQUIRE(t->tok_stride >= 0 && t->tok_stride < (1 << 24) && t->head_stride >= 0,
+                   "%s: token strides of 0 to 2^24 elements are taken", who);
+    }
+    return MG_OK;
+}
+
+// How the rows are cut: tiles of 32 rows by one wave each where a sequence's
+// rows (on the average) would leave most of a 128-row tile empty, and keys in
+// chunks where the tiles alone leave the GPU idle.
+struct FwdPlan {
+    int waves;
+    int64_t tiles;          // a key head's, at most
+    int split_keys;         // 0: whole rows
+    int64_t items;          // a key head's, at most
+    int64_t bytes;          // of partial results
+};
+
+static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int group, int dim,
+                        int n_seq) {
+    FwdPlan p{};
+    const int64_t rows = q_tokens * group;
+    p.waves = rows <= 64 * (int64_t)n_seq ? kNarrowWaves : kWideWaves;
+    const int64_t tile_rows = 32 * p.waves;
+    // Pseudo sequences before the first and past the last offset count too.
+    p.tiles = rows / tile_rows + n_seq + 2;
+    const int64_t likely = ceil_div(rows, tile_rows) + n_seq - 1;
+    p.items = p.tiles;
+    const int64_t mean_keys = k_tokens / n_seq + 1;
+    if (likely * k_heads < kSplitSlots && mean_keys > 2 * kTileRows) {
+        const int64_t chunks = kSplitSlots / (likely * k_heads) + 1;
+        int64_t keys = ceil_div(ceil_div(mean_keys, chunks), kTileRows) * kTileRows;
+        if (keys < 2 * kTileRows) keys = 2 * kTileRows;
+        p.split_keys = (int)keys;
+        // Sum of tiles * (1 + keys / chunk) over the sequences, no sequence
+        // having more tiles than all rows make.
+        p.items += (rows / tile_rows + 1) * (k_tokens / keys);
+        const int dk = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
+        p.bytes = p.items * k_heads * tile_rows * (dk + 2) * 4;
+    }
+    return p;
+}
+
+}  // namespace mg
+
+extern "C" {
+
+int64_t mg_attention_forward_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+                                             int32_t k_heads, int32_t dim, int32_t sequences) {
+    if (q_tokens <= 0 || k_tokens < 0 || k_heads < 1 || q_heads < k_heads || sequences < 1)
+        return 0;
+    return mg::fwd_plan(q_tokens, k_tokens, k_heads, q_heads / k_heads, dim, sequences).bytes;
+}
+
+int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+                             int32_t k_heads, int32_t dim, const void *q, int64_t q_token_stride,
+                             int64_t q_head_stride, const void *k, int64_t k_token_stride,
+                             int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                             int64_t v_head_stride, const int32_t *q_offsets,
+                             const int32_t *k_offsets, int32_t sequences, int32_t causal,
+                             float scale, void *out, float *lse, void *workspace,
+                             int64_t workspace_bytes, mg_stream_t stream) {
+    using namespace mg;
+    const char *who = "mg_attention_forward";
+    MG_REQUIRE(k_heads >= 1 && q_heads >= 1 && q_heads % k_heads == 0,
+               "%s: %d query heads are no multiple of %d key heads", who, q_heads, k_heads);
+    const int group = q_heads / k_heads;
+    MG_REQUIRE(q_tokens >= 0 && k_tokens >= 0 && q_tokens * group < (int64_t(1) << 30) &&
+                   k_tokens < (int64_t(1) << 30),
+               "%s: %lld query and %lld key tokens", who, (long long)q_tokens,
+               (long long)k_tokens);
+    AttnArgs a{};
+    a.q = {q, q_token_stride, q_head_stride};
+    a.k = {k, k_token_stride, k_head_stride};
+    a.v = {v, v_token_stride, v_head_stride};
+    a.q_off = q_offsets, a.k_off = k_offsets, a.n_seq = sequences;
+    a.q_tokens = (int32_t)q_tokens, a.k_tokens = (int32_t)k_tokens;
+    a.k_heads = k_heads, a.group = group, a.dim = dim, a.causal = causal != 0;
+    a.scale = scale, a.scale_log2 = scale_to_log2(scale);
+    a.out = out, a.lse = lse;
+    int32_t rc = attn_check(who, a, dtype);
+    if (rc != MG_OK) return rc;
+    if (q_tokens == 0) return MG_OK;
+    MG_REQUIRE(q && out && (k_tokens == 0 || (k && v)), "%s: a pointer is NULL", who);
+    const FwdPlan p = fwd_plan(q_tokens, k_tokens, k_heads, group, dim, sequences);
+    MG_REQUIRE(p.items * k_heads < (int64_t(1) << 31), "%s: too many work items", who);
+    MG_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes),
+               "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
+               (long long)p.bytes);
+    a.split_keys = p.split_keys, a.items = (int32_t)p.items;
+    a.partial = static_cast<float *>(workspace);
+    hipStream_t st = as_stream(stream);
+    const int64_t items = p.items * k_heads;
+    const unsigned grid = (unsigned)(p.split_keys && items > 2 * kSplitSlots ? 2 * kSplitSlots : items);
+    {
+        TimedScope ts("attention_fwd", st);
+        attn_form(dtype, dim, [&](auto t, auto d) {
+            using T = decltype(t);
+            constexpr int DK = decltype(d)::value;
+            if (p.waves == kWideWaves) {
+                if (p.split_keys)
+                    attn_fwd_kernel<T, DK, kWideWaves, true><<<grid, 64 * kWideWaves, 0, st>>>(a);
+                else
+                    attn_fwd_kernel<T, DK, kWideWaves, false>
+                        <<<grid, 64 * kWideWaves, 0, st>>>(a);
+            } else {
+                if (p.split_keys)
+                    attn_fwd_kernel<T, DK, kNarrowWaves, true>
+                        <<<grid, 64 * kNarrowWaves, 0, st>>>(a);
+                else
+                    attn_fwd_kernel<T, DK, kNarrowWaves, false>
+                        <<<grid, 64 * kNarrowWaves, 0, st>>>(a);
+            }
+        });
+        MG_LAUNCHED("attn_fwd_kernel");
+    }
+    if (p.split_keys) {
+        TimedScope ts("attention_join", st);
+        const unsigned joins = (unsigned)(p.tiles * k_heads);
+        attn_form(dtype, dim, [&](auto t, auto d) {
+            using T = decltype(t);
+            constexpr int DK = decltype(d)::value;
+            if (p.waves == kWideWaves)
+                attn_join_kernel<T, DK, kWideWaves><<<joins, 256, 0, st>>>(a);
+            else
+                attn_join_kernel<T, DK, kNarrowWaves><<<joins, 256, 0, st>>>(a);
+        });
+        MG_LAUNCHED("attn_join_kernel");
+    }
+    return MG_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,426 @@
+// Attention's backward pass, from the rows' lse of the forward:
+//
+//   p_ij = exp(scale q_i k_j - lse_i)
+//   dv_j = sum_i p_ij do_i
+//   ds_ij = p_ij (do_i v_j - delta_i),  delta_i = do_i o_i
+//   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
+//
+// Two kernels form the scores once each: the queries' gradient goes over the
+// keys and keeps its sums in registers, the keys' and values' goes over the
+// queries of all heads that share them. Seven products in place of the five of
+// a single pass, but no gradient is added to memory by several workgroups: no
+// atomics, no float32 copy of dq, and the same bits from call to call.
+//
+// float16: p and ds of a long row lie where float16 has few digits or none left
+// (p of 16000 equal keys is 6e-5), so p enters its product 2^15 times as large,
+// and ds by a power of two that takes the largest ds there can be,
+// 2 max|do| max|v|, to about 2^14; the results are scaled back in float32.
+// bfloat16 has float32's range and needs neither.
+#include "attention.h"
+
+namespace mg {
+
+constexpr int kBwdWaves = 4;
+constexpr int kBwdTile = 32 * kBwdWaves;         // rows, or keys, of a work item
+
+template <typename T>
+constexpr float kPowerP = sizeof(T) == 2 && std::is_same<T, f16_t>::value ? 15.f : 0.f;
+
+// The power of two that ds is taken by, from the largest |do|^2 and |v|^2.
+template <typename T>
+__device__ __forceinline__ float ds_power(const float *largest) {
+    if constexpr (kPowerP<T> == 0.f) return 0.f;
+    const float l = 14.f - (1.f + 0.5f * (__builtin_amdgcn_logf(largest[0]) +
+                                          __builtin_amdgcn_logf(largest[1])));
+    return l > -100.f && l < 100.f ? floorf(l) : 0.f;
+}
+
+// largest[0], [1]: the largest |row|^2 of do and of v (float bits order like
+// whole numbers from 0 on; a NaN counts as nothing).
+__global__ void attn_zero_kernel(float *largest) { largest[threadIdx.x] = 0.f; }
+
+template <typename T>
+__global__ __launch_bounds__(256) void attn_largest_kernel(AttnTensor x, int64_t rows, int heads,
+                                                           int dim, float *largest) {
+    // 16 lanes a row, eight elements each.
+    const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    const int at = threadIdx.x % 16 * 8;
+    float sq = 0.f;
+    if (row < rows && at < dim) {
+        const T *p = static_cast<const T *>(x.p) + row / heads * x.tok_stride +
+                     row % heads * x.head_stride;
+        float f[8];
+        load_vec<T, 8>(p + at, f);
+        for (int i = 0; i < 8; ++i) sq = fmaf(f[i], f[i], sq);
+    }
+    for (int o = 8; o >= 1; o >>= 1) sq += __shfl_xor(sq, o, 16);
+    sq = wave_max(sq);
+    if (lane_id() == 0 && sq > 0.f)
+        atomicMax(reinterpret_cast<unsigned *>(largest), __builtin_bit_cast(unsigned, sq));
+}
+
+// ------------------------------------------------------- the queries' gradient
+template <typename T, int DK>
+__global__ __launch_bounds__(64 * kBwdWaves) void attn_dq_kernel(AttnArgs a) {
+    constexpr int kSteps = DK / 16, kBlocks = DK / 32;
+    __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK>];
+    const int lane = lane_id(), half = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads, G = a.group;
+    const auto tiles_of = [&](int ql, int) { return (ql * G + kBwdTile - 1) / kBwdTile; };
+    const SeqItem s = find_item<false>(a, item, tiles_of, [](int, int) { return 0; });
+    if (!s.found) return;
+    const int tile = tiles_of(s.q_len, 0) - 1 - s.within;
+    const auto sees = [&](int token) {
+        return a.causal ? clamp_to(token + 1 + s.k_len - s.q_len, 0, s.k_len) : s.k_len;
+    };
+    const int row0 = tile * kBwdTile + wave * 32;
+    const int row = row0 + lane % 32;
+    const int token = row / G, head = kh * G + row % G;
+    const bool row_ok = token < s.q_len;
+    const int see = row_ok ? sees(token) : 0;
+    const int see_first = sees(min(row0 / G, s.q_len - 1));
+    const int see_last = sees(min((row0 + 31) / G, s.q_len - 1));
+    const int k_to = sees(min((tile * kBwdTile + kBwdTile - 1) / G, s.q_len - 1));
+
+    vec8<T> q[kSteps], dout[kSteps];
+    float lse = INFINITY, delta = 0.f;
+    {
+        const T *qr = static_cast<const T *>(a.q.p) + (int64_t)(s.q_lo + token) * a.q.tok_stride +
+                      (int64_t)head * a.q.head_stride;
+        const T *dor = static_cast<const T *>(a.dout.p) +
+                       (int64_t)(s.q_lo + token) * a.dout.tok_stride +
+                       (int64_t)head * a.dout.head_stride;
+        const T *outr = static_cast<const T *>(a.out) +
+                        ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int at = 16 * i + 8 * half;
+            const bool ok = row_ok && at < a.dim;
+            q[i] = memory_operand<T>(qr, at, ok);
+            dout[i] = memory_operand<T>(dor, at, ok);
+            const vec8<T> out = memory_operand<T>(outr, at, ok);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) delta = fmaf((float)dout[i][k], (float)out[k], delta);
+        }
+        delta = halves_sum(delta);
+        if (row_ok) {
+            const int64_t at = (int64_t)head * a.q_tokens + s.q_lo + token;
+            lse = a.lse[at];
+            if (half == 0) const_cast<float *>(a.delta)[at] = delta;
+        }
+    }
+    const char *kp = reinterpret_cast<const char *>(static_cast<const T *>(a.k.p) +
+                                                    (int64_t)s.k_lo * a.k.tok_stride +
+                                                    (int64_t)kh * a.k.head_stride);
+    const char *vp = reinterpret_cast<const char *>(static_cast<const T *>(a.v.p) +
+                                                    (int64_t)s.k_lo * a.v.tok_stride +
+                                                    (int64_t)kh * a.v.head_stride);
+    TileFill<DK, kBwdWaves> fill_k, fill_v;
+    fill_k.init(a.k.tok_stride, a.dim, wave);
+    fill_v.init(a.v.tok_stride, a.dim, wave);
+    const auto ask = [&](int key0, int buf) {
+        fill_k.ask(kp, a.k.tok_stride, a.dim, key0, s.k_len, wave, lds_address(s_tile[buf][0]));
+        fill_v.ask(vp, a.v.tok_stride, a.dim, key0, s.k_len, wave, lds_address(s_tile[buf][1]));
+    };
+    const float power = ds_power<T>(a.grad_scale);
+    const float up = __builtin_amdgcn_exp2f(power);
+    const float delta_up = delta * up;
+
+    f32x16 dq[kBlocks] = {};
+    int buf = 0;
+    if (k_to > 0) ask(0, 0);
+    for (int key0 = 0; key0 < k_to; key0 += kTileRows, buf ^= 1) {
+        tiles_ready();
+        if (key0 + kTileRows < k_to) ask(key0 + kTileRows, buf ^ 1);
+        if (key0 >= see_last) continue;
+        const char *kt = s_tile[buf][0], *vt = s_tile[buf][1];
+        const bool masked = key0 + kTileRows > see_first;
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            f32x16 sc = {}, dp = {};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                sc = mfma32(row_operand<T, DK>(kt, 32 * b, i), q[i], sc);
+                dp = mfma32(row_operand<T, DK>(vt, 32 * b, i), dout[i], dp);
+            }
+            vec8<T> ds[2];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale_log2, -lse));
+                float d = p * fmaf(dp[e], up, -delta_up);
+                // Selected: what is not seen may be anything.
+                if (masked && key0 + 32 * b + c_row(e, half) >= see) d = 0.f;
+                ds[e / 8][e % 8] = (T)d;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int c = 0; c < kBlocks; ++c)
+                    dq[c] = mfma32(column_operand<T, DK>(kt, 32 * b + 16 * i, c), ds[i], dq[c]);
+        }
+    }
+    lds_reads_done();
+    if (!row_ok) return;
+    const float down = a.scale * __builtin_amdgcn_exp2f(-power);
+    T *out = static_cast<T *>(a.dq) +
+             ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int at = 32 * b + c_row(e, half);
+            vec4<T> w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = (T)(dq[b][e + i] * down);
+            if (at < a.dim) *reinterpret_cast<vec4<T> *>(out + at) = w;
+        }
+}
+
+// ------------------------------------------- the keys' and values' gradients
+// Asks for 64 rows' lse and delta (past the last row, the last row's again).
+__device__ __forceinline__ void ask_row_values(const float *at, int rows, uint32_t lds) {
+    const uint32_t off = 4 * min(lane_id(), rows - 1);
+    const i32x4 rsrc = buffer_of(at, 4 * rows);
+    asm volatile("s_mov_b32 m0, %0\n\t"
+                 "s_nop 0\n\t"
+                 "buffer_load_dword %1, %2, 0 offen lds"
+                 :
+                 : "s"(uniform((int)lds)), "v"(off), "s"(rsrc)
+                 : "memory");
+}
+
+template <typename T, int DK>
+__global__ __launch_bounds__(64 * kBwdWaves) void attn_dkv_kernel(AttnArgs a) {
+    constexpr int kSteps = DK / 16, kBlocks = DK / 32;
+    __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK>];
+    __shared__ __align__(16) float s_row[2][2][kTileRows];     // lse, delta
+    const int lane = lane_id(), half = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
+    const SeqItem s = find_item<true>(
+        a, item, [](int, int kl) { return (kl + kBwdTile - 1) / kBwdTile; },
+        [](int, int) { return 0; });
+    if (!s.found) return;
+    // Causal: the first keys are seen by the most queries; they come first.
+    const int first_key = s.within * kBwdTile;
+    const int key0 = first_key + wave * 32, key = key0 + lane % 32;
+    const bool key_ok = key < s.k_len;
+    const int ahead = s.k_len - s.q_len;       // query i sees keys up to i + ahead
+    const int q_from = a.causal ? max(0, first_key - ahead) / kTileRows * kTileRows : 0;
+
+    vec8<T> k[kSteps], v[kSteps];
+    {
+        const T *kr = static_cast<const T *>(a.k.p) + (int64_t)(s.k_lo + key) * a.k.tok_stride +
+                      (int64_t)kh * a.k.head_stride;
+        const T *vr = static_cast<const T *>(a.v.p) + (int64_t)(s.k_lo + key) * a.v.tok_stride +
+                      (int64_t)kh * a.v.head_stride;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const int at = 16 * i + 8 * half;
+            const bool ok = key_ok && at < a.dim;
+            k[i] = memory_operand<T>(kr, at, ok);
+            v[i] = memory_operand<T>(vr, at, ok);
+        }
+    }
+    TileFill<DK, kBwdWaves> fill_q, fill_do;
+    fill_q.init(a.q.tok_stride, a.dim, wave);
+    fill_do.init(a.dout.tok_stride, a.dim, wave);
+    const auto ask = [&](int g, int row0, int buf) {
+        const int head = kh * a.group + g;
+        const char *qp = reinterpret_cast<const char *>(static_cast<const T *>(a.q.p) +
+                                                        (int64_t)s.q_lo * a.q.tok_stride +
+                                                        (int64_t)head * a.q.head_stride);
+        const char *dop = reinterpret_cast<const char *>(
+            static_cast<const T *>(a.dout.p) + (int64_t)s.q_lo * a.dout.tok_stride +
+            (int64_t)head * a.dout.head_stride);
+        fill_q.ask(qp, a.q.tok_stride, a.dim, row0, s.q_len, wave, lds_address(s_tile[buf][0]));
+        fill_do.ask(dop, a.dout.tok_stride, a.dim, row0, s.q_len, wave,
+                    lds_address(s_tile[buf][1]));
+        if (wave < 2) {
+            const float *from = wave == 0 ? a.lse : a.delta;
+            ask_row_values(from + (int64_t)head * a.q_tokens + s.q_lo + row0,
+                           min(s.q_len - row0, kTileRows),
+                           lds_address(reinterpret_cast<const char *>(s_row[buf][wave])));
+        }
+    };
+    const float power = ds_power<T>(a.grad_scale);
+    const float ds_up = __builtin_amdgcn_exp2f(power - kPowerP<T>);
+
+    f32x16 dk[kBlocks] = {}, dv[kBlocks] = {};
+    const int tiles = q_from < s.q_len ? (s.q_len - q_from + kTileRows - 1) / kTileRows : 0;
+    const int steps = tiles * a.group;
+    int g = 0, row0 = q_from, buf = 0;
+    if (steps > 0) ask(0, q_from, 0);
+    for (int step = 0; step < steps; ++step, buf ^= 1) {
+        tiles_ready();
+        const int at_row0 = row0;
+        row0 += kTileRows;
+        if (row0 >= s.q_len) {
+            row0 = q_from;
+            ++g;
+        }
+        if (step + 1 < steps) ask(g, row0, buf ^ 1);
+        const char *qt = s_tile[buf][0], *dot = s_tile[buf][1];
+        // Every row of the tile sees every key of the wave?
+        const bool masked = at_row0 + kTileRows > s.q_len || key0 + 32 > s.k_len ||
+                            (a.causal && at_row0 + ahead < key0 + 31);
+        if (a.causal && at_row0 + kTileRows - 1 + ahead < key0) continue;    // none sees any
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+            f32x16 sc = {}, dp = {};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                sc = mfma32(row_operand<T, DK>(qt, 32 * b, i), k[i], sc);
+                dp = mfma32(row_operand<T, DK>(dot, 32 * b, i), v[i], dp);
+            }
+            vec8<T> p[2], ds[2];
+#pragma unroll
+            for (int e4 = 0; e4 < 16; e4 += 4) {
+                const int r = 32 * b + c_row(e4, half);
+                const f32x4 lse = *reinterpret_cast<const f32x4 *>(&s_row[buf][0][r]);
+                const f32x4 delta = *reinterpret_cast<const f32x4 *>(&s_row[buf][1][r]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int e = e4 + i;
+                    float x = __builtin_amdgcn_exp2f(
+                        fmaf(sc[e], a.scale_log2, kPowerP<T> - lse[i]));
+                    float d = x * ((dp[e] - delta[i]) * ds_up);
+                    if (masked) {
+                        const int token = at_row0 + r + i;
+                        const bool seen = token < s.q_len && key_ok &&
+                                          (!a.causal || key <= token + ahead);
+                        x = seen ? x : 0.f;
+                        d = seen ? d : 0.f;
+                    }
+                    p[e / 8][e % 8] = (T)x;
+                    ds[e / 8][e % 8] = (T)d;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int c = 0; c < kBlocks; ++c) {
+                    dv[c] = mfma32(column_operand<T, DK>(dot, 32 * b + 16 * i, c), p[i], dv[c]);
+                    dk[c] = mfma32(column_operand<T, DK>(qt, 32 * b + 16 * i, c), ds[i], dk[c]);
+                }
+        }
+    }
+    lds_reads_done();
+    if (!key_ok) return;
+    const float down = a.scale * __builtin_amdgcn_exp2f(-power);
+    const float down_v = __builtin_amdgcn_exp2f(-kPowerP<T>);
+    const int64_t at_row = ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim;
+    T *dkr = static_cast<T *>(a.dk) + at_row, *dvr = static_cast<T *>(a.dv) + at_row;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int at = 32 * b + c_row(e, half);
+            vec4<T> w, x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = (T)(dk[b][e + i] * down);
+                x[i] = (T)(dv[b][e + i] * down_v);
+            }
+            if (at < a.dim) {
+                *reinterpret_cast<vec4<T> *>(dkr + at) = w;
+                *reinterpret_cast<vec4<T> *>(dvr + at) = x;
+            }
+        }
+}
+
+// Bytes of the backward's scratch: delta, and the two largest norms.
+static int64_t bwd_largest_at(int64_t q_tokens, int64_t q_heads) {
+    return align256(q_tokens * q_heads * 4);
+}
+
+}  // namespace mg
+
+extern "C" {
+
+int64_t mg_attention_backward_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+                                              int32_t k_heads, int32_t dim, int32_t sequences) {
+    (void)k_tokens, (void)k_heads, (void)dim, (void)sequences;
+    if (q_tokens < 0 || q_heads < 1) return 0;
+    return mg::bwd_largest_at(q_tokens, q_heads) + 256;
+}
+
+int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+                              int32_t k_heads, int32_t dim, const void *q, int64_t q_token_stride,
+                              int64_t q_head_stride, const void *k, int64_t k_token_stride,
+                              int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                              int64_t v_head_stride, const int32_t *q_offsets,
+                              const int32_t *k_offsets, int32_t sequences, int32_t causal,
+                              float scale, const void *out, const float *lse, const void *dout,
+                              int64_t dout_token_stride, int64_t dout_head_stride, void *dq,
+                              void *dk, void *dv, void *workspace, int64_t workspace_bytes,
+                              mg_stream_t stream) {
+    using namespace mg;
+    const char *who = "mg_attention_backward";
+    MG_REQUIRE(k_heads >= 1 && q_heads >= 1 && q_heads % k_heads == 0,
+               "%s: %d query heads are no multiple of %d key heads", who, q_heads, k_heads);
+    const int group = q_heads / k_heads;
+    MG_REQUIRE(q_tokens >= 0 && k_tokens >= 0 && q_tokens * group < (int64_t(1) << 30) &&
+                   k_tokens < (int64_t(1) << 30),
+               "%s: %lld query and %lld key tokens", who, (long long)q_tokens,
+               (long long)k_tokens);
+    AttnArgs a{};
+    a.q = {q, q_token_stride, q_head_stride};
+    a.k = {k, k_token_stride, k_head_stride};
+    a.v = {v, v_token_stride, v_head_stride};
+    a.dout = {dout, dout_token_stride, dout_head_stride};
+    a.q_off = q_offsets, a.k_off = k_offsets, a.n_seq = sequences;
+    a.q_tokens = (int32_t)q_tokens, a.k_tokens = (int32_t)k_tokens;
+    a.k_heads = k_heads, a.group = group, a.dim = dim, a.causal = causal != 0;
+    a.scale = scale, a.scale_log2 = scale_to_log2(scale);
+    a.out = const_cast<void *>(out), a.lse = const_cast<float *>(lse);
+    a.dq = dq, a.dk = dk, a.dv = dv;
+    int32_t rc = attn_check(who, a, dtype);
+    if (rc != MG_OK) return rc;
+    MG_REQUIRE(q_tokens == 0 || (q && out && lse && dout && dq), "%s: a pointer is NULL", who);
+    MG_REQUIRE(k_tokens == 0 || (k && v), "%s: a pointer is NULL", who);
+    MG_REQUIRE((dk == nullptr) == (dv == nullptr), "%s: dk and dv go together", who);
+    const int64_t need = mg_attention_backward_workspace_bytes(q_tokens, k_tokens, q_heads,
+                                                               k_heads, dim, sequences);
+    MG_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %lld bytes, %lld needed",
+               who, (long long)workspace_bytes, (long long)need);
+    a.delta = static_cast<float *>(workspace);
+    float *largest =
+        reinterpret_cast<float *>(static_cast<char *>(workspace) + bwd_largest_at(q_tokens, q_heads));
+    a.grad_scale = largest;
+    hipStream_t st = as_stream(stream);
+    const int64_t q_items = (q_tokens * group / kBwdTile + sequences + 2) * k_heads;
+    const int64_t k_items = (k_tokens / kBwdTile + sequences + 2) * k_heads;
+    MG_REQUIRE(q_items < (int64_t(1) << 31) && k_items < (int64_t(1) << 31),
+               "%s: too many work items", who);
+    if (dtype == MG_F16 && q_tokens > 0 && k_tokens > 0) {
+        TimedScope ts("attention_largest", st);
+        const int64_t rows_q = q_tokens * q_heads, rows_k = k_tokens * k_heads;
+        attn_zero_kernel<<<1, 2, 0, st>>>(largest);
+        attn_largest_kernel<f16_t><<<(unsigned)ceil_div(rows_q, 16), 256, 0, st>>>(
+            a.dout, rows_q, q_heads, dim, largest);
+        attn_largest_kernel<f16_t><<<(unsigned)ceil_div(rows_k, 16), 256, 0, st>>>(
+            a.v, rows_k, k_heads, dim, largest + 1);
+        MG_LAUNCHED("attn_largest_kernel");
+    }
+    if (q_tokens > 0) {
+        TimedScope ts("attention_dq", st);
+        attn_form(dtype, dim, [&](auto t, auto d) {
+            attn_dq_kernel<decltype(t), decltype(d)::value>
+                <<<(unsigned)q_items, 64 * kBwdWaves, 0, st>>>(a);
+        });
+        MG_LAUNCHED("attn_dq_kernel");
+    }
+    if (k_tokens > 0 && dk) {
+        TimedScope ts("attention_dkv", st);
+        attn_form(dtype, dim, [&](auto t, auto d) {
+            attn_dkv_kernel<decltype(t), decltype(d)::value>
+                <<<(unsigned)k_items, 64 * kBwdWaves, 0, st>>>(a);
+        });
+        MG_LAUNCHED("attn_dkv_kernel");
+    }
+    return MG_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,74 @@
+// Index rules of the attention kernels' tiles: plain constexpr functions, also
+// compiled by the host compiler alone for the index tests. Internal header.
+#pragma once
+
+#include <stdint.h>
+
+namespace mg {
+
+// ------------------------------------------------- 32x32x16 matrix products
+// C (32 x 32) += A (32 x 16) B (16 x 32), a wave's 64 lanes in two halves h:
+//   A: lane l holds row l % 32, eight of its 16 columns;
+//   B: lane l holds column l % 32, eight of its 16 rows;
+//   C: lane l holds column l % 32, element e (of 16) is row c_row(e, h).
+// The product sums over the 16 in any order as long as A and B agree on it.
+// Operands read along memory rows take them in memory order (half h has
+// 8h .. 8h + 7). An operand that is a C of an earlier product has its rows
+// where that product left them, elements 8s .. 8s + 7 being the s-th B, and the
+// A beside it is read in that order: 4h .. 4h + 3 and 8 + 4h .. 8 + 4h + 3.
+constexpr int c_row(int e, int h) { return 8 * (e / 4) + 4 * h + e % 4; }
+
+// --------------------------------------------------------------- LDS tiles
+// Rows of DK elements of two bytes in chunks of 16 bytes, tile_chunks<DK>() to
+// a row; chunk c of row r lies at place c ^ tile_swizzle<DK>(r) of its row.
+// Both ways of reading then spread over the banks: eight neighbouring rows at
+// one chunk (an operand along rows) take eight different places of 128 bytes,
+// and four neighbouring rows at a pair of chunks (an operand across rows, the
+// transposing read) four different pairs.
+template <int DK>
+constexpr int tile_chunks() {
+    return DK <= 32 ? 4 : DK <= 64 ? 8 : 16;
+}
+
+template <int DK>
+constexpr int tile_swizzle(int r) {
+    return tile_chunks<DK>() == 4   ? ((r >> 1 & 1) << 1 | (r >> 2 & 1))
+           : tile_chunks<DK>() == 8 ? ((r & 3) << 1 | (r >> 2 & 1))
+                                    : ((r & 3) << 1 | (r >> 2 & 1) | (r & 8));
+}
+
+// Byte of chunk c of row r.
+template <int DK>
+constexpr int tile_byte(int r, int c) {
+    return (r * tile_chunks<DK>() + (c ^ tile_swizzle<DK>(r))) * 16;
+}
+
+// Byte that lane l reads for rows row0 + l's chunk of a k step: an operand along
+// rows, 32 rows from row0, columns 16 step + 8 h ...
+template <int DK>
+constexpr int row_operand_byte(int lane, int row0, int step) {
+    return tile_byte<DK>(row0 + lane % 32, 2 * step + lane / 32);
+}
+
+// Byte that lane l points the transposing read at, for four rows row0 + 4 h ..
+// and the 32 columns from 32 block: 16 lanes hand over four rows of 16
+// columns, and get a column's four rows each.
+template <int DK>
+constexpr int column_operand_byte(int lane, int row0, int block) {
+    const int r = row0 + 4 * (lane / 32) + lane % 16 / 4;
+    const int col = 32 * block + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+    return tile_byte<DK>(r, col / 8) + col % 8 * 2;
+}
+
+// A tile is filled by loads of 64 chunks, in the order of their places: load i's
+// lane l fills place 64 i + l, whose row and chunk are these.
+template <int DK>
+constexpr int fill_row(int i, int lane) {
+    return (64 * i + lane) / tile_chunks<DK>();
+}
+template <int DK>
+constexpr int fill_chunk(int i, int lane) {
+    return (64 * i + lane) % tile_chunks<DK>() ^ tile_swizzle<DK>(fill_row<DK>(i, lane));
+}
+
+}  // namespace mg

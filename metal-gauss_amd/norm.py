@@ -1,0 +1,120 @@
+"""Layer norm on the GPU, forward and backward (mg_layer_norm_*).
+
+The reference has no counterpart: this is one of the operators of a network
+that predicts or refines splats, next to ``rotary`` and ``attention``.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+
+def _rows(x: torch.Tensor):
+    """(2-D view or copy of x, row stride): rows may lie apart, a row may not."""
+    n = x.shape[-1]
+    if x.dim() != 2:
+        x = x.reshape(-1, n)
+    if x.stride(1) != 1 and n != 1:
+        x = x.contiguous()
+    return x, x.stride(0)
+
+
+def _check_weight(w, x, what):
+    if w is None:
+        return
+    if w.shape != x.shape[-1:]:
+        raise ValueError(f"{what} must have shape ({x.shape[-1]},), got {tuple(w.shape)}")
+    if w.device != x.device:
+        raise RuntimeError(f"{what} must be on {x.device}, got device '{w.device}'")
+
+
+def _forward(x, weight, bias, eps, keep):
+    """y and, with ``keep``, what the backward pass needs."""
+    code = _lib.type_code(x, "x")
+    lib = _lib.load()
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise ValueError(f"layer_norm needs rows of at least one element, got {tuple(x.shape)}")
+    _check_weight(weight, x, "weight")
+    _check_weight(bias, x, "bias")
+    w = weight if weight is not None else bias
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"weight is {weight.dtype} and bias {bias.dtype}; one type is needed")
+    wcode = code if w is None else _lib.type_code(w, "weight")
+    if weight is not None:
+        weight = weight.contiguous()
+    if bias is not None:
+        bias = bias.contiguous()
+    rows, stride = _rows(x)
+    n = rows.shape[0]
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    stats = torch.empty(2, n, device=x.device) if keep else None
+    mean = stats.data_ptr() if keep else None
+    _lib.launch(lib.mg_layer_norm_forward, x, n, x.shape[-1], code, rows.data_ptr(), stride,
+                wcode, None if weight is None else weight.data_ptr(),
+                None if bias is None else bias.data_ptr(), eps, y.data_ptr(), mean,
+                mean + 4 * n if keep else None)
+    return y, rows, stats, weight
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, rows, stats, w = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(rows, w, stats)
+        ctx.x_shape = x.shape
+        ctx.has_bias = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        rows, w, stats = ctx.saved_tensors
+        lib = _lib.load()
+        n, width = rows.shape
+        dev = rows.device
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        if dy.dtype != rows.dtype:
+            dy = dy.to(rows.dtype)
+        dy, dy_stride = _rows(dy)
+        dx = torch.empty(ctx.x_shape, dtype=rows.dtype, device=dev) if need_x else None
+        wtype = w.dtype if w is not None else ctx.has_bias
+        make = torch.zeros if n == 0 else torch.empty
+        dw = make(width, dtype=wtype, device=dev) if need_w else None
+        db = make(width, dtype=wtype, device=dev) if need_b else None
+        if n == 0:
+            return dx, dw, db, None
+        ws = None
+        if need_w or need_b:
+            ws = torch.empty(lib.mg_layer_norm_backward_workspace_bytes(n, width),
+                             dtype=torch.uint8, device=dev)
+        code = _lib.TYPE_CODES[rows.dtype]
+        mean = stats.data_ptr()
+        _lib.launch(lib.mg_layer_norm_backward, rows, n, width, code, rows.data_ptr(),
+                    rows.stride(0), dy.data_ptr(), dy_stride,
+                    code if wtype is None else _lib.TYPE_CODES[wtype],
+                    None if w is None else w.data_ptr(), mean, mean + 4 * n,
+                    None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+                    None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
+                    0 if ws is None else ws.numel())
+        return dx, dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
+               bias: torch.Tensor | None = None, eps: float = 1e-5) -> torch.Tensor:
+    """Normalise the last dimension of ``x``:
+    ``(x - mean) / sqrt(var + eps) * weight + bias``.
+
+    ``x`` is float32, bfloat16 or float16, any shape; rows may be strided.
+    ``weight`` and ``bias`` (either may be None) are float32 or of x's type, and
+    their gradients come in that type. Means, variances and all sums are float32;
+    the result has x's type. Differentiable in all three, with the same bits from
+    call to call.
+    """
+    if torch.is_grad_enabled() and (
+            x.requires_grad or (weight is not None and weight.requires_grad) or
+            (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, float(eps))
+    return _forward(x, weight, bias, float(eps), False)[0]
