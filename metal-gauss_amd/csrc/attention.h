@@ -202,21 +202,33 @@ __device__ __forceinline__ uint32_t lds_address(const char *p) {
 }
 
 // ------------------------------------------------------------------ operands
+// A lane's places in any tile. fresh() keeps the compiler from holding an
+// address for every step in registers of its own: each is one exclusive or.
 template <typename T, int DK>
-__device__ __forceinline__ vec8<T> row_operand(const char *tile, int row0, int step) {
-    return *reinterpret_cast<const vec8<T> *>(tile + row_operand_byte<DK>(lane_id(), row0, step));
-}
+struct TileLane {
+    int row, column;
 
-// Rows row0 .. row0 + 15 in the order a C leaves its rows, columns 32 block ...
-template <typename T, int DK>
-__device__ __forceinline__ vec8<T> column_operand(const char *tile, int row0, int block) {
-    const auto read = [&](int r) {
-        return __builtin_bit_cast(
-            vec4<T>, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                         (lds_s16x4 *)(tile + column_operand_byte<DK>(lane_id(), r, block))));
-    };
-    return __builtin_shufflevector(read(row0), read(row0 + 8), 0, 1, 2, 3, 4, 5, 6, 7);
-}
+    __device__ __forceinline__ TileLane()
+        : row(row_lane_byte<DK>(lane_id())), column(column_lane_byte<DK>(lane_id())) {}
+
+    __device__ __forceinline__ void fresh() {
+        asm volatile("" : "+v"(row), "+v"(column));
+    }
+
+    __device__ __forceinline__ vec8<T> rows(const char *tile, int row0, int step) const {
+        return *reinterpret_cast<const vec8<T> *>(tile + row_operand_byte<DK>(row, row0, step));
+    }
+
+    // Rows row0 .. row0 + 15 in the order a C leaves its rows, columns 32 block ...
+    __device__ __forceinline__ vec8<T> columns(const char *tile, int row0, int block) const {
+        const auto read = [&](int r) {
+            return __builtin_bit_cast(
+                vec4<T>, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                             (lds_s16x4 *)(tile + column_operand_byte<DK>(column, r, block))));
+        };
+        return __builtin_shufflevector(read(row0), read(row0 + 8), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
 
 // Eight elements of row `row` from column `at` in memory, zeros if !ok.
 template <typename T>

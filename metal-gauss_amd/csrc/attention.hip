@@ -93,18 +93,20 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
 
     f32x16 o[kBlocks] = {};
     float top = -INFINITY, sum = 0.f;     // top: in powers of 2, what p goes by
+    TileLane<T, DK> lane_at;
     int buf = 0;
     if (k_from < k_to) ask(k_from, 0);
     for (int key0 = k_from; key0 < k_to; key0 += kTileRows, buf ^= 1) {
         tiles_ready();
+        lane_at.fresh();
         if (key0 + kTileRows < k_to) ask(key0 + kTileRows, buf ^ 1);
         if (key0 >= see_last) continue;   // the wave's rows see none of these keys
         const char *kt = s_tile[buf][0], *vt = s_tile[buf][1];
         f32x16 sc[2] = {};
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
-            sc[0] = mfma32(row_operand<T, DK>(kt, 0, i), q[i], sc[0]);
-            sc[1] = mfma32(row_operand<T, DK>(kt, 32, i), q[i], sc[1]);
+            sc[0] = mfma32(lane_at.rows(kt, 0, i), q[i], sc[0]);
+            sc[1] = mfma32(lane_at.rows(kt, 32, i), q[i], sc[1]);
         }
         if (key0 + kTileRows > see_first) {
             // Selected, not added to: a NaN of a key that is not seen goes too.
@@ -143,7 +145,7 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
-                o[b] = mfma32(column_operand<T, DK>(vt, 16 * i, b), p[i], o[b]);
+                o[b] = mfma32(lane_at.columns(vt, 16 * i, b), p[i], o[b]);
     }
     lds_reads_done();
     sum = halves_sum(sum);
@@ -185,7 +187,7 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
 // How many items the chunks make is known on the device alone: as many
 // workgroups as fill the GPU take them in turn.
 template <typename T, int DK, int kWaves, bool kSplit>
-__global__ __launch_bounds__(64 * kWaves) void attn_fwd_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, kWaves == 1 ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
     if constexpr (!kSplit) {
         attn_fwd_item<T, DK, kWaves, kSplit>(a, blockIdx.x);
     } else {

@@ -61,7 +61,7 @@ __global__ __launch_bounds__(256) void attn_largest_kernel(AttnTensor x, int64_t
 
 // ------------------------------------------------------- the queries' gradient
 template <typename T, int DK>
-__global__ __launch_bounds__(64 * kBwdWaves) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) {
     constexpr int kSteps = DK / 16, kBlocks = DK / 32;
     __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK>];
     const int lane = lane_id(), half = lane / 32;
@@ -128,10 +128,12 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_dq_kernel(AttnArgs a) {
     const float delta_up = delta * up;
 
     f32x16 dq[kBlocks] = {};
+    TileLane<T, DK> lane_at;
     int buf = 0;
     if (k_to > 0) ask(0, 0);
     for (int key0 = 0; key0 < k_to; key0 += kTileRows, buf ^= 1) {
         tiles_ready();
+        lane_at.fresh();
         if (key0 + kTileRows < k_to) ask(key0 + kTileRows, buf ^ 1);
         if (key0 >= see_last) continue;
         const char *kt = s_tile[buf][0], *vt = s_tile[buf][1];
@@ -141,8 +143,8 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_dq_kernel(AttnArgs a) {
             f32x16 sc = {}, dp = {};
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                sc = mfma32(row_operand<T, DK>(kt, 32 * b, i), q[i], sc);
-                dp = mfma32(row_operand<T, DK>(vt, 32 * b, i), dout[i], dp);
+                sc = mfma32(lane_at.rows(kt, 32 * b, i), q[i], sc);
+                dp = mfma32(lane_at.rows(vt, 32 * b, i), dout[i], dp);
             }
             vec8<T> ds[2];
 #pragma unroll
@@ -157,7 +159,7 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_dq_kernel(AttnArgs a) {
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int c = 0; c < kBlocks; ++c)
-                    dq[c] = mfma32(column_operand<T, DK>(kt, 32 * b + 16 * i, c), ds[i], dq[c]);
+                    dq[c] = mfma32(lane_at.columns(kt, 32 * b + 16 * i, c), ds[i], dq[c]);
         }
     }
     lds_reads_done();
@@ -191,7 +193,7 @@ __device__ __forceinline__ void ask_row_values(const float *at, int rows, uint32
 }
 
 template <typename T, int DK>
-__global__ __launch_bounds__(64 * kBwdWaves) void attn_dkv_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a) {
     constexpr int kSteps = DK / 16, kBlocks = DK / 32;
     __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK>];
     __shared__ __align__(16) float s_row[2][2][kTileRows];     // lse, delta
@@ -250,10 +252,12 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_dkv_kernel(AttnArgs a) {
     f32x16 dk[kBlocks] = {}, dv[kBlocks] = {};
     const int tiles = q_from < s.q_len ? (s.q_len - q_from + kTileRows - 1) / kTileRows : 0;
     const int steps = tiles * a.group;
+    TileLane<T, DK> lane_at;
     int g = 0, row0 = q_from, buf = 0;
     if (steps > 0) ask(0, q_from, 0);
     for (int step = 0; step < steps; ++step, buf ^= 1) {
         tiles_ready();
+        lane_at.fresh();
         const int at_row0 = row0;
         row0 += kTileRows;
         if (row0 >= s.q_len) {
@@ -266,13 +270,13 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_dkv_kernel(AttnArgs a) {
         const bool masked = at_row0 + kTileRows > s.q_len || key0 + 32 > s.k_len ||
                             (a.causal && at_row0 + ahead < key0 + 31);
         if (a.causal && at_row0 + kTileRows - 1 + ahead < key0) continue;    // none sees any
-#pragma unroll
+#pragma unroll 1
         for (int b = 0; b < 2; ++b) {
             f32x16 sc = {}, dp = {};
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                sc = mfma32(row_operand<T, DK>(qt, 32 * b, i), k[i], sc);
-                dp = mfma32(row_operand<T, DK>(dot, 32 * b, i), v[i], dp);
+                sc = mfma32(lane_at.rows(qt, 32 * b, i), k[i], sc);
+                dp = mfma32(lane_at.rows(dot, 32 * b, i), v[i], dp);
             }
             vec8<T> p[2], ds[2];
 #pragma unroll
@@ -301,8 +305,8 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_dkv_kernel(AttnArgs a) {
             for (int i = 0; i < 2; ++i)
 #pragma unroll
                 for (int c = 0; c < kBlocks; ++c) {
-                    dv[c] = mfma32(column_operand<T, DK>(dot, 32 * b + 16 * i, c), p[i], dv[c]);
-                    dk[c] = mfma32(column_operand<T, DK>(qt, 32 * b + 16 * i, c), ds[i], dk[c]);
+                    dv[c] = mfma32(lane_at.columns(dot, 32 * b + 16 * i, c), p[i], dv[c]);
+                    dk[c] = mfma32(lane_at.columns(qt, 32 * b + 16 * i, c), ds[i], dk[c]);
                 }
         }
     }

@@ -43,21 +43,32 @@ constexpr int tile_byte(int r, int c) {
     return (r * tile_chunks<DK>() + (c ^ tile_swizzle<DK>(r))) * 16;
 }
 
-// Byte that lane l reads for rows row0 + l's chunk of a k step: an operand along
-// rows, 32 rows from row0, columns 16 step + 8 h ...
+// An operand along rows, 32 rows from row0 (a multiple of 32), columns 16 step +
+// 8 h .. of a k step: byte that lane l reads. The lane's own part stands apart:
+// chunk 2 step + h differs from h in bits that the swizzle is added to without
+// carry, so a step is one exclusive or away.
 template <int DK>
-constexpr int row_operand_byte(int lane, int row0, int step) {
-    return tile_byte<DK>(row0 + lane % 32, 2 * step + lane / 32);
+constexpr int row_lane_byte(int lane) {
+    return tile_byte<DK>(lane % 32, lane / 32);
+}
+template <int DK>
+constexpr int row_operand_byte(int lane_byte, int row0, int step) {
+    return (lane_byte ^ 32 * step) + row0 * tile_chunks<DK>() * 16;
 }
 
-// Byte that lane l points the transposing read at, for four rows row0 + 4 h ..
-// and the 32 columns from 32 block: 16 lanes hand over four rows of 16
-// columns, and get a column's four rows each.
+// An operand across rows: byte that lane l points the transposing read at, for
+// four rows row0 + 4 h .. (row0 a multiple of 8) and the 32 columns from 32 block.
+// 16 lanes hand over four rows of 16 columns, and get a column's four rows each.
 template <int DK>
-constexpr int column_operand_byte(int lane, int row0, int block) {
-    const int r = row0 + 4 * (lane / 32) + lane % 16 / 4;
-    const int col = 32 * block + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+constexpr int column_lane_byte(int lane) {
+    const int r = 4 * (lane / 32) + lane % 16 / 4;
+    const int col = 16 * (lane / 16 % 2) + 4 * (lane % 4);
     return tile_byte<DK>(r, col / 8) + col % 8 * 2;
+}
+template <int DK>
+constexpr int column_operand_byte(int lane_byte, int row0, int block) {
+    return (lane_byte ^ (64 * block ^ 16 * (tile_swizzle<DK>(row0) & 8))) +
+           row0 * tile_chunks<DK>() * 16;
 }
 
 // A tile is filled by loads of 64 chunks, in the order of their places: load i's

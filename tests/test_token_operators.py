@@ -28,11 +28,11 @@ def test_fills_and_operands_agree_on_every_place(tmp_path, dk):
         for (int r = 0; r < 64; r += 32)
             for (int s = 0; s < {dk} / 16; ++s)
                 for (int l = 0; l < 64; ++l)
-                    std::printf("1 %d %d %d %d\\n", row_operand_byte<{dk}>(l, r, s), r, s, l);
+                    std::printf("1 %d %d %d %d\\n", row_operand_byte<{dk}>(row_lane_byte<{dk}>(l), r, s), r, s, l);
         for (int r = 0; r < 64; r += 8)
             for (int b = 0; b < {dk} / 32; ++b)
                 for (int l = 0; l < 64; ++l)
-                    std::printf("2 %d %d %d %d\\n", column_operand_byte<{dk}>(l, r, b), r, b, l);""")
+                    std::printf("2 %d %d %d %d\\n", column_operand_byte<{dk}>(column_lane_byte<{dk}>(l), r, b), r, b, l);""")
     chunks = rows[0][0]
     place = {}
     for _, byte, r, c in (x for x in rows[1:] if x[0] == 0):
@@ -58,7 +58,7 @@ def test_fills_and_operands_agree_on_every_place(tmp_path, dk):
 def test_rows_read_together_lie_in_different_banks(tmp_path, dk):
     rows = _run(tmp_path, "attention_tiles.h", f"""
         for (int s = 0; s < {dk} / 16; ++s)
-            for (int l = 0; l < 64; ++l) std::printf("%d\\n", row_operand_byte<{dk}>(l, 0, s));""")
+            for (int l = 0; l < 64; ++l) std::printf("%d\\n", row_operand_byte<{dk}>(row_lane_byte<{dk}>(l), 0, s));""")
     at = [r[0] % 128 for r in rows]
     for i in range(0, len(at), 8):
         assert len(set(at[i:i + 8])) == 8
