@@ -27,11 +27,8 @@ __device__ __forceinline__ f32x16 mfma32(vec8<f16_t> a, vec8<f16_t> b, f32x16 c)
 
 // Keys (or, in the keys' gradient, queries) of one LDS tile.
 constexpr int kTileRows = 64;
-template <int DK>
-constexpr int kTileBytes = kTileRows * tile_chunks<DK>() * 16;
-// Loads of 64 chunks that fill a tile.
-template <int DK>
-constexpr int kTileLoads = kTileRows * tile_chunks<DK>() / 64;
+template <int DK, int kTile = kTileRows>
+constexpr int kTileBytes = kTile * tile_chunks<DK>() * 16;
 
 struct AttnTensor {
     const void *p;
@@ -48,14 +45,19 @@ struct AttnArgs {
     float scale, scale_log2;             // scale, scale * log2(e)
     void *out;                           // (q_tokens, q_heads, dim)
     float *lse;                          // (q_heads, q_tokens), in powers of 2; NULL: not kept
-    // Split over the keys: chunks of split_keys, joined from `partial`, which has
-    // room for `items` of each key head.
+    // Split over the keys: chunks of split_keys, whose {top, sum} and unscaled
+    // sums of values are joined afterwards; there is room for `items` of each
+    // key head.
     int32_t split_keys, items;
-    float *partial;
+    float2 *part_stats;
+    float *part_o;
     // Backward.
     const float *delta;                  // (q_heads, q_tokens)
-    const float *grad_scale;             // {c, 1 / c}: see attention_bwd.hip
+    const float *largest;                // float16: see attention_bwd.hip
     void *dq, *dk, *dv;
+    // Keys' gradients over `splits` runs of queries, each in float32.
+    int32_t splits;
+    float *part_dk, *part_dv;            // (splits, k_tokens, k_heads, dim)
 };
 
 // ---------------------------------------------------------------- sequences
@@ -86,13 +88,17 @@ __device__ __forceinline__ void seq_bounds(const int32_t *off, int n, int tokens
     len = (s > n ? tokens : clamp_to(off[s], lo, tokens)) - lo;
 }
 
+template <int CTRL, int ROW_MASK = 0xf>
+__device__ __forceinline__ int dpp_i(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
+}
 __device__ __forceinline__ int wave_inclusive_sum(int v) {
-    const int lane = lane_id();
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int up = __shfl_up(v, o, 64);
-        v += lane >= o ? up : 0;
-    }
+    v += dpp_i<0x111>(v);        // row_shr:1
+    v += dpp_i<0x112>(v);        // row_shr:2
+    v += dpp_i<0x114>(v);        // row_shr:4
+    v += dpp_i<0x118>(v);        // row_shr:8
+    v += dpp_i<0x142, 0xa>(v);   // row_bcast:15
+    v += dpp_i<0x143, 0xc>(v);   // row_bcast:31
     return v;
 }
 
@@ -143,22 +149,22 @@ __device__ __forceinline__ i32x4 buffer_of(const void *base, uint32_t bytes) {
                  uniform((int)bytes), 0x00020000};
 }
 
-// Asks for rows row0 .. row0 + 63 (of n_rows; past the last, the last row again,
+// Asks for rows row0 .. row0 + kTile - 1 (of n_rows; past the last, the last row again,
 // whose products the masks leave out) of one head into an LDS tile, straight
 // from memory: nothing passes through registers, and the wave goes on at once.
 // tiles_ready() waits. Wave `wave` of kWaves makes every kWaves-th load.
 //
 // The loads are written in assembly because the compiler, which cannot tell
 // one LDS buffer from the other, would wait for them before the next LDS read.
-template <int DK, int kWaves>
+template <int DK, int kWaves, int kTile = kTileRows>
 struct TileFill {
-    static constexpr int kLoads = kTileLoads<DK> / kWaves;
-    static_assert(kTileLoads<DK> % kWaves == 0, "whole loads a wave");
+    static constexpr int kAll = kTileBytes<DK, kTile> / 1024, kLoads = kAll / kWaves;
+    static_assert(kAll % kWaves == 0, "whole loads a wave");
     uint32_t off[kLoads];          // bytes from row0's, of a whole tile
 
     __device__ __forceinline__ void init(int64_t tok_stride, int dim, int wave) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) off[i] = offset(i, tok_stride, dim, wave, kTileRows);
+        for (int i = 0; i < kLoads; ++i) off[i] = offset(i, tok_stride, dim, wave, kTile);
     }
 
     // Columns past the head's dimension read column 0 .. 7: the products beside
@@ -172,14 +178,14 @@ struct TileFill {
 
     __device__ __forceinline__ void ask(const char *head, int64_t tok_stride, int dim, int row0,
                                         int n_rows, int wave, uint32_t lds) const {
-        const int rows = min(n_rows - row0, kTileRows);
+        const int rows = min(n_rows - row0, kTile);
         const char *base = head + (int64_t)row0 * tok_stride * 2;
         const uint32_t bytes = (uint32_t)(rows - 1) * (uint32_t)(tok_stride * 2) + dim * 2;
         const i32x4 rsrc = buffer_of(base, bytes);
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const uint32_t at =
-                rows == kTileRows ? off[i] : offset(i, tok_stride, dim, wave, rows);
+                rows == kTile ? off[i] : offset(i, tok_stride, dim, wave, rows);
             const int to = uniform((int)lds + (i * kWaves + wave) * 1024);
             asm volatile("s_mov_b32 m0, %0\n\t"
                          "s_nop 0\n\t"

@@ -23,8 +23,15 @@
 namespace mg {
 
 constexpr float kMaxLag = 8.f;                   // powers of 2
+
+// Work items come in two widths. Wide: 128 rows by four waves, tiles of 64
+// keys that all four read. Narrow, where a sequence's rows would leave most of
+// that empty (single tokens): 32 rows by one wave, tiles of 32 keys; memory
+// bounds it, and ten waves (64 columns) or five (128) of a CU each have a
+// tile's loads under way.
 constexpr int kWideWaves = 4, kNarrowWaves = 1;
-constexpr int64_t kSplitSlots = 1024;            // work items that keep the GPU busy
+template <int kWaves>
+constexpr int kKeyTile = kWaves == kNarrowWaves ? 32 : kTileRows;
 
 // Keys that the last row of a tile sees bound its loop.
 __device__ __forceinline__ int keys_seen(const SeqItem &s, int token, int causal) {
@@ -36,7 +43,8 @@ __device__ __forceinline__ int keys_seen(const SeqItem &s, int token, int causal
 template <typename T, int DK, int kWaves, bool kSplit>
 __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     constexpr int kRows = 32 * kWaves, kSteps = DK / 16, kBlocks = DK / 32;
-    __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK>];
+    constexpr int kTile = kKeyTile<kWaves>, kParts = kTile / 32;
+    __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK, kTile>];
     const int lane = lane_id(), half = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kh = work % a.k_heads, item = work / a.k_heads, G = a.group;
@@ -83,7 +91,7 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     const char *vp = reinterpret_cast<const char *>(static_cast<const T *>(a.v.p) +
                                                     (int64_t)s.k_lo * a.v.tok_stride +
                                                     (int64_t)kh * a.v.head_stride);
-    TileFill<DK, kWaves> fill_k, fill_v;
+    TileFill<DK, kWaves, kTile> fill_k, fill_v;
     fill_k.init(a.k.tok_stride, a.dim, wave);
     fill_v.init(a.v.tok_stride, a.dim, wave);
     const auto ask = [&](int key0, int buf) {
@@ -96,29 +104,31 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     TileLane<T, DK> lane_at;
     int buf = 0;
     if (k_from < k_to) ask(k_from, 0);
-    for (int key0 = k_from; key0 < k_to; key0 += kTileRows, buf ^= 1) {
+    for (int key0 = k_from; key0 < k_to; key0 += kTile, buf ^= 1) {
         tiles_ready();
         lane_at.fresh();
-        if (key0 + kTileRows < k_to) ask(key0 + kTileRows, buf ^ 1);
+        if (key0 + kTile < k_to) ask(key0 + kTile, buf ^ 1);
         if (key0 >= see_last) continue;   // the wave's rows see none of these keys
         const char *kt = s_tile[buf][0], *vt = s_tile[buf][1];
-        f32x16 sc[2] = {};
+        f32x16 sc[kParts] = {};
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            sc[0] = mfma32(lane_at.rows(kt, 0, i), q[i], sc[0]);
-            sc[1] = mfma32(lane_at.rows(kt, 32, i), q[i], sc[1]);
-        }
-        if (key0 + kTileRows > see_first) {
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int b = 0; b < kParts; ++b)
+                sc[b] = mfma32(lane_at.rows(kt, 32 * b, i), q[i], sc[b]);
+        if (key0 + kTile > see_first) {
             // Selected, not added to: a NaN of a key that is not seen goes too.
 #pragma unroll
-            for (int b = 0; b < 2; ++b)
+            for (int b = 0; b < kParts; ++b)
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
                     if (key0 + 32 * b + c_row(e, half) >= see) sc[b][e] = -INFINITY;
         }
-        float most = fmaxf(sc[0][0], sc[1][0]);
+        float most = sc[0][0];
 #pragma unroll
-        for (int e = 1; e < 16; ++e) most = fmaxf(most, fmaxf(sc[0][e], sc[1][e]));
+        for (int b = 0; b < kParts; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) most = fmaxf(most, sc[b][e]);
         most = halves_max(most) * a.scale_log2;
         if (ballot(most > top + kMaxLag)) {
             const float next = fmaxf(top, most);
@@ -130,9 +140,9 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
             for (int b = 0; b < kBlocks; ++b) o[b] *= shrink;
         }
         const float by = top == -INFINITY ? 0.f : top;
-        vec8<T> p[4];
+        vec8<T> p[2 * kParts];
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < kParts; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
                 const float x = __builtin_amdgcn_exp2f(fmaf(sc[b][e], a.scale_log2, -by));
@@ -142,7 +152,7 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
                 p[2 * b + e / 8][e % 8] = (T)x;
             }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 2 * kParts; ++i)
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b)
                 o[b] = mfma32(lane_at.columns(vt, 16 * i, b), p[i], o[b]);
@@ -152,16 +162,15 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
 
     if constexpr (kSplit) {
         const int64_t slot = (int64_t)work * kRows + wave * 32 + lane % 32;
-        float *po = a.partial + slot * (DK + 2);
         if (!row_ok) return true;
+        float *po = a.part_o + slot * DK;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) po[2 + 32 * b + c_row(e, half)] = o[b][e];
-        if (half == 0) {
-            po[0] = top;
-            po[1] = sum;
-        }
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<f32x4 *>(po + 32 * b + c_row(e, half)) =
+                    f32x4{o[b][e], o[b][e + 1], o[b][e + 2], o[b][e + 3]};
+        if (half == 0) a.part_stats[slot] = make_float2(top, sum);
         return true;
     }
     if (!row_ok) return true;
@@ -197,49 +206,92 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 1 ? 1 : 2) void attn_fwd_ker
     }
 }
 
-// Joins the chunks of a tile's rows: o = sum 2^(top_c - top) o_c / sum of the
-// same of sum_c.
-template <typename T, int DK, int kWaves>
+// Joins the chunks of a row: o = sum 2^(top_c - top) o_c / sum of the same of
+// sum_c. kJoin waves a row (four where rows have many chunks), wave w with every
+// kJoin-th chunk from w; a lane first holds a chunk's weight, then DK / 64 columns.
+template <typename T, int DK, int kWaves, int kJoin>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    constexpr int kRows = 32 * kWaves;
-    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads, G = a.group;
-    const auto tiles_of = [&](int ql, int) { return (ql * G + kRows - 1) / kRows; };
+    constexpr int kRows = 32 * kWaves, kCols = DK <= 64 ? 1 : 2;
+    __shared__ float s_o[kJoin > 1 ? kJoin : 1][64 * kCols], s_top[kJoin], s_sum[kJoin];
+    const int lane = lane_id(), G = a.group, heads = a.k_heads * G;
+    const int wave = uniform(threadIdx.x / 64);
+    const int64_t row_head = kJoin > 1 ? blockIdx.x : (int64_t)blockIdx.x * 4 + wave;
+    const int at_token = (int)(row_head / heads), head = (int)(row_head % heads);
+    if (at_token >= a.q_tokens) return;
+    const int kh = head / G, first = kJoin > 1 ? wave : 0;
+    const auto tiles_of = [&](int ql) { return (ql * G + kRows - 1) / kRows; };
     const auto chunks_of = [&](int kl) { return max(1, (kl + a.split_keys - 1) / a.split_keys); };
-    const SeqItem s = find_item<false>(a, item, tiles_of, [&](int ql, int kl) {
-        return tiles_of(ql, kl) * chunks_of(kl);
-    });
+    const SeqItem s = find_item<false>(
+        a, at_token, [](int ql, int) { return ql; },
+        [&](int ql, int kl) { return tiles_of(ql) * chunks_of(kl); });
+    if (!s.found) return;
+    const int row = s.within * G + head % G, tile = row / kRows, chunks = chunks_of(s.k_len);
+    const int item0 = s.before + (tiles_of(s.q_len) - 1 - tile) * chunks;
     // Offsets that fall again could make more items than there are.
-    if (!s.found || s.before + (s.within + 1) * chunks_of(s.k_len) > a.items) return;
-    const int chunks = chunks_of(s.k_len), tile = tiles_of(s.q_len, 0) - 1 - s.within;
-    for (int i = threadIdx.x; i < kRows * (DK / 4); i += 256) {
-        const int r = i / (DK / 4), at = i % (DK / 4) * 4;
-        const int row = tile * kRows + r, token = row / G, head = kh * G + row % G;
-        if (token >= s.q_len || at >= a.dim) continue;
-        const auto part = [&](int c) {
-            const int64_t split_item = s.before + s.within * chunks + c;
-            return a.partial + ((split_item * a.k_heads + kh) * kRows + r) * (DK + 2);
+    if (item0 + chunks > a.items) return;
+    const auto slot = [&](int c) {
+        return ((int64_t)(item0 + c) * a.k_heads + kh) * kRows + row % kRows;
+    };
+    float top = -INFINITY, sum = 0.f, o[kCols] = {};
+    for (int c0 = first; c0 < chunks; c0 += 64 * kJoin) {
+        const int n = min((chunks - c0 + kJoin - 1) / kJoin, 64);
+        const float2 st =
+            lane < n ? a.part_stats[slot(c0 + kJoin * lane)] : make_float2(-INFINITY, 0.f);
+        const float next = fmaxf(top, wave_max(st.x));
+        const float shrink = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
+        const float w = st.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.x - next);
+        top = next;
+        // A NaN sum of a chunk without a finite score goes on.
+        sum = sum * shrink + wave_sum_all(st.y * w);
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) o[k] *= shrink;
+        const auto add = [&](int c) {
+            const float wc = __builtin_bit_cast(
+                float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), c));
+            const float *p = a.part_o + slot(c0 + kJoin * c) * DK + lane * kCols;
+            float f[kCols];
+            if (lane * kCols < DK) {
+                __builtin_memcpy(f, p, sizeof(f));
+#pragma unroll
+                for (int k = 0; k < kCols; ++k) o[k] = fmaf(f[k], wc, o[k]);
+            }
         };
-        float top = -INFINITY;
-        for (int c = 0; c < chunks; ++c) top = fmaxf(top, part(c)[0]);
-        float sum = 0.f, o[4] = {};
-        for (int c = 0; c < chunks; ++c) {
-            const float *p = part(c);
-            const float w = p[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[0] - top);
-            sum = fmaf(p[1], w, sum);
+        int c = 0;
+        for (; c + 8 <= n; c += 8)
 #pragma unroll
-            for (int k = 0; k < 4; ++k) o[k] = fmaf(p[2 + at + k], w, o[k]);
-        }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        T *out = static_cast<T *>(a.out) +
-                 ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim + at;
-        vec4<T> w;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) w[k] = (T)(o[k] * inv);
-        *reinterpret_cast<vec4<T> *>(out) = w;
-        if (a.lse && at == 0)
-            a.lse[(int64_t)head * a.q_tokens + s.q_lo + token] =
-                sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+            for (int k = 0; k < 8; ++k) add(c + k);
+        for (; c < n; ++c) add(c);
     }
+    if constexpr (kJoin > 1) {
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) s_o[wave][lane * kCols + k] = o[k];
+        if (lane == 0) {
+            s_top[wave] = top;
+            s_sum[wave] = sum;
+        }
+        __syncthreads();
+        if (wave != 0) return;
+        top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+        sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) o[k] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoin; ++w) {
+            const float by = s_top[w] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s_top[w] - top);
+            sum = fmaf(s_sum[w], by, sum);
+#pragma unroll
+            for (int k = 0; k < kCols; ++k) o[k] = fmaf(s_o[w][lane * kCols + k], by, o[k]);
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t at = ((int64_t)(s.q_lo + s.within) * heads + head) * a.dim + lane * kCols;
+    T w[kCols];
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) w[k] = (T)(o[k] * inv);
+    if (lane * kCols < a.dim) __builtin_memcpy(static_cast<T *>(a.out) + at, w, sizeof(w));
+    if (a.lse && lane == 0)
+        a.lse[(int64_t)head * a.q_tokens + s.q_lo + s.within] =
+            sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
 // -------------------------------------------------------------------- host
@@ -265,38 +317,41 @@ int32_t attn_check(const char *who, const AttnArgs &a, int32_t dtype) {
     return MG_OK;
 }
 
-// How the rows are cut: tiles of 32 rows by one wave each where a sequence's
-// rows (on the average) would leave most of a 128-row tile empty, and keys in
-// chunks where the tiles alone leave the GPU idle.
+// How the work is cut. Narrow items where rows fill half a wide item at most (on
+// the average of the sequences); chunks of keys where the items alone leave the
+// GPU idle and a row has keys enough to be worth the second launch.
 struct FwdPlan {
     int waves;
-    int64_t tiles;          // a key head's, at most
-    int split_keys;         // 0: whole rows
-    int64_t items;          // a key head's, at most
-    int64_t bytes;          // of partial results
+    int split_keys;             // 0: whole rows
+    int64_t items;              // a key head's, at most
+    int64_t stats_bytes, bytes; // of partial results
 };
+
+constexpr int64_t kWideSlots = 512, kNarrowSlots = 1536;
+constexpr int64_t kSplitLeast = 768, kChunkLeast = 256;
 
 static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int group, int dim,
                         int n_seq) {
     FwdPlan p{};
     const int64_t rows = q_tokens * group;
     p.waves = rows <= 64 * (int64_t)n_seq ? kNarrowWaves : kWideWaves;
-    const int64_t tile_rows = 32 * p.waves;
-    // Pseudo sequences before the first and past the last offset count too.
-    p.tiles = rows / tile_rows + n_seq + 2;
-    const int64_t likely = ceil_div(rows, tile_rows) + n_seq - 1;
-    p.items = p.tiles;
-    const int64_t mean_keys = k_tokens / n_seq + 1;
-    if (likely * k_heads < kSplitSlots && mean_keys > 2 * kTileRows) {
-        const int64_t chunks = kSplitSlots / (likely * k_heads) + 1;
-        int64_t keys = ceil_div(ceil_div(mean_keys, chunks), kTileRows) * kTileRows;
-        if (keys < 2 * kTileRows) keys = 2 * kTileRows;
+    const int64_t tile_rows = 32 * p.waves, tile = p.waves == kNarrowWaves ? 32 : kTileRows;
+    const int64_t slots = p.waves == kNarrowWaves ? kNarrowSlots : kWideSlots;
+    // The tokens before the first and past the last offset make tiles too.
+    p.items = rows / tile_rows + n_seq + 2;
+    const int64_t likely = (ceil_div(rows, tile_rows) + n_seq - 1) * k_heads;
+    const int64_t mean_keys = k_tokens / n_seq;
+    if (2 * likely <= slots && mean_keys >= kSplitLeast) {
+        int64_t keys = ceil_div(ceil_div(mean_keys * likely, slots), tile) * tile;
+        if (keys < kChunkLeast) keys = kChunkLeast;
         p.split_keys = (int)keys;
         // Sum of tiles * (1 + keys / chunk) over the sequences, no sequence
         // having more tiles than all rows make.
         p.items += (rows / tile_rows + 1) * (k_tokens / keys);
         const int dk = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
-        p.bytes = p.items * k_heads * tile_rows * (dk + 2) * 4;
+        const int64_t part_rows = p.items * k_heads * tile_rows;
+        p.stats_bytes = align256(part_rows * 8);
+        p.bytes = p.stats_bytes + part_rows * dk * 4;
     }
     return p;
 }
@@ -348,10 +403,13 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
                "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
                (long long)p.bytes);
     a.split_keys = p.split_keys, a.items = (int32_t)p.items;
-    a.partial = static_cast<float *>(workspace);
+    a.part_stats = static_cast<float2 *>(workspace);
+    a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.stats_bytes);
     hipStream_t st = as_stream(stream);
     const int64_t items = p.items * k_heads;
-    const unsigned grid = (unsigned)(p.split_keys && items > 2 * kSplitSlots ? 2 * kSplitSlots : items);
+    // Chunks are taken in turn by twice as many workgroups as run at once.
+    const int64_t most = 2 * (p.waves == kWideWaves ? kWideSlots : kNarrowSlots);
+    const unsigned grid = (unsigned)(p.split_keys && items > most ? most : items);
     {
         TimedScope ts("attention_fwd", st);
         attn_form(dtype, dim, [&](auto t, auto d) {
@@ -376,14 +434,25 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
     }
     if (p.split_keys) {
         TimedScope ts("attention_join", st);
-        const unsigned joins = (unsigned)(p.tiles * k_heads);
+        // Four waves a row where rows have more chunks than one wave asks for
+        // at once, on the average.
+        const bool many = k_tokens / sequences > 8 * (int64_t)p.split_keys;
+        const int64_t rows = q_tokens * q_heads;
+        const unsigned joins = (unsigned)(many ? rows : ceil_div(rows, 4));
         attn_form(dtype, dim, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int DK = decltype(d)::value;
-            if (p.waves == kWideWaves)
-                attn_join_kernel<T, DK, kWideWaves><<<joins, 256, 0, st>>>(a);
-            else
-                attn_join_kernel<T, DK, kNarrowWaves><<<joins, 256, 0, st>>>(a);
+            if (p.waves == kWideWaves) {
+                if (many)
+                    attn_join_kernel<T, DK, kWideWaves, 4><<<joins, 256, 0, st>>>(a);
+                else
+                    attn_join_kernel<T, DK, kWideWaves, 1><<<joins, 256, 0, st>>>(a);
+            } else {
+                if (many)
+                    attn_join_kernel<T, DK, kNarrowWaves, 4><<<joins, 256, 0, st>>>(a);
+                else
+                    attn_join_kernel<T, DK, kNarrowWaves, 1><<<joins, 256, 0, st>>>(a);
+            }
         });
         MG_LAUNCHED("attn_join_kernel");
     }

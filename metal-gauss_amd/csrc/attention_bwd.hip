@@ -26,37 +26,60 @@ constexpr int kBwdTile = 32 * kBwdWaves;         // rows, or keys, of a work ite
 template <typename T>
 constexpr float kPowerP = sizeof(T) == 2 && std::is_same<T, f16_t>::value ? 15.f : 0.f;
 
-// The power of two that ds is taken by, from the largest |do|^2 and |v|^2.
+// The largest |row|^2 of do (blockIdx.y 0) and of v (1) that each workgroup finds,
+// to largest[kNormGroups y + x]. A NaN counts as nothing.
+constexpr int kNormGroups = 256;
+
 template <typename T>
-__device__ __forceinline__ float ds_power(const float *largest) {
-    if constexpr (kPowerP<T> == 0.f) return 0.f;
-    const float l = 14.f - (1.f + 0.5f * (__builtin_amdgcn_logf(largest[0]) +
-                                          __builtin_amdgcn_logf(largest[1])));
-    return l > -100.f && l < 100.f ? floorf(l) : 0.f;
+__global__ __launch_bounds__(256) void attn_largest_kernel(AttnArgs a, float *largest) {
+    __shared__ float s_most[4];
+    const AttnTensor &x = blockIdx.y ? a.v : a.dout;
+    const int heads = blockIdx.y ? a.k_heads : a.k_heads * a.group;
+    const int64_t rows = (int64_t)(blockIdx.y ? a.k_tokens : a.q_tokens) * heads;
+    // 16 lanes a row, eight elements each.
+    const int at = threadIdx.x % 16 * 8;
+    float most = 0.f;
+    for (int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16; row < rows;
+         row += kNormGroups * 16) {
+        float sq = 0.f;
+        if (at < a.dim) {
+            const int token = (int)(row / heads), head = (int)(row % heads);
+            const T *p = static_cast<const T *>(x.p) + token * x.tok_stride + head * x.head_stride;
+            float f[8];
+            load_vec<T, 8>(p + at, f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sq = fmaf(f[i], f[i], sq);
+        }
+#pragma unroll
+        for (int o = 8; o >= 1; o >>= 1) sq += __shfl_xor(sq, o, 16);
+        most = fmaxf(most, sq);
+    }
+    most = wave_max(most);
+    if (lane_id() == 0) s_most[threadIdx.x / 64] = most;
+    __syncthreads();
+    if (threadIdx.x == 0)
+        largest[kNormGroups * blockIdx.y + blockIdx.x] =
+            fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
 }
 
-// largest[0], [1]: the largest |row|^2 of do and of v (float bits order like
-// whole numbers from 0 on; a NaN counts as nothing).
-__global__ void attn_zero_kernel(float *largest) { largest[threadIdx.x] = 0.f; }
-
+// The power of two that ds is taken by.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_largest_kernel(AttnTensor x, int64_t rows, int heads,
-                                                           int dim, float *largest) {
-    // 16 lanes a row, eight elements each.
-    const int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
-    const int at = threadIdx.x % 16 * 8;
-    float sq = 0.f;
-    if (row < rows && at < dim) {
-        const T *p = static_cast<const T *>(x.p) + row / heads * x.tok_stride +
-                     row % heads * x.head_stride;
-        float f[8];
-        load_vec<T, 8>(p + at, f);
-        for (int i = 0; i < 8; ++i) sq = fmaf(f[i], f[i], sq);
+__device__ __forceinline__ float ds_power(const float *largest) {
+    if constexpr (kPowerP<T> == 0.f) {
+        return 0.f;
+    } else {
+        float m[2] = {};
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+#pragma unroll
+            for (int i = 0; i < kNormGroups; i += 64)
+                m[y] = fmaxf(m[y], largest[kNormGroups * y + i + lane_id()]);
+            m[y] = wave_max(m[y]);
+        }
+        const float l =
+            13.f - 0.5f * (__builtin_amdgcn_logf(m[0]) + __builtin_amdgcn_logf(m[1]));
+        return l > -100.f && l < 100.f ? floorf(l) : 0.f;
     }
-    for (int o = 8; o >= 1; o >>= 1) sq += __shfl_xor(sq, o, 16);
-    sq = wave_max(sq);
-    if (lane_id() == 0 && sq > 0.f)
-        atomicMax(reinterpret_cast<unsigned *>(largest), __builtin_bit_cast(unsigned, sq));
 }
 
 // ------------------------------------------------------- the queries' gradient
@@ -123,7 +146,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
         fill_k.ask(kp, a.k.tok_stride, a.dim, key0, s.k_len, wave, lds_address(s_tile[buf][0]));
         fill_v.ask(vp, a.v.tok_stride, a.dim, key0, s.k_len, wave, lds_address(s_tile[buf][1]));
     };
-    const float power = ds_power<T>(a.grad_scale);
+    const float power = ds_power<T>(a.largest);
     const float up = __builtin_amdgcn_exp2f(power);
     const float delta_up = delta * up;
 
@@ -199,7 +222,8 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     __shared__ __align__(16) float s_row[2][2][kTileRows];     // lse, delta
     const int lane = lane_id(), half = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
+    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads / a.splits;
+    const int split = blockIdx.x / a.k_heads % a.splits;
     const SeqItem s = find_item<true>(
         a, item, [](int, int kl) { return (kl + kBwdTile - 1) / kBwdTile; },
         [](int, int) { return 0; });
@@ -246,15 +270,22 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
                            lds_address(reinterpret_cast<const char *>(s_row[buf][wave])));
         }
     };
-    const float power = ds_power<T>(a.grad_scale);
+    const float power = ds_power<T>(a.largest);
     const float ds_up = __builtin_amdgcn_exp2f(power - kPowerP<T>);
 
     f32x16 dk[kBlocks] = {}, dv[kBlocks] = {};
     const int tiles = q_from < s.q_len ? (s.q_len - q_from + kTileRows - 1) / kTileRows : 0;
-    const int steps = tiles * a.group;
+    // A split has a run of the steps: query tiles of one head after the other.
+    const int all = tiles * a.group;
+    const int from = (int)((int64_t)all * split / a.splits);
+    const int steps = (int)((int64_t)all * (split + 1) / a.splits) - from;
     TileLane<T, DK> lane_at;
     int g = 0, row0 = q_from, buf = 0;
-    if (steps > 0) ask(0, q_from, 0);
+    if (steps > 0) {
+        g = from / tiles;
+        row0 += from % tiles * kTileRows;
+        ask(g, row0, 0);
+    }
     for (int step = 0; step < steps; ++step, buf ^= 1) {
         tiles_ready();
         lane_at.fresh();
@@ -315,28 +346,66 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     const float down = a.scale * __builtin_amdgcn_exp2f(-power);
     const float down_v = __builtin_amdgcn_exp2f(-kPowerP<T>);
     const int64_t at_row = ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim;
+    const int64_t part = (int64_t)split * a.k_tokens * a.k_heads * a.dim + at_row;
     T *dkr = static_cast<T *>(a.dk) + at_row, *dvr = static_cast<T *>(a.dv) + at_row;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const int at = 32 * b + c_row(e, half);
-            vec4<T> w, x;
+            f32x4 w, x;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                w[i] = (T)(dk[b][e + i] * down);
-                x[i] = (T)(dv[b][e + i] * down_v);
+                w[i] = dk[b][e + i] * down;
+                x[i] = dv[b][e + i] * down_v;
             }
-            if (at < a.dim) {
-                *reinterpret_cast<vec4<T> *>(dkr + at) = w;
-                *reinterpret_cast<vec4<T> *>(dvr + at) = x;
+            if (at >= a.dim) continue;
+            if (a.splits > 1) {
+                *reinterpret_cast<f32x4 *>(a.part_dk + part + at) = w;
+                *reinterpret_cast<f32x4 *>(a.part_dv + part + at) = x;
+            } else {
+                *reinterpret_cast<vec4<T> *>(dkr + at) = __builtin_convertvector(w, vec4<T>);
+                *reinterpret_cast<vec4<T> *>(dvr + at) = __builtin_convertvector(x, vec4<T>);
             }
         }
 }
 
-// Bytes of the backward's scratch: delta, and the two largest norms.
-static int64_t bwd_largest_at(int64_t q_tokens, int64_t q_heads) {
-    return align256(q_tokens * q_heads * 4);
+// dk (blockIdx.y 0) and dv (1): the splits' sums, in order.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_sum_kernel(AttnArgs a, int64_t n) {
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= n) return;
+    const float *p = (blockIdx.y ? a.part_dv : a.part_dk) + i;
+    f32x4 sum = {};
+    for (int s = 0; s < a.splits; ++s) sum += *reinterpret_cast<const f32x4 *>(p + s * n);
+    *reinterpret_cast<vec4<T> *>(static_cast<T *>(blockIdx.y ? a.dv : a.dk) + i) =
+        __builtin_convertvector(sum, vec4<T>);
+}
+
+// Bytes of the backward's scratch: delta, the largest norms, and the splits'
+// sums. The keys' gradients are split where their tiles are fewer than fill the
+// GPU twice over, into runs of eight query tiles on the average at least.
+struct BwdPlan {
+    int64_t k_items, largest_at, part_at, bytes;
+    int splits;
+};
+
+constexpr int64_t kBwdSlots = 1024;
+
+static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int64_t group,
+                        int64_t dim, int64_t n_seq) {
+    BwdPlan p{};
+    p.k_items = k_tokens / kBwdTile + n_seq + 2;
+    const int64_t likely = (ceil_div(k_tokens, kBwdTile) + n_seq - 1) * k_heads;
+    const int64_t steps = ceil_div(q_tokens, n_seq * kTileRows) * group;
+    int64_t splits = kBwdSlots / (likely > 0 ? likely : 1);
+    if (splits > steps / 8) splits = steps / 8;
+    p.splits = (int)(splits < 1 ? 1 : splits > 8 ? 8 : splits);
+    p.largest_at = align256(q_tokens * k_heads * group * 4);
+    p.part_at = p.largest_at + 2 * kNormGroups * 4;
+    p.bytes = p.part_at;
+    if (p.splits > 1) p.bytes += 2 * p.splits * k_tokens * k_heads * dim * 4;
+    return p;
 }
 
 }  // namespace mg
@@ -345,9 +414,8 @@ extern "C" {
 
 int64_t mg_attention_backward_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
                                               int32_t k_heads, int32_t dim, int32_t sequences) {
-    (void)k_tokens, (void)k_heads, (void)dim, (void)sequences;
-    if (q_tokens < 0 || q_heads < 1) return 0;
-    return mg::bwd_largest_at(q_tokens, q_heads) + 256;
+    if (q_tokens < 0 || k_tokens < 0 || k_heads < 1 || q_heads < k_heads || sequences < 1) return 0;
+    return mg::bwd_plan(q_tokens, k_tokens, k_heads, q_heads / k_heads, dim, sequences).bytes;
 }
 
 int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
@@ -385,27 +453,25 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
     MG_REQUIRE(q_tokens == 0 || (q && out && lse && dout && dq), "%s: a pointer is NULL", who);
     MG_REQUIRE(k_tokens == 0 || (k && v), "%s: a pointer is NULL", who);
     MG_REQUIRE((dk == nullptr) == (dv == nullptr), "%s: dk and dv go together", who);
-    const int64_t need = mg_attention_backward_workspace_bytes(q_tokens, k_tokens, q_heads,
-                                                               k_heads, dim, sequences);
-    MG_REQUIRE(workspace && workspace_bytes >= need, "%s: workspace of %lld bytes, %lld needed",
-               who, (long long)workspace_bytes, (long long)need);
-    a.delta = static_cast<float *>(workspace);
-    float *largest =
-        reinterpret_cast<float *>(static_cast<char *>(workspace) + bwd_largest_at(q_tokens, q_heads));
-    a.grad_scale = largest;
+    const BwdPlan p = bwd_plan(q_tokens, k_tokens, k_heads, group, dim, sequences);
+    MG_REQUIRE(workspace && workspace_bytes >= p.bytes, "%s: workspace of %lld bytes, %lld needed",
+               who, (long long)workspace_bytes, (long long)p.bytes);
+    char *ws = static_cast<char *>(workspace);
+    a.delta = reinterpret_cast<float *>(ws);
+    float *largest = reinterpret_cast<float *>(ws + p.largest_at);
+    a.largest = largest;
+    const int64_t key_values = k_tokens * k_heads * dim;
+    a.splits = p.splits;
+    a.part_dk = reinterpret_cast<float *>(ws + p.part_at);
+    a.part_dv = a.part_dk + p.splits * key_values;
     hipStream_t st = as_stream(stream);
     const int64_t q_items = (q_tokens * group / kBwdTile + sequences + 2) * k_heads;
-    const int64_t k_items = (k_tokens / kBwdTile + sequences + 2) * k_heads;
+    const int64_t k_items = p.k_items * p.splits * k_heads;
     MG_REQUIRE(q_items < (int64_t(1) << 31) && k_items < (int64_t(1) << 31),
                "%s: too many work items", who);
-    if (dtype == MG_F16 && q_tokens > 0 && k_tokens > 0) {
+    if (dtype == MG_F16) {
         TimedScope ts("attention_largest", st);
-        const int64_t rows_q = q_tokens * q_heads, rows_k = k_tokens * k_heads;
-        attn_zero_kernel<<<1, 2, 0, st>>>(largest);
-        attn_largest_kernel<f16_t><<<(unsigned)ceil_div(rows_q, 16), 256, 0, st>>>(
-            a.dout, rows_q, q_heads, dim, largest);
-        attn_largest_kernel<f16_t><<<(unsigned)ceil_div(rows_k, 16), 256, 0, st>>>(
-            a.v, rows_k, k_heads, dim, largest + 1);
+        attn_largest_kernel<f16_t><<<dim3(kNormGroups, 2), 256, 0, st>>>(a, largest);
         MG_LAUNCHED("attn_largest_kernel");
     }
     if (q_tokens > 0) {
@@ -423,6 +489,15 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
                 <<<(unsigned)k_items, 64 * kBwdWaves, 0, st>>>(a);
         });
         MG_LAUNCHED("attn_dkv_kernel");
+    }
+    if (k_tokens > 0 && dk && p.splits > 1) {
+        TimedScope ts("attention_sum", st);
+        const dim3 grid((unsigned)ceil_div(key_values, 1024), 2);
+        if (dtype == MG_BF16)
+            attn_sum_kernel<bf16_t><<<grid, 256, 0, st>>>(a, key_values);
+        else
+            attn_sum_kernel<f16_t><<<grid, 256, 0, st>>>(a, key_values);
+        MG_LAUNCHED("attn_sum_kernel");
     }
     return MG_OK;
 }
