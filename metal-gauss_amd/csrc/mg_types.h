@@ -35,38 +35,50 @@ constexpr int kVec = 16 / (int)sizeof(T);
 // V neighbouring elements from any address an element may have: gfx950 takes
 // 16-byte accesses at element alignment, so rows of odd widths and strides
 // keep the wide form.
-template <typename T, int V>
+template <typename T, int V, bool kNt = false>
 __device__ __forceinline__ void load_vec(const T *p, float (&f)[V]) {
-    T t[V];
-    __builtin_memcpy(t, p, sizeof(t));
+    typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    if constexpr (kNt) {
+        const vec t = __builtin_nontemporal_load(reinterpret_cast<const vec *>(p));
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] = (float)t[i];
+        for (int i = 0; i < V; ++i) f[i] = (float)t[i];
+    } else {
+        T t[V];
+        __builtin_memcpy(t, p, sizeof(t));
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = (float)t[i];
+    }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool kNt = false>
 __device__ __forceinline__ void store_vec(T *p, const float (&f)[V]) {
-    T t[V];
+    typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    vec t;
 #pragma unroll
     for (int i = 0; i < V; ++i) t[i] = (T)f[i];
-    __builtin_memcpy(p, t, sizeof(t));
+    if constexpr (kNt) {
+        __builtin_nontemporal_store(t, reinterpret_cast<vec *>(p));
+    } else {
+        __builtin_memcpy(p, &t, sizeof(t));
+    }
 }
 
 // The same at element `at` of a row of n: what lies past the row reads as 0
 // and is not written.
-template <typename T, int V>
+template <typename T, int V, bool kNt = false>
 __device__ __forceinline__ void load_row(const T *row, int at, int n, float (&f)[V]) {
     if (at + V <= n) {
-        load_vec<T, V>(row + at, f);
+        load_vec<T, V, kNt>(row + at, f);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) f[i] = at + i < n ? (float)row[at + i] : 0.f;
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, bool kNt = false>
 __device__ __forceinline__ void store_row(T *row, int at, int n, const float (&f)[V]) {
     if (at + V <= n) {
-        store_vec<T, V>(row + at, f);
+        store_vec<T, V, kNt>(row + at, f);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i)

@@ -11,14 +11,18 @@
 // exact to 2^-53 of itself), so a token at position 10^6 is turned as exactly
 // as one at 10; sine and cosine are then float32, formed once per token and
 // pair and shared by all heads through LDS. What is left is memory: queries and
-// keys are read once and written once, in one launch.
+// keys are read once and written once, in one launch. A thread asks for all its
+// elements before it forms its cosines, whose chain (position, float64 product,
+// polynomial) is as long as a trip to memory.
 #include "mg_types.h"
 
 namespace mg {
 
 constexpr int kRotThreads = 256;
+constexpr int kRotUnits = 4;               // units a thread
 constexpr int kRotMaxPairs = 512;          // heads of up to 1024 elements
 constexpr int kRotTable = 1024;            // cosines and sines held by a workgroup
+constexpr int64_t kRotStreamBytes = 32 << 20;     // the L2 caches' together
 
 struct RotArgs {
     const void *x[2];
@@ -29,19 +33,68 @@ struct RotArgs {
     int32_t dim, pairs, axes;
     const void *positions;
     const double *freq;
-    int32_t tokens_at_once;
+    // A workgroup has tokens_at_once tokens, or one of `runs` runs of one token's
+    // units.
+    int32_t tokens_at_once, runs;
     float sign;
 };
+
+// kStream: results larger than the L2 caches pass by them (32640 tokens of 20
+// heads of 128 float32, forward and backward: 268 us, with streaming stores 258;
+// streaming loads gained nothing there and cost a third on smaller inputs).
+template <bool kStream, typename T, int V>
+__device__ __forceinline__ void copy_out(T *to, const T (&from)[V]) {
+    typedef T vec __attribute__((ext_vector_type(V), aligned(sizeof(T))));
+    if constexpr (kStream && V > 1) {
+        vec t;
+#pragma unroll
+        for (int i = 0; i < V; ++i) t[i] = from[i];
+        __builtin_nontemporal_store(t, reinterpret_cast<vec *>(to));
+    } else {
+        __builtin_memcpy(to, from, sizeof(from));
+    }
+}
 
 // A unit is V neighbouring elements of a head's rotated part together with
 // their partners (kHalf), V / 2 whole pairs (interleaved), or V elements that
 // are copied. V = 16 bytes' worth where units do not straddle the parts'
 // borders, else 1 (2 interleaved).
-template <typename T, typename P, int V, bool kHalf>
+template <typename T, typename P, int V, bool kHalf, bool kStream>
 __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
     __shared__ float2 s_cs[kRotTable];
-    const int64_t tok0 = (int64_t)blockIdx.x * a.tokens_at_once;
+    const int run = a.runs > 1 ? blockIdx.x % a.runs : 0;
+    const int64_t tok0 = (int64_t)(blockIdx.x / a.runs) * a.tokens_at_once;
     const int n_tok = (int)min((int64_t)a.tokens_at_once, a.tokens - tok0);
+    const int rot_units = (kHalf ? a.pairs : 2 * a.pairs) / V;
+    const int units = rot_units + (a.dim - 2 * a.pairs) / V;
+    const int per_tok = (a.heads[0] + a.heads[1]) * units;
+    struct Unit {
+        const T *x;
+        T *out;
+        int pair;      // of the workgroup's table; -1: copied, -2: none
+    };
+    Unit unit[kRotUnits];
+    T v[kRotUnits][V], w[kHalf ? kRotUnits : 1][V];
+#pragma unroll
+    for (int j = 0; j < kRotUnits; ++j) {
+        const int i = (run * kRotUnits + j) * kRotThreads + (int)threadIdx.x;
+        unit[j].pair = -2;
+        if (i >= n_tok * per_tok) continue;
+        const int tok = i / per_tok, r = i - tok * per_tok;
+        int h = r / units;
+        const int u = r - h * units;
+        const int which = h >= a.heads[0];
+        h -= which ? a.heads[0] : 0;
+        const bool turned = u < rot_units;
+        const int at = turned ? u * V : 2 * a.pairs + (u - rot_units) * V;
+        unit[j].pair = turned ? tok * a.pairs + (kHalf ? at : at / 2) : -1;
+        unit[j].x = static_cast<const T *>(a.x[which]) + (tok0 + tok) * a.tok_stride[which] +
+                    h * a.head_stride[which] + at;
+        unit[j].out = static_cast<T *>(a.out[which]) + (tok0 + tok) * a.out_tok_stride[which] +
+                      (int64_t)h * a.dim + at;
+        __builtin_memcpy(v[j], unit[j].x, sizeof(v[j]));
+        if (kHalf && turned) __builtin_memcpy(w[j], unit[j].x + a.pairs, sizeof(w[j]));
+    }
     const P *pos = static_cast<const P *>(a.positions);
     const int per_axis = a.pairs / a.axes;
     for (int i = threadIdx.x; i < n_tok * a.pairs; i += kRotThreads) {
@@ -54,70 +107,63 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
         s_cs[i] = make_float2(cs, a.sign * sn);
     }
     __syncthreads();
-    const int rot_units = (kHalf ? a.pairs : 2 * a.pairs) / V;
-    const int units = rot_units + (a.dim - 2 * a.pairs) / V;
-    const int heads = a.heads[0] + a.heads[1];
-    const int per_tok = heads * units;
-    for (int i = threadIdx.x; i < n_tok * per_tok; i += kRotThreads) {
-        const int tok = i / per_tok, r = i - tok * per_tok;
-        int h = r / units;
-        const int u = r - h * units;
-        const int which = h >= a.heads[0];
-        h -= which ? a.heads[0] : 0;
-        const T *x = static_cast<const T *>(a.x[which]) + (tok0 + tok) * a.tok_stride[which] +
-                     h * a.head_stride[which];
-        T *out = static_cast<T *>(a.out[which]) + (tok0 + tok) * a.out_tok_stride[which] +
-                 (int64_t)h * a.dim;
-        const float2 *cs = s_cs + tok * a.pairs;
-        float v[V];
-        if (u >= rot_units) {
-            const int at = 2 * a.pairs + (u - rot_units) * V;
-            load_vec<T, V>(x + at, v);
-            store_vec<T, V>(out + at, v);
-        } else if constexpr (kHalf) {
-            float w[V];
-            load_vec<T, V>(x + u * V, v);
-            load_vec<T, V>(x + a.pairs + u * V, w);
 #pragma unroll
-            for (int k = 0; k < V; ++k) {
-                const float2 c = cs[u * V + k];
-                const float p = v[k], q = w[k];
-                v[k] = p * c.x - q * c.y;
-                w[k] = q * c.x + p * c.y;
-            }
-            store_vec<T, V>(out + u * V, v);
-            store_vec<T, V>(out + a.pairs + u * V, w);
-        } else {
-            load_vec<T, V>(x + u * V, v);
+    for (int j = 0; j < kRotUnits; ++j) {
+        const Unit &m = unit[j];
+        if (m.pair == -2) continue;
+        if (m.pair >= 0) {
+            if constexpr (kHalf) {
 #pragma unroll
-            for (int k = 0; k + 1 < V; k += 2) {
-                const float2 c = cs[(u * V + k) / 2];
-                const float p = v[k], q = v[k + 1];
-                v[k] = p * c.x - q * c.y;
-                v[k + 1] = q * c.x + p * c.y;
+                for (int k = 0; k < V; ++k) {
+                    const float2 c = s_cs[m.pair + k];
+                    const float p = (float)v[j][k], q = (float)w[j][k];
+                    v[j][k] = (T)(p * c.x - q * c.y);
+                    w[j][k] = (T)(q * c.x + p * c.y);
+                }
+                copy_out<kStream>(m.out + a.pairs, w[j]);
+            } else {
+#pragma unroll
+                for (int k = 0; k + 1 < V; k += 2) {
+                    const float2 c = s_cs[m.pair + k / 2];
+                    const float p = (float)v[j][k], q = (float)v[j][k + 1];
+                    v[j][k] = (T)(p * c.x - q * c.y);
+                    v[j][k + 1] = (T)(q * c.x + p * c.y);
+                }
             }
-            store_vec<T, V>(out + u * V, v);
         }
+        copy_out<kStream>(m.out, v[j]);
     }
 }
 
+// Cuts the tokens among workgroups for units of V elements, and launches.
+template <typename T, typename P, int V, bool kHalf>
+static bool rotary_go(RotArgs a, hipStream_t st) {
+    const int units = ((kHalf ? a.pairs : 2 * a.pairs) + a.dim - 2 * a.pairs) / V;
+    const int64_t per_tok = (int64_t)(a.heads[0] + a.heads[1]) * units;
+    constexpr int64_t kAll = kRotUnits * kRotThreads;
+    int64_t at_once = kAll / per_tok;
+    if (at_once > kRotTable / a.pairs) at_once = kRotTable / a.pairs;
+    // A few tokens are spread over the GPU.
+    if (at_once > ceil_div(a.tokens, 512)) at_once = ceil_div(a.tokens, 512);
+    a.tokens_at_once = (int32_t)(at_once < 1 ? 1 : at_once);
+    a.runs = (int32_t)ceil_div(a.tokens_at_once * per_tok, kAll);
+    const int64_t grid = ceil_div(a.tokens, a.tokens_at_once) * a.runs;
+    if (grid >= (int64_t(1) << 31)) return false;
+    const int64_t bytes = a.tokens * (a.heads[0] + a.heads[1]) * a.dim * (int64_t)sizeof(T);
+    if (bytes > kRotStreamBytes)
+        rotary_kernel<T, P, V, kHalf, true><<<(unsigned)grid, kRotThreads, 0, st>>>(a);
+    else
+        rotary_kernel<T, P, V, kHalf, false><<<(unsigned)grid, kRotThreads, 0, st>>>(a);
+    return true;
+}
+
 template <typename T, typename P>
-static void rotary_launch(const RotArgs &a, bool half, hipStream_t st) {
+static bool rotary_launch(const RotArgs &a, bool half, hipStream_t st) {
     constexpr int V = kVec<T>;
-    const unsigned grid = (unsigned)ceil_div(a.tokens, a.tokens_at_once);
     const int rest = a.dim - 2 * a.pairs;
     const bool wide = (half ? a.pairs : 2 * a.pairs) % V == 0 && rest % V == 0;
-    if (half) {
-        if (wide)
-            rotary_kernel<T, P, V, true><<<grid, kRotThreads, 0, st>>>(a);
-        else
-            rotary_kernel<T, P, 1, true><<<grid, kRotThreads, 0, st>>>(a);
-    } else {
-        if (wide)
-            rotary_kernel<T, P, V, false><<<grid, kRotThreads, 0, st>>>(a);
-        else
-            rotary_kernel<T, P, 2, false><<<grid, kRotThreads, 0, st>>>(a);
-    }
+    if (half) return wide ? rotary_go<T, P, V, true>(a, st) : rotary_go<T, P, 1, true>(a, st);
+    return wide ? rotary_go<T, P, V, false>(a, st) : rotary_go<T, P, 2, false>(a, st);
 }
 
 }  // namespace mg
@@ -154,28 +200,19 @@ extern "C" int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q, int64
     a.tokens = tokens, a.dim = dim, a.pairs = pairs, a.axes = axes;
     a.positions = positions, a.freq = frequencies;
     a.sign = inverse ? -1.f : 1.f;
-    // Tokens of a workgroup: about 32 KB of heads, as many as the table holds.
-    const int64_t bytes = (int64_t)(q_heads + k_heads) * dim * type_bytes(dtype);
-    int64_t at_once = 32768 / bytes;
-    if (at_once > kRotTable / pairs) at_once = kRotTable / pairs;
-    if (at_once * 1024 > tokens) at_once = tokens / 1024;
-    a.tokens_at_once = (int32_t)(at_once < 1 ? 1 : at_once);
     hipStream_t st = as_stream(stream);
     TimedScope ts("rotary", st);
     const bool half = interleaved == 0;
-    auto go = [&](auto t) {
+    const auto go = [&](auto t) {
         using T = decltype(t);
-        if (positions_64)
-            rotary_launch<T, int64_t>(a, half, st);
-        else
-            rotary_launch<T, int32_t>(a, half, st);
+        return positions_64 ? rotary_launch<T, int64_t>(a, half, st)
+                            : rotary_launch<T, int32_t>(a, half, st);
     };
-    if (dtype == MG_F32)
-        go(float{});
-    else if (dtype == MG_BF16)
-        go(bf16_t{});
-    else
-        go(f16_t{});
+    const bool fits = dtype == MG_F32    ? go(float{})
+                      : dtype == MG_BF16 ? go(bf16_t{})
+                                         : go(f16_t{});
+    MG_REQUIRE(fits, "mg_rotary: %lld tokens of %d elements are too many for one call",
+               (long long)tokens, (q_heads + k_heads) * dim);
     MG_LAUNCHED("rotary_kernel");
     return MG_OK;
 }
