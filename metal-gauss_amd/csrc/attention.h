@@ -55,9 +55,10 @@ struct AttnArgs {
     const float *delta;                  // (q_heads, q_tokens)
     const float *largest;                // float16: see attention_bwd.hip
     void *dq, *dk, *dv;
-    // Keys' gradients over `splits` runs of queries, each in float32.
-    int32_t splits;
-    float *part_dk, *part_dv;            // (splits, k_tokens, k_heads, dim)
+    // Keys' gradients over up to `splits` runs of query tiles, of split_steps at
+    // least, each in float32 (part_of).
+    int32_t splits, split_steps;
+    float *part;
 };
 
 // ---------------------------------------------------------------- sequences
@@ -71,6 +72,9 @@ struct SeqItem {
     int before;        // sum of the second count over the sequences before
     bool found;
 };
+
+// A value that is the same in all lanes, where the compiler cannot tell.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 __device__ __forceinline__ int clamp_to(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
@@ -137,10 +141,82 @@ __device__ __forceinline__ SeqItem find_item(const AttnArgs &a, int item, Count 
     return r;
 }
 
-// ------------------------------------------------------------- filling tiles
-// A value that is the same in all lanes, where the compiler cannot tell.
-__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// ------------------------------------------------------------- longest first
+// Tiles of R rows (tokens by `per`) of a sequence that have at least w >= 1 pairs a
+// row to go through. By queries: the tile's last query's seen keys, rising with
+// the tile. By keys: the queries that see the tile's first key, falling with it.
+template <bool kByKeys>
+__device__ __forceinline__ int tiles_with(const AttnArgs &a, int R, int q_len, int k_len, int w) {
+    const int ahead = k_len - q_len;
+    if constexpr (kByKeys) {
+        const int tiles = (k_len + R - 1) / R;
+        if (q_len < w) return 0;
+        if (!a.causal) return tiles;
+        const int last = q_len - w + ahead;       // the last first key that w see
+        return last < 0 ? 0 : min(tiles, last / R + 1);
+    } else {
+        const int tiles = (q_len * a.group + R - 1) / R;
+        if (k_len < w) return 0;
+        if (!a.causal) return tiles;
+        const int query = w - 1 - ahead;          // the first query that sees w
+        if (query >= q_len) return 0;
+        return tiles - max(0, query) * a.group / R;
+    }
+}
 
+// Work item `item` of all sequences' tiles of R rows, in falling order of the
+// pairs a row has, in steps of 64: workgroups start in order, so that the
+// longest are not left for the end (packed sequences of 1 to 2500 tokens, causal:
+// see attention_bwd.hip). s.within is the tile. Up to 62 sequences; with more
+// the items come sequence by sequence.
+template <bool kByKeys>
+__device__ __forceinline__ SeqItem find_longest(const AttnArgs &a, int item, int R) {
+    const auto tiles_of = [&](int ql, int kl) {
+        return kByKeys ? (kl + R - 1) / R : (ql * a.group + R - 1) / R;
+    };
+    if (a.n_seq == 1 || a.n_seq + 2 > 64) {
+        SeqItem s = find_item<kByKeys>(a, item, tiles_of, [](int, int) { return 0; });
+        if (!kByKeys) s.within = tiles_of(s.q_len, 0) - 1 - s.within;
+        return s;
+    }
+    const int seq = lane_id();
+    int q_lo = 0, q_len = 0, k_lo = 0, k_len = 0, tiles = 0;
+    if (seq < a.n_seq + 2) {
+        seq_bounds(a.q_off, a.n_seq, a.q_tokens, seq, q_lo, q_len);
+        seq_bounds(a.k_off, a.n_seq, a.k_tokens, seq, k_lo, k_len);
+        if (seq == 0 || seq > a.n_seq) (kByKeys ? q_len : k_len) = 0;
+        tiles = tiles_of(q_len, k_len);
+    }
+    const auto with = [&](int w) {                // this lane's sequence's
+        return w == 0 ? tiles : tiles_with<kByKeys>(a, R, q_len, k_len, w * 64);
+    };
+    const auto all = [&](int w) {
+        return __builtin_amdgcn_readlane(wave_inclusive_sum(with(w)), 63);
+    };
+    SeqItem r{};
+    if (all(0) <= item) return r;
+    int lo = 0, hi = uniform(wave_max_i(kByKeys ? q_len : k_len)) / 64 + 1;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (all(mid) > item)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    // The item is among the tiles that lo has and lo + 1 has not.
+    const int longer = with(lo + 1), here = with(lo) - longer;
+    const int rank = item - all(lo + 1), upto = wave_inclusive_sum(here);
+    const uint64_t past = ballot(upto > rank);
+    const int l = past ? __builtin_ctzll(past) : 0;
+    const auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+    r.q_lo = get(q_lo), r.q_len = get(q_len), r.k_lo = get(k_lo), r.k_len = get(k_len);
+    const int nth = get(longer) + rank - (get(upto) - get(here));
+    r.within = clamp_to(kByKeys ? nth : get(tiles) - 1 - nth, 0, get(tiles) - 1);
+    r.found = past != 0;
+    return r;
+}
+
+// ------------------------------------------------------------- filling tiles
 // Descriptor of `bytes` bytes from a wave-uniform address; accesses past them
 // do not reach memory.
 __device__ __forceinline__ i32x4 buffer_of(const void *base, uint32_t bytes) {

@@ -52,12 +52,21 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     const auto chunks_of = [&](int, int kl) {
         return kSplit ? max(1, (kl + a.split_keys - 1) / a.split_keys) : 1;
     };
-    const SeqItem s = find_item<false>(
-        a, item, [&](int ql, int kl) { return tiles_of(ql, kl) * chunks_of(ql, kl); },
-        [](int, int) { return 0; });
-    if (!s.found || (kSplit && item >= a.items)) return false;
-    const int chunks = chunks_of(s.q_len, s.k_len);
-    const int tile = tiles_of(s.q_len, 0) - 1 - s.within / chunks, chunk = s.within % chunks;
+    SeqItem s;
+    int tile, chunk = 0;
+    if constexpr (kSplit) {
+        s = find_item<false>(
+            a, item, [&](int ql, int kl) { return tiles_of(ql, kl) * chunks_of(ql, kl); },
+            [](int, int) { return 0; });
+        if (!s.found || item >= a.items) return false;
+        const int chunks = chunks_of(s.q_len, s.k_len);
+        tile = tiles_of(s.q_len, 0) - 1 - s.within / chunks;
+        chunk = s.within % chunks;
+    } else {
+        s = find_longest<false>(a, item, kRows);
+        if (!s.found) return false;
+        tile = s.within;
+    }
 
     // This lane's row.
     const int row0 = tile * kRows + wave * 32;

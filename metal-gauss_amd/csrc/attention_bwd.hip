@@ -28,7 +28,7 @@ constexpr float kPowerP = sizeof(T) == 2 && std::is_same<T, f16_t>::value ? 15.f
 
 // The largest |row|^2 of do (blockIdx.y 0) and of v (1) that each workgroup finds,
 // to largest[kNormGroups y + x]. A NaN counts as nothing.
-constexpr int kNormGroups = 256;
+constexpr int kNormGroups = 512;
 
 template <typename T>
 __global__ __launch_bounds__(256) void attn_largest_kernel(AttnArgs a, float *largest) {
@@ -36,23 +36,29 @@ __global__ __launch_bounds__(256) void attn_largest_kernel(AttnArgs a, float *la
     const AttnTensor &x = blockIdx.y ? a.v : a.dout;
     const int heads = blockIdx.y ? a.k_heads : a.k_heads * a.group;
     const int64_t rows = (int64_t)(blockIdx.y ? a.k_tokens : a.q_tokens) * heads;
-    // 16 lanes a row, eight elements each.
+    // 16 lanes a row, eight elements each, four rows asked for at once.
     const int at = threadIdx.x % 16 * 8;
+    constexpr int64_t kStep = kNormGroups * 16;
     float most = 0.f;
-    for (int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16; row < rows;
-         row += kNormGroups * 16) {
-        float sq = 0.f;
-        if (at < a.dim) {
-            const int token = (int)(row / heads), head = (int)(row % heads);
-            const T *p = static_cast<const T *>(x.p) + token * x.tok_stride + head * x.head_stride;
-            float f[8];
-            load_vec<T, 8>(p + at, f);
+    for (int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16; row < rows; row += 4 * kStep) {
+        float f[4][8] = {};
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sq = fmaf(f[i], f[i], sq);
+        for (int k = 0; k < 4; ++k) {
+            const int64_t r = row + k * kStep;
+            const int token = (int)(r / heads), head = (int)(r % heads);
+            if (r < rows && at < a.dim)
+                load_vec<T, 8>(static_cast<const T *>(x.p) + token * x.tok_stride +
+                                   head * x.head_stride + at, f[k]);
         }
 #pragma unroll
-        for (int o = 8; o >= 1; o >>= 1) sq += __shfl_xor(sq, o, 16);
-        most = fmaxf(most, sq);
+        for (int k = 0; k < 4; ++k) {
+            float sq = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sq = fmaf(f[k][i], f[k][i], sq);
+#pragma unroll
+            for (int o = 8; o >= 1; o >>= 1) sq += __shfl_xor(sq, o, 16);
+            most = fmaxf(most, sq);
+        }
     }
     most = wave_max(most);
     if (lane_id() == 0) s_most[threadIdx.x / 64] = most;
@@ -90,10 +96,9 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
     const int lane = lane_id(), half = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads, G = a.group;
-    const auto tiles_of = [&](int ql, int) { return (ql * G + kBwdTile - 1) / kBwdTile; };
-    const SeqItem s = find_item<false>(a, item, tiles_of, [](int, int) { return 0; });
+    const SeqItem s = find_longest<false>(a, item, kBwdTile);
     if (!s.found) return;
-    const int tile = tiles_of(s.q_len, 0) - 1 - s.within;
+    const int tile = s.within;
     const auto sees = [&](int token) {
         return a.causal ? clamp_to(token + 1 + s.k_len - s.q_len, 0, s.k_len) : s.k_len;
     };
@@ -215,6 +220,35 @@ __device__ __forceinline__ void ask_row_values(const float *at, int rows, uint32
                  : "memory");
 }
 
+// A run's sums for one key tile, in the order the waves hold them (a store is
+// 1024 bytes in a row): dk, then dv, a wave's blocks one after the other.
+template <int DK>
+constexpr int kPartFours = 2 * kBwdTile * DK / 4;
+
+template <int DK>
+__device__ __forceinline__ f32x4 *part_of(const AttnArgs &a, int item, int kh, int split) {
+    return reinterpret_cast<f32x4 *>(a.part) +
+           (((int64_t)item * a.k_heads + kh) * a.splits + split) * kPartFours<DK>;
+}
+
+// The query tiles that see a key tile (tiles of each of the group's heads, from
+// q_from), and the runs they are cut into: whole heads, or `parts` of each head
+// where there are more runs than heads. Key tiles that run at the same time then
+// read the same heads' queries, which stay in their XCD's L2.
+struct KeySteps {
+    int q_from, tiles, runs, parts;
+};
+
+__device__ __forceinline__ KeySteps key_steps(const AttnArgs &a, const SeqItem &s, int first_key) {
+    const int ahead = s.k_len - s.q_len, G = a.group;
+    const int from = a.causal ? max(0, first_key - ahead) / kTileRows * kTileRows : 0;
+    const int tiles = from < s.q_len ? (s.q_len - from + kTileRows - 1) / kTileRows : 0;
+    int runs = (int)(((int64_t)tiles * G + a.split_steps - 1) / a.split_steps);
+    runs = clamp_to(runs, 1, a.splits);
+    const int parts = runs > G ? runs / G : 1;
+    return {from, tiles, parts > 1 ? parts * G : min(runs, G), parts};
+}
+
 template <typename T, int DK>
 __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a) {
     constexpr int kSteps = DK / 16, kBlocks = DK / 32;
@@ -224,16 +258,21 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads / a.splits;
     const int split = blockIdx.x / a.k_heads % a.splits;
-    const SeqItem s = find_item<true>(
-        a, item, [](int, int kl) { return (kl + kBwdTile - 1) / kBwdTile; },
-        [](int, int) { return 0; });
+    const SeqItem s = find_longest<true>(a, item, kBwdTile);
     if (!s.found) return;
-    // Causal: the first keys are seen by the most queries; they come first.
     const int first_key = s.within * kBwdTile;
+    const KeySteps steps_of = key_steps(a, s, first_key);
+    if (split >= steps_of.runs) return;
     const int key0 = first_key + wave * 32, key = key0 + lane % 32;
     const bool key_ok = key < s.k_len;
     const int ahead = s.k_len - s.q_len;       // query i sees keys up to i + ahead
-    const int q_from = a.causal ? max(0, first_key - ahead) / kTileRows * kTileRows : 0;
+    // This run's heads, and its query tiles of each.
+    const int parts = steps_of.parts, runs = steps_of.runs / parts, run = split / parts;
+    const int g_from = run * a.group / runs, heads = (run + 1) * a.group / runs - g_from;
+    const int t_from = steps_of.tiles * (split % parts) / parts;
+    const int tiles = steps_of.tiles * (split % parts + 1) / parts - t_from;
+    const int q_from = steps_of.q_from + t_from * kTileRows;
+    const int q_to = q_from + tiles * kTileRows;
 
     vec8<T> k[kSteps], v[kSteps];
     {
@@ -274,24 +313,16 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     const float ds_up = __builtin_amdgcn_exp2f(power - kPowerP<T>);
 
     f32x16 dk[kBlocks] = {}, dv[kBlocks] = {};
-    const int tiles = q_from < s.q_len ? (s.q_len - q_from + kTileRows - 1) / kTileRows : 0;
-    // A split has a run of the steps: query tiles of one head after the other.
-    const int all = tiles * a.group;
-    const int from = (int)((int64_t)all * split / a.splits);
-    const int steps = (int)((int64_t)all * (split + 1) / a.splits) - from;
+    const int steps = tiles * heads;
     TileLane<T, DK> lane_at;
-    int g = 0, row0 = q_from, buf = 0;
-    if (steps > 0) {
-        g = from / tiles;
-        row0 += from % tiles * kTileRows;
-        ask(g, row0, 0);
-    }
+    int g = g_from, row0 = q_from, buf = 0;
+    if (steps > 0) ask(g, row0, 0);
     for (int step = 0; step < steps; ++step, buf ^= 1) {
         tiles_ready();
         lane_at.fresh();
         const int at_row0 = row0;
         row0 += kTileRows;
-        if (row0 >= s.q_len) {
+        if (row0 >= q_to) {
             row0 = q_from;
             ++g;
         }
@@ -342,69 +373,100 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
         }
     }
     lds_reads_done();
-    if (!key_ok) return;
     const float down = a.scale * __builtin_amdgcn_exp2f(-power);
     const float down_v = __builtin_amdgcn_exp2f(-kPowerP<T>);
+    if (steps_of.runs > 1) {
+        f32x4 *part = part_of<DK>(a, item, kh, split) + wave * kBlocks * 4 * 64 + lane;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                f32x4 w, x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = dk[b][e + i] * down;
+                    x[i] = dv[b][e + i] * down_v;
+                }
+                part[(b * 4 + e / 4) * 64] = w;
+                part[(b * 4 + e / 4) * 64 + kPartFours<DK> / 2] = x;
+            }
+        return;
+    }
+    if (!key_ok) return;
     const int64_t at_row = ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim;
-    const int64_t part = (int64_t)split * a.k_tokens * a.k_heads * a.dim + at_row;
     T *dkr = static_cast<T *>(a.dk) + at_row, *dvr = static_cast<T *>(a.dv) + at_row;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const int at = 32 * b + c_row(e, half);
-            f32x4 w, x;
+            vec4<T> w, x;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                w[i] = dk[b][e + i] * down;
-                x[i] = dv[b][e + i] * down_v;
+                w[i] = (T)(dk[b][e + i] * down);
+                x[i] = (T)(dv[b][e + i] * down_v);
             }
-            if (at >= a.dim) continue;
-            if (a.splits > 1) {
-                *reinterpret_cast<f32x4 *>(a.part_dk + part + at) = w;
-                *reinterpret_cast<f32x4 *>(a.part_dv + part + at) = x;
-            } else {
-                *reinterpret_cast<vec4<T> *>(dkr + at) = __builtin_convertvector(w, vec4<T>);
-                *reinterpret_cast<vec4<T> *>(dvr + at) = __builtin_convertvector(x, vec4<T>);
+            if (at < a.dim) {
+                *reinterpret_cast<vec4<T> *>(dkr + at) = w;
+                *reinterpret_cast<vec4<T> *>(dvr + at) = x;
             }
         }
 }
 
-// dk (blockIdx.y 0) and dv (1): the splits' sums, in order.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_sum_kernel(AttnArgs a, int64_t n) {
-    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= n) return;
-    const float *p = (blockIdx.y ? a.part_dv : a.part_dk) + i;
-    f32x4 sum = {};
-    for (int s = 0; s < a.splits; ++s) sum += *reinterpret_cast<const f32x4 *>(p + s * n);
-    *reinterpret_cast<vec4<T> *>(static_cast<T *>(blockIdx.y ? a.dv : a.dk) + i) =
-        __builtin_convertvector(sum, vec4<T>);
+// The sums of the keys' tiles that were cut into runs, in order. A workgroup has
+// 32 columns of dk or dv of one tile of one key head, its threads the elements
+// that attn_dkv_kernel's have.
+template <typename T, int DK>
+__global__ __launch_bounds__(64 * kBwdWaves) void attn_sum_kernel(AttnArgs a) {
+    constexpr int kBlocks = DK / 32;
+    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
+    const SeqItem s = find_longest<true>(a, item, kBwdTile);
+    if (!s.found) return;
+    const int first_key = s.within * kBwdTile;
+    const int runs = key_steps(a, s, first_key).runs;
+    if (runs == 1) return;
+    const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / 64);
+    const int key = first_key + wave * 32 + lane % 32;
+    const int64_t at_row = ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim;
+    const f32x4 *part = part_of<DK>(a, item, kh, 0) + wave * kBlocks * 4 * 64 + lane;
+    const int which = blockIdx.y % 2, block = blockIdx.y / 2;
+#pragma unroll
+    for (int i = 4 * block; i < 4 * block + 4; ++i) {
+        const f32x4 *p = part + i * 64 + which * kPartFours<DK> / 2;
+        f32x4 sum = *p;
+        for (int k = 1; k < runs; ++k) sum += p[k * kPartFours<DK>];
+        const int at = 32 * block + c_row(i % 4 * 4, half);
+        if (key < s.k_len && at < a.dim)
+            *reinterpret_cast<vec4<T> *>(static_cast<T *>(which ? a.dv : a.dk) + at_row + at) =
+                __builtin_convertvector(sum, vec4<T>);
+    }
 }
 
-// Bytes of the backward's scratch: delta, the largest norms, and the splits'
-// sums. The keys' gradients are split where their tiles are fewer than fill the
-// GPU twice over, into runs of eight query tiles on the average at least.
+// Bytes of the backward's scratch: delta, the largest norms, and the runs' sums.
+// The keys' gradients are cut into runs where their tiles are fewer than fill
+// the GPU twice over, of eight query tiles at least.
 struct BwdPlan {
     int64_t k_items, largest_at, part_at, bytes;
-    int splits;
+    int splits, split_steps;
 };
 
-constexpr int64_t kBwdSlots = 1024;
+constexpr int64_t kBwdRuns = 1024, kBwdRunLeast = 8, kBwdMostSplits = 8;
 
 static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int64_t group,
                         int64_t dim, int64_t n_seq) {
     BwdPlan p{};
     p.k_items = k_tokens / kBwdTile + n_seq + 2;
-    const int64_t likely = (ceil_div(k_tokens, kBwdTile) + n_seq - 1) * k_heads;
+    const int64_t tiles = (ceil_div(k_tokens, kBwdTile) + n_seq - 1) * k_heads;
     const int64_t steps = ceil_div(q_tokens, n_seq * kTileRows) * group;
-    int64_t splits = kBwdSlots / (likely > 0 ? likely : 1);
-    if (splits > steps / 8) splits = steps / 8;
-    p.splits = (int)(splits < 1 ? 1 : splits > 8 ? 8 : splits);
+    int64_t splits = kBwdRuns / (tiles > 0 ? tiles : 1);
+    if (splits > steps / kBwdRunLeast) splits = steps / kBwdRunLeast;
+    p.splits = (int)(splits < 1 ? 1 : splits > kBwdMostSplits ? kBwdMostSplits : splits);
+    p.split_steps = (int)kBwdRunLeast;
     p.largest_at = align256(q_tokens * k_heads * group * 4);
     p.part_at = p.largest_at + 2 * kNormGroups * 4;
     p.bytes = p.part_at;
-    if (p.splits > 1) p.bytes += 2 * p.splits * k_tokens * k_heads * dim * 4;
+    const int64_t dk = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
+    if (p.splits > 1) p.bytes += p.k_items * k_heads * p.splits * 2 * kBwdTile * dk * 4;
     return p;
 }
 
@@ -460,10 +522,8 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
     a.delta = reinterpret_cast<float *>(ws);
     float *largest = reinterpret_cast<float *>(ws + p.largest_at);
     a.largest = largest;
-    const int64_t key_values = k_tokens * k_heads * dim;
-    a.splits = p.splits;
-    a.part_dk = reinterpret_cast<float *>(ws + p.part_at);
-    a.part_dv = a.part_dk + p.splits * key_values;
+    a.splits = p.splits, a.split_steps = p.split_steps;
+    a.part = reinterpret_cast<float *>(ws + p.part_at);
     hipStream_t st = as_stream(stream);
     const int64_t q_items = (q_tokens * group / kBwdTile + sequences + 2) * k_heads;
     const int64_t k_items = p.k_items * p.splits * k_heads;
@@ -492,11 +552,11 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
     }
     if (k_tokens > 0 && dk && p.splits > 1) {
         TimedScope ts("attention_sum", st);
-        const dim3 grid((unsigned)ceil_div(key_values, 1024), 2);
-        if (dtype == MG_BF16)
-            attn_sum_kernel<bf16_t><<<grid, 256, 0, st>>>(a, key_values);
-        else
-            attn_sum_kernel<f16_t><<<grid, 256, 0, st>>>(a, key_values);
+        attn_form(dtype, dim, [&](auto t, auto d) {
+            constexpr int DK = decltype(d)::value;
+            const dim3 grid((unsigned)(p.k_items * k_heads), 2 * DK / 32);
+            attn_sum_kernel<decltype(t), DK><<<grid, 64 * kBwdWaves, 0, st>>>(a);
+        });
         MG_LAUNCHED("attn_sum_kernel");
     }
     return MG_OK;
