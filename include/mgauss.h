@@ -702,7 +702,9 @@ int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q,
  *
  * lse (q_heads, q_tokens, float32; NULL: not kept) is the base 2 logarithm of a
  * row's sum of exponentials, +inf for a row that sees nothing: the backward
- * pass needs it. The workspace holds partial sums where few rows attend to
+ * pass needs it. out_rest (as out; NULL: not kept) is what rounding to the type
+ * took from out, rounded in turn: with it the backward pass's row sums do . o are
+ * those of the unrounded out. The workspace holds partial sums where few rows attend to
  * many keys; its size depends on the arguments of the query alone. */
 int64_t mg_attention_forward_workspace_bytes(int64_t q_tokens, int64_t k_tokens,
                                              int32_t q_heads, int32_t k_heads,
@@ -713,8 +715,8 @@ int32_t mg_attention_forward(
     int64_t q_head_stride, const void *k, int64_t k_token_stride,
     int64_t k_head_stride, const void *v, int64_t v_token_stride,
     int64_t v_head_stride, const int32_t *q_offsets, const int32_t *k_offsets,
-    int32_t sequences, int32_t causal, float scale, void *out, float *lse,
-    void *workspace, int64_t workspace_bytes, mg_stream_t stream);
+    int32_t sequences, int32_t causal, float scale, void *out, void *out_rest,
+    float *lse, void *workspace, int64_t workspace_bytes, mg_stream_t stream);
 /* Gradients of the above from its out and lse and the gradient dout of out
  * (strided as q): dq, dk, dv (contiguous; dk and dv may both be NULL). Heads
  * that share keys have their gradients summed in float32. Equal calls give
@@ -729,7 +731,7 @@ int32_t mg_attention_backward(
     int64_t k_head_stride, const void *v, int64_t v_token_stride,
     int64_t v_head_stride, const int32_t *q_offsets, const int32_t *k_offsets,
     int32_t sequences, int32_t causal, float scale, const void *out,
-    const float *lse, const void *dout, int64_t dout_token_stride,
+    const void *out_rest, const float *lse, const void *dout, int64_t dout_token_stride,
     int64_t dout_head_stride, void *dq, void *dk, void *dv, void *workspace,
     int64_t workspace_bytes, mg_stream_t stream);
 

@@ -131,11 +131,12 @@ _SIGNATURES = {
     "mg_attention_forward_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
     "mg_attention_forward": (_i32, [_i32, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _vp,
                                     _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _f32,
-                                    _vp, _vp, _vp, _i64, _vp]),
+                                    _vp, _vp, _vp, _vp, _i64, _vp]),
     "mg_attention_backward_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
     "mg_attention_backward": (_i32, [_i32, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _vp,
                                      _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _f32,
-                                     _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64, _vp]),
+                                     _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64,
+                                     _vp]),
 }
 
 EXPORTS = tuple(_SIGNATURES)

@@ -35,7 +35,9 @@ def _forward(q, k, v, q_offsets, k_offsets, causal, scale, keep):
     Tq, Hq, D = q.shape
     Tk, Hk = k.shape[0], k.shape[1]
     n = 1 if q_offsets is None else q_offsets.numel() - 1
+    # With a backward pass ahead, what rounding takes from the result is kept too.
     out = torch.empty(Tq, Hq, D, dtype=q.dtype, device=q.device)
+    rest = torch.empty_like(out) if keep else None
     lse = torch.empty(Hq, Tq, device=q.device) if keep else None
     need = lib.mg_attention_forward_workspace_bytes(Tq, Tk, Hq, Hk, D, n)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
@@ -43,23 +45,24 @@ def _forward(q, k, v, q_offsets, k_offsets, causal, scale, keep):
                 *_where(q), *_where(k), *_where(v),
                 None if q_offsets is None else q_offsets.data_ptr(),
                 None if k_offsets is None else k_offsets.data_ptr(), n, causal, scale,
-                out.data_ptr(), lse.data_ptr() if keep else None,
+                out.data_ptr(), rest.data_ptr() if keep else None,
+                lse.data_ptr() if keep else None,
                 ws.data_ptr() if need else None, need)
-    return out, lse, q, k, v
+    return out, rest, lse, q, k, v
 
 
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, q_offsets, k_offsets, causal, scale):
-        out, lse, q, k, v = _forward(q, k, v, q_offsets, k_offsets, causal, scale, True)
-        ctx.save_for_backward(q, k, v, q_offsets, k_offsets, out, lse)
+        out, rest, lse, q, k, v = _forward(q, k, v, q_offsets, k_offsets, causal, scale, True)
+        ctx.save_for_backward(q, k, v, q_offsets, k_offsets, out, rest, lse)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, q_offsets, k_offsets, out, lse = ctx.saved_tensors
+        q, k, v, q_offsets, k_offsets, out, rest, lse = ctx.saved_tensors
         lib = _lib.load()
         Tq, Hq, D = q.shape
         Tk, Hk = k.shape[0], k.shape[1]
@@ -75,7 +78,7 @@ class _Attention(torch.autograd.Function):
                     *_where(q), *_where(k), *_where(v),
                     None if q_offsets is None else q_offsets.data_ptr(),
                     None if k_offsets is None else k_offsets.data_ptr(), n, ctx.causal,
-                    ctx.scale, out.data_ptr(), lse.data_ptr(), *_where(dout), dq.data_ptr(),
+                    ctx.scale, out.data_ptr(), rest.data_ptr(), lse.data_ptr(), *_where(dout), dq.data_ptr(),
                     dk.data_ptr() if keys else None, dv.data_ptr() if keys else None,
                     ws.data_ptr(), need)
         return dq, dk, dv, None, None, None, None

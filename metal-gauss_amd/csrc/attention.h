@@ -44,6 +44,7 @@ struct AttnArgs {
     int32_t causal;
     float scale, scale_log2;             // scale, scale * log2(e)
     void *out;                           // (q_tokens, q_heads, dim)
+    void *out_rest;                      // what rounding took from out, or NULL
     float *lse;                          // (q_heads, q_tokens), in powers of 2; NULL: not kept
     // Split over the keys: chunks of split_keys, whose {top, sum} and unscaled
     // sums of values are joined afterwards; there is room for `items` of each

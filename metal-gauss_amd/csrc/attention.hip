@@ -184,17 +184,23 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     }
     if (!row_ok) return true;
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T *out = static_cast<T *>(a.out) +
-             ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim;
+    const int64_t at_row = ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim;
+    T *out = static_cast<T *>(a.out) + at_row, *rest = static_cast<T *>(a.out_rest) + at_row;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int e = 0; e < 16; e += 4) {
             const int at = 32 * b + c_row(e, half);
-            vec4<T> w;
+            vec4<T> w, x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = (T)(o[b][e + i] * inv);
-            if (at < a.dim) *reinterpret_cast<vec4<T> *>(out + at) = w;
+            for (int i = 0; i < 4; ++i) {
+                const float f = o[b][e + i] * inv;
+                w[i] = (T)f;
+                x[i] = (T)(f - (float)w[i]);
+            }
+            if (at >= a.dim) continue;
+            *reinterpret_cast<vec4<T> *>(out + at) = w;
+            if (a.out_rest) *reinterpret_cast<vec4<T> *>(rest + at) = x;
         }
     if (a.lse && half == 0)
         a.lse[(int64_t)head * a.q_tokens + s.q_lo + token] =
@@ -294,10 +300,16 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int64_t at = ((int64_t)(s.q_lo + s.within) * heads + head) * a.dim + lane * kCols;
-    T w[kCols];
+    T w[kCols], x[kCols];
 #pragma unroll
-    for (int k = 0; k < kCols; ++k) w[k] = (T)(o[k] * inv);
-    if (lane * kCols < a.dim) __builtin_memcpy(static_cast<T *>(a.out) + at, w, sizeof(w));
+    for (int k = 0; k < kCols; ++k) {
+        w[k] = (T)(o[k] * inv);
+        x[k] = (T)(o[k] * inv - (float)w[k]);
+    }
+    if (lane * kCols < a.dim) {
+        __builtin_memcpy(static_cast<T *>(a.out) + at, w, sizeof(w));
+        if (a.out_rest) __builtin_memcpy(static_cast<T *>(a.out_rest) + at, x, sizeof(x));
+    }
     if (a.lse && lane == 0)
         a.lse[(int64_t)head * a.q_tokens + s.q_lo + s.within] =
             sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
@@ -382,8 +394,8 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
                              int64_t k_head_stride, const void *v, int64_t v_token_stride,
                              int64_t v_head_stride, const int32_t *q_offsets,
                              const int32_t *k_offsets, int32_t sequences, int32_t causal,
-                             float scale, void *out, float *lse, void *workspace,
-                             int64_t workspace_bytes, mg_stream_t stream) {
+                             float scale, void *out, void *out_rest, float *lse,
+                             void *workspace, int64_t workspace_bytes, mg_stream_t stream) {
     using namespace mg;
     const char *who = "mg_attention_forward";
     MG_REQUIRE(k_heads >= 1 && q_heads >= 1 && q_heads % k_heads == 0,
@@ -401,7 +413,7 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
     a.q_tokens = (int32_t)q_tokens, a.k_tokens = (int32_t)k_tokens;
     a.k_heads = k_heads, a.group = group, a.dim = dim, a.causal = causal != 0;
     a.scale = scale, a.scale_log2 = scale_to_log2(scale);
-    a.out = out, a.lse = lse;
+    a.out = out, a.out_rest = out_rest, a.lse = lse;
     int32_t rc = attn_check(who, a, dtype);
     if (rc != MG_OK) return rc;
     if (q_tokens == 0) return MG_OK;

@@ -5,6 +5,9 @@
 //   ds_ij = p_ij (do_i v_j - delta_i),  delta_i = do_i o_i
 //   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i
 //
+// delta takes o with what rounding took from it (out_rest), where the forward
+// kept that: delta's error enters every ds of a row with the same sign.
+//
 // Two kernels form the scores once each: the queries' gradient goes over the
 // keys and keeps its sums in registers, the keys' and values' goes over the
 // queries of all heads that share them. Seven products in place of the five of
@@ -119,8 +122,9 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
         const T *dor = static_cast<const T *>(a.dout.p) +
                        (int64_t)(s.q_lo + token) * a.dout.tok_stride +
                        (int64_t)head * a.dout.head_stride;
-        const T *outr = static_cast<const T *>(a.out) +
-                        ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim;
+        const int64_t at_row = ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim;
+        const T *outr = static_cast<const T *>(a.out) + at_row;
+        const T *restr = static_cast<const T *>(a.out_rest) + at_row;
 #pragma unroll
         for (int i = 0; i < kSteps; ++i) {
             const int at = 16 * i + 8 * half;
@@ -128,8 +132,10 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
             q[i] = memory_operand<T>(qr, at, ok);
             dout[i] = memory_operand<T>(dor, at, ok);
             const vec8<T> out = memory_operand<T>(outr, at, ok);
+            const vec8<T> rest = memory_operand<T>(restr, at, ok && a.out_rest);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) delta = fmaf((float)dout[i][k], (float)out[k], delta);
+            for (int k = 0; k < 8; ++k)
+                delta = fmaf((float)dout[i][k], (float)out[k] + (float)rest[k], delta);
         }
         delta = halves_sum(delta);
         if (row_ok) {
@@ -486,7 +492,8 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
                               int64_t k_head_stride, const void *v, int64_t v_token_stride,
                               int64_t v_head_stride, const int32_t *q_offsets,
                               const int32_t *k_offsets, int32_t sequences, int32_t causal,
-                              float scale, const void *out, const float *lse, const void *dout,
+                              float scale, const void *out, const void *out_rest,
+                              const float *lse, const void *dout,
                               int64_t dout_token_stride, int64_t dout_head_stride, void *dq,
                               void *dk, void *dv, void *workspace, int64_t workspace_bytes,
                               mg_stream_t stream) {
@@ -508,7 +515,7 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
     a.q_tokens = (int32_t)q_tokens, a.k_tokens = (int32_t)k_tokens;
     a.k_heads = k_heads, a.group = group, a.dim = dim, a.causal = causal != 0;
     a.scale = scale, a.scale_log2 = scale_to_log2(scale);
-    a.out = const_cast<void *>(out), a.lse = const_cast<float *>(lse);
+    a.out = const_cast<void *>(out), a.out_rest = const_cast<void *>(out_rest), a.lse = const_cast<float *>(lse);
     a.dq = dq, a.dk = dk, a.dv = dv;
     int32_t rc = attn_check(who, a, dtype);
     if (rc != MG_OK) return rc;

@@ -111,8 +111,8 @@ def test_frequencies_refusals(args, kw):
 def _attn(lib, dtype=1, nq=4, nk=4, heads=2, kv=2, dim=64, q=16, stride=64, off=None, n=1,
           scale=1.0, out=16, ws=None, ws_bytes=0):
     return lib.mg_attention_forward(dtype, nq, nk, heads, kv, dim, q, stride, 64, 16, stride, 64,
-                                    16, stride, 64, off, off, n, 0, scale, out, None, ws,
-                                    ws_bytes, None)
+                                    16, stride, 64, off, off, n, 0, scale, out, None, None,
+                                    ws, ws_bytes, None)
 
 
 def test_refusals_before_any_launch():
@@ -154,11 +154,11 @@ def test_refusals_before_any_launch():
     refused(_attn(lib, out=None), "NULL")
     refused(_attn(lib, nk=100000), "workspace")
     refused(lib.mg_attention_backward(1, 4, 4, 2, 2, 64, 16, 64, 64, 16, 64, 64, 16, 64, 64, None,
-                                      None, 1, 0, 1.0, 16, 16, 16, 64, 64, 16, 16, None, 16,
-                                      1 << 20, None), "go together")
+                                      None, 1, 0, 1.0, 16, None, 16, 16, 64, 64, 16, 16, None,
+                                      16, 1 << 20, None), "go together")
     refused(lib.mg_attention_backward(1, 4, 4, 2, 2, 64, 16, 64, 64, 16, 64, 64, 16, 64, 64, None,
-                                      None, 1, 0, 1.0, 16, 16, 16, 64, 64, 16, 16, 16, 16, 8,
-                                      None), "workspace of 8 bytes")
+                                      None, 1, 0, 1.0, 16, None, 16, 16, 64, 64, 16, 16, 16,
+                                      16, 8, None), "workspace of 8 bytes")
 
 
 def test_workspace_queries():
