@@ -280,6 +280,10 @@ __device__ __forceinline__ void tiles_ready() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// Ends the loads made so far, in a way that the compiler counts: a loop after it
+// holds no wait for them, which would be one for the tiles asked for in between.
+__device__ __forceinline__ void loads_done() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+
 __device__ __forceinline__ uint32_t lds_address(const char *p) {
     return (uint32_t)(uintptr_t)(const lds_char *)p;
 }

@@ -113,6 +113,7 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     TileLane<T, DK> lane_at;
     int buf = 0;
     if (k_from < k_to) ask(k_from, 0);
+    loads_done();
     for (int key0 = k_from; key0 < k_to; key0 += kTile, buf ^= 1) {
         tiles_ready();
         lane_at.fresh();

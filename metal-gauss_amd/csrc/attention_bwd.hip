@@ -165,6 +165,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
     TileLane<T, DK> lane_at;
     int buf = 0;
     if (k_to > 0) ask(0, 0);
+    loads_done();
     for (int key0 = 0; key0 < k_to; key0 += kTileRows, buf ^= 1) {
         tiles_ready();
         lane_at.fresh();
@@ -323,6 +324,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     TileLane<T, DK> lane_at;
     int g = g_from, row0 = q_from, buf = 0;
     if (steps > 0) ask(g, row0, 0);
+    loads_done();
     for (int step = 0; step < steps; ++step, buf ^= 1) {
         tiles_ready();
         lane_at.fresh();
