@@ -233,6 +233,9 @@ __device__ __forceinline__ i32x4 buffer_of(const void *base, uint32_t bytes) {
 //
 // The loads are written in assembly because the compiler, which cannot tell
 // one LDS buffer from the other, would wait for them before the next LDS read.
+// Its hazard pass does not look into assembly: the five wait states between a
+// vector instruction's scalar result (v_readfirstlane, in the descriptor) and a
+// memory access that reads it are in each load, and cover m0's one.
 template <int DK, int kWaves, int kTile = kTileRows>
 struct TileFill {
     static constexpr int kAll = kTileBytes<DK, kTile> / 1024, kLoads = kAll / kWaves;
@@ -265,7 +268,7 @@ struct TileFill {
                 rows == kTile ? off[i] : offset(i, tok_stride, dim, wave, rows);
             const int to = uniform((int)lds + (i * kWaves + wave) * 1024);
             asm volatile("s_mov_b32 m0, %0\n\t"
-                         "s_nop 0\n\t"
+                         "s_nop 4\n\t"
                          "buffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
                          : "s"(to), "v"(at), "s"(rsrc)

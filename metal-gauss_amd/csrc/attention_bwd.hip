@@ -220,7 +220,7 @@ __device__ __forceinline__ void ask_row_values(const float *at, int rows, uint32
     const uint32_t off = 4 * min(lane_id(), rows - 1);
     const i32x4 rsrc = buffer_of(at, 4 * rows);
     asm volatile("s_mov_b32 m0, %0\n\t"
-                 "s_nop 0\n\t"
+                 "s_nop 4\n\t"
                  "buffer_load_dword %1, %2, 0 offen lds"
                  :
                  : "s"(uniform((int)lds)), "v"(off), "s"(rsrc)

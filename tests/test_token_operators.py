@@ -224,3 +224,21 @@ def test_oracle_rotation_keeps_lengths_and_turns_back():
         assert np.array_equal(y[..., 8:], x[..., 8:])
         back = token_ref.rotary(y, pos, np.array([1.0, 0.1, 1.0, 0.1]), layout, inverse=True)
         assert np.allclose(back, x)
+
+
+# ------------------------------------------------------------ compiled loads
+
+@pytest.mark.parametrize("source", ["attention.hip", "attention_bwd.hip"])
+def test_tile_loads_wait_for_their_scalars(tmp_path, source):
+    """The loads into LDS are assembly that the compiler does not look into: each
+    has five wait states (s_nop 4) between anything that may have written its
+    descriptor and itself, and m0 is written just before them."""
+    from test_lds_barrier_audit import _assemble, _build_module
+
+    out = _assemble(_build_module().CSRC / source, tmp_path / "out.s", source)
+    lines = [s.split(";")[0].strip() for s in out.read_text().splitlines()]
+    lines = [s for s in lines if s and not s.startswith(".")]
+    at = [i for i, s in enumerate(lines) if s.startswith("buffer_load") and s.endswith(" lds")]
+    assert len(at) > 50
+    for i in at:
+        assert lines[i - 1] == "s_nop 4" and lines[i - 2].startswith("s_mov_b32 m0,"), lines[i - 2:i + 1]
