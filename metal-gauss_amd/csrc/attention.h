@@ -235,7 +235,8 @@ __device__ __forceinline__ i32x4 buffer_of(const void *base, uint32_t bytes) {
 // one LDS buffer from the other, would wait for them before the next LDS read.
 // Its hazard pass does not look into assembly: the five wait states between a
 // vector instruction's scalar result (v_readfirstlane, in the descriptor) and a
-// memory access that reads it are in each load, and cover m0's one.
+// memory access that reads it stand before the first load, and m0's one before
+// each.
 template <int DK, int kWaves, int kTile = kTileRows>
 struct TileFill {
     static constexpr int kAll = kTileBytes<DK, kTile> / 1024, kLoads = kAll / kWaves;
@@ -262,18 +263,33 @@ struct TileFill {
         const char *base = head + (int64_t)row0 * tok_stride * 2;
         const uint32_t bytes = (uint32_t)(rows - 1) * (uint32_t)(tok_stride * 2) + dim * 2;
         const i32x4 rsrc = buffer_of(base, bytes);
+        const int to = uniform((int)lds + wave * 1024);
+        if (rows == kTile) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const uint32_t at =
-                rows == kTile ? off[i] : offset(i, tok_stride, dim, wave, rows);
-            const int to = uniform((int)lds + (i * kWaves + wave) * 1024);
+            for (int i = 0; i < kLoads; ++i) load(i, to, off[i], rsrc);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                load(i, to, offset(i, tok_stride, dim, wave, rows), rsrc);
+        }
+    }
+
+    static __device__ __forceinline__ void load(int i, int to, uint32_t at, i32x4 rsrc) {
+        // The descriptor is the same for all of them: the first waits for it.
+        if (i == 0)
             asm volatile("s_mov_b32 m0, %0\n\t"
                          "s_nop 4\n\t"
                          "buffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
                          : "s"(to), "v"(at), "s"(rsrc)
                          : "memory");
-        }
+        else
+            asm volatile("s_mov_b32 m0, %0\n\t"
+                         "s_nop 0\n\t"
+                         "buffer_load_dwordx4 %1, %2, 0 offen lds"
+                         :
+                         : "s"(to + i * kWaves * 1024), "v"(at), "s"(rsrc)
+                         : "memory");
     }
 };
 
