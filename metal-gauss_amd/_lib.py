@@ -200,14 +200,18 @@ def dev_tensor(t: torch.Tensor, what: str, dtype: torch.dtype | None = torch.flo
 TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
-def launch(fn, t: torch.Tensor, *args) -> None:
-    """fn(*args, stream) on the device of ``t`` and that device's current stream."""
-    index = t.device.index
-    if index != torch.cuda.current_device():
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else None
+
+
+def launch(fn, index: int, *args) -> None:
+    """fn(*args, stream) on GPU `index` and that GPU's current stream."""
+    if index != _current_device():
         with torch.cuda.device(index):
             check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
     else:
-        check(fn(*args, torch._C._cuda_getCurrentRawStream(index)))
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+        if rc != 0:
+            check(rc)
 
 
 def type_code(t: torch.Tensor, what: str) -> int:

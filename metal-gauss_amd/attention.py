@@ -13,36 +13,37 @@ from torch.autograd.function import once_differentiable
 from . import _lib
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x, or a copy of it whose rows lie as the kernels read them: contiguous and
-    16-byte aligned. Slices of a projection do as they are."""
-    st = x.stride()
-    if (st[2] != 1 or x.data_ptr() % 16 or (st[0] % 8 and x.shape[0] > 1) or
-            (st[1] % 8 and x.shape[1] > 1) or st[0] >= 1 << 24):
-        return x.contiguous() if not x.is_contiguous() else x.clone()
-    return x
-
-
-def _where(x: torch.Tensor):
-    """Pointer, token stride and head stride."""
-    return (x.data_ptr() if x.numel() else None, x.stride(0) if x.shape[0] > 1 else 0,
-            x.stride(1) if x.shape[1] > 1 else 0)
+def _rows(x: torch.Tensor):
+    """x, or a copy of it whose rows lie as the kernels read them (contiguous and
+    16-byte aligned; slices of a projection do as they are), with its pointer,
+    token stride and head stride."""
+    tok, head, one = x.stride()
+    tokens, heads, _ = x.shape
+    if tokens <= 1:
+        tok = 0
+    if heads <= 1:
+        head = 0
+    at = x.data_ptr()
+    if one != 1 or at % 16 or tok % 8 or head % 8 or tok >= 1 << 24:
+        x = x.clone(memory_format=torch.contiguous_format)
+        at, tok, head = x.data_ptr(), x.stride(0), x.stride(1)
+    return x, (at if tokens else None, tok, head)
 
 
 def _forward(q, k, v, q_offsets, k_offsets, causal, scale, keep):
     lib = _lib.load()
-    q, k, v = _rows(q), _rows(k), _rows(v)
+    (q, q_at), (k, k_at), (v, v_at) = _rows(q), _rows(k), _rows(v)
     Tq, Hq, D = q.shape
-    Tk, Hk = k.shape[0], k.shape[1]
+    Tk, Hk, _ = k.shape
     n = 1 if q_offsets is None else q_offsets.numel() - 1
     # With a backward pass ahead, what rounding takes from the result is kept too.
-    out = torch.empty(Tq, Hq, D, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     rest = torch.empty_like(out) if keep else None
     lse = torch.empty(Hq, Tq, device=q.device) if keep else None
     need = lib.mg_attention_forward_workspace_bytes(Tq, Tk, Hq, Hk, D, n)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _lib.launch(lib.mg_attention_forward, q, _lib.TYPE_CODES[q.dtype], Tq, Tk, Hq, Hk, D,
-                *_where(q), *_where(k), *_where(v),
+    _lib.launch(lib.mg_attention_forward, q.get_device(), _lib.TYPE_CODES[q.dtype], Tq, Tk, Hq,
+                Hk, D, *q_at, *k_at, *v_at,
                 None if q_offsets is None else q_offsets.data_ptr(),
                 None if k_offsets is None else k_offsets.data_ptr(), n, causal, scale,
                 out.data_ptr(), rest.data_ptr() if keep else None,
@@ -67,18 +68,18 @@ class _Attention(torch.autograd.Function):
         Tq, Hq, D = q.shape
         Tk, Hk = k.shape[0], k.shape[1]
         n = 1 if q_offsets is None else q_offsets.numel() - 1
-        dout = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype))
-        dq = torch.empty(Tq, Hq, D, dtype=q.dtype, device=q.device)
+        dout, dout_at = _rows(dout if dout.dtype == q.dtype else dout.to(q.dtype))
+        dq = torch.empty_like(out)
         keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dk = torch.empty(Tk, Hk, D, dtype=q.dtype, device=q.device) if keys else None
         dv = torch.empty(Tk, Hk, D, dtype=q.dtype, device=q.device) if keys else None
         need = lib.mg_attention_backward_workspace_bytes(Tq, Tk, Hq, Hk, D, n)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _lib.launch(lib.mg_attention_backward, q, _lib.TYPE_CODES[q.dtype], Tq, Tk, Hq, Hk, D,
-                    *_where(q), *_where(k), *_where(v),
+        _lib.launch(lib.mg_attention_backward, q.get_device(), _lib.TYPE_CODES[q.dtype], Tq, Tk,
+                    Hq, Hk, D, *_rows(q)[1], *_rows(k)[1], *_rows(v)[1],
                     None if q_offsets is None else q_offsets.data_ptr(),
                     None if k_offsets is None else k_offsets.data_ptr(), n, ctx.causal,
-                    ctx.scale, out.data_ptr(), rest.data_ptr(), lse.data_ptr(), *_where(dout), dq.data_ptr(),
+                    ctx.scale, out.data_ptr(), rest.data_ptr(), lse.data_ptr(), *dout_at, dq.data_ptr(),
                     dk.data_ptr() if keys else None, dv.data_ptr() if keys else None,
                     ws.data_ptr(), need)
         return dq, dk, dv, None, None, None, None
@@ -88,7 +89,7 @@ def _check_offsets(off, what, q):
     if off.dim() != 1 or off.numel() < 2:
         raise ValueError(f"{what} must be (sequences + 1,), got {tuple(off.shape)}")
     _lib.dev_tensor(off, what, torch.int32)
-    if off.device != q.device:
+    if off.get_device() != q.get_device():
         raise RuntimeError(f"{what} must be on {q.device}, got device '{off.device}'")
 
 
@@ -122,7 +123,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             raise RuntimeError(f"{what} must be bfloat16 or float16, got {t.dtype}")
         if t.dim() != 3:
             raise ValueError(f"{what} must be (tokens, heads, dim), got {tuple(t.shape)}")
-        if t.dtype != q.dtype or t.device != q.device or t.shape[2] != q.shape[2]:
+        if (t.dtype != q.dtype or t.get_device() != q.get_device() or
+                t.shape[2] != q.shape[2]):
             raise ValueError(f"{what} must match q's type, device and head dimension; got "
                              f"{t.dtype} {tuple(t.shape)} on {t.device}")
     if k.shape != v.shape:

@@ -22,40 +22,41 @@ def _rows(x: torch.Tensor):
     return x, x.stride(0)
 
 
-def _check_weight(w, x, what):
-    if w is None:
-        return
-    if w.shape != x.shape[-1:]:
-        raise ValueError(f"{what} must have shape ({x.shape[-1]},), got {tuple(w.shape)}")
-    if w.device != x.device:
-        raise RuntimeError(f"{what} must be on {x.device}, got device '{w.device}'")
+def _check_weight(w, n, index, what):
+    if w.dim() != 1 or w.shape[0] != n:
+        raise ValueError(f"{what} must have shape ({n},), got {tuple(w.shape)}")
+    if w.get_device() != index:
+        raise RuntimeError(f"{what} must be on GPU {index}, got device '{w.device}'")
+    return w if w.is_contiguous() else w.contiguous()
 
 
 def _forward(x, weight, bias, eps, keep):
     """y and, with ``keep``, what the backward pass needs."""
     code = _lib.type_code(x, "x")
     lib = _lib.load()
-    if x.dim() == 0 or x.shape[-1] == 0:
+    width = x.shape[-1] if x.dim() else 0
+    if width == 0:
         raise ValueError(f"layer_norm needs rows of at least one element, got {tuple(x.shape)}")
-    _check_weight(weight, x, "weight")
-    _check_weight(bias, x, "bias")
-    w = weight if weight is not None else bias
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError(f"weight is {weight.dtype} and bias {bias.dtype}; one type is needed")
-    wcode = code if w is None else _lib.type_code(w, "weight")
+    index = x.get_device()
+    wcode, w_at, b_at = code, None, None
     if weight is not None:
-        weight = weight.contiguous()
+        weight = _check_weight(weight, width, index, "weight")
+        wcode, w_at = _lib.type_code(weight, "weight"), weight.data_ptr()
     if bias is not None:
-        bias = bias.contiguous()
+        bias = _check_weight(bias, width, index, "bias")
+        if weight is not None and bias.dtype != weight.dtype:
+            raise ValueError(f"weight is {weight.dtype} and bias {bias.dtype}; one type is needed")
+        wcode, b_at = _lib.type_code(bias, "bias"), bias.data_ptr()
     rows, stride = _rows(x)
     n = rows.shape[0]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty(2, n, device=x.device) if keep else None
-    mean = stats.data_ptr() if keep else None
-    _lib.launch(lib.mg_layer_norm_forward, x, n, x.shape[-1], code, rows.data_ptr(), stride,
-                wcode, None if weight is None else weight.data_ptr(),
-                None if bias is None else bias.data_ptr(), eps, y.data_ptr(), mean,
-                mean + 4 * n if keep else None)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    stats = mean = rstd = None
+    if keep:
+        stats = torch.empty(2 * n, device=x.device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * n
+    _lib.launch(lib.mg_layer_norm_forward, index, n, width, code, rows.data_ptr(), stride, wcode,
+                w_at, b_at, eps, y.data_ptr(), mean, rstd)
     return y, rows, stats, weight
 
 
@@ -92,7 +93,7 @@ class _LayerNorm(torch.autograd.Function):
                              dtype=torch.uint8, device=dev)
         code = _lib.TYPE_CODES[rows.dtype]
         mean = stats.data_ptr()
-        _lib.launch(lib.mg_layer_norm_backward, rows, n, width, code, rows.data_ptr(),
+        _lib.launch(lib.mg_layer_norm_backward, rows.get_device(), n, width, code, rows.data_ptr(),
                     rows.stride(0), dy.data_ptr(), dy_stride,
                     code if wtype is None else _lib.TYPE_CODES[wtype],
                     None if w is None else w.data_ptr(), mean, mean + 4 * n,

@@ -62,19 +62,18 @@ def _heads(x: torch.Tensor):
 def _turn(q, k, positions, frequencies, layout, inverse):
     lib = _lib.load()
     q = _heads(q)
-    k = None if k is None else _heads(k)
     T, Hq, D = q.shape
-    dtype = q.dtype
-    q_out = torch.empty(T, Hq, D, dtype=dtype, device=q.device)
-    k_out = None if k is None else torch.empty(T, k.shape[1], D, dtype=dtype, device=q.device)
-    _lib.launch(lib.mg_rotary, q, T, _lib.TYPE_CODES[dtype], q.data_ptr(), q.stride(0),
-                q.stride(1), Hq, None if k is None else k.data_ptr(),
-                0 if k is None else k.stride(0), 0 if k is None else k.stride(1),
-                0 if k is None else k.shape[1], D, positions.data_ptr(),
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out, k_args, k_to = None, (None, 0, 0, 0), None
+    if k is not None:
+        k = _heads(k)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_args, k_to = (k.data_ptr(), k.stride(0), k.stride(1), k.shape[1]), k_out.data_ptr()
+    _lib.launch(lib.mg_rotary, q.get_device(), T, _lib.TYPE_CODES[q.dtype], q.data_ptr(),
+                q.stride(0), q.stride(1), Hq, *k_args, D, positions.data_ptr(),
                 positions.dtype == torch.int64,
                 1 if positions.dim() == 1 else positions.shape[1], frequencies.data_ptr(),
-                frequencies.numel(), layout == "interleaved", inverse, q_out.data_ptr(),
-                None if k is None else k_out.data_ptr())
+                frequencies.numel(), layout == "interleaved", inverse, q_out.data_ptr(), k_to)
     return q_out, k_out
 
 
@@ -118,8 +117,10 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     code = _lib.type_code(q, "q")
     if q.dim() != 3:
         raise ValueError(f"q must be (tokens, heads, dim), got {tuple(q.shape)}")
-    if k is not None and (k.dim() != 3 or _lib.type_code(k, "k") != code or k.shape[0] != q.shape[0] or
-                          k.shape[-1] != q.shape[-1] or k.device != q.device):
+    index = q.get_device()
+    if k is not None and (k.dim() != 3 or _lib.type_code(k, "k") != code or
+                          k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2] or
+                          k.get_device() != index):
         raise ValueError(f"k must match q's type, device, tokens and head dimension; got "
                          f"{k.dtype} {tuple(k.shape)} against {q.dtype} {tuple(q.shape)}")
     if layout not in LAYOUTS:
@@ -129,10 +130,14 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     if positions.dim() not in (1, 2) or positions.shape[0] != q.shape[0]:
         raise ValueError(f"positions must be ({q.shape[0]},) or ({q.shape[0]}, axes), got "
                          f"{tuple(positions.shape)}")
-    if positions.device != q.device:
+    if not positions.is_cuda or positions.get_device() != index:
         raise RuntimeError(f"positions must be on {q.device}, got device '{positions.device}'")
     _lib.dev_tensor(frequencies, "frequencies", torch.float64)
-    positions = positions.contiguous()
+    if frequencies.get_device() != index:
+        raise RuntimeError(f"frequencies must be on {q.device}, got device "
+                           f"'{frequencies.device}'")
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         out = _Rotary.apply(q, k, positions, frequencies, layout)
     else:
