@@ -697,8 +697,9 @@ int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q,
  * made to rise; tokens outside every sequence get zeros. A query sees its
  * sequence's keys, causal those that stand at or before it, the last query
  * standing at the last key; a query that sees none gets zeros. softmax(scale *
- * q k) v, scale >= 0. What a query does not see may hold anything in k; in v
- * too, as long as it is finite.
+ * q k) v, scale >= 0. Keys and values that a query does not see may be
+ * infinities or NaN without a trace in its result; the backward pass asks for
+ * finite ones.
  *
  * lse (q_heads, q_tokens, float32; NULL: not kept) is the base 2 logarithm of a
  * row's sum of exponentials, +inf for a row that sees nothing: the backward

@@ -111,7 +111,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     tokens. A sequence may have more keys than queries (new tokens over a
     memory, down to one token), fewer, or none of either. ``causal``: a query sees
     the keys that stand at or before it, a sequence's last query standing at its
-    last key. A query that sees no key, or belongs to no sequence, gets zeros.
+    last key. A query that sees no key, or belongs to no sequence, gets zeros;
+    infinities and NaN in keys and values that it does not see leave no trace in
+    its result (the backward pass asks for finite inputs within a sequence).
     ``scale`` (default dim ** -0.5) may not be negative.
 
     Scores, softmax and sums are float32; p is rounded to the inputs' type for

@@ -39,12 +39,74 @@ __device__ __forceinline__ int keys_seen(const SeqItem &s, int token, int causal
     return clamp_to(token + 1 + s.k_len - s.q_len, 0, s.k_len);
 }
 
+// Infinities and NaN among values that a mask leaves out for some rows: 0 times
+// one would reach rows that do not see it. Tiles that some row of the item does
+// not see whole are cleared of them before their products, and they are added
+// after the last tile to the rows that see them (add_seen_values).
+
+// Bits of the halves of a word that are not finite: their exponents are all ones.
+template <typename T>
+__device__ __forceinline__ uint32_t not_finite(uint32_t w) {
+    constexpr uint32_t lo = std::is_same<T, f16_t>::value ? 0x7c00u : 0x7f80u, hi = lo << 16;
+    return ((w & lo) == lo ? 0xffffu : 0u) | ((w & hi) == hi ? 0xffff0000u : 0u);
+}
+
+// Clears wave `wave`'s part of a tile; whether anything was there.
+template <typename T, int DK, int kTile, int kWaves>
+__device__ __forceinline__ bool clear_not_finite(char *tile, int wave) {
+    constexpr int kPart = kTileBytes<DK, kTile> / kWaves;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < kPart / 1024; ++i) {
+        i32x4 *at = reinterpret_cast<i32x4 *>(tile + wave * kPart + 1024 * i + 16 * lane_id());
+        i32x4 w = *at;
+        uint32_t bad[4], any = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) any |= bad[k] = not_finite<T>(w[k]);
+        if (any) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] &= ~bad[k];
+            *at = w;
+            found = true;
+        }
+    }
+    return ballot(found) != 0;
+}
+
+// Adds what is not finite of keys from .. to - 1 to the rows that see them.
+template <typename T, int DK>
+__device__ __forceinline__ void add_seen_values(const char *head, int64_t tok_stride, int dim,
+                                                int from, int to, int see, int half,
+                                                f32x16 (&o)[DK / 32]) {
+#pragma unroll 1
+    for (int key = from; key < to; ++key) {
+        const T *row = reinterpret_cast<const T *>(head) + (int64_t)key * tok_stride;
+        // No branches: a row that does not see the key adds 0.
+#pragma unroll
+        for (int b = 0; b < DK / 32; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int at = 32 * b + c_row(e, half);
+                const vec4<T> v = *reinterpret_cast<const vec4<T> *>(row + min(at, dim - 4));
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float f = (float)v[k];
+                    o[b][e + k] += key < see && f - f != 0.f ? f : 0.f;
+                }
+            }
+    }
+}
+
 // One work item: false if there is none of this number.
 template <typename T, int DK, int kWaves, bool kSplit>
 __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     constexpr int kRows = 32 * kWaves, kSteps = DK / 16, kBlocks = DK / 32;
     constexpr int kTile = kKeyTile<kWaves>, kParts = kTile / 32;
     __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK, kTile>];
+    // The first key of a tile that was cleared: a register of the only wave, or in
+    // LDS.
+    __shared__ int s_not_finite;
+    int not_finite_from = 0;
     const int lane = lane_id(), half = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kh = work % a.k_heads, item = work / a.k_heads, G = a.group;
@@ -74,7 +136,8 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     const int token = row / G, head = kh * G + row % G;
     const bool row_ok = token < s.q_len;
     const int see = row_ok ? keys_seen(s, token, a.causal) : 0;
-    // The keys of its wave's first and last row, and of the tile's last.
+    // The keys of its wave's first and last row, and of the tile's.
+    const int see_least = keys_seen(s, min(tile * kRows / G, s.q_len - 1), a.causal);
     const int last_token = min((tile * kRows + kRows - 1) / G, s.q_len - 1);
     const int see_first = keys_seen(s, min(row0 / G, s.q_len - 1), a.causal);
     const int see_last = keys_seen(s, min((row0 + 31) / G, s.q_len - 1), a.causal);
@@ -110,6 +173,10 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
 
     f32x16 o[kBlocks] = {};
     float top = -INFINITY, sum = 0.f;     // top: in powers of 2, what p goes by
+    if constexpr (kWaves == 1)
+        not_finite_from = k_to;
+    else if (threadIdx.x == 0)
+        s_not_finite = k_to;
     TileLane<T, DK> lane_at;
     int buf = 0;
     if (k_from < k_to) ask(k_from, 0);
@@ -117,6 +184,15 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     for (int key0 = k_from; key0 < k_to; key0 += kTile, buf ^= 1) {
         tiles_ready();
         lane_at.fresh();
+        if (key0 + kTile > see_least) {
+            const bool found = clear_not_finite<T, DK, kTile, kWaves>(s_tile[buf][1], wave);
+            if constexpr (kWaves == 1) {
+                if (found) not_finite_from = min(not_finite_from, key0);
+            } else {
+                if (found && lane == 0 && key0 < s_not_finite) s_not_finite = key0;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
         if (key0 + kTile < k_to) ask(key0 + kTile, buf ^ 1);
         if (key0 >= see_last) continue;   // the wave's rows see none of these keys
         const char *kt = s_tile[buf][0], *vt = s_tile[buf][1];
@@ -168,6 +244,12 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
                 o[b] = mfma32(lane_at.columns(vt, 16 * i, b), p[i], o[b]);
     }
     lds_reads_done();
+    if (k_from < k_to) {
+        if constexpr (kWaves > 1) not_finite_from = uniform(s_not_finite);
+        if (not_finite_from < k_to)
+            add_seen_values<T, DK>(vp, a.v.tok_stride, a.dim, not_finite_from,
+                                   min(see_last, k_to), see, half, o);
+    }
     sum = halves_sum(sum);
 
     if constexpr (kSplit) {

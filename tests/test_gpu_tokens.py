@@ -424,8 +424,8 @@ def test_attention_offsets_are_held_to_the_tensors(dev):
 
 
 def test_attention_unseen_keys_may_hold_anything(dev):
-    """NaN and infinities in keys that the mask leaves out, in neighbours'
-    sequences and (finite) in values."""
+    """NaN and infinities in keys and values that the mask leaves out, in their own
+    sequence and in its neighbours'."""
     from metal_gauss_amd import attention
 
     q, k, v, _ = (t.to(dev) for t in attn_inputs(("unseen",), 100, 100, 2, 2, 64, "bf16"))
@@ -439,6 +439,71 @@ def test_attention_unseen_keys_may_hold_anything(dev):
     v[:50] = float("nan")
     got = attention(q, k, v, off, causal=True)
     assert torch.equal(got[50:99], clean[50:99])
+
+
+@pytest.mark.parametrize("ty,heads,kv,dim", [("bf16", 2, 2, 64), ("f16", 4, 1, 128),
+                                             ("bf16", 1, 1, 32)])
+@pytest.mark.parametrize("nq,nk", [(200, 200), (3, 700), (90, 300)])
+def test_attention_values_that_are_not_finite_reach_those_who_see_them(dev, ty, heads, kv, dim,
+                                                                       nq, nk):
+    from metal_gauss_amd import attention
+
+    q, k, v, _ = (t.to(dev) for t in attn_inputs(("poison", nq, nk), nq, nk, heads, kv, dim, ty))
+    clean = attention(q, k, v, causal=True).float()
+    first = nk - nq                  # the key at which query 0 stands
+    plus, minus, nan = first + nq // 3, first + nq // 2, first + nq - 1
+    v[plus, :, 3], v[minus, :, 3], v[minus, :, 5], v[nan, :, 7] = (
+        float("inf"), float("-inf"), float("-inf"), float("nan"))
+    got = attention(q, k, v, causal=True).float()
+    stands = torch.arange(nq, device=dev) + first
+    for column in range(dim):
+        want = clean[:, :, column].clone()
+        if column == 3:              # of three queries both stand at one key
+            want[stands >= plus] = float("inf")
+            want[stands >= minus] = float("nan" if plus != minus else "-inf")
+        elif column == 5:
+            want[stands >= minus] = float("-inf")
+        elif column == 7:
+            want[stands >= nan] = float("nan")
+        assert torch.equal(got[:, :, column].isnan(), want.isnan()), column
+        fine = want.isfinite()
+        assert torch.equal(got[:, :, column][~fine & ~want.isnan()], want[~fine & ~want.isnan()])
+        # The finite part is the same products in the same order.
+        assert torch.equal(got[:, :, column][fine], want[fine]), column
+
+
+def test_attention_in_a_graph(dev):
+    """A token step captured once and replayed on new inputs, with eager work
+    between: chunks of keys and their joining allocate nothing and clear nothing."""
+    from metal_gauss_amd import attention, layer_norm, rotary, rotary_frequencies
+
+    g = gen("graph")
+    q = torch.randn(4, 8, 64, generator=g).to(dev, torch.bfloat16)
+    kv = torch.randn(9000, 2, 2, 64, generator=g).to(dev, torch.bfloat16)
+    pos = torch.arange(4, dtype=torch.int32, device=dev)
+    freq = rotary_frequencies(64, device=dev)
+    qo = torch.arange(5, dtype=torch.int32, device=dev)
+    ko = torch.tensor([0, 3000, 3100, 8990, 9000], dtype=torch.int32, device=dev)
+
+    def step():
+        x = rotary(layer_norm(q), None, pos, freq)
+        return attention(x, kv[:, 0], kv[:, 1], qo, ko, causal=True)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for i in range(4):
+        q.copy_(torch.randn(4, 8, 64, generator=g))
+        kv.copy_(torch.randn(9000, 2, 2, 64, generator=g))
+        graph.replay()
+        got = out.clone()
+        torch.cuda.synchronize()
+        assert torch.equal(got, step())
 
 
 def test_attention_strided_views_and_broadcast_heads(dev):
