@@ -97,6 +97,36 @@ __device__ __forceinline__ void add_seen_values(const char *head, int64_t tok_st
     }
 }
 
+// The result of a lane's row in columns 32 block0 .. of DK, its sums of values o
+// unscaled.
+template <typename T, int DK>
+__device__ __forceinline__ void store_row_result(const AttnArgs &a, int token, int head, int half,
+                                                 int block0, float top, float sum,
+                                                 const f32x16 (&o)[DK / 32]) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int64_t at_row = ((int64_t)token * (a.k_heads * a.group) + head) * a.dim;
+    T *out = static_cast<T *>(a.out) + at_row, *rest = static_cast<T *>(a.out_rest) + at_row;
+#pragma unroll
+    for (int b = 0; b < DK / 32; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int at = 32 * (block0 + b) + c_row(e, half);
+            vec4<T> w, x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float f = o[b][e + i] * inv;
+                w[i] = (T)f;
+                x[i] = (T)(f - (float)w[i]);
+            }
+            if (at >= a.dim) continue;
+            *reinterpret_cast<vec4<T> *>(out + at) = w;
+            if (a.out_rest) *reinterpret_cast<vec4<T> *>(rest + at) = x;
+        }
+    if (a.lse && half == 0 && block0 == 0)
+        a.lse[(int64_t)head * a.q_tokens + token] =
+            sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+}
+
 // One work item: false if there is none of this number.
 template <typename T, int DK, int kWaves, bool kSplit>
 __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
@@ -255,39 +285,22 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     if constexpr (kSplit) {
         const int64_t slot = (int64_t)work * kRows + wave * 32 + lane % 32;
         if (!row_ok) return true;
-        float *po = a.part_o + slot * DK;
+        // Narrow items hold few rows, and keep them one after the other; wide
+        // ones are kept as their waves hold them, 1024 bytes a store.
+        float *po = kWaves == kNarrowWaves
+                        ? a.part_o + slot * DK + 4 * half
+                        : a.part_o + (int64_t)work * kRows * DK + wave * 32 * DK + 4 * lane;
+        constexpr int kApart = kWaves == kNarrowWaves ? 8 : 4 * 64;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<f32x4 *>(po + 32 * b + c_row(e, half)) =
+                *reinterpret_cast<f32x4 *>(po + (4 * b + e / 4) * kApart) =
                     f32x4{o[b][e], o[b][e + 1], o[b][e + 2], o[b][e + 3]};
         if (half == 0) a.part_stats[slot] = make_float2(top, sum);
         return true;
     }
-    if (!row_ok) return true;
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int64_t at_row = ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim;
-    T *out = static_cast<T *>(a.out) + at_row, *rest = static_cast<T *>(a.out_rest) + at_row;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int at = 32 * b + c_row(e, half);
-            vec4<T> w, x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float f = o[b][e + i] * inv;
-                w[i] = (T)f;
-                x[i] = (T)(f - (float)w[i]);
-            }
-            if (at >= a.dim) continue;
-            *reinterpret_cast<vec4<T> *>(out + at) = w;
-            if (a.out_rest) *reinterpret_cast<vec4<T> *>(rest + at) = x;
-        }
-    if (a.lse && half == 0)
-        a.lse[(int64_t)head * a.q_tokens + s.q_lo + token] =
-            sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
+    if (row_ok) store_row_result<T, DK>(a, s.q_lo + token, head, half, 0, top, sum, o);
     return true;
 }
 
@@ -304,12 +317,59 @@ __global__ __launch_bounds__(64 * kWaves, kWaves == 1 ? 1 : 2) void attn_fwd_ker
     }
 }
 
-// Joins the chunks of a row: o = sum 2^(top_c - top) o_c / sum of the same of
-// sum_c. kJoin waves a row (four where rows have many chunks), wave w with every
-// kJoin-th chunk from w; a lane first holds a chunk's weight, then DK / 64 columns.
-template <typename T, int DK, int kWaves, int kJoin>
-__global__ __launch_bounds__(256) void attn_join_kernel(AttnArgs a) {
-    constexpr int kRows = 32 * kWaves, kCols = DK <= 64 ? 1 : 2;
+// Joining the chunks of a row: o = sum 2^(top_c - top) o_c / sum of the same of
+// sum_c.
+//
+// Wide items: a workgroup has 32 columns of a tile of one key head, its threads
+// the elements that the item's had.
+template <typename T, int DK>
+__global__ __launch_bounds__(64 * kWideWaves) void attn_join_tile_kernel(AttnArgs a) {
+    constexpr int kRows = 32 * kWideWaves;
+    const int lane = lane_id(), half = lane / 32, G = a.group, block = blockIdx.y;
+    const int wave = uniform(threadIdx.x / 64);
+    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
+    const auto tiles_of = [&](int ql, int) { return (ql * G + kRows - 1) / kRows; };
+    const auto chunks_of = [&](int kl) { return max(1, (kl + a.split_keys - 1) / a.split_keys); };
+    const SeqItem s = find_item<false>(
+        a, item, tiles_of, [&](int ql, int kl) { return tiles_of(ql, kl) * chunks_of(kl); });
+    if (!s.found) return;
+    const int chunks = chunks_of(s.k_len), item0 = s.before + s.within * chunks;
+    // Offsets that fall again could make more items than there are.
+    if (item0 + chunks > a.items) return;
+    const int row = (tiles_of(s.q_len, 0) - 1 - s.within) * kRows + wave * 32 + lane % 32;
+    const int token = row / G, head = kh * G + row % G;
+    if (token >= s.q_len) return;
+    const int64_t work0 = (int64_t)item0 * a.k_heads + kh;
+    const float2 *stats = a.part_stats + work0 * kRows + wave * 32 + lane % 32;
+    const float *po =
+        a.part_o + work0 * kRows * DK + wave * 32 * DK + 4 * lane + 4 * block * 4 * 64;
+    float top = -INFINITY, sum = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < chunks; ++c) top = fmaxf(top, stats[(int64_t)c * a.k_heads * kRows].x);
+    f32x16 o[1] = {};
+#pragma unroll 4
+    for (int c = 0; c < chunks; ++c) {
+        const float2 st = stats[(int64_t)c * a.k_heads * kRows];
+        const float *p = po + (int64_t)c * a.k_heads * kRows * DK;
+        const float by = st.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st.x - top);
+        // A NaN sum of a chunk without a finite score goes on.
+        sum = fmaf(st.y, by, sum);
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(p + e * 64);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[0][e + i] = fmaf(x[i], by, o[0][e + i]);
+        }
+    }
+    store_row_result<T, 32>(a, s.q_lo + token, head, half, block, top, sum, o);
+}
+
+// Narrow items: kJoin waves a row (four where rows have many chunks), wave w with
+// every kJoin-th chunk from w; a lane first holds a chunk's weight, then DK / 64
+// columns.
+template <typename T, int DK, int kJoin>
+__global__ __launch_bounds__(256) void attn_join_row_kernel(AttnArgs a) {
+    constexpr int kRows = 32 * kNarrowWaves, kCols = DK <= 64 ? 1 : 2;
     __shared__ float s_o[kJoin > 1 ? kJoin : 1][64 * kCols], s_top[kJoin], s_sum[kJoin];
     const int lane = lane_id(), G = a.group, heads = a.k_heads * G;
     const int wave = uniform(threadIdx.x / 64);
@@ -427,10 +487,14 @@ int32_t attn_check(const char *who, const AttnArgs &a, int32_t dtype) {
 struct FwdPlan {
     int waves;
     int split_keys;             // 0: whole rows
-    int64_t items;              // a key head's, at most
+    int64_t tiles, items;       // a key head's, at most
     int64_t stats_bytes, bytes; // of partial results
 };
 
+// Items that run at once. Of several sequences the longer ones have more chunks
+// than the average says, so half as many are aimed at (chunks of 475, 256, 1 and
+// 64 queries over up to 16320 keys: 106 us, aimed at 512 it is 109 and 384 124;
+// one sequence of 2500, 8 heads of 64: 40 aimed at 256, 26 at 512).
 constexpr int64_t kWideSlots = 512, kNarrowSlots = 1536;
 constexpr int64_t kSplitLeast = 768, kChunkLeast = 256;
 
@@ -440,9 +504,11 @@ static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int gro
     const int64_t rows = q_tokens * group;
     p.waves = rows <= 64 * (int64_t)n_seq ? kNarrowWaves : kWideWaves;
     const int64_t tile_rows = 32 * p.waves, tile = p.waves == kNarrowWaves ? 32 : kTileRows;
-    const int64_t slots = p.waves == kNarrowWaves ? kNarrowSlots : kWideSlots;
+    const int64_t slots = p.waves == kNarrowWaves ? kNarrowSlots
+                          : n_seq == 1            ? kWideSlots
+                                                  : kWideSlots / 2;
     // The tokens before the first and past the last offset make tiles too.
-    p.items = rows / tile_rows + n_seq + 2;
+    p.items = p.tiles = rows / tile_rows + n_seq + 2;
     const int64_t likely = (ceil_div(rows, tile_rows) + n_seq - 1) * k_heads;
     const int64_t mean_keys = k_tokens / n_seq;
     if (2 * likely <= slots && mean_keys >= kSplitLeast) {
@@ -542,23 +608,19 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
         // at once, on the average.
         const bool many = k_tokens / sequences > 8 * (int64_t)p.split_keys;
         const int64_t rows = q_tokens * q_heads;
-        const unsigned joins = (unsigned)(many ? rows : ceil_div(rows, 4));
+        const unsigned tiles = (unsigned)(p.tiles * k_heads);
         attn_form(dtype, dim, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int DK = decltype(d)::value;
-            if (p.waves == kWideWaves) {
-                if (many)
-                    attn_join_kernel<T, DK, kWideWaves, 4><<<joins, 256, 0, st>>>(a);
-                else
-                    attn_join_kernel<T, DK, kWideWaves, 1><<<joins, 256, 0, st>>>(a);
-            } else {
-                if (many)
-                    attn_join_kernel<T, DK, kNarrowWaves, 4><<<joins, 256, 0, st>>>(a);
-                else
-                    attn_join_kernel<T, DK, kNarrowWaves, 1><<<joins, 256, 0, st>>>(a);
-            }
+            if (p.waves == kWideWaves)
+                attn_join_tile_kernel<T, DK>
+                    <<<dim3(tiles, DK / 32), 64 * kWideWaves, 0, st>>>(a);
+            else if (many)
+                attn_join_row_kernel<T, DK, 4><<<(unsigned)rows, 256, 0, st>>>(a);
+            else
+                attn_join_row_kernel<T, DK, 1><<<(unsigned)ceil_div(rows, 4), 256, 0, st>>>(a);
         });
-        MG_LAUNCHED("attn_join_kernel");
+        MG_LAUNCHED("attn_join kernels");
     }
     return MG_OK;
 }
