@@ -20,11 +20,14 @@ constexpr int c_row(int e, int h) { return 8 * (e / 4) + 4 * h + e % 4; }
 
 // --------------------------------------------------------------- LDS tiles
 // Rows of DK elements of two bytes in chunks of 16 bytes, tile_chunks<DK>() to
-// a row; chunk c of row r lies at place c ^ tile_swizzle<DK>(r) of its row.
-// Both ways of reading then spread over the banks: eight neighbouring rows at
-// one chunk (an operand along rows) take eight different places of 128 bytes,
-// and four neighbouring rows at a pair of chunks (an operand across rows, the
-// transposing read) four different pairs.
+// a row; chunk c of row r lies at place c ^ tile_swizzle<DK>(r) of its row. Both
+// ways of reading then spread over the 64 banks (256 bytes): four neighbouring
+// rows at four chunks (an operand across rows, the transposing read, 32 lanes at
+// a time), and 16 neighbouring rows at one chunk (an operand along rows, 16 lanes
+// at a time). The shorter rows take the latter in two turns: a swizzle that
+// spared that needs twice the addresses, and cost 3% (forward, 64 columns) to 9%
+// (keys' gradient) where the vector unit is the bound; of 128 columns a swizzle
+// with conflicts in both (a third of the LDS cycles) was 1% slower.
 template <int DK>
 constexpr int tile_chunks() {
     return DK <= 32 ? 4 : DK <= 64 ? 8 : 16;
@@ -34,7 +37,7 @@ template <int DK>
 constexpr int tile_swizzle(int r) {
     return tile_chunks<DK>() == 4   ? ((r >> 1 & 1) << 1 | (r >> 2 & 1))
            : tile_chunks<DK>() == 8 ? ((r & 3) << 1 | (r >> 2 & 1))
-                                    : ((r & 3) << 1 | (r >> 2 & 1) | (r & 8));
+                                    : ((r & 3) << 2 | (r >> 2 & 3));
 }
 
 // Byte of chunk c of row r.
@@ -67,7 +70,7 @@ constexpr int column_lane_byte(int lane) {
 }
 template <int DK>
 constexpr int column_operand_byte(int lane_byte, int row0, int block) {
-    return (lane_byte ^ (64 * block ^ 16 * (tile_swizzle<DK>(row0) & 8))) +
+    return (lane_byte ^ (64 * block ^ 16 * tile_swizzle<DK>(row0))) +
            row0 * tile_chunks<DK>() * 16;
 }
 

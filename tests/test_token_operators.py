@@ -50,9 +50,9 @@ def test_fills_and_operands_agree_on_every_place(tmp_path, dk):
         want_col = 32 * b + 16 * (l // 16 % 2) + 4 * (l % 4)
         at, within = byte - byte % 16, byte % 16
         assert place[at] == (want_row, want_col // 8) and within == want_col % 8 * 2
-        banks.setdefault((r, b, l // 16), []).append(byte % 128)
+        banks.setdefault((r, b, l // 32), []).append(byte % 256)
     for seen in banks.values():
-        assert len(set(seen)) == 16, "16 lanes' reads spread over 128 bytes"
+        assert len(set(seen)) == 32, "32 lanes' reads of 8 bytes spread over 256"
 
 
 @pytest.mark.parametrize("dk", [32, 64, 96, 128])
@@ -60,9 +60,9 @@ def test_rows_read_together_lie_in_different_banks(tmp_path, dk):
     rows = _run(tmp_path, "attention_tiles.h", f"""
         for (int s = 0; s < {dk} / 16; ++s)
             for (int l = 0; l < 64; ++l) std::printf("%d\\n", row_operand_byte<{dk}>(row_lane_byte<{dk}>(l), 0, s));""")
-    at = [r[0] % 128 for r in rows]
-    for i in range(0, len(at), 8):
-        assert len(set(at[i:i + 8])) == 8
+    at = [r[0] % 256 for r in rows]
+    for i in range(0, len(at), 16):
+        assert len(set(at[i:i + 16])) == (16 if dk > 64 else 8)
 
 
 def test_a_products_rows_are_the_next_ones_operand(tmp_path):
