@@ -257,39 +257,52 @@ struct TileFill {
         return (uint32_t)r * (uint32_t)(tok_stride * 2) + (c * 8 < dim ? c * 16 : 0);
     }
 
-    __device__ __forceinline__ void ask(const char *head, int64_t tok_stride, int dim, int row0,
-                                        int n_rows, int wave, uint32_t lds) const {
+    // A tile to be asked for, load by load.
+    struct Order {
+        i32x4 rsrc;
+        int to, rows;
+    };
+
+    __device__ __forceinline__ Order order(const char *head, int64_t tok_stride, int dim, int row0,
+                                           int n_rows, int wave, uint32_t lds) const {
         const int rows = min(n_rows - row0, kTile);
         const char *base = head + (int64_t)row0 * tok_stride * 2;
         const uint32_t bytes = (uint32_t)(rows - 1) * (uint32_t)(tok_stride * 2) + dim * 2;
-        const i32x4 rsrc = buffer_of(base, bytes);
-        const int to = uniform((int)lds + wave * 1024);
-        if (rows == kTile) {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i) load(i, to, off[i], rsrc);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kLoads; ++i)
-                load(i, to, offset(i, tok_stride, dim, wave, rows), rsrc);
-        }
+        return {buffer_of(base, bytes), uniform((int)lds + wave * 1024), rows};
     }
 
-    static __device__ __forceinline__ void load(int i, int to, uint32_t at, i32x4 rsrc) {
+    // Load i of a whole tile.
+    __device__ __forceinline__ void load(int i, const Order &o) const { load(i, o, off[i]); }
+
+    // The compiler knows nothing of the LDS that this writes: it is ordered by
+    // the barriers of tiles_ready() alone, and LDS reads may pass it.
+    static __device__ __forceinline__ void load(int i, const Order &o, uint32_t at) {
         // The descriptor is the same for all of them: the first waits for it.
         if (i == 0)
             asm volatile("s_mov_b32 m0, %0\n\t"
                          "s_nop 4\n\t"
                          "buffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
-                         : "s"(to), "v"(at), "s"(rsrc)
-                         : "memory");
+                         : "s"(o.to), "v"(at), "s"(o.rsrc));
         else
             asm volatile("s_mov_b32 m0, %0\n\t"
                          "s_nop 0\n\t"
                          "buffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
-                         : "s"(to + i * kWaves * 1024), "v"(at), "s"(rsrc)
-                         : "memory");
+                         : "s"(o.to + i * kWaves * 1024), "v"(at), "s"(o.rsrc));
+    }
+
+    __device__ __forceinline__ void ask(const char *head, int64_t tok_stride, int dim, int row0,
+                                        int n_rows, int wave, uint32_t lds) const {
+        const Order o = order(head, tok_stride, dim, row0, n_rows, wave, lds);
+        if (o.rows == kTile) {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) load(i, o);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                load(i, o, offset(i, tok_stride, dim, wave, o.rows));
+        }
     }
 };
 
