@@ -14,9 +14,11 @@ point raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 from pathlib import Path
 
 import torch
+from torch.autograd.function import once_differentiable
 
 _HERE = Path(__file__).resolve().parent
 LIB_PATH = _HERE / "libmgauss.so"
@@ -212,6 +214,18 @@ def launch(fn, index: int, *args) -> None:
         rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
         if rc != 0:
             check(rc)
+
+
+def differentiable_once(fn):
+    """torch's once_differentiable for an autograd function's backward, at no cost
+    where no graph of the backward pass is being made (the usual case)."""
+    checked = once_differentiable(fn)
+
+    @functools.wraps(fn)
+    def backward(ctx, *grads):
+        return (checked if torch.is_grad_enabled() else fn)(ctx, *grads)
+
+    return backward
 
 
 def type_code(t: torch.Tensor, what: str) -> int:

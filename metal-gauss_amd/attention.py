@@ -8,7 +8,6 @@ that predicts or refines splats, next to ``layer_norm`` and ``rotary``.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -61,7 +60,7 @@ class _Attention(torch.autograd.Function):
         return out
 
     @staticmethod
-    @once_differentiable
+    @_lib.differentiable_once
     def backward(ctx, dout):
         q, k, v, q_offsets, k_offsets, out, rest, lse = ctx.saved_tensors
         lib = _lib.load()

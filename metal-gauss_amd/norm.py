@@ -7,7 +7,6 @@ that predicts or refines splats, next to ``rotary`` and ``attention``.
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -70,36 +69,35 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_lib.differentiable_once
     def backward(ctx, dy):
         rows, w, stats = ctx.saved_tensors
         lib = _lib.load()
         n, width = rows.shape
-        dev = rows.device
+        dtype, dev, index = rows.dtype, rows.device, rows.get_device()
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        if dy.dtype != rows.dtype:
-            dy = dy.to(rows.dtype)
+        if dy.dtype != dtype:
+            dy = dy.to(dtype)
         dy, dy_stride = _rows(dy)
-        dx = torch.empty(ctx.x_shape, dtype=rows.dtype, device=dev) if need_x else None
+        code = _lib.TYPE_CODES[dtype]
         wtype = w.dtype if w is not None else ctx.has_bias
+        dx = torch.empty(ctx.x_shape, dtype=dtype, device=dev) if need_x else None
         make = torch.zeros if n == 0 else torch.empty
         dw = make(width, dtype=wtype, device=dev) if need_w else None
         db = make(width, dtype=wtype, device=dev) if need_b else None
         if n == 0:
             return dx, dw, db, None
-        ws = None
+        ws, size = None, 0
         if need_w or need_b:
-            ws = torch.empty(lib.mg_layer_norm_backward_workspace_bytes(n, width),
-                             dtype=torch.uint8, device=dev)
-        code = _lib.TYPE_CODES[rows.dtype]
+            size = lib.mg_layer_norm_backward_workspace_bytes(n, width)
+            ws = torch.empty(size, dtype=torch.uint8, device=dev)
         mean = stats.data_ptr()
-        _lib.launch(lib.mg_layer_norm_backward, rows.get_device(), n, width, code, rows.data_ptr(),
+        _lib.launch(lib.mg_layer_norm_backward, index, n, width, code, rows.data_ptr(),
                     rows.stride(0), dy.data_ptr(), dy_stride,
                     code if wtype is None else _lib.TYPE_CODES[wtype],
                     None if w is None else w.data_ptr(), mean, mean + 4 * n,
-                    None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
-                    None if db is None else db.data_ptr(), None if ws is None else ws.data_ptr(),
-                    0 if ws is None else ws.numel())
+                    dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,
+                    db.data_ptr() if need_b else None, ws.data_ptr() if size else None, size)
         return dx, dw, db, None
 
 

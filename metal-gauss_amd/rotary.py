@@ -9,7 +9,6 @@ from __future__ import annotations
 import math
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -86,7 +85,7 @@ class _Rotary(torch.autograd.Function):
         return _turn(q, k, positions, frequencies, layout, False)
 
     @staticmethod
-    @once_differentiable
+    @_lib.differentiable_once
     def backward(ctx, dq, dk):
         positions, frequencies = ctx.saved_tensors
         dtype = ctx.dtype

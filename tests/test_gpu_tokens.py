@@ -635,3 +635,14 @@ def test_refusals(dev):
     for kind, text, call in bad:
         with pytest.raises(kind, match=text):
             call()
+
+
+def test_second_derivatives_are_refused(dev):
+    """A graph of the backward pass can be made; going through it is refused, not
+    answered with zeros."""
+    from metal_gauss_amd import layer_norm
+
+    x = torch.randn(3, 8, generator=gen("twice")).to(dev).requires_grad_(True)
+    dx, = torch.autograd.grad(layer_norm(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
