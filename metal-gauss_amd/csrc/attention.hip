@@ -15,6 +15,11 @@
 // lane's own registers (and its partner's, 32 lanes on), and the scores are
 // already where the product O^T = V^T P^T wants them.
 //
+// With 128 columns a tile's products take as long as its softmax, with 64 the
+// softmax (exponentials) is the bound; two to four waves a SIMD take turns at
+// both. 16320 tokens, causal, 16 heads on 4 of 128: 950 to 1050 us (1150 to 1040
+// TFLOP/s, as the GPU's clock holds); 10000 tokens, 16 heads of 64: 440 us (930).
+//
 // The running maximum lags: the accumulators are rescaled only when a score
 // passes the maximum they go by by more than 2^8, which leaves every sum exact
 // to its 24 bits and skips nearly all rescaling.
@@ -28,7 +33,9 @@ constexpr float kMaxLag = 8.f;                   // powers of 2
 // keys that all four read. Narrow, where a sequence's rows would leave most of
 // that empty (single tokens): 32 rows by one wave, tiles of 32 keys; memory
 // bounds it, and ten waves (64 columns) or five (128) of a CU each have a
-// tile's loads under way.
+// tile's loads under way. 16 tokens of 16 heads on 4 of 64 over 75000 keys: 16 us
+// and 6.4 to join (tiles of 64 keys: 19, half as many waves), 75 MB of keys and
+// values at 7 TB/s once the loop runs.
 constexpr int kWideWaves = 4, kNarrowWaves = 1;
 template <int kWaves>
 constexpr int kKeyTile = kWaves == kNarrowWaves ? 32 : kTileRows;

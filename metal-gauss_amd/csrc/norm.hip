@@ -10,14 +10,20 @@
 // from zero keeps its variance's digits), and written once. All arithmetic is
 // in float32 whatever the type of x; a row's mean and s are kept as float32 for
 // the backward pass.
+//
+// 65280 rows of 1024 bfloat16, float32 weights: forward 45 us (5.9 TB/s), backward
+// 66 (6.1 TB/s) and 4 to join the weights' gradients; 64 rows of 256 float32: 3 us,
+// the launch.
 #include "mg_types.h"
 
 namespace mg {
 
 // A row is held by kWaves waves, C accesses of V elements a thread: thread t
 // has elements (t + i * 64 kWaves) V .. + V - 1 for i < C. Rows longer than the
-// widest form are read once per pass instead (norm_loop_*).
-//
+// widest form are read once per pass instead (norm_loop_*). A workgroup keeps the
+// weights in registers over all its rows (from memory for each row they would be
+// twice a bfloat16 row's own bytes).
+
 // Sum over the threads that hold a row, in all of them. `slot` alternates so
 // that one barrier a reduction suffices: a slot is written again only after
 // the barrier of the reduction between.

@@ -13,7 +13,9 @@
 // pair and shared by all heads through LDS. What is left is memory: queries and
 // keys are read once and written once, in one launch. A thread asks for all its
 // elements before it forms its cosines, whose chain (position, float64 product,
-// polynomial) is as long as a trip to memory.
+// polynomial) is as long as a trip to memory: 10000 tokens of 32 heads of 64
+// bfloat16 16 us (5.1 TB/s; 23 us with the cosines first), 32640 of 20 heads of
+// 128 float32, a quarter of them elsewhere in their rows, 125 us (5.3 TB/s).
 #include "mg_types.h"
 
 namespace mg {
