@@ -84,12 +84,13 @@ class _Attention(torch.autograd.Function):
         return dq, dk, dv, None, None, None, None
 
 
-def _check_offsets(off, what, q):
-    if off.dim() != 1 or off.numel() < 2:
+def _check_offsets(off, what, index):
+    if off.dim() != 1 or off.shape[0] < 2:
         raise ValueError(f"{what} must be (sequences + 1,), got {tuple(off.shape)}")
-    _lib.dev_tensor(off, what, torch.int32)
-    if off.get_device() != q.get_device():
-        raise RuntimeError(f"{what} must be on {q.device}, got device '{off.device}'")
+    if not off.is_cuda or off.dtype != torch.int32 or not off.is_contiguous():
+        _lib.dev_tensor(off, what, torch.int32)
+    if off.get_device() != index:
+        raise RuntimeError(f"{what} must be on GPU {index}, got device '{off.device}'")
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
@@ -119,32 +120,32 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     its product with v. Differentiable in q, k and v, with the same bits from
     call to call.
     """
+    dtype, dim, index = q.dtype, q.shape[-1] if q.dim() else 0, q.get_device()
     for t, what in ((q, "q"), (k, "k"), (v, "v")):
         if _lib.type_code(t, what) == 0:
             raise RuntimeError(f"{what} must be bfloat16 or float16, got {t.dtype}")
         if t.dim() != 3:
             raise ValueError(f"{what} must be (tokens, heads, dim), got {tuple(t.shape)}")
-        if (t.dtype != q.dtype or t.get_device() != q.get_device() or
-                t.shape[2] != q.shape[2]):
+        if t.dtype != dtype or t.shape[2] != dim or t.get_device() != index:
             raise ValueError(f"{what} must match q's type, device and head dimension; got "
                              f"{t.dtype} {tuple(t.shape)} on {t.device}")
     if k.shape != v.shape:
         raise ValueError(f"k is {tuple(k.shape)} and v {tuple(v.shape)}; one shape is needed")
     if q_offsets is not None:
-        _check_offsets(q_offsets, "q_offsets", q)
+        _check_offsets(q_offsets, "q_offsets", index)
         if k_offsets is None:
             if k.shape[0] != q.shape[0]:
                 raise ValueError(f"k_offsets is needed: {q.shape[0]} query tokens and "
                                  f"{k.shape[0]} key tokens")
             k_offsets = q_offsets
-    if k_offsets is not None:
+    if k_offsets is not None and k_offsets is not q_offsets:
         if q_offsets is None:
             raise ValueError("k_offsets needs q_offsets")
-        _check_offsets(k_offsets, "k_offsets", q)
-        if k_offsets.shape != q_offsets.shape:
+        _check_offsets(k_offsets, "k_offsets", index)
+        if k_offsets.shape[0] != q_offsets.shape[0]:
             raise ValueError(f"q_offsets is {tuple(q_offsets.shape)} and k_offsets "
                              f"{tuple(k_offsets.shape)}; one number of sequences is needed")
-    scale = q.shape[2] ** -0.5 if scale is None else float(scale)
+    scale = dim ** -0.5 if scale is None else float(scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
         return _Attention.apply(q, k, v, q_offsets, k_offsets, bool(causal), scale)
     return _forward(q, k, v, q_offsets, k_offsets, bool(causal), scale, False)[0]

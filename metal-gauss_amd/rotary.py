@@ -131,8 +131,9 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
                          f"{tuple(positions.shape)}")
     if not positions.is_cuda or positions.get_device() != index:
         raise RuntimeError(f"positions must be on {q.device}, got device '{positions.device}'")
-    _lib.dev_tensor(frequencies, "frequencies", torch.float64)
-    if frequencies.get_device() != index:
+    if frequencies.dtype != torch.float64 or not frequencies.is_contiguous():
+        _lib.dev_tensor(frequencies, "frequencies", torch.float64)
+    if not frequencies.is_cuda or frequencies.get_device() != index:
         raise RuntimeError(f"frequencies must be on {q.device}, got device "
                            f"'{frequencies.device}'")
     if not positions.is_contiguous():

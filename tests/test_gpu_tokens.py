@@ -378,6 +378,23 @@ def test_attention_long_memory_of_few_rows(dev):
     check_attention(dev, q, k, v, do, q_lens, k_lens, "f16", True)
 
 
+@pytest.mark.parametrize("seed", range(8))
+def test_attention_random_packs(dev, seed):
+    """Every tile of every sequence is given out once, in whatever order: up to 80
+    sequences (62 are ordered by length, more are not) of any two lengths."""
+    rng = np.random.default_rng(100 + seed)
+    n = int((3, 9, 30, 61, 62, 63, 64, 80)[seed])
+    most = 900 if n < 10 else 150
+    q_lens = [int(x) for x in rng.integers(0, most, n)]
+    k_lens = [int(x) for x in rng.integers(0, most, n)]
+    if seed % 2:
+        k_lens = list(q_lens)
+    heads, kv, dim = ((4, 2, 64), (2, 2, 128), (3, 1, 32), (2, 1, 64))[seed % 4]
+    ty = ("bf16", "f16")[seed // 4]
+    q, k, v, do = attn_inputs(("packs", seed), sum(q_lens), sum(k_lens), heads, kv, dim, ty)
+    check_attention(dev, q, k, v, do, q_lens, k_lens, ty, bool(seed % 3))
+
+
 def test_attention_one_sequence_without_offsets(dev):
     from metal_gauss_amd import attention
 
