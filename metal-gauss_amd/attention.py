@@ -62,7 +62,11 @@ class _Attention(torch.autograd.Function):
     @staticmethod
     @_lib.differentiable_once
     def backward(ctx, dout):
-        q, k, v, q_offsets, k_offsets, out, rest, lse = ctx.saved_tensors
+        # Hooks on saved tensors may give them back in another layout.
+        q, k, v, *others = ctx.saved_tensors
+        q_offsets, k_offsets, out, rest, lse = (
+            None if t is None else t.contiguous() for t in others)
+        (q, q_at), (k, k_at), (v, v_at) = _rows(q), _rows(k), _rows(v)
         lib = _lib.load()
         Tq, Hq, D = q.shape
         Tk, Hk = k.shape[0], k.shape[1]
@@ -75,7 +79,7 @@ class _Attention(torch.autograd.Function):
         need = lib.mg_attention_backward_workspace_bytes(Tq, Tk, Hq, Hk, D, n)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
         _lib.launch(lib.mg_attention_backward, q.get_device(), _lib.TYPE_CODES[q.dtype], Tq, Tk,
-                    Hq, Hk, D, *_rows(q)[1], *_rows(k)[1], *_rows(v)[1],
+                    Hq, Hk, D, *q_at, *k_at, *v_at,
                     None if q_offsets is None else q_offsets.data_ptr(),
                     None if k_offsets is None else k_offsets.data_ptr(), n, ctx.causal,
                     ctx.scale, out.data_ptr(), rest.data_ptr(), lse.data_ptr(), *dout_at, dq.data_ptr(),

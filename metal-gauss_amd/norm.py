@@ -71,7 +71,12 @@ class _LayerNorm(torch.autograd.Function):
     @staticmethod
     @_lib.differentiable_once
     def backward(ctx, dy):
+        # Hooks on saved tensors may give them back in another layout.
         rows, w, stats = ctx.saved_tensors
+        rows, row_stride = _rows(rows)
+        stats = stats.contiguous()
+        if w is not None:
+            w = w.contiguous()
         lib = _lib.load()
         n, width = rows.shape
         dtype, dev, index = rows.dtype, rows.device, rows.get_device()
@@ -93,7 +98,7 @@ class _LayerNorm(torch.autograd.Function):
             ws = torch.empty(size, dtype=torch.uint8, device=dev)
         mean = stats.data_ptr()
         _lib.launch(lib.mg_layer_norm_backward, index, n, width, code, rows.data_ptr(),
-                    rows.stride(0), dy.data_ptr(), dy_stride,
+                    row_stride, dy.data_ptr(), dy_stride,
                     code if wtype is None else _lib.TYPE_CODES[wtype],
                     None if w is None else w.data_ptr(), mean, mean + 4 * n,
                     dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None,

@@ -87,7 +87,8 @@ class _Rotary(torch.autograd.Function):
     @staticmethod
     @_lib.differentiable_once
     def backward(ctx, dq, dk):
-        positions, frequencies = ctx.saved_tensors
+        # Hooks on saved tensors may give them back in another layout.
+        positions, frequencies = (t.contiguous() for t in ctx.saved_tensors)
         dtype = ctx.dtype
         if dq is None and dk is None:
             return None, None, None, None, None

@@ -607,6 +607,37 @@ def test_attention_of_nothing(dev):
     assert bool((dk == 0).all())
 
 
+def test_saved_tensors_may_come_back_in_another_layout(dev):
+    """Hooks on saved tensors (they offload, or pack) keep values, not strides."""
+    from metal_gauss_amd import attention, layer_norm, rotary, rotary_frequencies
+
+    def spread(t):
+        """t's values with gaps between all elements."""
+        wide = torch.full((*t.shape, 3), 7, dtype=t.dtype, device=t.device)
+        wide[..., 1] = t
+        return wide[..., 1]
+
+    g = gen("hooks")
+    q, k, v = (torch.randn(90, h, 32, generator=g).to(dev, torch.bfloat16).requires_grad_(True)
+               for h in (4, 2, 2))
+    x = torch.randn(9, 40, generator=g).to(dev).requires_grad_(True)
+    w, b = (torch.randn(40, generator=g).to(dev).requires_grad_(True) for _ in range(2))
+    off = torch.tensor([0, 33, 90], dtype=torch.int32, device=dev)
+    pos = torch.arange(90, dtype=torch.int32, device=dev)
+    freq = rotary_frequencies(32, device=dev)
+    calls = [(lambda: attention(q, k, v, off, causal=True), (q, k, v)),
+             (lambda: layer_norm(x, w, b), (x, w, b)),
+             (lambda: torch.cat(rotary(q, k, pos, freq), 1), (q, k))]
+    for call, leaves in calls:
+        y = call()
+        dy = torch.randn(y.shape, generator=g).to(y)
+        want = torch.autograd.grad(y, leaves, dy)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+            y = call()
+        got = torch.autograd.grad(y, leaves, dy)
+        assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
 # ---------------------------------------------------------------- refusals
 
 def test_refusals(dev):
