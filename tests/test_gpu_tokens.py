@@ -685,6 +685,14 @@ def test_refusals(dev):
             call()
 
 
+def test_heads_of_no_elements_are_refused(dev):
+    from metal_gauss_amd import attention
+
+    b = torch.zeros(4, 2, 0, dtype=torch.bfloat16, device=dev)
+    with pytest.raises(RuntimeError, match="multiples of 8"):
+        attention(b, b, b)
+
+
 def test_second_derivatives_are_refused(dev):
     """A graph of the backward pass can be made; going through it is refused, not
     answered with zeros."""
