@@ -256,9 +256,8 @@ __device__ __forceinline__ KeySteps key_steps(const AttnArgs &a, const SeqItem &
     const int from = a.causal ? max(0, first_key - ahead) / kTileRows * kTileRows : 0;
     const int tiles = from < s.q_len ? (s.q_len - from + kTileRows - 1) / kTileRows : 0;
     int runs = (int)(((int64_t)tiles * G + a.split_steps - 1) / a.split_steps);
-    runs = clamp_to(runs, 1, a.splits);
-    const int parts = runs > G ? runs / G : 1;
-    return {from, tiles, parts > 1 ? parts * G : min(runs, G), parts};
+    runs = even_runs(clamp_to(runs, 1, a.splits), G, a.splits);
+    return {from, tiles, runs, runs > G ? runs / G : 1};
 }
 
 template <typename T, int DK>
@@ -474,7 +473,8 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     const int64_t steps = ceil_div(q_tokens, n_seq * kTileRows) * group;
     int64_t splits = kBwdRuns / (tiles > 0 ? tiles : 1);
     if (splits > steps / kBwdRunLeast) splits = steps / kBwdRunLeast;
-    p.splits = (int)(splits < 1 ? 1 : splits > kBwdMostSplits ? kBwdMostSplits : splits);
+    splits = splits < 1 ? 1 : splits > kBwdMostSplits ? kBwdMostSplits : splits;
+    p.splits = even_runs((int)splits, (int)group, (int)kBwdMostSplits);
     p.split_steps = (int)kBwdRunLeast;
     p.largest_at = align256(q_tokens * k_heads * group * 4);
     p.part_at = p.largest_at + 2 * kNormGroups * 4;

@@ -395,6 +395,16 @@ def test_attention_random_packs(dev, seed):
     check_attention(dev, q, k, v, do, q_lens, k_lens, ty, bool(seed % 3))
 
 
+@pytest.mark.parametrize("heads,kv", [(5, 1), (6, 1), (7, 1), (11, 1), (12, 2), (2, 1), (9, 3)])
+def test_attention_gradients_of_shared_heads_in_runs(dev, heads, kv):
+    """The keys' gradients in runs of whole heads, of parts of heads, and of heads
+    that no number of runs divides."""
+    q_lens, k_lens = [700, 40, 300], [650, 300, 1]
+    q, k, v, do = attn_inputs(("runs", heads), 1040, 951, heads, kv, 16, "bf16")
+    for causal in (False, True):
+        check_attention(dev, q, k, v, do, q_lens, k_lens, "bf16", causal)
+
+
 def test_attention_one_sequence_without_offsets(dev):
     from metal_gauss_amd import attention
 

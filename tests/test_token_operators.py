@@ -77,6 +77,16 @@ def test_a_products_rows_are_the_next_ones_operand(tmp_path):
     assert sorted(r for _, _, r in rows) == list(range(32))
 
 
+def test_runs_are_even_where_they_can_be(tmp_path):
+    cases = [(r, g, m) for g in range(1, 20) for m in (1, 4, 8) for r in range(1, m + 1)]
+    rows = _run(tmp_path, "attention_tiles.h", "".join(
+        f'std::printf("%d\\n", even_runs({r}, {g}, {m}));' for r, g, m in cases))
+    for (r, g, m), (got,) in zip(cases, rows):
+        assert 1 <= got <= m
+        if got % g and g % got:                      # uneven: no even number was left
+            assert got == r and all(g % n for n in range(r, m + 1))
+
+
 # ------------------------------------------------------------- frequencies
 
 def test_frequencies():
