@@ -48,8 +48,8 @@ struct AttnArgs {
     float *lse;                          // (q_heads, q_tokens), in powers of 2; NULL: not kept
     // Split over the keys: chunks of split_keys, whose {top, sum} and unscaled
     // sums of values are joined afterwards; there is room for `items` of each
-    // key head.
-    int32_t split_keys, items;
+    // key head. longer_chunks: uneven sequences may make more (chunk_keys).
+    int32_t split_keys, items, longer_chunks;
     float2 *part_stats;
     float *part_o;
     // Backward.

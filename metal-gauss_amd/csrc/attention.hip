@@ -134,9 +134,34 @@ __device__ __forceinline__ void store_row_result(const AttnArgs &a, int token, i
             sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
+// Keys of a chunk: split_keys, doubled until the chunks of all sequences' tiles
+// find room, as chunks of whole sequences do. Every wave of every kernel comes to
+// the same.
+template <int kRows>
+__device__ __forceinline__ int chunk_keys(const AttnArgs &a) {
+    int keys = a.split_keys;
+    if (!a.longer_chunks) return keys;
+    for (;; keys *= 2) {
+        int items = 0;
+        for (int s0 = 0; s0 < a.n_seq + 2; s0 += 64) {
+            const int s = s0 + lane_id();
+            int n = 0;
+            if (s < a.n_seq + 2) {
+                int lo, q_len, k_len;
+                seq_bounds(a.q_off, a.n_seq, a.q_tokens, s, lo, q_len);
+                seq_bounds(a.k_off, a.n_seq, a.k_tokens, s, lo, k_len);
+                if (s == 0 || s > a.n_seq) k_len = 0;
+                n = (q_len * a.group + kRows - 1) / kRows * max(1, (k_len + keys - 1) / keys);
+            }
+            items += __builtin_amdgcn_readlane(wave_inclusive_sum(n), 63);
+        }
+        if (items <= a.items || keys >= a.k_tokens) return keys;
+    }
+}
+
 // One work item: false if there is none of this number.
 template <typename T, int DK, int kWaves, bool kSplit>
-__device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
+__device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work, int split_keys) {
     constexpr int kRows = 32 * kWaves, kSteps = DK / 16, kBlocks = DK / 32;
     constexpr bool kInterleave = kWaves == kWideWaves;
     constexpr int kTile = kKeyTile<kWaves>, kParts = kTile / 32;
@@ -150,7 +175,7 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     const int kh = work % a.k_heads, item = work / a.k_heads, G = a.group;
     const auto tiles_of = [&](int ql, int) { return (ql * G + kRows - 1) / kRows; };
     const auto chunks_of = [&](int, int kl) {
-        return kSplit ? max(1, (kl + a.split_keys - 1) / a.split_keys) : 1;
+        return kSplit ? max(1, (kl + split_keys - 1) / split_keys) : 1;
     };
     SeqItem s;
     int tile, chunk = 0;
@@ -181,8 +206,8 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     const int see_last = keys_seen(s, min((row0 + 31) / G, s.q_len - 1), a.causal);
     int k_from = 0, k_to = keys_seen(s, last_token, a.causal);
     if (kSplit) {
-        k_from = min(chunk * a.split_keys, k_to);
-        k_to = min(k_from + a.split_keys, k_to);
+        k_from = min(chunk * split_keys, k_to);
+        k_to = min(k_from + split_keys, k_to);
     }
 
     vec8<T> q[kSteps];
@@ -341,9 +366,10 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
 template <typename T, int DK, int kWaves, bool kSplit>
 __global__ __launch_bounds__(64 * kWaves, kWaves == 1 ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
     if constexpr (!kSplit) {
-        attn_fwd_item<T, DK, kWaves, kSplit>(a, blockIdx.x);
+        attn_fwd_item<T, DK, kWaves, kSplit>(a, blockIdx.x, 0);
     } else {
-        for (int work = blockIdx.x; attn_fwd_item<T, DK, kWaves, kSplit>(a, work);
+        const int keys = chunk_keys<32 * kWaves>(a);
+        for (int work = blockIdx.x; attn_fwd_item<T, DK, kWaves, kSplit>(a, work, keys);
              work += gridDim.x)
             tiles_ready();
     }
@@ -361,7 +387,8 @@ __global__ __launch_bounds__(64 * kWideWaves) void attn_join_tile_kernel(AttnArg
     const int wave = uniform(threadIdx.x / 64);
     const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
     const auto tiles_of = [&](int ql, int) { return (ql * G + kRows - 1) / kRows; };
-    const auto chunks_of = [&](int kl) { return max(1, (kl + a.split_keys - 1) / a.split_keys); };
+    const int keys = chunk_keys<kRows>(a);
+    const auto chunks_of = [&](int kl) { return max(1, (kl + keys - 1) / keys); };
     const SeqItem s = find_item<false>(
         a, item, tiles_of, [&](int ql, int kl) { return tiles_of(ql, kl) * chunks_of(kl); });
     if (!s.found) return;
@@ -410,7 +437,8 @@ __global__ __launch_bounds__(256) void attn_join_row_kernel(AttnArgs a) {
     if (at_token >= a.q_tokens) return;
     const int kh = head / G, first = kJoin > 1 ? wave : 0;
     const auto tiles_of = [&](int ql) { return (ql * G + kRows - 1) / kRows; };
-    const auto chunks_of = [&](int kl) { return max(1, (kl + a.split_keys - 1) / a.split_keys); };
+    const int keys = chunk_keys<kRows>(a);
+    const auto chunks_of = [&](int kl) { return max(1, (kl + keys - 1) / keys); };
     const SeqItem s = find_item<false>(
         a, at_token, [](int ql, int) { return ql; },
         [&](int ql, int kl) { return tiles_of(ql) * chunks_of(kl); });
@@ -520,6 +548,7 @@ struct FwdPlan {
     int waves;
     int split_keys;             // 0: whole rows
     int64_t tiles, items;       // a key head's, at most
+    bool longer_chunks;         // see chunk_keys
     int64_t stats_bytes, bytes; // of partial results
 };
 
@@ -548,8 +577,13 @@ static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int gro
         if (keys < kChunkLeast) keys = kChunkLeast;
         p.split_keys = (int)keys;
         // Sum of tiles * (1 + keys / chunk) over the sequences, no sequence
-        // having more tiles than all rows make.
-        p.items += (rows / tile_rows + 1) * (k_tokens / keys);
+        // having more tiles than all rows make. Many sequences are alike enough
+        // for four times what equal ones make; room for any would be gigabytes
+        // (384 tokens of 32 heads on one of 128, 1000 keys each: 4.8, now 0.11).
+        const int64_t any = (rows / tile_rows + 1) * (k_tokens / keys);
+        const int64_t equal = ceil_div(rows / tile_rows + n_seq, n_seq) * (k_tokens / keys);
+        p.longer_chunks = any > 4 * equal;
+        p.items += p.longer_chunks ? 4 * equal : any;
         const int dk = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
         const int64_t part_rows = p.items * k_heads * tile_rows;
         p.stats_bytes = align256(part_rows * 8);
@@ -604,7 +638,7 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
     MG_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes),
                "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
                (long long)p.bytes);
-    a.split_keys = p.split_keys, a.items = (int32_t)p.items;
+    a.split_keys = p.split_keys, a.items = (int32_t)p.items, a.longer_chunks = p.longer_chunks;
     a.part_stats = static_cast<float2 *>(workspace);
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.stats_bytes);
     hipStream_t st = as_stream(stream);

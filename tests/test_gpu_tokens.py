@@ -378,6 +378,22 @@ def test_attention_long_memory_of_few_rows(dev):
     check_attention(dev, q, k, v, do, q_lens, k_lens, "f16", True)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_chunks_of_very_unequal_sequences(dev, causal):
+    """One of many sequences holds nearly all queries and keys: its chunks of the
+    length that suits the average find no room, and grow."""
+    q_lens, k_lens = [1] * 39 + [250], [3 + i for i in range(39)] + [36001]   # narrow items
+    q, k, v, do = attn_inputs(("unequal", 1), sum(q_lens), sum(k_lens), 8, 1, 64, "bf16")
+    check_attention(dev, q, k, v, do, q_lens, k_lens, "bf16", causal, grad=False)
+    q_lens = [700] + [1] * 69                     # narrow, over 64 sequences
+    k_lens = [60001] + [5] * 69
+    q, k, v, do = attn_inputs(("unequal", 2), sum(q_lens), sum(k_lens), 1, 1, 40, "f16")
+    check_attention(dev, q, k, v, do, q_lens, k_lens, "f16", causal, grad=False)
+    q_lens, k_lens = [5] * 6 + [2900] + [3] * 5, [7] * 6 + [11900] + [0] * 5   # wide items
+    q, k, v, do = attn_inputs(("unequal", 3), sum(q_lens), sum(k_lens), 2, 2, 128, "f16")
+    check_attention(dev, q, k, v, do, q_lens, k_lens, "f16", causal, grad=False)
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_attention_random_packs(dev, seed):
     """Every tile of every sequence is given out once, in whatever order: up to 80

@@ -185,6 +185,19 @@ def test_workspace_queries():
     assert lib.mg_layer_norm_backward_workspace_bytes(0, 100) == 0
 
 
+@pytest.mark.parametrize("streams,heads,kv,keys", [(384, 32, 1, 1000), (128, 32, 1, 4096),
+                                                   (64, 32, 8, 4096), (300, 8, 1, 800)])
+def test_workspace_of_single_tokens_over_many_memories(streams, heads, kv, keys):
+    """Partial results of at most 1536 items at once and two more chunks a sequence
+    and head, of 32 rows of 128 columns: eight times that is the most asked for."""
+    from metal_gauss_amd import _lib
+
+    lib = _lib.open_library()
+    need = lib.mg_attention_forward_workspace_bytes(streams, streams * keys, heads, kv, 128,
+                                                    streams)
+    assert 0 < need <= 8 * (1536 + 2 * streams * kv) * 32 * 128 * 4
+
+
 # ---------------------------------------------------- the oracle's own checks
 
 def _difference(f, x, d):
