@@ -46,10 +46,10 @@ struct AttnArgs {
     void *out;                           // (q_tokens, q_heads, dim)
     void *out_rest;                      // what rounding took from out, or NULL
     float *lse;                          // (q_heads, q_tokens), in powers of 2; NULL: not kept
-    // Split over the keys: chunks of split_keys, whose {top, sum} and unscaled
-    // sums of values are joined afterwards; there is room for `items` of each
-    // key head. longer_chunks: uneven sequences may make more (chunk_keys).
-    int32_t split_keys, items, longer_chunks;
+    // Split over the keys: chunks of split_keys (more with over chunk_tiles tiles:
+    // chunks_of), whose {top, sum} and unscaled sums of values are joined
+    // afterwards; there is room for `items` of each key head.
+    int32_t split_keys, chunk_tiles, items;
     float2 *part_stats;
     float *part_o;
     // Backward.

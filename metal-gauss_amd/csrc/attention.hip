@@ -134,34 +134,21 @@ __device__ __forceinline__ void store_row_result(const AttnArgs &a, int token, i
             sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
 }
 
-// Keys of a chunk: split_keys, doubled until the chunks of all sequences' tiles
-// find room, as chunks of whole sequences do. Every wave of every kernel comes to
-// the same.
-template <int kRows>
-__device__ __forceinline__ int chunk_keys(const AttnArgs &a) {
-    int keys = a.split_keys;
-    if (!a.longer_chunks) return keys;
-    for (;; keys *= 2) {
-        int items = 0;
-        for (int s0 = 0; s0 < a.n_seq + 2; s0 += 64) {
-            const int s = s0 + lane_id();
-            int n = 0;
-            if (s < a.n_seq + 2) {
-                int lo, q_len, k_len;
-                seq_bounds(a.q_off, a.n_seq, a.q_tokens, s, lo, q_len);
-                seq_bounds(a.k_off, a.n_seq, a.k_tokens, s, lo, k_len);
-                if (s == 0 || s > a.n_seq) k_len = 0;
-                n = (q_len * a.group + kRows - 1) / kRows * max(1, (k_len + keys - 1) / keys);
-            }
-            items += __builtin_amdgcn_readlane(wave_inclusive_sum(n), 63);
-        }
-        if (items <= a.items || keys >= a.k_tokens) return keys;
-    }
+// Keys of the chunks of a sequence of so many tiles. One of many more tiles than
+// most have longer chunks by as much, so that tiles * (keys / chunk) adds up to
+// chunk_tiles * (all keys / split_keys) at most.
+__device__ __forceinline__ int chunk_keys(const AttnArgs &a, int tiles) {
+    if (tiles <= a.chunk_tiles) return a.split_keys;
+    return a.split_keys * ((tiles + a.chunk_tiles - 1) / a.chunk_tiles);
+}
+__device__ __forceinline__ int chunks_of(const AttnArgs &a, int tiles, int keys) {
+    const int each = chunk_keys(a, tiles);
+    return max(1, (keys + each - 1) / each);
 }
 
 // One work item: false if there is none of this number.
 template <typename T, int DK, int kWaves, bool kSplit>
-__device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work, int split_keys) {
+__device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     constexpr int kRows = 32 * kWaves, kSteps = DK / 16, kBlocks = DK / 32;
     constexpr bool kInterleave = kWaves == kWideWaves;
     constexpr int kTile = kKeyTile<kWaves>, kParts = kTile / 32;
@@ -174,18 +161,20 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work, int s
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kh = work % a.k_heads, item = work / a.k_heads, G = a.group;
     const auto tiles_of = [&](int ql, int) { return (ql * G + kRows - 1) / kRows; };
-    const auto chunks_of = [&](int, int kl) {
-        return kSplit ? max(1, (kl + split_keys - 1) / split_keys) : 1;
-    };
     SeqItem s;
-    int tile, chunk = 0;
+    int tile, chunk = 0, split_keys = 0;
     if constexpr (kSplit) {
         s = find_item<false>(
-            a, item, [&](int ql, int kl) { return tiles_of(ql, kl) * chunks_of(ql, kl); },
+            a, item,
+            [&](int ql, int kl) {
+                const int tiles = tiles_of(ql, kl);
+                return tiles * chunks_of(a, tiles, kl);
+            },
             [](int, int) { return 0; });
         if (!s.found || item >= a.items) return false;
-        const int chunks = chunks_of(s.q_len, s.k_len);
-        tile = tiles_of(s.q_len, 0) - 1 - s.within / chunks;
+        const int tiles = tiles_of(s.q_len, 0), chunks = chunks_of(a, tiles, s.k_len);
+        split_keys = chunk_keys(a, tiles);
+        tile = tiles - 1 - s.within / chunks;
         chunk = s.within % chunks;
     } else {
         s = find_longest<false>(a, item, kRows);
@@ -366,10 +355,9 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work, int s
 template <typename T, int DK, int kWaves, bool kSplit>
 __global__ __launch_bounds__(64 * kWaves, kWaves == 1 ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
     if constexpr (!kSplit) {
-        attn_fwd_item<T, DK, kWaves, kSplit>(a, blockIdx.x, 0);
+        attn_fwd_item<T, DK, kWaves, kSplit>(a, blockIdx.x);
     } else {
-        const int keys = chunk_keys<32 * kWaves>(a);
-        for (int work = blockIdx.x; attn_fwd_item<T, DK, kWaves, kSplit>(a, work, keys);
+        for (int work = blockIdx.x; attn_fwd_item<T, DK, kWaves, kSplit>(a, work);
              work += gridDim.x)
             tiles_ready();
     }
@@ -387,15 +375,16 @@ __global__ __launch_bounds__(64 * kWideWaves) void attn_join_tile_kernel(AttnArg
     const int wave = uniform(threadIdx.x / 64);
     const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
     const auto tiles_of = [&](int ql, int) { return (ql * G + kRows - 1) / kRows; };
-    const int keys = chunk_keys<kRows>(a);
-    const auto chunks_of = [&](int kl) { return max(1, (kl + keys - 1) / keys); };
-    const SeqItem s = find_item<false>(
-        a, item, tiles_of, [&](int ql, int kl) { return tiles_of(ql, kl) * chunks_of(kl); });
+    const SeqItem s = find_item<false>(a, item, tiles_of, [&](int ql, int kl) {
+        const int tiles = tiles_of(ql, kl);
+        return tiles * chunks_of(a, tiles, kl);
+    });
     if (!s.found) return;
-    const int chunks = chunks_of(s.k_len), item0 = s.before + s.within * chunks;
+    const int tiles = tiles_of(s.q_len, 0), chunks = chunks_of(a, tiles, s.k_len);
+    const int item0 = s.before + s.within * chunks;
     // Offsets that fall again could make more items than there are.
     if (item0 + chunks > a.items) return;
-    const int row = (tiles_of(s.q_len, 0) - 1 - s.within) * kRows + wave * 32 + lane % 32;
+    const int row = (tiles - 1 - s.within) * kRows + wave * 32 + lane % 32;
     const int token = row / G, head = kh * G + row % G;
     if (token >= s.q_len) return;
     const int64_t work0 = (int64_t)item0 * a.k_heads + kh;
@@ -437,14 +426,15 @@ __global__ __launch_bounds__(256) void attn_join_row_kernel(AttnArgs a) {
     if (at_token >= a.q_tokens) return;
     const int kh = head / G, first = kJoin > 1 ? wave : 0;
     const auto tiles_of = [&](int ql) { return (ql * G + kRows - 1) / kRows; };
-    const int keys = chunk_keys<kRows>(a);
-    const auto chunks_of = [&](int kl) { return max(1, (kl + keys - 1) / keys); };
     const SeqItem s = find_item<false>(
         a, at_token, [](int ql, int) { return ql; },
-        [&](int ql, int kl) { return tiles_of(ql) * chunks_of(kl); });
+        [&](int ql, int kl) {
+            const int tiles = tiles_of(ql);
+            return tiles * chunks_of(a, tiles, kl);
+        });
     if (!s.found) return;
-    const int row = s.within * G + head % G, tile = row / kRows, chunks = chunks_of(s.k_len);
-    const int item0 = s.before + (tiles_of(s.q_len) - 1 - tile) * chunks;
+    const int row = s.within * G + head % G, tile = row / kRows, tiles = tiles_of(s.q_len);
+    const int chunks = chunks_of(a, tiles, s.k_len), item0 = s.before + (tiles - 1 - tile) * chunks;
     // Offsets that fall again could make more items than there are.
     if (item0 + chunks > a.items) return;
     const auto slot = [&](int c) {
@@ -547,8 +537,8 @@ int32_t attn_check(const char *who, const AttnArgs &a, int32_t dtype) {
 struct FwdPlan {
     int waves;
     int split_keys;             // 0: whole rows
+    int64_t chunk_tiles;        // see chunk_keys
     int64_t tiles, items;       // a key head's, at most
-    bool longer_chunks;         // see chunk_keys
     int64_t stats_bytes, bytes; // of partial results
 };
 
@@ -576,14 +566,15 @@ static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int gro
         int64_t keys = ceil_div(ceil_div(mean_keys * likely, slots), tile) * tile;
         if (keys < kChunkLeast) keys = kChunkLeast;
         p.split_keys = (int)keys;
-        // Sum of tiles * (1 + keys / chunk) over the sequences, no sequence
-        // having more tiles than all rows make. Many sequences are alike enough
-        // for four times what equal ones make; room for any would be gigabytes
-        // (384 tokens of 32 heads on one of 128, 1000 keys each: 4.8, now 0.11).
-        const int64_t any = (rows / tile_rows + 1) * (k_tokens / keys);
-        const int64_t equal = ceil_div(rows / tile_rows + n_seq, n_seq) * (k_tokens / keys);
-        p.longer_chunks = any > 4 * equal;
-        p.items += p.longer_chunks ? 4 * equal : any;
+        // Sum of tiles * (1 + keys / chunk) over the sequences. No sequence has
+        // more tiles than all rows make; of many sequences those that have over
+        // four times the average take longer chunks, as room for any would be
+        // gigabytes (384 tokens of 32 heads on one of 128, 1000 keys each: 4.8,
+        // now 0.11).
+        const int64_t most = rows / tile_rows + 1;
+        p.chunk_tiles = 4 * ceil_div(rows / tile_rows + n_seq, n_seq);
+        p.items += most <= p.chunk_tiles ? most * (k_tokens / keys)
+                                         : p.chunk_tiles * k_tokens / keys;
         const int dk = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
         const int64_t part_rows = p.items * k_heads * tile_rows;
         p.stats_bytes = align256(part_rows * 8);
@@ -638,7 +629,8 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
     MG_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes),
                "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
                (long long)p.bytes);
-    a.split_keys = p.split_keys, a.items = (int32_t)p.items, a.longer_chunks = p.longer_chunks;
+    a.split_keys = p.split_keys, a.chunk_tiles = (int32_t)p.chunk_tiles;
+    a.items = (int32_t)p.items;
     a.part_stats = static_cast<float2 *>(workspace);
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.stats_bytes);
     hipStream_t st = as_stream(stream);
