@@ -190,6 +190,10 @@ extern "C" int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q, int64
                "mg_rotary: interleaved pairs need an even head dimension, got %d", dim);
     MG_REQUIRE(axes >= 1 && pairs % axes == 0,
                "mg_rotary: %d frequencies do not divide among %d axes", pairs, axes);
+    // A workgroup's units are numbered in 32 bits.
+    MG_REQUIRE((int64_t)(q_heads + k_heads) * dim <= (int64_t(1) << 30),
+               "mg_rotary: tokens of %d heads of %d elements are too long", q_heads + k_heads,
+               dim);
     if (tokens == 0) return MG_OK;
     MG_REQUIRE(q && q_out && positions && frequencies && (k_heads == 0 || (k && k_out)),
                "mg_rotary: a pointer is NULL");

@@ -185,6 +185,17 @@ def test_workspace_queries():
     assert lib.mg_layer_norm_backward_workspace_bytes(0, 100) == 0
 
 
+def test_rotary_refuses_tokens_of_more_elements_than_are_counted():
+    """Before any launch: 65537 heads of 65536 elements pass 32 bits."""
+    from metal_gauss_amd import _lib
+
+    lib = _lib.open_library()
+    for heads, k_heads in ((65536, 1), (16384, 1), (65536, 65536)):
+        rc = lib.mg_rotary(1, 0, None, 65536, 65536, heads, None, 65536, 65536, k_heads, 65536,
+                           None, 0, 1, None, 32, 0, 0, None, None, None)
+        assert rc == 1 and "too long" in lib.mg_last_error().decode(), lib.mg_last_error()
+
+
 @pytest.mark.parametrize("streams,heads,kv,keys", [(384, 32, 1, 1000), (128, 32, 1, 4096),
                                                    (64, 32, 8, 4096), (300, 8, 1, 800)])
 def test_workspace_of_single_tokens_over_many_memories(streams, heads, kv, keys):
