@@ -378,6 +378,16 @@ def test_attention_long_memory_of_few_rows(dev):
     check_attention(dev, q, k, v, do, q_lens, k_lens, "f16", True)
 
 
+@pytest.mark.parametrize("n", [62, 63, 64, 127, 385, 4094, 4095, 4300])
+def test_attention_of_many_sequences(dev, n):
+    """Sequences found in one step of 64, in several, and in many."""
+    rng = np.random.default_rng(n)
+    q_lens, k_lens = (rng.integers(0, 4, n).tolist() for _ in range(2))
+    q_lens[n // 2], k_lens[n // 2] = 150, 140
+    q, k, v, do = attn_inputs(("sequences", n), sum(q_lens), sum(k_lens), 2, 1, 32, "f16")
+    check_attention(dev, q, k, v, do, q_lens, k_lens, "f16", n % 2 == 1)
+
+
 @pytest.mark.parametrize("causal", [False, True])
 def test_attention_chunks_of_very_unequal_sequences(dev, causal):
     """One of many sequences holds nearly all queries and keys: its chunks of the
