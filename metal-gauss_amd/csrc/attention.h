@@ -54,7 +54,7 @@ struct AttnArgs {
     float *part_o;
     // Backward.
     const float *delta;                  // (q_heads, q_tokens)
-    const float *largest;                // float16: see attention_bwd.hip
+    float *largest_do, *largest_v;       // float16: see attention_bwd.hip
     void *dq, *dk, *dv;
     // Keys' gradients over up to `splits` runs of query tiles, of split_steps at
     // least, each in float32 (part_of).
@@ -69,6 +69,7 @@ struct AttnArgs {
 // are zeros and no row stays unwritten.
 struct SeqItem {
     int q_lo, q_len, k_lo, k_len;
+    int seq;           // 1 .. n; 0 and n + 1: the tokens of no sequence
     int within;        // the item's number within its sequence
     int before;        // sum of the second count over the sequences before
     bool found;
@@ -129,6 +130,7 @@ __device__ __forceinline__ SeqItem find_item(const AttnArgs &a, int item, Count 
         const uint64_t past = ballot(base + upto > item);
         if (past) {
             const int l = __builtin_ctzll(past);
+            r.seq = s0 + l;
             const auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
             r.q_lo = get(q_lo), r.q_len = get(q_len), r.k_lo = get(k_lo), r.k_len = get(k_len);
             r.within = clamp_to(item - (base + get(upto) - get(n)), 0, get(n) - 1);
@@ -209,6 +211,7 @@ __device__ __forceinline__ SeqItem find_longest(const AttnArgs &a, int item, int
     const int rank = item - all(lo + 1), upto = wave_inclusive_sum(here);
     const uint64_t past = ballot(upto > rank);
     const int l = past ? __builtin_ctzll(past) : 0;
+    r.seq = l;
     const auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
     r.q_lo = get(q_lo), r.q_len = get(q_len), r.k_lo = get(k_lo), r.k_len = get(k_len);
     const int nth = get(longer) + rank - (get(upto) - get(here));

@@ -17,8 +17,11 @@
 // float16: p and ds of a long row lie where float16 has few digits or none left
 // (p of 16000 equal keys is 6e-5), so p enters its product 2^15 times as large,
 // and ds by a power of two that takes the largest ds there can be,
-// 2 max|do| max|v|, to about 2^14; the results are scaled back in float32.
-// bfloat16 has float32's range and needs neither.
+// 2 max|do| max|v|, to about 2^14; the results are scaled back in float32. The
+// maxima are those of the item's own sequence and key head (in the queries'
+// gradient, whose sums are a row's own, of the row's do), so that neither a
+// sequence packed with it nor tokens of none take digits from it. bfloat16 has
+// float32's range and needs neither.
 //
 // 8192 tokens, 16 heads of 128: queries 740 us, keys 1015 (1110 and 1080 TFLOP/s);
 // of 64: 454 and 611 (905 and 900). As the forward, both need two waves a SIMD to
@@ -34,29 +37,43 @@ constexpr int kBwdTile = 32 * kBwdWaves;         // rows, or keys, of a work ite
 template <typename T>
 constexpr float kPowerP = sizeof(T) == 2 && std::is_same<T, f16_t>::value ? 15.f : 0.f;
 
-// The largest |row|^2 of do (blockIdx.y 0) and of v (1) that each workgroup finds,
-// to largest[kNormGroups y + x]. A NaN counts as nothing.
-constexpr int kNormGroups = 512;
+// A sequence's tokens in tiles of 64 have a place each in an array of this many:
+// tile t of sequence seq, whose tokens begin at lo, is at lo / 64 + seq + t.
+__host__ __device__ constexpr int64_t norm_places(int64_t tokens, int64_t n_seq) {
+    return tokens / kTileRows + n_seq + 2;
+}
 
+// The largest |row|^2 of a tile's tokens in do (blockIdx.y 0: over the query heads
+// that share the key head) and in v (1). Tokens of no sequence are not looked at.
+// A NaN counts as nothing.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_largest_kernel(AttnArgs a, float *largest) {
+__global__ __launch_bounds__(256) void attn_largest_kernel(AttnArgs a) {
     __shared__ float s_most[4];
-    const AttnTensor &x = blockIdx.y ? a.v : a.dout;
-    const int heads = blockIdx.y ? a.k_heads : a.k_heads * a.group;
-    const int64_t rows = (int64_t)(blockIdx.y ? a.k_tokens : a.q_tokens) * heads;
+    const bool of_v = blockIdx.y != 0;
+    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
+    const auto tiles_of = [&](int ql, int kl) {
+        return ((of_v ? kl : ql) + kTileRows - 1) / kTileRows;
+    };
+    const auto none = [](int, int) { return 0; };
+    const SeqItem s = of_v ? find_item<true>(a, item, tiles_of, none)
+                           : find_item<false>(a, item, tiles_of, none);
+    if (!s.found || s.seq == 0 || s.seq > a.n_seq) return;
+    const AttnTensor &x = of_v ? a.v : a.dout;
+    const int heads = of_v ? 1 : a.group, lo = of_v ? s.k_lo : s.q_lo;
+    const int tokens = min((of_v ? s.k_len : s.q_len) - s.within * kTileRows, kTileRows);
+    const T *from = static_cast<const T *>(x.p) +
+                    (int64_t)(lo + s.within * kTileRows) * x.tok_stride +
+                    (int64_t)(kh * heads) * x.head_stride;
     // 16 lanes a row, eight elements each, four rows asked for at once.
-    const int at = threadIdx.x % 16 * 8;
-    constexpr int64_t kStep = kNormGroups * 16;
+    const int at = threadIdx.x % 16 * 8, rows = tokens * heads;
     float most = 0.f;
-    for (int64_t row = (int64_t)blockIdx.x * 16 + threadIdx.x / 16; row < rows; row += 4 * kStep) {
+    for (int row = threadIdx.x / 16; row < rows; row += 4 * 16) {
         float f[4][8] = {};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int64_t r = row + k * kStep;
-            const int token = (int)(r / heads), head = (int)(r % heads);
+            const int r = row + k * 16, token = r / heads, head = r % heads;
             if (r < rows && at < a.dim)
-                load_vec<T, 8>(static_cast<const T *>(x.p) + token * x.tok_stride +
-                                   head * x.head_stride + at, f[k]);
+                load_vec<T, 8>(from + token * x.tok_stride + head * x.head_stride + at, f[k]);
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -72,28 +89,25 @@ __global__ __launch_bounds__(256) void attn_largest_kernel(AttnArgs a, float *la
     if (lane_id() == 0) s_most[threadIdx.x / 64] = most;
     __syncthreads();
     if (threadIdx.x == 0)
-        largest[kNormGroups * blockIdx.y + blockIdx.x] =
-            fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
+        (of_v ? a.largest_v : a.largest_do)[
+            kh * norm_places(of_v ? a.k_tokens : a.q_tokens, a.n_seq) + lo / kTileRows + s.seq +
+            s.within] = fmaxf(fmaxf(s_most[0], s_most[1]), fmaxf(s_most[2], s_most[3]));
 }
 
-// The power of two that ds is taken by.
-template <typename T>
-__device__ __forceinline__ float ds_power(const float *largest) {
-    if constexpr (kPowerP<T> == 0.f) {
-        return 0.f;
-    } else {
-        float m[2] = {};
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-#pragma unroll
-            for (int i = 0; i < kNormGroups; i += 64)
-                m[y] = fmaxf(m[y], largest[kNormGroups * y + i + lane_id()]);
-            m[y] = wave_max(m[y]);
-        }
-        const float l =
-            13.f - 0.5f * (__builtin_amdgcn_logf(m[0]) + __builtin_amdgcn_logf(m[1]));
-        return l > -100.f && l < 100.f ? floorf(l) : 0.f;
-    }
+// The largest of a sequence, whose `len` tokens of `tokens` begin at lo.
+__device__ __forceinline__ float seq_largest(const AttnArgs &a, const float *largest, int kh,
+                                             int tokens, int seq, int lo, int len) {
+    const float *p = largest + kh * norm_places(tokens, a.n_seq) + lo / kTileRows + seq;
+    float most = 0.f;
+    for (int t = lane_id(); t * kTileRows < len; t += 64) most = fmaxf(most, p[t]);
+    return wave_max(most);
+}
+
+// The power of two that ds is taken by, from the largest |do|^2 and |v|^2 it can
+// be of.
+__device__ __forceinline__ float ds_power(float do_sq, float v_sq) {
+    const float l = 13.f - 0.5f * (__builtin_amdgcn_logf(do_sq) + __builtin_amdgcn_logf(v_sq));
+    return l > -100.f && l < 100.f ? floorf(l) : 0.f;
 }
 
 // ------------------------------------------------------- the queries' gradient
@@ -120,7 +134,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
     const int k_to = sees(min((tile * kBwdTile + kBwdTile - 1) / G, s.q_len - 1));
 
     vec8<T> q[kSteps], dout[kSteps];
-    float lse = INFINITY, delta = 0.f;
+    float lse = INFINITY, delta = 0.f, do_sq = 0.f;
     {
         const T *qr = static_cast<const T *>(a.q.p) + (int64_t)(s.q_lo + token) * a.q.tok_stride +
                       (int64_t)head * a.q.head_stride;
@@ -139,8 +153,11 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
             const vec8<T> out = memory_operand<T>(outr, at, ok);
             const vec8<T> rest = memory_operand<T>(restr, at, ok && a.out_rest);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+            for (int k = 0; k < 8; ++k) {
                 delta = fmaf((float)dout[i][k], (float)out[k] + (float)rest[k], delta);
+                if constexpr (kPowerP<T> != 0.f)
+                    do_sq = fmaf((float)dout[i][k], (float)dout[i][k], do_sq);
+            }
         }
         delta = halves_sum(delta);
         if (row_ok) {
@@ -162,7 +179,10 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
         fill_k.ask(kp, a.k.tok_stride, a.dim, key0, s.k_len, wave, lds_address(s_tile[buf][0]));
         fill_v.ask(vp, a.v.tok_stride, a.dim, key0, s.k_len, wave, lds_address(s_tile[buf][1]));
     };
-    const float power = ds_power<T>(a.largest);
+    float power = 0.f;                   // this lane's row's
+    if constexpr (kPowerP<T> != 0.f)
+        power = ds_power(halves_sum(do_sq), seq_largest(a, a.largest_v, kh, a.k_tokens, s.seq,
+                                                        s.k_lo, s.k_len));
     const float up = __builtin_amdgcn_exp2f(power);
     const float delta_up = delta * up;
 
@@ -320,7 +340,11 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
                            lds_address(reinterpret_cast<const char *>(s_row[buf][wave])));
         }
     };
-    const float power = ds_power<T>(a.largest);
+    float power = 0.f;
+    if constexpr (kPowerP<T> != 0.f)
+        power = ds_power(
+            seq_largest(a, a.largest_do, kh, a.q_tokens, s.seq, s.q_lo, s.q_len),
+            seq_largest(a, a.largest_v, kh, a.k_tokens, s.seq, s.k_lo, s.k_len));
     const float ds_up = __builtin_amdgcn_exp2f(power - kPowerP<T>);
 
     f32x16 dk[kBlocks] = {}, dv[kBlocks] = {};
@@ -477,7 +501,8 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     p.splits = even_runs((int)splits, (int)group, (int)kBwdMostSplits);
     p.split_steps = (int)kBwdRunLeast;
     p.largest_at = align256(q_tokens * k_heads * group * 4);
-    p.part_at = p.largest_at + 2 * kNormGroups * 4;
+    p.part_at = align256(p.largest_at + k_heads * 4 * (norm_places(q_tokens, n_seq) +
+                                                       norm_places(k_tokens, n_seq)));
     p.bytes = p.part_at;
     const int64_t dk = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
     if (p.splits > 1) p.bytes += p.k_items * k_heads * p.splits * 2 * kBwdTile * dk * 4;
@@ -535,8 +560,8 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
                who, (long long)workspace_bytes, (long long)p.bytes);
     char *ws = static_cast<char *>(workspace);
     a.delta = reinterpret_cast<float *>(ws);
-    float *largest = reinterpret_cast<float *>(ws + p.largest_at);
-    a.largest = largest;
+    a.largest_do = reinterpret_cast<float *>(ws + p.largest_at);
+    a.largest_v = a.largest_do + k_heads * norm_places(q_tokens, sequences);
     a.splits = p.splits, a.split_steps = p.split_steps;
     a.part = reinterpret_cast<float *>(ws + p.part_at);
     hipStream_t st = as_stream(stream);
@@ -546,7 +571,8 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
                "%s: too many work items", who);
     if (dtype == MG_F16) {
         TimedScope ts("attention_largest", st);
-        attn_largest_kernel<f16_t><<<dim3(kNormGroups, 2), 256, 0, st>>>(a, largest);
+        const int64_t places = norm_places(q_tokens > k_tokens ? q_tokens : k_tokens, sequences);
+        attn_largest_kernel<f16_t><<<dim3((unsigned)(places * k_heads), 2), 256, 0, st>>>(a);
         MG_LAUNCHED("attn_largest_kernel");
     }
     if (q_tokens > 0) {

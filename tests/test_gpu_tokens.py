@@ -627,6 +627,37 @@ def test_attention_float16_small_gradients(dev):
     check_attention(dev, q, k, v, (do.float() * 1e-3).half(), [64], [3000], "f16", False)
 
 
+@pytest.mark.parametrize("fill", [6e4, float("inf"), float("nan")])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_float16_gradients_without_tokens_of_no_sequence(dev, fill, causal):
+    """The unused ends of the tensors hold anything: the powers of two that float16's
+    ds is taken by come of the sequences' own tokens."""
+    from metal_gauss_amd import attention
+
+    q, k, v, do = (t.to(dev) for t in attn_inputs(("ends",), 300, 3100, 4, 2, 64, "f16"))
+    do *= 1e-3
+    off = [torch.tensor(o, dtype=torch.int32, device=dev) for o in ([20, 90, 220], [10, 80, 3010])]
+    got = []
+    for value in (0.0, fill):
+        for t, a, b in ((q, 20, 220), (k, 10, 3010), (v, 10, 3010), (do, 20, 220)):
+            t[:a], t[b:] = value, value
+        leaves = [t.detach().clone().requires_grad_(True) for t in (q, k, v)]
+        o = attention(*leaves, *off, causal=causal)
+        got.append((o, *torch.autograd.grad(o, leaves, do)))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
+def test_attention_float16_gradients_of_sequences_and_rows_of_unlike_size(dev):
+    """Gradients of 1e-3 packed with others of 1e3, in another sequence and (their own
+    gradients, the queries') in other rows of theirs."""
+    q_lens, k_lens = [64, 70, 33], [3000, 300, 500]
+    q, k, v, do = attn_inputs(("unlike",), 167, 3800, 2, 1, 64, "f16")
+    size = torch.full((167, 1, 1), 1e-3)
+    size[64:134], size[140:150] = 1e3, 1e3
+    check_attention(dev, q, k, v, (do.float() * size).half(), q_lens, k_lens, "f16", False)
+
+
 def test_attention_of_nothing(dev):
     from metal_gauss_amd import attention
 
