@@ -21,13 +21,22 @@
 // TFLOP/s, as the GPU's clock holds); 10000 tokens, 16 heads of 64: 440 us (930).
 //
 // The running maximum lags: the accumulators are rescaled only when a score
-// passes the maximum they go by by more than 2^8, which leaves every sum exact
+// passes the maximum they go by by more than kMaxLag, which leaves every sum exact
 // to its 24 bits and skips nearly all rescaling.
+//
+// float16: p is kept 2^kRise times as large, sum and all, for the product. As they
+// are, keys of less than 2^-14 of the largest would lose digits and those of less
+// than 2^-25 everything, which many of them add up to (16000 keys at 2^-22 beside
+// one whose value is zero: a result 9% off); so it is 2^-25 and 2^-36. Lag and
+// rise together stay below float16's 2^16. bfloat16 has float32's range.
 #include "attention.h"
 
 namespace mg {
 
-constexpr float kMaxLag = 8.f;                   // powers of 2
+template <typename T>                             // powers of 2
+constexpr float kMaxLag = std::is_same<T, f16_t>::value ? 4.f : 8.f;
+template <typename T>
+constexpr float kRise = std::is_same<T, f16_t>::value ? 11.f : 0.f;
 
 // Work items come in two widths. Wide: 128 rows by four waves, tiles of 64
 // keys that all four read. Narrow, where a sequence's rows would leave most of
@@ -224,7 +233,8 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     };
 
     f32x16 o[kBlocks] = {};
-    float top = -INFINITY, sum = 0.f;     // top: in powers of 2, what p goes by
+    // top: in powers of 2, what p goes by: kRise below a maximum seen.
+    float top = -INFINITY, sum = 0.f;
     if constexpr (kWaves == 1)
         not_finite_from = k_to;
     else if (threadIdx.x == 0)
@@ -291,8 +301,8 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
         for (int b = 0; b < kParts; ++b)
 #pragma unroll
             for (int e = 0; e < 16; ++e) most = fmaxf(most, sc[b][e]);
-        most = halves_max(most) * a.scale_log2;
-        if (ballot(most > top + kMaxLag)) {
+        most = fmaf(halves_max(most), a.scale_log2, -kRise<T>);
+        if (ballot(most > top + kMaxLag<T>)) {
             const float next = fmaxf(top, most);
             // A row that has seen no finite score yet keeps zeros.
             const float shrink = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
@@ -310,7 +320,8 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
                 const float x = __builtin_amdgcn_exp2f(fmaf(sc[b][e], a.scale_log2, -by));
                 sum += x;
                 // Rounded to the type of the values for the product, after
-                // the sum has its full digits: half an ulp of each p at most.
+                // the sum has its full digits: half an ulp of each p (in float16
+                // below 2^-25 of the largest: of 2^-25).
                 p[2 * b + e / 8][e % 8] = (T)x;
             }
 #pragma unroll

@@ -658,6 +658,26 @@ def test_attention_float16_gradients_of_sequences_and_rows_of_unlike_size(dev):
     check_attention(dev, q, k, v, (do.float() * size).half(), q_lens, k_lens, "f16", False)
 
 
+@pytest.mark.parametrize("q_lens,k_lens", [([16], [16000]), ([100], [16000]),
+                                           ([16] + [1] * 39, [16000] + [1] * 39),
+                                           ([900] + [1] * 21, [16000] + [1] * 21)],
+                         ids=["narrow-split", "wide-split", "narrow-whole", "wide-whole"])
+@pytest.mark.parametrize("ty", ["f16", "bf16"])
+@pytest.mark.parametrize("bits", [18, 22, 24])
+@pytest.mark.parametrize("where", [0, 40, 15999])
+def test_attention_many_keys_far_below_one(dev, ty, q_lens, k_lens, bits, where):
+    """One key whose value is zero, and 15999 others of 1.37 * 2^-bits of its
+    weight, which make the result: their weights keep the digits of the type
+    (float16's own end at 2^-14, and the kernels take them 2^11 times as large)."""
+    nq, nk = sum(q_lens), sum(k_lens)
+    q, k, v, do = attn_inputs(("far", bits, where), nq, nk, 2, 1, 64, "f32")
+    q, k, v = 2.0 + 0.05 * q, 0.02 * k, 1.0 + 0.1 * v
+    k[where] = (bits * np.log(2.0) - np.log(1.37)) / 16.0      # a score of 16 times that
+    v[where] = 0.0
+    q, k, v, do = (t.to(TYPES[ty]) for t in (q, k, v, do))
+    check_attention(dev, q, k, v, do, q_lens, k_lens, ty, False, grad=nq < 200)
+
+
 def test_attention_of_nothing(dev):
     from metal_gauss_amd import attention
 
