@@ -48,8 +48,8 @@ struct AttnArgs {
     float *lse;                          // (q_heads, q_tokens), in powers of 2; NULL: not kept
     // Split over the keys: chunks of split_keys (more with over chunk_tiles tiles:
     // chunks_of), whose {top, sum} and unscaled sums of values are joined
-    // afterwards; there is room for `items` of each key head.
-    int32_t split_keys, chunk_tiles, items;
+    // afterwards.
+    int32_t split_keys, chunk_tiles;
     float2 *part_stats;
     float *part_o;
     // Backward.
@@ -80,20 +80,6 @@ __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirs
 
 __device__ __forceinline__ int clamp_to(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-// Tokens of pseudo sequence s of n + 2 (0: before the first, n + 1: past the
-// last). Offsets are held to [0, tokens] and made to rise, so that no value of
-// theirs leads out of the tensors.
-__device__ __forceinline__ void seq_bounds(const int32_t *off, int n, int tokens, int s, int &lo,
-                                           int &len) {
-    if (!off) {
-        lo = 0;
-        len = s == 1 ? tokens : 0;
-        return;
-    }
-    lo = s == 0 ? 0 : clamp_to(off[s - 1], 0, tokens);
-    len = (s > n ? tokens : clamp_to(off[s], lo, tokens)) - lo;
-}
-
 template <int CTRL, int ROW_MASK = 0xf>
 __device__ __forceinline__ int dpp_i(int v) {
     return __builtin_amdgcn_update_dpp(0, v, CTRL, ROW_MASK, 0xf, false);
@@ -107,6 +93,35 @@ __device__ __forceinline__ int wave_inclusive_sum(int v) {
     v += dpp_i<0x143, 0xc>(v);   // row_bcast:31
     return v;
 }
+__device__ __forceinline__ int wave_inclusive_max(int v) {       // v >= 0
+    v = max(v, dpp_i<0x111>(v));
+    v = max(v, dpp_i<0x112>(v));
+    v = max(v, dpp_i<0x114>(v));
+    v = max(v, dpp_i<0x118>(v));
+    v = max(v, dpp_i<0x142, 0xa>(v));
+    v = max(v, dpp_i<0x143, 0xc>(v));
+    return v;
+}
+
+// Tokens of pseudo sequences s0 + lane of n + 2 (0: before the first, n + 1: past
+// the last), s0 a multiple of 64 and `end` where the one before s0 ends, which is
+// carried on. Offsets are held to [0, tokens] and made to rise (an offset below
+// one before it counts as that one), so that no value of theirs leads out of the
+// tensors and every token is in one pseudo sequence. For all lanes of a wave.
+__device__ __forceinline__ void seq_bounds(const int32_t *off, int n, int tokens, int s0, int &end,
+                                           int &lo, int &len) {
+    const int s = s0 + lane_id();
+    int to = tokens;
+    if (off) {
+        if (s <= n) to = clamp_to(off[s], 0, tokens);
+    } else if (s == 0) {
+        to = 0;
+    }
+    to = max(end, wave_inclusive_max(to));
+    lo = __builtin_amdgcn_update_dpp(end, to, 0x138, 0xf, 0xf, false);   // wave_shr:1
+    len = to - lo;
+    end = __builtin_amdgcn_readlane(to, 63);
+}
 
 // The sequence that has `item` when a sequence has count(q_len, k_len) items;
 // `before` sums second(q_len, k_len). Every lane of a wave calls with the same
@@ -115,17 +130,14 @@ template <bool kByKeys, typename Count, typename Second>
 __device__ __forceinline__ SeqItem find_item(const AttnArgs &a, int item, Count count,
                                              Second second) {
     SeqItem r{};
-    int base = 0, base2 = 0;
+    int base = 0, base2 = 0, q_end = 0, k_end = 0;
     for (int s0 = 0; s0 < a.n_seq + 2; s0 += 64) {
         const int s = s0 + lane_id();
-        int q_lo = 0, q_len = 0, k_lo = 0, k_len = 0, n = 0, n2 = 0;
-        if (s < a.n_seq + 2) {
-            seq_bounds(a.q_off, a.n_seq, a.q_tokens, s, q_lo, q_len);
-            seq_bounds(a.k_off, a.n_seq, a.k_tokens, s, k_lo, k_len);
-            if (s == 0 || s > a.n_seq) (kByKeys ? q_len : k_len) = 0;
-            n = count(q_len, k_len);
-            n2 = second(q_len, k_len);
-        }
+        int q_lo, q_len, k_lo, k_len;
+        seq_bounds(a.q_off, a.n_seq, a.q_tokens, s0, q_end, q_lo, q_len);
+        seq_bounds(a.k_off, a.n_seq, a.k_tokens, s0, k_end, k_lo, k_len);
+        if (s == 0 || s > a.n_seq) (kByKeys ? q_len : k_len) = 0;
+        const int n = count(q_len, k_len), n2 = second(q_len, k_len);
         const int upto = wave_inclusive_sum(n), upto2 = wave_inclusive_sum(n2);
         const uint64_t past = ballot(base + upto > item);
         if (past) {
@@ -183,13 +195,11 @@ __device__ __forceinline__ SeqItem find_longest(const AttnArgs &a, int item, int
         return s;
     }
     const int seq = lane_id();
-    int q_lo = 0, q_len = 0, k_lo = 0, k_len = 0, tiles = 0;
-    if (seq < a.n_seq + 2) {
-        seq_bounds(a.q_off, a.n_seq, a.q_tokens, seq, q_lo, q_len);
-        seq_bounds(a.k_off, a.n_seq, a.k_tokens, seq, k_lo, k_len);
-        if (seq == 0 || seq > a.n_seq) (kByKeys ? q_len : k_len) = 0;
-        tiles = tiles_of(q_len, k_len);
-    }
+    int q_end = 0, k_end = 0, q_lo, q_len, k_lo, k_len;
+    seq_bounds(a.q_off, a.n_seq, a.q_tokens, 0, q_end, q_lo, q_len);
+    seq_bounds(a.k_off, a.n_seq, a.k_tokens, 0, k_end, k_lo, k_len);
+    if (seq == 0 || seq > a.n_seq) (kByKeys ? q_len : k_len) = 0;
+    const int tiles = tiles_of(q_len, k_len);
     const auto with = [&](int w) {                // this lane's sequence's
         return w == 0 ? tiles : tiles_with<kByKeys>(a, R, q_len, k_len, w * 64);
     };

@@ -180,7 +180,7 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
                 return tiles * chunks_of(a, tiles, kl);
             },
             [](int, int) { return 0; });
-        if (!s.found || item >= a.items) return false;
+        if (!s.found) return false;
         const int tiles = tiles_of(s.q_len, 0), chunks = chunks_of(a, tiles, s.k_len);
         split_keys = chunk_keys(a, tiles);
         tile = tiles - 1 - s.within / chunks;
@@ -393,8 +393,6 @@ __global__ __launch_bounds__(64 * kWideWaves) void attn_join_tile_kernel(AttnArg
     if (!s.found) return;
     const int tiles = tiles_of(s.q_len, 0), chunks = chunks_of(a, tiles, s.k_len);
     const int item0 = s.before + s.within * chunks;
-    // Offsets that fall again could make more items than there are.
-    if (item0 + chunks > a.items) return;
     const int row = (tiles - 1 - s.within) * kRows + wave * 32 + lane % 32;
     const int token = row / G, head = kh * G + row % G;
     if (token >= s.q_len) return;
@@ -446,8 +444,6 @@ __global__ __launch_bounds__(256) void attn_join_row_kernel(AttnArgs a) {
     if (!s.found) return;
     const int row = s.within * G + head % G, tile = row / kRows, tiles = tiles_of(s.q_len);
     const int chunks = chunks_of(a, tiles, s.k_len), item0 = s.before + (tiles - 1 - tile) * chunks;
-    // Offsets that fall again could make more items than there are.
-    if (item0 + chunks > a.items) return;
     const auto slot = [&](int c) {
         return ((int64_t)(item0 + c) * a.k_heads + kh) * kRows + row % kRows;
     };
@@ -577,7 +573,9 @@ static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int gro
         int64_t keys = ceil_div(ceil_div(mean_keys * likely, slots), tile) * tile;
         if (keys < kChunkLeast) keys = kChunkLeast;
         p.split_keys = (int)keys;
-        // Sum of tiles * (1 + keys / chunk) over the sequences. No sequence has
+        // Sum of tiles * (1 + keys / chunk) over the sequences, which have each
+        // token once whatever the offsets hold (seq_bounds): the partial results
+        // of every item have room, without a check on the device. No sequence has
         // more tiles than all rows make; of many sequences those that have over
         // four times the average take longer chunks, as room for any would be
         // gigabytes (384 tokens of 32 heads on one of 128, 1000 keys each: 4.8,
@@ -641,7 +639,6 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
                "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
                (long long)p.bytes);
     a.split_keys = p.split_keys, a.chunk_tiles = (int32_t)p.chunk_tiles;
-    a.items = (int32_t)p.items;
     a.part_stats = static_cast<float2 *>(workspace);
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.stats_bytes);
     hipStream_t st = as_stream(stream);

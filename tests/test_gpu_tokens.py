@@ -476,6 +476,56 @@ def test_attention_offsets_are_held_to_the_tensors(dev):
     assert attention(q, k, v, fall).shape == q.shape
 
 
+FALLING = [   # queries' tokens and offsets, keys'
+    (100, [0, 60, 20, 100], 100, [0, 60, 20, 100]),
+    (300, [300, 0, 300, 0, 300], 280, [0, 280, 0, 280, 0]),          # all in one, or none
+    (50, [7, 3, -9, 40, 39, 10 ** 9, 5], 9000, [20, 8000, 7000, 8500, 0, 8600, 1]),   # few, many keys
+    (400, [0, 10, 390, 2, 395], 9000, [9, 1, 8000, 0, 7000]),
+]
+
+
+@pytest.mark.parametrize("tokens_q,q_off,tokens_k,k_off", FALLING)
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_offsets_that_fall_are_made_to_rise(dev, tokens_q, q_off, tokens_k, k_off, ty,
+                                                      causal):
+    check_falling_offsets(dev, tokens_q, q_off, tokens_k, k_off, ty, causal)
+
+
+@pytest.mark.parametrize("n", [61, 62, 63, 64, 126, 127, 200])
+def test_attention_offsets_of_many_sequences_that_fall(dev, n):
+    """The rise goes on from one step of 64 sequences to the next."""
+    rng = np.random.default_rng(n)
+    offs = [np.sort(rng.integers(0, 3000, n + 1)) + rng.integers(-200, 200, n + 1)
+            for _ in range(2)]
+    offs[0][n // 3], offs[1][n // 2] = 2950, 2900      # most that follow lie below
+    check_falling_offsets(dev, 3000, offs[0], 3000, offs[1], "f16", n % 2 == 0)
+
+
+def check_falling_offsets(dev, tokens_q, q_off, tokens_k, k_off, ty, causal):
+    """Result and gradients are, bit for bit, those of the offsets' running maximum,
+    held to the tensors."""
+    from metal_gauss_amd import attention
+
+    q, k, v, do = (t.to(dev) for t in attn_inputs(("fall", tokens_q, tokens_k), tokens_q, tokens_k,
+                                                  4, 2, 64, ty))
+    got = []
+    for rising in (False, True):
+        offs = []
+        for off, tokens in ((q_off, tokens_q), (k_off, tokens_k)):
+            off = np.asarray(off)
+            if rising:
+                off = np.maximum.accumulate(off.clip(0, tokens))
+            offs.append(torch.tensor(off, dtype=torch.int32, device=dev))
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        o = attention(*leaves, *offs, causal=causal)
+        got.append((o, *torch.autograd.grad(o, leaves, do)))
+        with torch.no_grad():
+            assert torch.equal(attention(*leaves, *offs, causal=causal), o)
+    for a, b in zip(*got):
+        assert bool(a.isfinite().all()) and torch.equal(a, b)
+
+
 def test_attention_unseen_keys_may_hold_anything(dev):
     """NaN and infinities in keys and values that the mask leaves out, in their own
     sequence and in its neighbours'."""
