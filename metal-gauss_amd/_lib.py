@@ -18,6 +18,7 @@ import functools
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 _HERE = Path(__file__).resolve().parent
@@ -216,13 +217,24 @@ def launch(fn, index: int, *args) -> None:
             check(rc)
 
 
+def forward_mode() -> bool:
+    """Whether forward-mode derivatives are being taken. An operator's call then goes
+    through autograd even where no input requires a gradient: autograd refuses
+    an input with a tangent, which would be lost without a word otherwise."""
+    return forward_ad._current_level >= 0
+
+
 def differentiable_once(fn):
     """torch's once_differentiable for an autograd function's backward, at no cost
-    where no graph of the backward pass is being made (the usual case)."""
+    where no graph of the backward pass is being made (the usual case). Gradients
+    with a tangent are refused."""
     checked = once_differentiable(fn)
 
     @functools.wraps(fn)
     def backward(ctx, *grads):
+        if forward_mode() and any(g is not None and forward_ad.unpack_dual(g).tangent is not None
+                                  for g in grads):
+            raise NotImplementedError("the backward pass has no forward-mode derivative")
         return (checked if torch.is_grad_enabled() else fn)(ctx, *grads)
 
     return backward

@@ -150,6 +150,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             raise ValueError(f"q_offsets is {tuple(q_offsets.shape)} and k_offsets "
                              f"{tuple(k_offsets.shape)}; one number of sequences is needed")
     scale = max(dim, 1) ** -0.5 if scale is None else float(scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) \
+            or _lib.forward_mode():
         return _Attention.apply(q, k, v, q_offsets, k_offsets, bool(causal), scale)
     return _forward(q, k, v, q_offsets, k_offsets, bool(causal), scale, False)[0]

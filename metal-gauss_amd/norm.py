@@ -117,8 +117,8 @@ def layer_norm(x: torch.Tensor, weight: torch.Tensor | None = None,
     the result has x's type. Differentiable in all three, with the same bits from
     call to call.
     """
-    if torch.is_grad_enabled() and (
+    if (torch.is_grad_enabled() and (
             x.requires_grad or (weight is not None and weight.requires_grad) or
-            (bias is not None and bias.requires_grad)):
+            (bias is not None and bias.requires_grad))) or _lib.forward_mode():
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _forward(x, weight, bias, float(eps), False)[0]

@@ -139,7 +139,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
                            f"'{frequencies.device}'")
     if not positions.is_contiguous():
         positions = positions.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) \
+            or _lib.forward_mode():
         out = _Rotary.apply(q, k, positions, frequencies, layout)
     else:
         out = _turn(q, k, positions, frequencies, layout, False)

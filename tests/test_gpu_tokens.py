@@ -839,3 +839,36 @@ def test_second_derivatives_are_refused(dev):
     dx, = torch.autograd.grad(layer_norm(x).square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dx.sum().backward()
+
+
+def test_forward_mode_derivatives_are_refused(dev):
+    """A tangent of an input, or of a result's gradient, is refused, not dropped;
+    tensors without one are served while others' are taken."""
+    import torch.autograd.forward_ad as fw
+    from metal_gauss_amd import attention, layer_norm, rotary, rotary_frequencies
+
+    g = gen("tangents")
+    q, k, v = (torch.randn(9, 2, 32, generator=g).to(dev, torch.bfloat16) for _ in range(3))
+    x, w, b = (torch.randn(*s, generator=g).to(dev) for s in ((5, 24), (24,), (24,)))
+    pos, freq = torch.arange(9, device=dev), rotary_frequencies(32, device=dev)
+    calls = [(lambda q, k, v: attention(q, k, v), (q, k, v), 3),
+             (lambda x, w, b: layer_norm(x, w, b), (x, w, b), 3),
+             (lambda q, k, f: rotary(q, k, pos, f)[0], (q, k, freq), 2),
+             (lambda q, f: rotary(q, None, pos, f), (q, freq), 1)]
+    for call, inputs, leaves in calls:
+        plain = call(*inputs)
+        with fw.dual_level():
+            assert torch.equal(call(*inputs), plain) and not call(*inputs).requires_grad
+            for i in range(len(inputs)):
+                dual = list(inputs)
+                dual[i] = fw.make_dual(inputs[i], torch.ones_like(inputs[i]))
+                with pytest.raises(NotImplementedError):
+                    call(*dual)
+                with torch.no_grad(), pytest.raises(NotImplementedError):
+                    call(*dual)
+            at = [t.detach().requires_grad_(i < leaves) for i, t in enumerate(inputs)]
+            y = call(*at)
+            dy = torch.ones_like(y)
+            torch.autograd.grad(y, at[:leaves], dy, retain_graph=True, allow_unused=True)
+            with pytest.raises(NotImplementedError):
+                torch.autograd.grad(y, at[:leaves], fw.make_dual(dy, dy), allow_unused=True)

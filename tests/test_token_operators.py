@@ -209,6 +209,38 @@ def test_workspace_of_single_tokens_over_many_memories(streams, heads, kv, keys)
     assert 0 < need <= 8 * (1536 + 2 * streams * kv) * 32 * 128 * 4
 
 
+# ----------------------------------------------------------------- autograd
+
+def test_a_backward_pass_refuses_tangents():
+    """The decorator of the operators' backward passes: a gradient with a tangent is
+    refused, one without is passed on, and second derivatives are refused."""
+    import torch.autograd.forward_ad as fw
+    from metal_gauss_amd import _lib
+
+    class Twice(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return 2.0 * x
+
+        @staticmethod
+        @_lib.differentiable_once
+        def backward(ctx, dy):
+            return torch.from_numpy(2.0 * dy.detach().numpy())
+
+    x = torch.randn(4).requires_grad_(True)
+    dy = torch.ones(4)
+    assert not _lib.forward_mode()
+    assert torch.equal(torch.autograd.grad(Twice.apply(x), x, dy)[0], 2.0 * dy)
+    with fw.dual_level():
+        assert _lib.forward_mode()
+        assert torch.equal(torch.autograd.grad(Twice.apply(x), x, dy)[0], 2.0 * dy)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(Twice.apply(x), x, fw.make_dual(dy, dy))
+    dx, = torch.autograd.grad(Twice.apply(x).square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.sum().backward()
+
+
 # ---------------------------------------------------- the oracle's own checks
 
 def _difference(f, x, d):
