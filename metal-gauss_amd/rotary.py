@@ -112,7 +112,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     ("half") or (2i, 2i + 1) ("interleaved").
 
     Returns new contiguous tensors (q, k), or q alone where k is None; one launch
-    for both, one for both gradients. Differentiable in q and k.
+    for both, one for both gradients. Differentiable in q and k; frequencies that
+    require a gradient are refused.
     """
     code = _lib.type_code(q, "q")
     if q.dim() != 3:
@@ -137,6 +138,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
     if not frequencies.is_cuda or frequencies.get_device() != index:
         raise RuntimeError(f"frequencies must be on {q.device}, got device "
                            f"'{frequencies.device}'")
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("frequencies must not require a gradient: there is none for them")
     if not positions.is_contiguous():
         positions = positions.contiguous()
     if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) \

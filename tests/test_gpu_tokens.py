@@ -872,3 +872,18 @@ def test_forward_mode_derivatives_are_refused(dev):
             torch.autograd.grad(y, at[:leaves], dy, retain_graph=True, allow_unused=True)
             with pytest.raises(NotImplementedError):
                 torch.autograd.grad(y, at[:leaves], fw.make_dual(dy, dy), allow_unused=True)
+
+
+def test_rotary_refuses_frequencies_that_require_a_gradient(dev):
+    """Learned frequencies would stay as they are in silence."""
+    from metal_gauss_amd import rotary, rotary_frequencies
+
+    x = torch.randn(4, 2, 32, generator=gen("learned")).to(dev)
+    pos = torch.arange(4, device=dev)
+    freq = rotary_frequencies(32, device=dev).requires_grad_(True)
+    for q in (x, x.detach().requires_grad_(True)):
+        with pytest.raises(RuntimeError, match="frequencies must not require"):
+            rotary(q, None, pos, freq)
+    want = rotary(x, None, pos, freq.detach())
+    with torch.no_grad():
+        assert torch.equal(rotary(x, None, pos, freq), want)
