@@ -296,13 +296,15 @@ struct TileFill {
                          "s_nop 4\n\t"
                          "buffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
-                         : "s"(o.to), "v"(at), "s"(o.rsrc));
+                         : "s"(o.to), "v"(at), "s"(o.rsrc)
+                         : "m0");
         else
             asm volatile("s_mov_b32 m0, %0\n\t"
                          "s_nop 0\n\t"
                          "buffer_load_dwordx4 %1, %2, 0 offen lds"
                          :
-                         : "s"(o.to + i * kWaves * 1024), "v"(at), "s"(o.rsrc));
+                         : "s"(o.to + i * kWaves * 1024), "v"(at), "s"(o.rsrc)
+                         : "m0");
     }
 
     __device__ __forceinline__ void ask(const char *head, int64_t tok_stride, int dim, int row0,

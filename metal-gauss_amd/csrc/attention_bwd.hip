@@ -249,7 +249,7 @@ __device__ __forceinline__ void ask_row_values(const float *at, int rows, uint32
                  "buffer_load_dword %1, %2, 0 offen lds"
                  :
                  : "s"(uniform((int)lds)), "v"(off), "s"(rsrc)
-                 : "memory");
+                 : "m0", "memory");
 }
 
 // A run's sums for one key tile, in the order the waves hold them (a store is

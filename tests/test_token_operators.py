@@ -342,3 +342,50 @@ def test_the_check_flags_a_descriptor_just_written():
     assert not unready_lds_loads(["v_readfirstlane_b32 s12, v3", *wait, load])
     assert not unready_lds_loads(["v_readfirstlane_b32 s9, v3", "s_mov_b32 m0, s2", "s_nop 4", load])
     assert unready_lds_loads(["s_nop 4", "s_mov_b32 m0, s2", load])
+
+
+def undeclared_m0(text):
+    """Assembly statements that write m0 and do not say so."""
+    bad = []
+    for start in re.finditer(r"\basm\b[^(;]*\(", text):
+        depth, at = 1, start.end()
+        while depth:
+            depth += {"(": 1, ")": -1}.get(text[at], 0)
+            at += 1
+        statement = text[start.end():at - 1]
+        if re.search(r"s_\w+ m0,", statement) and '"m0"' not in statement.rpartition(":")[2]:
+            bad.append(statement)
+    return bad
+
+
+def test_assembly_that_writes_m0_says_so():
+    """The compiler may hold a value of its own there."""
+    from test_lds_barrier_audit import _build_module
+
+    sources = [p for p in sorted(_build_module().CSRC.iterdir()) if p.suffix in (".h", ".hip")]
+    texts = {p.name: p.read_text() for p in sources}
+    assert sum(len(re.findall(r"s_\w+ m0,", t)) for t in texts.values()) >= 3
+    assert not {n: u for n, t in texts.items() if (u := undeclared_m0(t))}
+
+
+def test_the_check_flags_an_undeclared_m0():
+    write = 'asm volatile("s_mov_b32 m0, %0\\n\\t" "buffer_load_dword %1, %2, 0 offen lds" : : "s"(f((int)a)), "v"(b)'
+    assert undeclared_m0(write + ");")
+    assert undeclared_m0(write + ' : "memory");')
+    assert not undeclared_m0(write + ' : "m0", "memory");')
+    assert not undeclared_m0('asm volatile("s_waitcnt vmcnt(0)" ::: "memory");')
+
+
+@pytest.mark.parametrize("source", ["attention.hip", "attention_bwd.hip"])
+def test_m0_is_for_the_tile_loads_alone(tmp_path, source):
+    """Nothing else in the compiled kernels reads or writes it."""
+    from test_lds_barrier_audit import _assemble, _build_module
+
+    out = _assemble(_build_module().CSRC / source, tmp_path / "out.s", source)
+    lines = [s.split(";")[0].strip() for s in out.read_text().splitlines()]
+    lines = [s for s in lines if s and not s.startswith(".") and not s.endswith(":")]
+    at = [i for i, s in enumerate(lines) if re.search(r"\bm0\b", s)]
+    assert len(at) > 50
+    for i in at:
+        assert re.fullmatch(r"s_mov_b32 m0, (s\d+|vcc_lo|vcc_hi)", lines[i])
+        assert re.fullmatch(r"s_nop \d", lines[i + 1]) and lines[i + 2].endswith(" lds"), lines[i]
