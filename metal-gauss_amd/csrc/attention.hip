@@ -634,7 +634,7 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
     if (q_tokens == 0) return MG_OK;
     MG_REQUIRE(q && out && (k_tokens == 0 || (k && v)), "%s: a pointer is NULL", who);
     const FwdPlan p = fwd_plan(q_tokens, k_tokens, k_heads, group, dim, sequences);
-    MG_REQUIRE(p.items * k_heads < (int64_t(1) << 31), "%s: too many work items", who);
+    MG_REQUIRE(grid_fits(p.items * k_heads, 64 * p.waves), "%s: too many work items", who);
     MG_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes),
                "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
                (long long)p.bytes);

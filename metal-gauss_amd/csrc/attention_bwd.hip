@@ -46,9 +46,11 @@ __host__ __device__ constexpr int64_t norm_places(int64_t tokens, int64_t n_seq)
 // The largest |row|^2 of a tile's tokens in do (blockIdx.y 0: over the query heads
 // that share the key head) and in v (1). Tokens of no sequence are not looked at.
 // A NaN counts as nothing.
+constexpr int kLargestThreads = 256;
+
 template <typename T>
-__global__ __launch_bounds__(256) void attn_largest_kernel(AttnArgs a) {
-    __shared__ float s_most[4];
+__global__ __launch_bounds__(kLargestThreads) void attn_largest_kernel(AttnArgs a) {
+    __shared__ float s_most[kLargestThreads / 64];
     const bool of_v = blockIdx.y != 0;
     const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
     const auto tiles_of = [&](int ql, int kl) {
@@ -567,12 +569,14 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
     hipStream_t st = as_stream(stream);
     const int64_t q_items = (q_tokens * group / kBwdTile + sequences + 2) * k_heads;
     const int64_t k_items = p.k_items * p.splits * k_heads;
-    MG_REQUIRE(q_items < (int64_t(1) << 31) && k_items < (int64_t(1) << 31),
+    const int64_t places =
+        k_heads * norm_places(q_tokens > k_tokens ? q_tokens : k_tokens, sequences);
+    MG_REQUIRE(grid_fits(q_items, 64 * kBwdWaves) && grid_fits(k_items, 64 * kBwdWaves) &&
+                   (dtype != MG_F16 || grid_fits(places, kLargestThreads)),
                "%s: too many work items", who);
     if (dtype == MG_F16) {
         TimedScope ts("attention_largest", st);
-        const int64_t places = norm_places(q_tokens > k_tokens ? q_tokens : k_tokens, sequences);
-        attn_largest_kernel<f16_t><<<dim3((unsigned)(places * k_heads), 2), 256, 0, st>>>(a);
+        attn_largest_kernel<f16_t><<<dim3((unsigned)places, 2), kLargestThreads, 0, st>>>(a);
         MG_LAUNCHED("attn_largest_kernel");
     }
     if (q_tokens > 0) {

@@ -28,6 +28,11 @@ struct TypeCode<f16_t> {
 inline int64_t type_bytes(int32_t code) { return code == MG_F32 ? 4 : 2; }
 inline bool type_known(int32_t code) { return code == MG_F32 || code == MG_BF16 || code == MG_F16; }
 
+// A launch counts its threads in 32 bits.
+inline bool grid_fits(int64_t groups, int threads) {
+    return groups * threads < (int64_t(1) << 32);
+}
+
 // Elements of one 16-byte access.
 template <typename T>
 constexpr int kVec = 16 / (int)sizeof(T);

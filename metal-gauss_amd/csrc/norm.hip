@@ -438,6 +438,9 @@ static int32_t norm_check(const char *who, int64_t rows, int64_t n, int32_t dtyp
     MG_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31), "%s: %lld rows", who, (long long)rows);
     MG_REQUIRE(n >= 1 && n <= (int64_t(1) << 24), "%s: rows of %lld elements; 1 to 2^24 are taken",
                who, (long long)n);
+    MG_REQUIRE(n <= kNormLoopWidth || grid_fits(rows, kLoopThreads),
+               "%s: %lld rows of %lld elements are too many for one call", who, (long long)rows,
+               (long long)n);
     MG_REQUIRE(type_known(dtype), "%s: type code %d", who, dtype);
     MG_REQUIRE(wtype == MG_F32 || wtype == dtype,
                "%s: the weights must be float32 or of the input's type", who);

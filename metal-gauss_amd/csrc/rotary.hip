@@ -150,7 +150,7 @@ static bool rotary_go(RotArgs a, hipStream_t st) {
     a.tokens_at_once = (int32_t)(at_once < 1 ? 1 : at_once);
     a.runs = (int32_t)ceil_div(a.tokens_at_once * per_tok, kAll);
     const int64_t grid = ceil_div(a.tokens, a.tokens_at_once) * a.runs;
-    if (grid >= (int64_t(1) << 31)) return false;
+    if (!grid_fits(grid, kRotThreads)) return false;
     const int64_t bytes = a.tokens * (a.heads[0] + a.heads[1]) * a.dim * (int64_t)sizeof(T);
     if (bytes > kRotStreamBytes)
         rotary_kernel<T, P, V, kHalf, true><<<(unsigned)grid, kRotThreads, 0, st>>>(a);

@@ -172,6 +172,27 @@ def test_refusals_before_any_launch():
                                       16, 8, None), "workspace of 8 bytes")
 
 
+def test_launches_of_more_threads_than_are_counted_are_refused():
+    """Before the launch: 2^32 threads are too many."""
+    from metal_gauss_amd import _lib
+
+    lib = _lib.open_library()
+
+    def refused(rc, text):
+        assert rc == 1 and text in lib.mg_last_error().decode(), lib.mg_last_error()
+
+    off, many = 16, 1 << 24          # one work item a sequence and head at least
+    refused(_attn(lib, nq=many, nk=many, heads=4, kv=4, off=off, n=many), "too many work items")
+    for n, kv in ((many, 1), (many // 8, 8)):
+        refused(lib.mg_attention_backward(2, n, n, kv, kv, 64, 16, 64, 64, 16, 64, 64, 16, 64, 64,
+                                          off, off, n, 0, 1.0, 16, None, 16, 16, 64, 64, 16, 16,
+                                          16, 16, 1 << 50, None), "too many work items")
+    refused(lib.mg_layer_norm_forward(1 << 22, 16385, 0, 16, 16385, 0, None, None, 1e-5, 16, None,
+                                      None, None), "too many for one call")
+    refused(lib.mg_rotary(1 << 24, 1, 16, 2046, 1023, 2, None, 0, 0, 0, 1023, 16, 0, 1, 16, 32, 0,
+                          0, 16, None, None), "too many for one call")
+
+
 def test_workspace_queries():
     from metal_gauss_amd import _lib
 
