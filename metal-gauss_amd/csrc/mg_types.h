@@ -10,22 +10,6 @@ namespace mg {
 typedef __bf16 bf16_t;
 typedef _Float16 f16_t;
 
-template <typename T>
-struct TypeCode;
-template <>
-struct TypeCode<float> {
-    static constexpr int32_t value = MG_F32;
-};
-template <>
-struct TypeCode<bf16_t> {
-    static constexpr int32_t value = MG_BF16;
-};
-template <>
-struct TypeCode<f16_t> {
-    static constexpr int32_t value = MG_F16;
-};
-
-inline int64_t type_bytes(int32_t code) { return code == MG_F32 ? 4 : 2; }
 inline bool type_known(int32_t code) { return code == MG_F32 || code == MG_BF16 || code == MG_F16; }
 
 // A launch counts its threads in 32 bits.
