@@ -404,6 +404,19 @@ def test_attention_chunks_of_very_unequal_sequences(dev, causal):
     check_attention(dev, q, k, v, do, q_lens, k_lens, "f16", causal, grad=False)
 
 
+@pytest.mark.parametrize("q_lens,k_lens,heads,kv", [
+    ([1] * 40, [64] * 39 + [16320], 4, 1),            # one long memory: narrow, whole
+    ([1] * 100, [9000, 1, 0] + [30] * 97, 8, 8),      # items enough by their number alone
+    ([2000] + [1] * 63, [2000] + [40] * 63, 1, 1),    # a prompt in narrow items
+    ([1] * 10 + [900], [3] * 10 + [5000], 2, 1)],     # wide, whole
+    ids=["streams", "heads", "prompt", "chunk"])
+@pytest.mark.parametrize("ty", ["bf16", "f16"])
+def test_attention_unequal_sequences_that_are_not_cut(dev, q_lens, k_lens, heads, kv, ty):
+    """Packs whose average sequence is too short to cut any over its keys."""
+    q, k, v, do = attn_inputs(("uncut", heads, kv), sum(q_lens), sum(k_lens), heads, kv, 64, ty)
+    check_attention(dev, q, k, v, do, q_lens, k_lens, ty, True)
+
+
 @pytest.mark.parametrize("seed", range(8))
 def test_attention_random_packs(dev, seed):
     """Every tile of every sequence is given out once, in whatever order: up to 80
