@@ -122,7 +122,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
     Scores, softmax and sums are float32; p is rounded to the inputs' type for
     its product with v. Differentiable in q, k and v, with the same bits from
-    call to call.
+    call to call; for that, what rounding took from the result is kept, a second
+    tensor of its size.
     """
     dtype, dim, index = q.dtype, q.shape[-1] if q.dim() else 0, q.get_device()
     for t, what in ((q, "q"), (k, "k"), (v, "v")):

@@ -18,7 +18,8 @@
 // With 128 columns a tile's products take as long as its softmax, with 64 the
 // softmax (exponentials) is the bound; two to four waves a SIMD take turns at
 // both. 16320 tokens, causal, 16 heads on 4 of 128: 950 to 1050 us (1150 to 1040
-// TFLOP/s, as the GPU's clock holds); 10000 tokens, 16 heads of 64: 440 us (930).
+// TFLOP/s, as the GPU's clock holds); 10000 tokens, 16 heads of 64: 440 us (930), of 80
+// 620 (830) and of 96 627 (980): 80 columns take the form of 96.
 //
 // The running maximum lags: the accumulators are rescaled only when a score
 // passes the maximum they go by by more than kMaxLag, which leaves every sum exact
@@ -42,8 +43,8 @@ constexpr float kRise = std::is_same<T, f16_t>::value ? 11.f : 0.f;
 // keys that all four read. Narrow, where a sequence's rows would leave most of
 // that empty (single tokens): 32 rows by one wave, tiles of 32 keys; memory
 // bounds it, and ten waves (64 columns) or five (128) of a CU each have a
-// tile's loads under way. 16 tokens of 16 heads on 4 of 64 over 75000 keys: 16 us
-// and 6.4 to join (tiles of 64 keys: 19, half as many waves), 75 MB of keys and
+// tile's loads under way. 16 tokens of 16 heads on 4 of 64 over 75000 keys: 16.5 us
+// and 8 to join (tiles of 64 keys: 19, half as many waves), 75 MB of keys and
 // values at 7 TB/s once the loop runs.
 constexpr int kWideWaves = 4, kNarrowWaves = 1;
 template <int kWaves>
@@ -540,7 +541,10 @@ int32_t attn_check(const char *who, const AttnArgs &a, int32_t dtype) {
 
 // How the work is cut. Narrow items where rows fill half a wide item at most (on
 // the average of the sequences); chunks of keys where the items alone leave the
-// GPU idle and a row has keys enough to be worth the second launch.
+// GPU idle and a row has keys enough to be worth the second launch. The host
+// knows the average alone: one long memory among many short ones is not cut (40
+// tokens, 16 heads on 4 of 64, over 16320 keys and 39 times 64: 358 us, over 40
+// times 470: 16).
 struct FwdPlan {
     int waves;
     int split_keys;             // 0: whole rows

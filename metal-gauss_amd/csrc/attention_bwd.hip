@@ -23,8 +23,9 @@
 // sequence packed with it nor tokens of none take digits from it. bfloat16 has
 // float32's range and needs neither.
 //
-// 8192 tokens, 16 heads of 128: queries 740 us, keys 1015 (1110 and 1080 TFLOP/s);
-// of 64: 454 and 611 (905 and 900). As the forward, both need two waves a SIMD to
+// 8192 tokens, 16 heads of 128: queries 748 us, keys 1047 (1100 and 1050 TFLOP/s);
+// of 64: 462 and 623 (890 and 880). The queries' kernel is never cut over its keys:
+// 64 queries over 16000 of them, 16 heads on 4 of 128, take 417 us. As the forward, both need two waves a SIMD to
 // keep products and exponentials going side by side: the keys' kernel with one
 // (256 columns of sums and operands in 472 registers) took 1970.
 #include "attention.h"
@@ -483,7 +484,7 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_sum_kernel(AttnArgs a) {
 // Bytes of the backward's scratch: delta, the largest norms, and the runs' sums.
 // The keys' gradients are cut into runs where their tiles are fewer than fill
 // the GPU twice over, of eight query tiles at least (7033 packed tokens, 62 tiles
-// on 4 key heads: 528 us uncut, 177 and 29 to add the runs in four).
+// on 4 key heads: 528 us uncut, 187 and 27 to add the runs in four).
 struct BwdPlan {
     int64_t k_items, largest_at, part_at, bytes;
     int splits, split_steps;

@@ -13,7 +13,9 @@
 //
 // 65280 rows of 1024 bfloat16, float32 weights: forward 45 us (5.9 TB/s), backward
 // 66 (6.1 TB/s) and 4 to join the weights' gradients; 64 rows of 256 float32: 3 us,
-// the launch.
+// the launch. Few or wide rows: 2048 of 8192 take 16 us forward, and 40 and 12 to
+// join backward, where the workgroups' sums of columns (67 MB written, then read)
+// move more bytes than the rows (101 MB).
 #include "mg_types.h"
 
 namespace mg {
@@ -235,7 +237,8 @@ __global__ __launch_bounds__(kJoinThreads) void norm_join_kernel(const float *__
 
 // ------------------------------------------------------------- longest rows
 // Rows past 16 waves' registers: one workgroup a row, the row read again for
-// each of its three passes (from L2 where it fits).
+// each of its three passes (from L2 where it fits), an element a lane. 1024 rows of
+// 20000 bfloat16: forward 48 us (1.7 TB/s), backward 46 and 20 for the weights' sums.
 constexpr int kLoopThreads = 1024;
 
 template <typename T, typename W>
