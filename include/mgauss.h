@@ -688,6 +688,60 @@ int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q,
                   int32_t inverse, void *q_out, void *k_out,
                   mg_stream_t stream);
 
+/* mg_rotary with pair i going by axis axis_of[i] (host, `pairs` bytes below
+ * `axes`; at most 256 pairs), in place of equal runs. */
+int32_t mg_rotary_axes(int64_t tokens, int32_t dtype, const void *q,
+                       int64_t q_token_stride, int64_t q_head_stride,
+                       int32_t q_heads, const void *k, int64_t k_token_stride,
+                       int64_t k_head_stride, int32_t k_heads, int32_t dim,
+                       const void *positions, int32_t positions_64,
+                       int32_t axes, const uint8_t *axis_of,
+                       const double *frequencies, int32_t pairs,
+                       int32_t interleaved, int32_t inverse, void *q_out,
+                       void *k_out, mg_stream_t stream);
+
+/* Heads normed by their root mean square, x / sqrt(mean(x^2) + eps) * weight, and
+ * then turned as mg_rotary_axes does (axis_of NULL: equal runs), in one pass.
+ * dim 2 to 512; either tensor may have no heads. The weights (dim; NULL: ones)
+ * are shared by a tensor's heads, float32 or of the inputs' type. */
+int32_t mg_norm_rotary_forward(
+    int64_t tokens, int32_t dtype, const void *q, int64_t q_token_stride,
+    int64_t q_head_stride, int32_t q_heads, const void *k,
+    int64_t k_token_stride, int64_t k_head_stride, int32_t k_heads, int32_t dim,
+    int32_t weight_dtype, const void *q_weight, const void *k_weight, float eps,
+    const void *positions, int32_t positions_64, int32_t axes,
+    const uint8_t *axis_of, const double *frequencies, int32_t pairs,
+    int32_t interleaved, void *q_out, void *k_out, mg_stream_t stream);
+/* Its gradients from the inputs and the results' gradients dq_out and dk_out
+ * (strided as the inputs): dq, dk (contiguous), dq_weight and dk_weight (of the
+ * weights' type), each of which may be NULL. Sums over tokens and heads are
+ * formed in a fixed order: equal calls give equal bits. The workspace is needed
+ * where a weight's gradient is. */
+int64_t mg_norm_rotary_backward_workspace_bytes(int32_t dim);
+int32_t mg_norm_rotary_backward(
+    int64_t tokens, int32_t dtype, const void *q, int64_t q_token_stride,
+    int64_t q_head_stride, int32_t q_heads, const void *k,
+    int64_t k_token_stride, int64_t k_head_stride, int32_t k_heads, int32_t dim,
+    int32_t weight_dtype, const void *q_weight, const void *k_weight, float eps,
+    const void *positions, int32_t positions_64, int32_t axes,
+    const uint8_t *axis_of, const double *frequencies, int32_t pairs,
+    int32_t interleaved, const void *dq_out, int64_t dq_token_stride,
+    int64_t dq_head_stride, const void *dk_out, int64_t dk_token_stride,
+    int64_t dk_head_stride, void *dq, void *dk, void *dq_weight,
+    void *dk_weight, void *workspace, int64_t workspace_bytes,
+    mg_stream_t stream);
+
+/* Dropout of n contiguous elements: out = residual + (kept ? x * 65536 / (65536 -
+ * drop) : 0); residual may be NULL (0) and has out's type. out_dtype is x's, or
+ * either is MG_F32 (the gradient of x from that of a float32 result is the same
+ * call on the gradient). Element i is kept where 16 bits of Philox4x32-10 are at
+ * least `drop` (of 65536): key the seed (low word first), counter (i / 8, site) in
+ * four words, low ones first; its bits are half i % 2 (the low one first) of word
+ * i % 8 / 2. The seed is read from seed_at (device) unless that is NULL. */
+int32_t mg_dropout(int64_t n, int32_t dtype, const void *x, int32_t out_dtype,
+                   const void *residual, void *out, int32_t drop, uint64_t seed,
+                   const int64_t *seed_at, uint64_t site, mg_stream_t stream);
+
 /* Attention over packed sequences: q (q_tokens, q_heads, dim), k and v
  * (k_tokens, k_heads, dim), bfloat16 or float16, dim a multiple of 8 up to 128,
  * q_heads a multiple of k_heads (a key head serves as many query heads, in

@@ -20,7 +20,9 @@ counterpart in the reference):
     layer_norm             layer norm and its gradients
     rotary, rotary_frequencies
                            rotary positions of queries and keys
+    norm_rotary            heads normed and turned in one pass, and its gradients
     attention              attention over packed sequences and its gradients
+    dropout                dropout onto a residual stream, and its gradients
 """
 
 from .api import BACKENDS, render  # noqa: F401
@@ -31,6 +33,8 @@ from .mipfilter import apply_3d_filter, compute_3d_filter  # noqa: F401
 from .backend import ListCapacity  # noqa: F401
 from .norm import layer_norm  # noqa: F401
 from .rotary import rotary, rotary_frequencies  # noqa: F401
+from .norm_rotary import norm_rotary  # noqa: F401
+from .dropout import dropout  # noqa: F401
 from .attention import attention  # noqa: F401
 from . import backend, ext  # noqa: F401
 

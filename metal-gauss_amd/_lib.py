@@ -131,6 +131,17 @@ _SIGNATURES = {
                                       _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "mg_rotary": (_i32, [_i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32, _i32, _vp,
                          _i32, _i32, _vp, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "mg_rotary_axes": (_i32, [_i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32, _i32,
+                              _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp]),
+    "mg_norm_rotary_forward": (_i32, [_i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32,
+                                      _i32, _i32, _vp, _vp, _f32, _vp, _i32, _i32, _vp, _vp,
+                                      _i32, _i32, _vp, _vp, _vp]),
+    "mg_norm_rotary_backward_workspace_bytes": (_i64, [_i32]),
+    "mg_norm_rotary_backward": (_i32, [_i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32,
+                                       _i32, _i32, _vp, _vp, _f32, _vp, _i32, _i32, _vp, _vp,
+                                       _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp,
+                                       _vp, _vp, _vp, _i64, _vp]),
+    "mg_dropout": (_i32, [_i64, _i32, _vp, _i32, _vp, _vp, _i32, _u64, _vp, _u64, _vp]),
     "mg_attention_forward_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
     "mg_attention_forward": (_i32, [_i32, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _vp,
                                     _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _f32,

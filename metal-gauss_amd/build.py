@@ -24,6 +24,7 @@ ARCH = "gfx950"
 
 SOURCES = ["runtime.hip", "adam.hip", "preprocess.hip", "mip.hip", "mcmc.hip", "binning.hip", "sort.hip",
            "rasterize.hip", "ssim.hip", "ply.hip", "norm.hip", "rotary.hip",
+           "norm_rotary.hip", "dropout.hip",
            "attention.hip", "attention_bwd.hip"]
 
 # -packed-fp32-ops keeps the compiler from emitting packed fp32 VALU forms;

@@ -16,7 +16,7 @@
 // polynomial) is as long as a trip to memory: 10000 tokens of 32 heads of 64
 // bfloat16 16 us (5.1 TB/s; 23 us with the cosines first), 32640 of 20 heads of
 // 128 float32, a quarter of them elsewhere in their rows, 125 us (5.3 TB/s).
-#include "mg_types.h"
+#include "rotary.h"
 
 namespace mg {
 
@@ -40,6 +40,9 @@ struct RotArgs {
     int32_t tokens_at_once, runs;
     float sign;
 };
+struct RotAxisArgs : RotArgs {
+    AxisTable axis;                        // in place of equal runs
+};
 
 // kStream: results larger than the L2 caches pass by them (32640 tokens of 20
 // heads of 128 float32, forward and backward: 268 us, with streaming stores 258;
@@ -61,8 +64,8 @@ __device__ __forceinline__ void copy_out(T *to, const T (&from)[V]) {
 // their partners (kHalf), V / 2 whole pairs (interleaved), or V elements that
 // are copied. V = 16 bytes' worth where units do not straddle the parts'
 // borders, else 1 (2 interleaved).
-template <typename T, typename P, int V, bool kHalf, bool kStream>
-__global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
+template <typename T, typename P, int V, bool kHalf, bool kStream, typename Args>
+__global__ __launch_bounds__(kRotThreads) void rotary_kernel(Args a) {
     __shared__ float2 s_cs[kRotTable];
     const int run = a.runs > 1 ? blockIdx.x % a.runs : 0;
     const int64_t tok0 = (int64_t)(blockIdx.x / a.runs) * a.tokens_at_once;
@@ -101,12 +104,12 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
     const int per_axis = a.pairs / a.axes;
     for (int i = threadIdx.x; i < n_tok * a.pairs; i += kRotThreads) {
         const int tok = i / a.pairs, pair = i - tok * a.pairs;
-        const double turns = (double)pos[(tok0 + tok) * a.axes + pair / per_axis] * a.freq[pair] *
-                             0.15915494309189533577;
-        float sn, cs;
-        // turns - rint(turns) in [-1/2, 1/2]; sincospi takes half turns.
-        sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cs);
-        s_cs[i] = make_float2(cs, a.sign * sn);
+        int axis;
+        if constexpr (std::is_same<Args, RotAxisArgs>::value)
+            axis = a.axis.axis[pair];
+        else
+            axis = pair / per_axis;
+        s_cs[i] = turn_of((double)pos[(tok0 + tok) * a.axes + axis], a.freq[pair], a.sign);
     }
     __syncthreads();
 #pragma unroll
@@ -138,8 +141,8 @@ __global__ __launch_bounds__(kRotThreads) void rotary_kernel(RotArgs a) {
 }
 
 // Cuts the tokens among workgroups for units of V elements, and launches.
-template <typename T, typename P, int V, bool kHalf>
-static bool rotary_go(RotArgs a, hipStream_t st) {
+template <typename T, typename P, int V, bool kHalf, typename Args>
+static bool rotary_go(Args a, hipStream_t st) {
     const int units = ((kHalf ? a.pairs : 2 * a.pairs) + a.dim - 2 * a.pairs) / V;
     const int64_t per_tok = (int64_t)(a.heads[0] + a.heads[1]) * units;
     constexpr int64_t kAll = kRotUnits * kRotThreads;
@@ -153,14 +156,14 @@ static bool rotary_go(RotArgs a, hipStream_t st) {
     if (!grid_fits(grid, kRotThreads)) return false;
     const int64_t bytes = a.tokens * (a.heads[0] + a.heads[1]) * a.dim * (int64_t)sizeof(T);
     if (bytes > kRotStreamBytes)
-        rotary_kernel<T, P, V, kHalf, true><<<(unsigned)grid, kRotThreads, 0, st>>>(a);
+        rotary_kernel<T, P, V, kHalf, true, Args><<<(unsigned)grid, kRotThreads, 0, st>>>(a);
     else
-        rotary_kernel<T, P, V, kHalf, false><<<(unsigned)grid, kRotThreads, 0, st>>>(a);
+        rotary_kernel<T, P, V, kHalf, false, Args><<<(unsigned)grid, kRotThreads, 0, st>>>(a);
     return true;
 }
 
-template <typename T, typename P>
-static bool rotary_launch(const RotArgs &a, bool half, hipStream_t st) {
+template <typename T, typename P, typename Args>
+static bool rotary_launch(const Args &a, bool half, hipStream_t st) {
     constexpr int V = kVec<T>;
     const int rest = a.dim - 2 * a.pairs;
     const bool wide = (half ? a.pairs : 2 * a.pairs) % V == 0 && rest % V == 0;
@@ -168,16 +171,13 @@ static bool rotary_launch(const RotArgs &a, bool half, hipStream_t st) {
     return wide ? rotary_go<T, P, V, false>(a, st) : rotary_go<T, P, 2, false>(a, st);
 }
 
-}  // namespace mg
-
-extern "C" int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q, int64_t q_token_stride,
-                             int64_t q_head_stride, int32_t q_heads, const void *k,
-                             int64_t k_token_stride, int64_t k_head_stride, int32_t k_heads,
-                             int32_t dim, const void *positions, int32_t positions_64,
-                             int32_t axes, const double *frequencies, int32_t pairs,
-                             int32_t interleaved, int32_t inverse, void *q_out, void *k_out,
-                             mg_stream_t stream) {
-    using namespace mg;
+static int32_t rotary_entry(int64_t tokens, int32_t dtype, const void *q, int64_t q_token_stride,
+                            int64_t q_head_stride, int32_t q_heads, const void *k,
+                            int64_t k_token_stride, int64_t k_head_stride, int32_t k_heads,
+                            int32_t dim, const void *positions, int32_t positions_64,
+                            int32_t axes, const uint8_t *axis_of, const double *frequencies,
+                            int32_t pairs, int32_t interleaved, int32_t inverse, void *q_out,
+                            void *k_out, mg_stream_t stream) {
     MG_REQUIRE(type_known(dtype), "mg_rotary: type code %d", dtype);
     MG_REQUIRE(tokens >= 0 && tokens < (int64_t(1) << 31), "mg_rotary: %lld tokens",
                (long long)tokens);
@@ -188,7 +188,7 @@ extern "C" int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q, int64
                "frequencies are taken", pairs, 2 * pairs, dim, kRotMaxPairs);
     MG_REQUIRE(interleaved == 0 || dim % 2 == 0,
                "mg_rotary: interleaved pairs need an even head dimension, got %d", dim);
-    MG_REQUIRE(axes >= 1 && pairs % axes == 0,
+    MG_REQUIRE(axes >= 1 && (axis_of || pairs % axes == 0),
                "mg_rotary: %d frequencies do not divide among %d axes", pairs, axes);
     // A workgroup's units are numbered in 32 bits.
     MG_REQUIRE((int64_t)(q_heads + k_heads) * dim <= (int64_t(1) << 30),
@@ -197,7 +197,10 @@ extern "C" int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q, int64
     if (tokens == 0) return MG_OK;
     MG_REQUIRE(q && q_out && positions && frequencies && (k_heads == 0 || (k && k_out)),
                "mg_rotary: a pointer is NULL");
-    RotArgs a{};
+    RotAxisArgs a{};
+    MG_REQUIRE(!axis_of || (pairs <= kAxisPairs && fill_axes(a.axis, axis_of, pairs, axes)),
+               "mg_rotary_axes: %d pairs, at most %d are taken, each by one of the %d axes of the "
+               "positions", pairs, kAxisPairs, axes);
     a.x[0] = q, a.x[1] = k, a.out[0] = q_out, a.out[1] = k_out;
     a.tok_stride[0] = q_token_stride, a.tok_stride[1] = k_token_stride;
     a.head_stride[0] = q_head_stride, a.head_stride[1] = k_head_stride;
@@ -211,8 +214,11 @@ extern "C" int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q, int64
     const bool half = interleaved == 0;
     const auto go = [&](auto t) {
         using T = decltype(t);
-        return positions_64 ? rotary_launch<T, int64_t>(a, half, st)
-                            : rotary_launch<T, int32_t>(a, half, st);
+        const auto with = [&](const auto &args) {
+            return positions_64 ? rotary_launch<T, int64_t>(args, half, st)
+                                : rotary_launch<T, int32_t>(args, half, st);
+        };
+        return axis_of ? with(a) : with(static_cast<const RotArgs &>(a));
     };
     const bool fits = dtype == MG_F32    ? go(float{})
                       : dtype == MG_BF16 ? go(bf16_t{})
@@ -222,3 +228,35 @@ extern "C" int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q, int64
     MG_LAUNCHED("rotary_kernel");
     return MG_OK;
 }
+
+}  // namespace mg
+
+extern "C" {
+
+int32_t mg_rotary(int64_t tokens, int32_t dtype, const void *q, int64_t q_token_stride,
+                  int64_t q_head_stride, int32_t q_heads, const void *k, int64_t k_token_stride,
+                  int64_t k_head_stride, int32_t k_heads, int32_t dim, const void *positions,
+                  int32_t positions_64, int32_t axes, const double *frequencies, int32_t pairs,
+                  int32_t interleaved, int32_t inverse, void *q_out, void *k_out,
+                  mg_stream_t stream) {
+    return mg::rotary_entry(tokens, dtype, q, q_token_stride, q_head_stride, q_heads, k,
+                            k_token_stride, k_head_stride, k_heads, dim, positions, positions_64,
+                            axes, nullptr, frequencies, pairs, interleaved, inverse, q_out, k_out,
+                            stream);
+}
+
+int32_t mg_rotary_axes(int64_t tokens, int32_t dtype, const void *q, int64_t q_token_stride,
+                       int64_t q_head_stride, int32_t q_heads, const void *k,
+                       int64_t k_token_stride, int64_t k_head_stride, int32_t k_heads,
+                       int32_t dim, const void *positions, int32_t positions_64, int32_t axes,
+                       const uint8_t *axis_of, const double *frequencies, int32_t pairs,
+                       int32_t interleaved, int32_t inverse, void *q_out, void *k_out,
+                       mg_stream_t stream) {
+    MG_REQUIRE(axis_of, "mg_rotary_axes: the pairs' axes are NULL");
+    return mg::rotary_entry(tokens, dtype, q, q_token_stride, q_head_stride, q_heads, k,
+                            k_token_stride, k_head_stride, k_heads, dim, positions, positions_64,
+                            axes, axis_of, frequencies, pairs, interleaved, inverse, q_out, k_out,
+                            stream);
+}
+
+}  // extern "C"

@@ -6,6 +6,8 @@ that predicts or refines splats, next to ``layer_norm`` and ``attention``.
 
 from __future__ import annotations
 
+import ctypes
+import functools
 import math
 
 import torch
@@ -13,6 +15,7 @@ import torch
 from . import _lib
 
 LAYOUTS = ("half", "interleaved")
+ORDERS = ("runs", "turns")
 
 
 def rotary_frequencies(dims: int, base: float = 10000.0, *, axes: int = 1,
@@ -58,7 +61,36 @@ def _heads(x: torch.Tensor):
     return x if x.stride(2) == 1 or x.shape[2] == 1 else x.contiguous()
 
 
-def _turn(q, k, positions, frequencies, layout, inverse):
+@functools.lru_cache(maxsize=256)
+def _table(sections: tuple, order: str):
+    """The axis of each pair, a byte each."""
+    if order not in ORDERS:
+        raise ValueError(f"unknown order {order!r}; expected one of {ORDERS}")
+    if not 1 <= len(sections) <= 256 or any(n < 0 for n in sections) \
+            or not 1 <= sum(sections) <= 256:
+        raise ValueError(f"sections {sections} must be numbers of pairs, up to 256 in all")
+    turn = [(n, a) for a, count in enumerate(sections) for n in range(count)]
+    if order == "turns":
+        turn.sort()
+    return ctypes.create_string_buffer(bytes(a for _, a in turn), len(turn))
+
+
+def axis_table(sections, order, positions, frequencies):
+    """The axis of each pair as the C calls take it, or None for equal runs."""
+    if sections is None:
+        if order != "runs":
+            raise ValueError(f"order {order!r} needs sections")
+        return None
+    sections = tuple(sections)
+    table = _table(sections, order)
+    axes = 1 if positions.dim() == 1 else positions.shape[1]
+    if len(sections) != axes or len(table) != frequencies.numel():
+        raise ValueError(f"sections {sections} must be one for each of the {axes} axes and add "
+                         f"up to the {frequencies.numel()} frequencies")
+    return table
+
+
+def _turn(q, k, positions, frequencies, layout, table, inverse):
     lib = _lib.load()
     q = _heads(q)
     T, Hq, D = q.shape
@@ -68,21 +100,23 @@ def _turn(q, k, positions, frequencies, layout, inverse):
         k = _heads(k)
         k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
         k_args, k_to = (k.data_ptr(), k.stride(0), k.stride(1), k.shape[1]), k_out.data_ptr()
-    _lib.launch(lib.mg_rotary, q.get_device(), T, _lib.TYPE_CODES[q.dtype], q.data_ptr(),
+    fn, axis_of = (lib.mg_rotary, ()) if table is None else (lib.mg_rotary_axes, (table,))
+    _lib.launch(fn, q.get_device(), T, _lib.TYPE_CODES[q.dtype], q.data_ptr(),
                 q.stride(0), q.stride(1), Hq, *k_args, D, positions.data_ptr(),
                 positions.dtype == torch.int64,
-                1 if positions.dim() == 1 else positions.shape[1], frequencies.data_ptr(),
-                frequencies.numel(), layout == "interleaved", inverse, q_out.data_ptr(), k_to)
+                1 if positions.dim() == 1 else positions.shape[1], *axis_of,
+                frequencies.data_ptr(), frequencies.numel(), layout == "interleaved", inverse,
+                q_out.data_ptr(), k_to)
     return q_out, k_out
 
 
 class _Rotary(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, positions, frequencies, layout):
+    def forward(ctx, q, k, positions, frequencies, layout, table):
         ctx.save_for_backward(positions, frequencies)
-        ctx.layout, ctx.dtype = layout, q.dtype
+        ctx.layout, ctx.table, ctx.dtype = layout, table, q.dtype
         ctx.set_materialize_grads(False)
-        return _turn(q, k, positions, frequencies, layout, False)
+        return _turn(q, k, positions, frequencies, layout, table, False)
 
     @staticmethod
     @_lib.differentiable_once
@@ -91,30 +125,17 @@ class _Rotary(torch.autograd.Function):
         positions, frequencies = (t.contiguous() for t in ctx.saved_tensors)
         dtype = ctx.dtype
         if dq is None and dk is None:
-            return None, None, None, None, None
+            return None, None, None, None, None, None
         first, second = (dq, dk) if dq is not None else (dk, None)
         first = first.to(dtype)
         second = None if second is None else second.to(dtype)
-        a, b = _turn(first, second, positions, frequencies, ctx.layout, True)
-        return (a, b, None, None, None) if dq is not None else (None, a, None, None, None)
+        a, b = _turn(first, second, positions, frequencies, ctx.layout, ctx.table, True)
+        return (a, b, None, None, None, None) if dq is not None else \
+            (None, a, None, None, None, None)
 
 
-def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
-           frequencies: torch.Tensor, *, layout: str = "half"):
-    """Turn pairs of each head's first ``2 * frequencies.numel()`` elements by
-    ``position * frequency`` radians; the rest of the head is copied.
-
-    ``q`` (tokens, heads, dim) and ``k`` (tokens, its own heads, dim; or None) are
-    float32, bfloat16 or float16, with any strides over tokens and heads, so
-    slices of one projection go as they are. ``positions`` is (tokens,) or
-    (tokens, axes), int32 or int64, of any size or sign; ``frequencies`` comes from
-    ``rotary_frequencies`` (float64 on the GPU). ``layout`` pairs elements (i, P + i)
-    ("half") or (2i, 2i + 1) ("interleaved").
-
-    Returns new contiguous tensors (q, k), or q alone where k is None; one launch
-    for both, one for both gradients. Differentiable in q and k; frequencies that
-    require a gradient are refused.
-    """
+def _check(q, k, positions, frequencies, layout):
+    """The GPU of all of them, and contiguous positions."""
     code = _lib.type_code(q, "q")
     if q.dim() != 3:
         raise ValueError(f"q must be (tokens, heads, dim), got {tuple(q.shape)}")
@@ -140,11 +161,37 @@ def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
                            f"'{frequencies.device}'")
     if frequencies.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("frequencies must not require a gradient: there is none for them")
-    if not positions.is_contiguous():
-        positions = positions.contiguous()
+    return index, positions if positions.is_contiguous() else positions.contiguous()
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
+           frequencies: torch.Tensor, *, layout: str = "half",
+           sections: tuple[int, ...] | None = None, order: str = "runs"):
+    """Turn pairs of each head's first ``2 * frequencies.numel()`` elements by
+    ``position * frequency`` radians; the rest of the head is copied.
+
+    ``q`` (tokens, heads, dim) and ``k`` (tokens, its own heads, dim; or None) are
+    float32, bfloat16 or float16, with any strides over tokens and heads, so
+    slices of one projection go as they are. ``positions`` is (tokens,) or
+    (tokens, axes), int32 or int64, of any size or sign; ``frequencies`` comes from
+    ``rotary_frequencies`` (float64 on the GPU). ``layout`` pairs elements (i, P + i)
+    ("half") or (2i, 2i + 1) ("interleaved").
+
+    With several axes (frame, row and column) the pairs are dealt to them in equal
+    runs, or as ``sections`` says: one number of pairs for each axis (0 is taken),
+    in all those of ``frequencies`` and 256 at most. ``order="runs"`` gives each axis
+    neighbouring pairs; ``"turns"`` deals pair after pair to the axes in turn, an axis
+    with its pairs dealt being left out, so that every axis has fast and slow ones.
+
+    Returns new contiguous tensors (q, k), or q alone where k is None; one launch
+    for both, one for both gradients. Differentiable in q and k; frequencies that
+    require a gradient are refused.
+    """
+    _, positions = _check(q, k, positions, frequencies, layout)
+    table = axis_table(sections, order, positions, frequencies)
     if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) \
             or _lib.forward_mode():
-        out = _Rotary.apply(q, k, positions, frequencies, layout)
+        out = _Rotary.apply(q, k, positions, frequencies, layout, table)
     else:
-        out = _turn(q, k, positions, frequencies, layout, False)
+        out = _turn(q, k, positions, frequencies, layout, table, False)
     return out if k is not None else out[0]

@@ -1,6 +1,7 @@
 """Plain float64 restatements of the token operators (layer norm, rotary
-positions, attention over packed sequences) and of their gradients, one row,
-head and sequence at a time, from the definitions alone. CPU, numpy."""
+positions, heads normed and turned, dropout, attention over packed sequences) and
+of their gradients, one row, head and sequence at a time, from the definitions
+alone. CPU, numpy."""
 
 from __future__ import annotations
 
@@ -47,6 +48,67 @@ def rotary(x, positions, frequencies, layout, inverse=False):
         p, q = np.array(x[..., a], np.float64), np.array(x[..., b], np.float64)
         y[..., a], y[..., b] = p * c - q * s, q * c + p * s
     return y
+
+
+def axes_of(sections, order):
+    """The axis of each pair: each axis's pairs as neighbours ("runs"), or pair after
+    pair dealt to the axes that have pairs left ("turns")."""
+    if order == "runs":
+        return [a for a, n in enumerate(sections) for _ in range(n)]
+    return [a for n in range(max(sections)) for a in range(len(sections)) if n < sections[a]]
+
+
+def rotary_axes(x, positions, frequencies, layout, axes, inverse=False):
+    """`rotary` with pair i going by positions[:, axes[i]]."""
+    return rotary(x, np.asarray(positions)[:, axes], frequencies, layout, inverse)
+
+
+# ------------------------------------------------------- heads normed and turned
+
+def norm_rotary(x, weight, eps, turn):
+    """turn(x / sqrt(mean(x^2) + eps) * weight), of heads x (tokens, heads, dim)."""
+    x = np.asarray(x, np.float64)
+    u = x / np.sqrt((x ** 2).mean(-1, keepdims=True) + eps)
+    return turn(u if weight is None else u * weight)
+
+
+def norm_rotary_grad(x, weight, eps, turn_back, dy):
+    """(dx, dweight), each head by its Jacobian."""
+    x, n = np.asarray(x, np.float64), x.shape[-1]
+    w = np.ones(n) if weight is None else np.asarray(weight, np.float64)
+    g = turn_back(np.asarray(dy, np.float64))
+    dx, dw = np.zeros_like(x), np.zeros(n)
+    for t in range(x.shape[0]):
+        for h in range(x.shape[1]):
+            s = 1.0 / np.sqrt((x[t, h] ** 2).mean() + eps)
+            u = x[t, h] * s
+            d = g[t, h] * w
+            dx[t, h] = s * (d - u * (d * u).mean())
+            dw += g[t, h] * u
+    return dx, dw
+
+
+# ----------------------------------------------------------------- dropout
+
+def philox4x32(counter, key):
+    """One block of Philox4x32-10: four words of 32 bits of four and two."""
+    c, k = list(counter), list(key)
+    for _ in range(10):
+        a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
+        c = [(b >> 32) ^ c[1] ^ k[0], b & 0xFFFFFFFF, (a >> 32) ^ c[3] ^ k[1], a & 0xFFFFFFFF]
+        k = [(k[0] + 0x9E3779B9) & 0xFFFFFFFF, (k[1] + 0xBB67AE85) & 0xFFFFFFFF]
+    return c
+
+
+def kept(n, drop, seed, site=0, first=0):
+    """Truth values of elements first .. first + n - 1: 16 bits of the block of every
+    eight, at least `drop`."""
+    out = []
+    for i in range(first, first + n):
+        w = philox4x32((i // 8 & 0xFFFFFFFF, i // 8 >> 32, site & 0xFFFFFFFF, site >> 32),
+                       (seed & 0xFFFFFFFF, seed >> 32))[i % 8 // 2]
+        out.append((w >> 16 if i % 2 else w & 0xFFFF) >= drop)
+    return np.array(out, bool)
 
 
 # --------------------------------------------------------------- attention
