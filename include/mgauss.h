@@ -790,6 +790,34 @@ int32_t mg_attention_backward(
     int64_t dout_head_stride, void *dq, void *dk, void *dv, void *workspace,
     int64_t workspace_bytes, mg_stream_t stream);
 
+/* The same with a window, causal: a query sees the last `window` (1 or more) of the
+ * keys at or before it, and the first `sinks` of its sequence. */
+int64_t mg_attention_window_forward_workspace_bytes(
+    int64_t q_tokens, int64_t k_tokens, int32_t q_heads, int32_t k_heads,
+    int32_t dim, int32_t sequences, int32_t window, int32_t sinks);
+int32_t mg_attention_window_forward(
+    int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+    int32_t k_heads, int32_t dim, const void *q, int64_t q_token_stride,
+    int64_t q_head_stride, const void *k, int64_t k_token_stride,
+    int64_t k_head_stride, const void *v, int64_t v_token_stride,
+    int64_t v_head_stride, const int32_t *q_offsets, const int32_t *k_offsets,
+    int32_t sequences, int32_t window, int32_t sinks, float scale, void *out,
+    void *out_rest, float *lse, void *workspace, int64_t workspace_bytes,
+    mg_stream_t stream);
+int64_t mg_attention_window_backward_workspace_bytes(
+    int64_t q_tokens, int64_t k_tokens, int32_t q_heads, int32_t k_heads,
+    int32_t dim, int32_t sequences, int32_t window, int32_t sinks);
+int32_t mg_attention_window_backward(
+    int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+    int32_t k_heads, int32_t dim, const void *q, int64_t q_token_stride,
+    int64_t q_head_stride, const void *k, int64_t k_token_stride,
+    int64_t k_head_stride, const void *v, int64_t v_token_stride,
+    int64_t v_head_stride, const int32_t *q_offsets, const int32_t *k_offsets,
+    int32_t sequences, int32_t window, int32_t sinks, float scale,
+    const void *out, const void *out_rest, const float *lse, const void *dout,
+    int64_t dout_token_stride, int64_t dout_head_stride, void *dq, void *dk,
+    void *dv, void *workspace, int64_t workspace_bytes, mg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

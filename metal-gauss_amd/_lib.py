@@ -151,6 +151,17 @@ _SIGNATURES = {
                                      _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32, _f32,
                                      _vp, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _vp, _i64,
                                      _vp]),
+    "mg_attention_window_forward_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32,
+                                                           _i32, _i32]),
+    "mg_attention_window_forward": (_i32, [_i32, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64,
+                                           _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32, _i32,
+                                           _i32, _f32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mg_attention_window_backward_workspace_bytes": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32,
+                                                            _i32, _i32]),
+    "mg_attention_window_backward": (_i32, [_i32, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64,
+                                            _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32,
+                                            _i32, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _i64, _vp,
+                                            _vp, _vp, _vp, _i64, _vp]),
 }
 
 EXPORTS = tuple(_SIGNATURES)

@@ -29,8 +29,18 @@ def _rows(x: torch.Tensor):
     return x, (at if tokens else None, tok, head)
 
 
-def _forward(q, k, v, q_offsets, k_offsets, causal, scale, keep):
+def _calls(lib, which, causal, window):
+    """The C entry and its workspace query, with what each takes of the mask."""
+    if window is None:
+        return (getattr(lib, f"mg_attention_{which}"), (causal,),
+                getattr(lib, f"mg_attention_{which}_workspace_bytes"), ())
+    return (getattr(lib, f"mg_attention_window_{which}"), window,
+            getattr(lib, f"mg_attention_window_{which}_workspace_bytes"), window)
+
+
+def _forward(q, k, v, q_offsets, k_offsets, causal, window, scale, keep):
     lib = _lib.load()
+    call, mask, workspace, more = _calls(lib, "forward", causal, window)
     (q, q_at), (k, k_at), (v, v_at) = _rows(q), _rows(k), _rows(v)
     Tq, Hq, D = q.shape
     Tk, Hk, _ = k.shape
@@ -39,12 +49,12 @@ def _forward(q, k, v, q_offsets, k_offsets, causal, scale, keep):
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     rest = torch.empty_like(out) if keep else None
     lse = torch.empty(Hq, Tq, device=q.device) if keep else None
-    need = lib.mg_attention_forward_workspace_bytes(Tq, Tk, Hq, Hk, D, n)
+    need = workspace(Tq, Tk, Hq, Hk, D, n, *more)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    _lib.launch(lib.mg_attention_forward, q.get_device(), _lib.TYPE_CODES[q.dtype], Tq, Tk, Hq,
+    _lib.launch(call, q.get_device(), _lib.TYPE_CODES[q.dtype], Tq, Tk, Hq,
                 Hk, D, *q_at, *k_at, *v_at,
                 None if q_offsets is None else q_offsets.data_ptr(),
-                None if k_offsets is None else k_offsets.data_ptr(), n, causal, scale,
+                None if k_offsets is None else k_offsets.data_ptr(), n, *mask, scale,
                 out.data_ptr(), rest.data_ptr() if keep else None,
                 lse.data_ptr() if keep else None,
                 ws.data_ptr() if need else None, need)
@@ -53,10 +63,11 @@ def _forward(q, k, v, q_offsets, k_offsets, causal, scale, keep):
 
 class _Attention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, q_offsets, k_offsets, causal, scale):
-        out, rest, lse, q, k, v = _forward(q, k, v, q_offsets, k_offsets, causal, scale, True)
+    def forward(ctx, q, k, v, q_offsets, k_offsets, causal, window, scale):
+        out, rest, lse, q, k, v = _forward(q, k, v, q_offsets, k_offsets, causal, window, scale,
+                                           True)
         ctx.save_for_backward(q, k, v, q_offsets, k_offsets, out, rest, lse)
-        ctx.causal, ctx.scale = causal, scale
+        ctx.causal, ctx.window, ctx.scale = causal, window, scale
         return out
 
     @staticmethod
@@ -67,7 +78,7 @@ class _Attention(torch.autograd.Function):
         q_offsets, k_offsets, out, rest, lse = (
             None if t is None else t.contiguous() for t in others)
         (q, q_at), (k, k_at), (v, v_at) = _rows(q), _rows(k), _rows(v)
-        lib = _lib.load()
+        call, mask, workspace, more = _calls(_lib.load(), "backward", ctx.causal, ctx.window)
         Tq, Hq, D = q.shape
         Tk, Hk = k.shape[0], k.shape[1]
         n = 1 if q_offsets is None else q_offsets.numel() - 1
@@ -76,16 +87,16 @@ class _Attention(torch.autograd.Function):
         keys = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dk = torch.empty(Tk, Hk, D, dtype=q.dtype, device=q.device) if keys else None
         dv = torch.empty(Tk, Hk, D, dtype=q.dtype, device=q.device) if keys else None
-        need = lib.mg_attention_backward_workspace_bytes(Tq, Tk, Hq, Hk, D, n)
+        need = workspace(Tq, Tk, Hq, Hk, D, n, *more)
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _lib.launch(lib.mg_attention_backward, q.get_device(), _lib.TYPE_CODES[q.dtype], Tq, Tk,
+        _lib.launch(call, q.get_device(), _lib.TYPE_CODES[q.dtype], Tq, Tk,
                     Hq, Hk, D, *q_at, *k_at, *v_at,
                     None if q_offsets is None else q_offsets.data_ptr(),
-                    None if k_offsets is None else k_offsets.data_ptr(), n, ctx.causal,
+                    None if k_offsets is None else k_offsets.data_ptr(), n, *mask,
                     ctx.scale, out.data_ptr(), rest.data_ptr(), lse.data_ptr(), *dout_at, dq.data_ptr(),
                     dk.data_ptr() if keys else None, dv.data_ptr() if keys else None,
                     ws.data_ptr(), need)
-        return dq, dk, dv, None, None, None, None
+        return dq, dk, dv, None, None, None, None, None
 
 
 def _check_offsets(off, what, index):
@@ -99,7 +110,8 @@ def _check_offsets(off, what, index):
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
               q_offsets: torch.Tensor | None = None, k_offsets: torch.Tensor | None = None, *,
-              causal: bool = False, scale: float | None = None) -> torch.Tensor:
+              causal: bool = False, window: int | None = None, sinks: int = 0,
+              scale: float | None = None) -> torch.Tensor:
     """softmax(scale * q k^T) v within each of the sequences packed one after the
     other along the tokens.
 
@@ -118,6 +130,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     last key. A query that sees no key, or belongs to no sequence, gets zeros;
     infinities and NaN in keys and values that it does not see leave no trace in
     its result (the backward pass asks for finite inputs within a sequence).
+
+    ``window`` (with ``causal``; 1 or more) leaves a query the last ``window`` of these
+    keys, its own included, and the sequence's first ``sinks``; time and memory go by
+    the keys that are left.
+
     ``scale`` (default dim ** -0.5) may not be negative.
 
     Scores, softmax and sums are float32; p is rounded to the inputs' type for
@@ -151,7 +168,16 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             raise ValueError(f"q_offsets is {tuple(q_offsets.shape)} and k_offsets "
                              f"{tuple(k_offsets.shape)}; one number of sequences is needed")
     scale = max(dim, 1) ** -0.5 if scale is None else float(scale)
+    if window is not None:
+        if not causal:
+            raise ValueError("window needs causal=True")
+        if window < 1 or sinks < 0:
+            raise ValueError(f"window must be at least 1 and sinks 0, got {window} and {sinks}")
+        # More than any tensor has is all of them.
+        window = (min(int(window), 2 ** 31 - 1), min(int(sinks), 2 ** 31 - 1))
+    elif sinks:
+        raise ValueError("sinks needs window: without one all first keys are seen")
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) \
             or _lib.forward_mode():
-        return _Attention.apply(q, k, v, q_offsets, k_offsets, bool(causal), scale)
-    return _forward(q, k, v, q_offsets, k_offsets, bool(causal), scale, False)[0]
+        return _Attention.apply(q, k, v, q_offsets, k_offsets, bool(causal), window, scale)
+    return _forward(q, k, v, q_offsets, k_offsets, bool(causal), window, scale, False)[0]

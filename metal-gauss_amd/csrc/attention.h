@@ -42,6 +42,9 @@ struct AttnArgs {
     int32_t q_tokens, k_tokens;
     int32_t k_heads, group, dim;         // q_heads = k_heads * group
     int32_t causal;
+    // With a window (causal): a query sees the last `window` keys up to where it
+    // stands, and the sequence's first `sinks`. 0: no window.
+    int32_t window, sinks;
     float scale, scale_log2;             // scale, scale * log2(e)
     void *out;                           // (q_tokens, q_heads, dim)
     void *out_rest;                      // what rounding took from out, or NULL
@@ -50,6 +53,7 @@ struct AttnArgs {
     // chunks_of), whose {top, sum} and unscaled sums of values are joined
     // afterwards.
     int32_t split_keys, chunk_tiles;
+    int32_t span_extra, span_most;       // of the keys an item goes through: span_keys
     float2 *part_stats;
     float *part_o;
     // Backward.
@@ -60,6 +64,10 @@ struct AttnArgs {
     // least, each in float32 (part_of).
     int32_t splits, split_steps;
     float *part;
+    // With sinks: the first keys' gradients from queries further on than the
+    // window, in runs of sink_steps query tiles of one head (attention_bwd.hip).
+    int32_t sink_items, sink_steps, sink_rows;
+    float *sink_part;
 };
 
 // ---------------------------------------------------------------- sequences
@@ -154,6 +162,47 @@ __device__ __forceinline__ SeqItem find_item(const AttnArgs &a, int item, Count 
         base2 += __builtin_amdgcn_readlane(upto2, 63);
     }
     return r;
+}
+
+// ------------------------------------------------------------------ windows
+// The first key of a query's window.
+__device__ __forceinline__ int key_low(const AttnArgs &a, const SeqItem &s, int token) {
+    return max(0, token + 1 + s.k_len - s.q_len - a.window);
+}
+
+// The keys that the queries from `first` to `last` go through, numbered in the order
+// they are: all from the first to the last seen, or, with a window, first the
+// sinks in whole tiles, then those from the first query's window on that are
+// none. A sink lies in a query's window or before it: it counts as a sink.
+struct KeyRun {
+    int sink, sink_up, start, end;
+};
+template <bool kWin, int kTile>
+__device__ __forceinline__ KeyRun key_run(const AttnArgs &a, const SeqItem &s, int first,
+                                          int seen_to) {
+    if constexpr (!kWin) return {0, 0, 0, seen_to};
+    const int sink = min(a.sinks, seen_to), start = max(key_low(a, s, first), sink);
+    const int sink_up = (sink + kTile - 1) / kTile * kTile;
+    return {sink, sink_up, start, sink_up + max(0, seen_to - start)};
+}
+
+// The key of a number in the run.
+template <bool kWin>
+__device__ __forceinline__ int key_at(const KeyRun &r, int number) {
+    return !kWin ? number : number < r.sink_up ? number : number - r.sink_up + r.start;
+}
+
+// The bounds of what a query sees, within the tile of a number: among the sinks,
+// they alone; past them, the window alone.
+struct TileSees {
+    bool sinks;
+    int sink;
+    __device__ __forceinline__ int to(int see) const { return sinks ? min(see, sink) : see; }
+    __device__ __forceinline__ int from(int low) const { return sinks ? 0 : low; }
+};
+template <bool kWin>
+__device__ __forceinline__ TileSees tile_sees(const KeyRun &r, int number) {
+    return {kWin && number < r.sink_up, r.sink};
 }
 
 // ------------------------------------------------------------- longest first
@@ -410,6 +459,12 @@ static void attn_form(int32_t dtype, int dim, F f) {
 inline float scale_to_log2(float scale) {
     const float s = scale * 1.44269504088896340736f;
     return s < 1e-30f ? 1e-30f : s;
+}
+
+// Window and sinks held to the keys: a window of all of them is none.
+inline void hold_window(AttnArgs &a) {
+    if (a.window >= a.k_tokens) a.window = a.sinks = 0;
+    if (a.sinks > a.k_tokens) a.sinks = a.k_tokens;
 }
 
 int32_t attn_check(const char *who, const AttnArgs &a, int32_t dtype);

@@ -3,8 +3,9 @@
 //   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i k_j - lse_i)
 //
 // over the keys j of query i's own sequence, causal: those that stand at or
-// before it, a sequence's last query standing at its last key. Queries that see
-// no key give zeros.
+// before it, a sequence's last query standing at its last key; with a window, the
+// last `window` of these and the sequence's first `sinks`. Queries that see no key
+// give zeros.
 //
 // A work item is a tile of rows of one key head, a row being a query token
 // together with one of the `group` query heads that share the head: a single
@@ -90,13 +91,17 @@ __device__ __forceinline__ bool clear_not_finite(char *tile, int wave) {
     return ballot(found) != 0;
 }
 
-// Adds what is not finite of keys from .. to - 1 to the rows that see them.
-template <typename T, int DK>
+// Adds what is not finite of the run's keys from .. to - 1 to the rows that see
+// them.
+template <typename T, int DK, bool kWin>
 __device__ __forceinline__ void add_seen_values(const char *head, int64_t tok_stride, int dim,
-                                                int from, int to, int see, int half,
-                                                f32x16 (&o)[DK / 32]) {
+                                                const KeyRun &run, int from, int to, int low,
+                                                int see, int half, f32x16 (&o)[DK / 32]) {
 #pragma unroll 1
-    for (int key = from; key < to; ++key) {
+    for (int number = from; number < to; ++number) {
+        if (kWin && number >= run.sink && number < run.sink_up) continue;
+        const int key = key_at<kWin>(run, number);
+        const bool sees = key < see && (!kWin || number < run.sink_up || key >= low);
         const T *row = reinterpret_cast<const T *>(head) + (int64_t)key * tok_stride;
         // No branches: a row that does not see the key adds 0.
 #pragma unroll
@@ -108,7 +113,7 @@ __device__ __forceinline__ void add_seen_values(const char *head, int64_t tok_st
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float f = (float)v[k];
-                    o[b][e + k] += key < see && f - f != 0.f ? f : 0.f;
+                    o[b][e + k] += sees && f - f != 0.f ? f : 0.f;
                 }
             }
     }
@@ -151,13 +156,18 @@ __device__ __forceinline__ int chunk_keys(const AttnArgs &a, int tiles) {
     if (tiles <= a.chunk_tiles) return a.split_keys;
     return a.split_keys * ((tiles + a.chunk_tiles - 1) / a.chunk_tiles);
 }
+// Keys that an item goes through at most: with a window, its own and the sinks'
+// tiles, whatever the sequence has.
+__device__ __forceinline__ int span_keys(const AttnArgs &a, int keys) {
+    return min(keys + a.span_extra, a.span_most);
+}
 __device__ __forceinline__ int chunks_of(const AttnArgs &a, int tiles, int keys) {
     const int each = chunk_keys(a, tiles);
-    return max(1, (keys + each - 1) / each);
+    return max(1, (span_keys(a, keys) + each - 1) / each);
 }
 
 // One work item: false if there is none of this number.
-template <typename T, int DK, int kWaves, bool kSplit>
+template <typename T, int DK, int kWaves, bool kSplit, bool kWin>
 __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     constexpr int kRows = 32 * kWaves, kSteps = DK / 16, kBlocks = DK / 32;
     constexpr bool kInterleave = kWaves == kWideWaves;
@@ -186,6 +196,11 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
         split_keys = chunk_keys(a, tiles);
         tile = tiles - 1 - s.within / chunks;
         chunk = s.within % chunks;
+    } else if constexpr (kWin) {
+        // Most tiles have a window's keys: no order would even them out.
+        s = find_item<false>(a, item, tiles_of, [](int, int) { return 0; });
+        if (!s.found) return false;
+        tile = tiles_of(s.q_len, 0) - 1 - s.within;
     } else {
         s = find_longest<false>(a, item, kRows);
         if (!s.found) return false;
@@ -203,7 +218,13 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     const int last_token = min((tile * kRows + kRows - 1) / G, s.q_len - 1);
     const int see_first = keys_seen(s, min(row0 / G, s.q_len - 1), a.causal);
     const int see_last = keys_seen(s, min((row0 + 31) / G, s.q_len - 1), a.causal);
-    int k_from = 0, k_to = keys_seen(s, last_token, a.causal);
+    const int low = kWin ? key_low(a, s, token) : 0;
+    const int low_first = kWin ? key_low(a, s, min(row0 / G, s.q_len - 1)) : 0;
+    const int low_last = kWin ? key_low(a, s, min((row0 + 31) / G, s.q_len - 1)) : 0;
+    const int low_most = kWin ? key_low(a, s, last_token) : 0;
+    const KeyRun run = key_run<kWin, kTile>(a, s, min(tile * kRows / G, s.q_len - 1),
+                                            keys_seen(s, last_token, a.causal));
+    int k_from = 0, k_to = run.end;               // numbers in the run
     if (kSplit) {
         k_from = min(chunk * split_keys, k_to);
         k_to = min(k_from + split_keys, k_to);
@@ -242,25 +263,31 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
         s_not_finite = k_to;
     TileLane<T, DK> lane_at;
     int buf = 0;
-    if (k_from < k_to) ask(k_from, 0);
+    if (k_from < k_to) ask(key_at<kWin>(run, k_from), 0);
     loads_done();
-    for (int key0 = k_from; key0 < k_to; key0 += kTile, buf ^= 1) {
+    for (int number = k_from; number < k_to; number += kTile, buf ^= 1) {
+        const int key0 = key_at<kWin>(run, number);
+        const TileSees sees = tile_sees<kWin>(run, number);
         tiles_ready();
         lane_at.fresh();
-        if (key0 + kTile > see_least) {
+        if (key0 + kTile > sees.to(see_least) || (kWin && key0 < sees.from(low_most))) {
             const bool found = clear_not_finite<T, DK, kTile, kWaves>(s_tile[buf][1], wave);
             if constexpr (kWaves == 1) {
-                if (found) not_finite_from = min(not_finite_from, key0);
+                if (found) not_finite_from = min(not_finite_from, number);
             } else {
-                if (found && lane == 0 && key0 < s_not_finite) s_not_finite = key0;
+                if (found && lane == 0 && number < s_not_finite) s_not_finite = number;
             }
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
         const char *kt = s_tile[buf][0], *vt = s_tile[buf][1];
         f32x16 sc[kParts] = {};
-        const int next0 = key0 + kTile;
+        const bool more = number + kTile < k_to;
+        const int next0 = key_at<kWin>(run, number + kTile);
+        // The wave's rows see none of these keys.
+        const bool none =
+            key0 >= sees.to(see_last) || (kWin && key0 + kTile <= sees.from(low_first));
         constexpr int kEach = decltype(fill_k)::kLoads;
-        if (kInterleave && next0 + kTile <= s.k_len && next0 < k_to && key0 < see_last) {
+        if (kInterleave && next0 + kTile <= s.k_len && more && !none) {
             // The next tile's loads one by one between the products: all at once
             // they queue before the wave's first product (2.4% of a prompt of
             // 16320 with 128 columns, 1% with 64).
@@ -281,21 +308,24 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
                         fill_v.load(l - kEach, ov);
             }
         } else {
-            if (next0 < k_to) ask(next0, buf ^ 1);
-            if (key0 >= see_last) continue;   // the wave's rows see none of these keys
+            if (more) ask(next0, buf ^ 1);
+            if (none) continue;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
 #pragma unroll
                 for (int b = 0; b < kParts; ++b)
                     sc[b] = mfma32(lane_at.rows(kt, 32 * b, i), q[i], sc[b]);
         }
-        if (key0 + kTile > see_first) {
+        if (key0 + kTile > sees.to(see_first) || (kWin && key0 < sees.from(low_last))) {
             // Selected, not added to: a NaN of a key that is not seen goes too.
+            const int to = sees.to(see), from = sees.from(low);
 #pragma unroll
             for (int b = 0; b < kParts; ++b)
 #pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (key0 + 32 * b + c_row(e, half) >= see) sc[b][e] = -INFINITY;
+                for (int e = 0; e < 16; ++e) {
+                    const int key = key0 + 32 * b + c_row(e, half);
+                    if (key >= to || (kWin && key < from)) sc[b][e] = -INFINITY;
+                }
         }
         float most = sc[0][0];
 #pragma unroll
@@ -335,8 +365,8 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     if (k_from < k_to) {
         if constexpr (kWaves > 1) not_finite_from = uniform(s_not_finite);
         if (not_finite_from < k_to)
-            add_seen_values<T, DK>(vp, a.v.tok_stride, a.dim, not_finite_from,
-                                   min(see_last, k_to), see, half, o);
+            add_seen_values<T, DK, kWin>(vp, a.v.tok_stride, a.dim, run, not_finite_from,
+                                         kWin ? k_to : min(see_last, k_to), low, see, half, o);
     }
     sum = halves_sum(sum);
 
@@ -364,12 +394,12 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
 
 // How many items the chunks make is known on the device alone: as many
 // workgroups as fill the GPU take them in turn.
-template <typename T, int DK, int kWaves, bool kSplit>
+template <typename T, int DK, int kWaves, bool kSplit, bool kWin>
 __global__ __launch_bounds__(64 * kWaves, kWaves == 1 ? 1 : 2) void attn_fwd_kernel(AttnArgs a) {
     if constexpr (!kSplit) {
-        attn_fwd_item<T, DK, kWaves, kSplit>(a, blockIdx.x);
+        attn_fwd_item<T, DK, kWaves, kSplit, kWin>(a, blockIdx.x);
     } else {
-        for (int work = blockIdx.x; attn_fwd_item<T, DK, kWaves, kSplit>(a, work);
+        for (int work = blockIdx.x; attn_fwd_item<T, DK, kWaves, kSplit, kWin>(a, work);
              work += gridDim.x)
             tiles_ready();
     }
@@ -529,6 +559,9 @@ int32_t attn_check(const char *who, const AttnArgs &a, int32_t dtype) {
     MG_REQUIRE((a.q_off == nullptr) == (a.k_off == nullptr),
                "%s: offsets of queries and keys go together", who);
     MG_REQUIRE(a.scale >= 0.f && a.scale < INFINITY, "%s: scale %g", who, (double)a.scale);
+    MG_REQUIRE(a.window >= 0 && a.sinks >= 0 && (a.window > 0 || a.sinks == 0),
+               "%s: a window of %d keys and %d first ones", who, a.window, a.sinks);
+    MG_REQUIRE(a.window == 0 || a.causal, "%s: a window is for causal attention", who);
     for (const AttnTensor *t : {&a.q, &a.k, &a.v, &a.dout}) {
         MG_REQUIRE(((uintptr_t)t->p & 15) == 0 && t->tok_stride % 8 == 0 &&
                        t->head_stride % 8 == 0,
@@ -550,6 +583,7 @@ struct FwdPlan {
     int split_keys;             // 0: whole rows
     int64_t chunk_tiles;        // see chunk_keys
     int64_t tiles, items;       // a key head's, at most
+    int32_t span_extra, span_most;
     int64_t stats_bytes, bytes; // of partial results
 };
 
@@ -561,7 +595,7 @@ constexpr int64_t kWideSlots = 512, kNarrowSlots = 1536;
 constexpr int64_t kSplitLeast = 768, kChunkLeast = 256;
 
 static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int group, int dim,
-                        int n_seq) {
+                        int n_seq, int window, int sinks) {
     FwdPlan p{};
     const int64_t rows = q_tokens * group;
     p.waves = rows <= 64 * (int64_t)n_seq ? kNarrowWaves : kWideWaves;
@@ -572,6 +606,16 @@ static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int gro
     // The tokens before the first and past the last offset make tiles too.
     p.items = p.tiles = rows / tile_rows + n_seq + 2;
     const int64_t likely = (ceil_div(rows, tile_rows) + n_seq - 1) * k_heads;
+    // A window bounds the keys that an item goes through: its queries', and the
+    // sinks' in whole tiles, which may pass the sequence's own by a tile.
+    p.span_most = INT32_MAX;
+    if (window > 0) {
+        p.span_extra = sinks > 0 ? (int)tile : 0;
+        const int64_t most = ceil_div(sinks, tile) * tile + window + (tile_rows - 1) / group + 2;
+        if (most < INT32_MAX) p.span_most = (int)most;
+        k_tokens += (int64_t)n_seq * p.span_extra;
+        if (k_tokens > n_seq * most) k_tokens = n_seq * most;
+    }
     const int64_t mean_keys = k_tokens / n_seq;
     if (2 * likely <= slots && mean_keys >= kSplitLeast) {
         int64_t keys = ceil_div(ceil_div(mean_keys * likely, slots), tile) * tile;
@@ -596,27 +640,28 @@ static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int gro
     return p;
 }
 
-}  // namespace mg
-
-extern "C" {
-
-int64_t mg_attention_forward_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
-                                             int32_t k_heads, int32_t dim, int32_t sequences) {
+static int64_t forward_workspace(int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+                                 int32_t k_heads, int32_t dim, int32_t sequences, int32_t window,
+                                 int32_t sinks) {
     if (q_tokens <= 0 || k_tokens < 0 || k_heads < 1 || q_heads < k_heads || sequences < 1)
         return 0;
-    return mg::fwd_plan(q_tokens, k_tokens, k_heads, q_heads / k_heads, dim, sequences).bytes;
+    AttnArgs a{};
+    a.k_tokens = (int32_t)k_tokens, a.window = window, a.sinks = sinks;
+    hold_window(a);
+    return fwd_plan(q_tokens, k_tokens, k_heads, q_heads / k_heads, dim, sequences, a.window,
+                    a.sinks)
+        .bytes;
 }
 
-int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
-                             int32_t k_heads, int32_t dim, const void *q, int64_t q_token_stride,
-                             int64_t q_head_stride, const void *k, int64_t k_token_stride,
-                             int64_t k_head_stride, const void *v, int64_t v_token_stride,
-                             int64_t v_head_stride, const int32_t *q_offsets,
-                             const int32_t *k_offsets, int32_t sequences, int32_t causal,
-                             float scale, void *out, void *out_rest, float *lse,
-                             void *workspace, int64_t workspace_bytes, mg_stream_t stream) {
-    using namespace mg;
-    const char *who = "mg_attention_forward";
+static int32_t attention_forward(const char *who, int32_t dtype, int64_t q_tokens,
+                                 int64_t k_tokens, int32_t q_heads, int32_t k_heads, int32_t dim,
+                                 const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                                 const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                                 const void *v, int64_t v_token_stride, int64_t v_head_stride,
+                                 const int32_t *q_offsets, const int32_t *k_offsets,
+                                 int32_t sequences, int32_t causal, int32_t window, int32_t sinks,
+                                 float scale, void *out, void *out_rest, float *lse,
+                                 void *workspace, int64_t workspace_bytes, mg_stream_t stream) {
     MG_REQUIRE(k_heads >= 1 && q_heads >= 1 && q_heads % k_heads == 0,
                "%s: %d query heads are no multiple of %d key heads", who, q_heads, k_heads);
     const int group = q_heads / k_heads;
@@ -631,18 +676,22 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
     a.q_off = q_offsets, a.k_off = k_offsets, a.n_seq = sequences;
     a.q_tokens = (int32_t)q_tokens, a.k_tokens = (int32_t)k_tokens;
     a.k_heads = k_heads, a.group = group, a.dim = dim, a.causal = causal != 0;
+    a.window = window, a.sinks = sinks;
     a.scale = scale, a.scale_log2 = scale_to_log2(scale);
     a.out = out, a.out_rest = out_rest, a.lse = lse;
     int32_t rc = attn_check(who, a, dtype);
     if (rc != MG_OK) return rc;
     if (q_tokens == 0) return MG_OK;
     MG_REQUIRE(q && out && (k_tokens == 0 || (k && v)), "%s: a pointer is NULL", who);
-    const FwdPlan p = fwd_plan(q_tokens, k_tokens, k_heads, group, dim, sequences);
+    hold_window(a);
+    const FwdPlan p =
+        fwd_plan(q_tokens, k_tokens, k_heads, group, dim, sequences, a.window, a.sinks);
     MG_REQUIRE(grid_fits(p.items * k_heads, 64 * p.waves), "%s: too many work items", who);
     MG_REQUIRE(p.bytes == 0 || (workspace && workspace_bytes >= p.bytes),
                "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
                (long long)p.bytes);
     a.split_keys = p.split_keys, a.chunk_tiles = (int32_t)p.chunk_tiles;
+    a.span_extra = p.span_extra, a.span_most = p.span_most;
     a.part_stats = static_cast<float2 *>(workspace);
     a.part_o = reinterpret_cast<float *>(static_cast<char *>(workspace) + p.stats_bytes);
     hipStream_t st = as_stream(stream);
@@ -655,20 +704,29 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
         attn_form(dtype, dim, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int DK = decltype(d)::value;
-            if (p.waves == kWideWaves) {
-                if (p.split_keys)
-                    attn_fwd_kernel<T, DK, kWideWaves, true><<<grid, 64 * kWideWaves, 0, st>>>(a);
+            using std::bool_constant;
+            using std::integral_constant;
+            const auto go = [&](auto waves, auto split, auto win) {
+                constexpr int kWaves = decltype(waves)::value;
+                attn_fwd_kernel<T, DK, kWaves, decltype(split)::value, decltype(win)::value>
+                    <<<grid, 64 * kWaves, 0, st>>>(a);
+            };
+            const auto with = [&](auto waves, auto split) {
+                if (a.window)
+                    go(waves, split, bool_constant<true>{});
                 else
-                    attn_fwd_kernel<T, DK, kWideWaves, false>
-                        <<<grid, 64 * kWideWaves, 0, st>>>(a);
-            } else {
+                    go(waves, split, bool_constant<false>{});
+            };
+            const auto cut = [&](auto waves) {
                 if (p.split_keys)
-                    attn_fwd_kernel<T, DK, kNarrowWaves, true>
-                        <<<grid, 64 * kNarrowWaves, 0, st>>>(a);
+                    with(waves, bool_constant<true>{});
                 else
-                    attn_fwd_kernel<T, DK, kNarrowWaves, false>
-                        <<<grid, 64 * kNarrowWaves, 0, st>>>(a);
-            }
+                    with(waves, bool_constant<false>{});
+            };
+            if (p.waves == kWideWaves)
+                cut(integral_constant<int, kWideWaves>{});
+            else
+                cut(integral_constant<int, kNarrowWaves>{});
         });
         MG_LAUNCHED("attn_fwd_kernel");
     }
@@ -676,7 +734,8 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
         TimedScope ts("attention_join", st);
         // Four waves a row where rows have more chunks than one wave asks for
         // at once, on the average.
-        const bool many = k_tokens / sequences > 8 * (int64_t)p.split_keys;
+        const int64_t mean = k_tokens / sequences;
+        const bool many = (mean < p.span_most ? mean : p.span_most) > 8 * (int64_t)p.split_keys;
         const int64_t rows = q_tokens * q_heads;
         const unsigned tiles = (unsigned)(p.tiles * k_heads);
         attn_form(dtype, dim, [&](auto t, auto d) {
@@ -693,6 +752,55 @@ int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, 
         MG_LAUNCHED("attn_join kernels");
     }
     return MG_OK;
+}
+
+}  // namespace mg
+
+extern "C" {
+
+int64_t mg_attention_forward_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+                                             int32_t k_heads, int32_t dim, int32_t sequences) {
+    return mg::forward_workspace(q_tokens, k_tokens, q_heads, k_heads, dim, sequences, 0, 0);
+}
+
+int32_t mg_attention_forward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+                             int32_t k_heads, int32_t dim, const void *q, int64_t q_token_stride,
+                             int64_t q_head_stride, const void *k, int64_t k_token_stride,
+                             int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                             int64_t v_head_stride, const int32_t *q_offsets,
+                             const int32_t *k_offsets, int32_t sequences, int32_t causal,
+                             float scale, void *out, void *out_rest, float *lse,
+                             void *workspace, int64_t workspace_bytes, mg_stream_t stream) {
+    return mg::attention_forward("mg_attention_forward", dtype, q_tokens, k_tokens, q_heads,
+                                 k_heads, dim, q, q_token_stride, q_head_stride, k, k_token_stride,
+                                 k_head_stride, v, v_token_stride, v_head_stride, q_offsets,
+                                 k_offsets, sequences, causal, 0, 0, scale, out, out_rest, lse,
+                                 workspace, workspace_bytes, stream);
+}
+
+int64_t mg_attention_window_forward_workspace_bytes(int64_t q_tokens, int64_t k_tokens,
+                                                    int32_t q_heads, int32_t k_heads, int32_t dim,
+                                                    int32_t sequences, int32_t window,
+                                                    int32_t sinks) {
+    if (window < 1 || sinks < 0) return 0;
+    return mg::forward_workspace(q_tokens, k_tokens, q_heads, k_heads, dim, sequences, window,
+                                 sinks);
+}
+
+int32_t mg_attention_window_forward(
+    int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads, int32_t k_heads,
+    int32_t dim, const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
+    int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+    int64_t v_head_stride, const int32_t *q_offsets, const int32_t *k_offsets, int32_t sequences,
+    int32_t window, int32_t sinks, float scale, void *out, void *out_rest, float *lse,
+    void *workspace, int64_t workspace_bytes, mg_stream_t stream) {
+    const char *who = "mg_attention_window_forward";
+    MG_REQUIRE(window >= 1, "%s: a window of %d keys", who, window);
+    return mg::attention_forward(who, dtype, q_tokens, k_tokens, q_heads, k_heads, dim, q,
+                                 q_token_stride, q_head_stride, k, k_token_stride, k_head_stride,
+                                 v, v_token_stride, v_head_stride, q_offsets, k_offsets, sequences,
+                                 1, window, sinks, scale, out, out_rest, lse, workspace,
+                                 workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -114,16 +114,18 @@ __device__ __forceinline__ float ds_power(float do_sq, float v_sq) {
 }
 
 // ------------------------------------------------------- the queries' gradient
-template <typename T, int DK>
+template <typename T, int DK, bool kWin>
 __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) {
     constexpr int kSteps = DK / 16, kBlocks = DK / 32;
     __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK>];
     const int lane = lane_id(), half = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads, G = a.group;
-    const SeqItem s = find_longest<false>(a, item, kBwdTile);
+    const auto tiles_of = [&](int ql, int) { return (ql * G + kBwdTile - 1) / kBwdTile; };
+    const SeqItem s = kWin ? find_item<false>(a, item, tiles_of, [](int, int) { return 0; })
+                           : find_longest<false>(a, item, kBwdTile);
     if (!s.found) return;
-    const int tile = s.within;
+    const int tile = kWin ? tiles_of(s.q_len, 0) - 1 - s.within : s.within;
     const auto sees = [&](int token) {
         return a.causal ? clamp_to(token + 1 + s.k_len - s.q_len, 0, s.k_len) : s.k_len;
     };
@@ -134,7 +136,12 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
     const int see = row_ok ? sees(token) : 0;
     const int see_first = sees(min(row0 / G, s.q_len - 1));
     const int see_last = sees(min((row0 + 31) / G, s.q_len - 1));
-    const int k_to = sees(min((tile * kBwdTile + kBwdTile - 1) / G, s.q_len - 1));
+    const int low = kWin ? key_low(a, s, token) : 0;
+    const int low_first = kWin ? key_low(a, s, min(row0 / G, s.q_len - 1)) : 0;
+    const int low_last = kWin ? key_low(a, s, min((row0 + 31) / G, s.q_len - 1)) : 0;
+    const KeyRun run = key_run<kWin, kTileRows>(
+        a, s, min(tile * kBwdTile / G, s.q_len - 1),
+        sees(min((tile * kBwdTile + kBwdTile - 1) / G, s.q_len - 1)));
 
     vec8<T> q[kSteps], dout[kSteps];
     float lse = INFINITY, delta = 0.f, do_sq = 0.f;
@@ -192,15 +199,19 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
     f32x16 dq[kBlocks] = {};
     TileLane<T, DK> lane_at;
     int buf = 0;
-    if (k_to > 0) ask(0, 0);
+    if (run.end > 0) ask(key_at<kWin>(run, 0), 0);
     loads_done();
-    for (int key0 = 0; key0 < k_to; key0 += kTileRows, buf ^= 1) {
+    for (int number = 0; number < run.end; number += kTileRows, buf ^= 1) {
+        const int key0 = key_at<kWin>(run, number);
+        const TileSees in = tile_sees<kWin>(run, number);
         tiles_ready();
         lane_at.fresh();
-        if (key0 + kTileRows < k_to) ask(key0 + kTileRows, buf ^ 1);
-        if (key0 >= see_last) continue;
+        if (number + kTileRows < run.end) ask(key_at<kWin>(run, number + kTileRows), buf ^ 1);
+        if (key0 >= in.to(see_last) || (kWin && key0 + kTileRows <= in.from(low_first))) continue;
         const char *kt = s_tile[buf][0], *vt = s_tile[buf][1];
-        const bool masked = key0 + kTileRows > see_first;
+        const bool masked =
+            key0 + kTileRows > in.to(see_first) || (kWin && key0 < in.from(low_last));
+        const int to = in.to(see), from = in.from(low);
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
             f32x16 sc = {}, dp = {};
@@ -215,7 +226,8 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
                 const float p = __builtin_amdgcn_exp2f(fmaf(sc[e], a.scale_log2, -lse));
                 float d = p * fmaf(dp[e], up, -delta_up);
                 // Selected: what is not seen may be anything.
-                if (masked && key0 + 32 * b + c_row(e, half) >= see) d = 0.f;
+                const int key = key0 + 32 * b + c_row(e, half);
+                if (masked && (key >= to || (kWin && key < from))) d = 0.f;
                 ds[e / 8][e % 8] = (T)d;
             }
 #pragma unroll
@@ -266,6 +278,35 @@ __device__ __forceinline__ f32x4 *part_of(const AttnArgs &a, int item, int kh, i
            (((int64_t)item * a.k_heads + kh) * a.splits + split) * kPartFours<DK>;
 }
 
+// With a window, the queries that see a key tile are few, but those further on all
+// see the sinks. Their sums for the sinks are work items of their own, which go
+// first: one tile of kBwdTile keys, one head and sink_steps query tiles each. Item
+// i keeps them, of sink_rows keys, in place i of sink_part; the sequence's
+// window items, after them, a place each key tile that has sinks (sink_items has them
+// all), where they are not cut into runs.
+struct SinkItems {
+    int key_tiles, from, tiles, pieces;    // from: the first query past the window
+
+    __device__ __forceinline__ SinkItems(const AttnArgs &a, int q_len, int k_len) {
+        key_tiles = (min(a.sinks, k_len) + kBwdTile - 1) / kBwdTile;
+        from = (int)min((int64_t)q_len, max((int64_t)0, (int64_t)a.window + q_len - k_len));
+        tiles = (q_len - from + kTileRows - 1) / kTileRows;
+        pieces = (tiles + a.sink_steps - 1) / a.sink_steps;
+        if (q_len == 0) key_tiles = 0;
+    }
+    __device__ __forceinline__ int runs(const AttnArgs &a) const { return pieces * a.group; }
+    // Items, and places, of a sequence.
+    __device__ __forceinline__ int all(const AttnArgs &a) const {
+        return key_tiles * (runs(a) + 1);
+    }
+};
+
+template <int DK>
+__device__ __forceinline__ f32x4 *sink_part_of(const AttnArgs &a, int place, int kh) {
+    return reinterpret_cast<f32x4 *>(a.sink_part) +
+           ((int64_t)place * a.k_heads + kh) * (2 * a.sink_rows * DK / 4);
+}
+
 // The query tiles that see a key tile (tiles of each of the group's heads, from
 // q_from), and the runs they are cut into: whole heads, or `parts` of each head
 // where there are more runs than heads. Key tiles that run at the same time then
@@ -274,37 +315,70 @@ struct KeySteps {
     int q_from, tiles, runs, parts;
 };
 
+template <bool kWin>
 __device__ __forceinline__ KeySteps key_steps(const AttnArgs &a, const SeqItem &s, int first_key) {
     const int ahead = s.k_len - s.q_len, G = a.group;
-    const int from = a.causal ? max(0, first_key - ahead) / kTileRows * kTileRows : 0;
-    const int tiles = from < s.q_len ? (s.q_len - from + kTileRows - 1) / kTileRows : 0;
+    int from = a.causal ? max(0, first_key - ahead) / kTileRows * kTileRows : 0, to = s.q_len;
+    if constexpr (kWin) {
+        from = max(0, first_key - ahead);
+        const int last = min(first_key + kBwdTile, s.k_len) - 1;
+        to = (int)min((int64_t)s.q_len, max((int64_t)0, (int64_t)last + a.window - ahead));
+    }
+    const int tiles = from < to ? (to - from + kTileRows - 1) / kTileRows : 0;
     int runs = (int)(((int64_t)tiles * G + a.split_steps - 1) / a.split_steps);
     runs = even_runs(clamp_to(runs, 1, a.splits), G, a.splits);
     return {from, tiles, runs, runs > G ? runs / G : 1};
 }
 
-template <typename T, int DK>
+template <typename T, int DK, bool kWin>
 __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a) {
     constexpr int kSteps = DK / 16, kBlocks = DK / 32;
     __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK>];
     __shared__ __align__(16) float s_row[2][2][kTileRows];     // lse, delta
     const int lane = lane_id(), half = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads / a.splits;
-    const int split = blockIdx.x / a.k_heads % a.splits;
-    const SeqItem s = find_longest<true>(a, item, kBwdTile);
+    const int kh = blockIdx.x % a.k_heads, at_item = blockIdx.x / a.k_heads;
+    // Queries past the window, for the sinks.
+    const bool far = kWin && at_item < a.sink_items;
+    const auto sink_count = [&](int ql, int kl) { return SinkItems(a, ql, kl).all(a); };
+    const auto key_tiles = [&](int, int kl) { return (kl + kBwdTile - 1) / kBwdTile; };
+    const int after = kWin ? at_item - a.sink_items : at_item;
+    const int item = after / a.splits, split = after % a.splits;
+    SeqItem s;
+    if constexpr (kWin)
+        s = far ? find_item<true>(a, at_item, sink_count, key_tiles)
+                : find_item<true>(a, item, key_tiles, sink_count);
+    else
+        s = find_longest<true>(a, item, kBwdTile);
     if (!s.found) return;
-    const int first_key = s.within * kBwdTile;
-    const KeySteps steps_of = key_steps(a, s, first_key);
-    if (split >= steps_of.runs) return;
+    KeySteps steps_of;
+    int first_key = s.within * kBwdTile, sink_run = 0, sink_runs = 0, sink_place = 0;
+    if (kWin && a.sinks > 0) {
+        const SinkItems of(a, s.q_len, s.k_len);
+        sink_runs = of.runs(a);
+        if (far) {
+            first_key = s.within / (sink_runs + 1) * kBwdTile;
+            sink_run = s.within % (sink_runs + 1);
+            if (sink_run == sink_runs) return;         // the window item's place
+            sink_place = at_item;
+            steps_of = {of.from, of.tiles, sink_runs, of.pieces};
+        } else {
+            sink_place = s.before + s.within * (sink_runs + 1) + sink_runs;
+        }
+    }
+    if (!far) {
+        steps_of = key_steps<kWin>(a, s, first_key);
+        if (split >= steps_of.runs) return;
+    }
     const int key0 = first_key + wave * 32, key = key0 + lane % 32;
     const bool key_ok = key < s.k_len;
     const int ahead = s.k_len - s.q_len;       // query i sees keys up to i + ahead
     // This run's heads, and its query tiles of each.
-    const int parts = steps_of.parts, runs = steps_of.runs / parts, run = split / parts;
+    const int parts = steps_of.parts, runs = steps_of.runs / parts;
+    const int nth = far ? sink_run : split, run = nth / parts, piece = nth % parts;
     const int g_from = run * a.group / runs, heads = (run + 1) * a.group / runs - g_from;
-    const int t_from = steps_of.tiles * (split % parts) / parts;
-    const int tiles = steps_of.tiles * (split % parts + 1) / parts - t_from;
+    const int t_from = (int)((int64_t)steps_of.tiles * piece / parts);
+    const int tiles = (int)((int64_t)steps_of.tiles * (piece + 1) / parts) - t_from;
     const int q_from = steps_of.q_from + t_from * kTileRows;
     const int q_to = q_from + tiles * kTileRows;
 
@@ -368,9 +442,16 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
         if (step + 1 < steps) ask(g, row0, buf ^ 1);
         const char *qt = s_tile[buf][0], *dot = s_tile[buf][1];
         // Every row of the tile sees every key of the wave?
-        const bool masked = at_row0 + kTileRows > s.q_len || key0 + 32 > s.k_len ||
-                            (a.causal && at_row0 + ahead < key0 + 31);
+        bool masked = at_row0 + kTileRows > s.q_len || key0 + 32 > s.k_len ||
+                      (a.causal && at_row0 + ahead < key0 + 31);
         if (a.causal && at_row0 + kTileRows - 1 + ahead < key0) continue;    // none sees any
+        if constexpr (kWin) {
+            // How far on the tile's rows stand, of the wave's keys.
+            const int least = at_row0 + ahead - (key0 + 31);
+            const int most = at_row0 + kTileRows - 1 + ahead - key0;
+            if (far ? key0 >= a.sinks || most < a.window : least >= a.window) continue;
+            masked |= far ? key0 + 32 > a.sinks || least < a.window : most >= a.window;
+        }
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
             f32x16 sc = {}, dp = {};
@@ -393,8 +474,12 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
                     float d = x * ((dp[e] - delta[i]) * ds_up);
                     if (masked) {
                         const int token = at_row0 + r + i;
-                        const bool seen = token < s.q_len && key_ok &&
-                                          (!a.causal || key <= token + ahead);
+                        bool seen = token < s.q_len && key_ok &&
+                                    (!a.causal || key <= token + ahead);
+                        if constexpr (kWin) {
+                            const bool within = token + ahead - key < a.window;
+                            seen = seen && (far ? !within && key < a.sinks : within);
+                        }
                         x = seen ? x : 0.f;
                         d = seen ? d : 0.f;
                     }
@@ -414,6 +499,26 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     lds_reads_done();
     const float down = a.scale * __builtin_amdgcn_exp2f(-power);
     const float down_v = __builtin_amdgcn_exp2f(-kPowerP<T>);
+    // With sinks, the sums of those that queries past the window see too.
+    const bool sinks_too = kWin && sink_runs > 0 && key < a.sinks;
+    if (kWin && (far || (steps_of.runs == 1 && sinks_too))) {
+        if (key >= a.sinks) return;
+        f32x4 *part = sink_part_of<DK>(a, sink_place, kh) + wave * kBlocks * 4 * 64 + lane;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                f32x4 w, x;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[i] = dk[b][e + i] * down;
+                    x[i] = dv[b][e + i] * down_v;
+                }
+                part[(b * 4 + e / 4) * 64] = w;
+                part[(b * 4 + e / 4) * 64 + a.sink_rows * DK / 4] = x;
+            }
+        return;
+    }
     if (steps_of.runs > 1) {
         f32x4 *part = part_of<DK>(a, item, kh, split) + wave * kBlocks * 4 * 64 + lane;
 #pragma unroll
@@ -455,25 +560,51 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
 // The sums of the keys' tiles that were cut into runs, in order. A workgroup has
 // 32 columns of dk or dv of one tile of one key head, its threads the elements
 // that attn_dkv_kernel's have.
-template <typename T, int DK>
+template <typename T, int DK, bool kWin>
 __global__ __launch_bounds__(64 * kBwdWaves) void attn_sum_kernel(AttnArgs a) {
     constexpr int kBlocks = DK / 32;
     const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
-    const SeqItem s = find_longest<true>(a, item, kBwdTile);
+    SeqItem s;
+    if constexpr (kWin)
+        s = find_item<true>(
+            a, item, [&](int, int kl) { return (kl + kBwdTile - 1) / kBwdTile; },
+            [&](int ql, int kl) { return a.sinks > 0 ? SinkItems(a, ql, kl).all(a) : 0; });
+    else
+        s = find_longest<true>(a, item, kBwdTile);
     if (!s.found) return;
     const int first_key = s.within * kBwdTile;
-    const int runs = key_steps(a, s, first_key).runs;
-    if (runs == 1) return;
+    const int runs = key_steps<kWin>(a, s, first_key).runs;
+    int sink_runs = 0, sink_place = 0;
+    if (kWin && first_key < a.sinks) {
+        sink_runs = SinkItems(a, s.q_len, s.k_len).runs(a);
+        sink_place = s.before + s.within * (sink_runs + 1);
+    }
+    if (runs == 1 && sink_runs == 0) return;
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / 64);
     const int key = first_key + wave * 32 + lane % 32;
     const int64_t at_row = ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim;
     const f32x4 *part = part_of<DK>(a, item, kh, 0) + wave * kBlocks * 4 * 64 + lane;
     const int which = blockIdx.y % 2, block = blockIdx.y / 2;
+    const bool sinks_too = kWin && sink_runs > 0 && key < a.sinks;
+    if (kWin && runs == 1 && !sinks_too) return;       // written by its only item
+    const f32x4 *far = nullptr;
+    int64_t far_step = 0;
+    if (sinks_too) {
+        far = sink_part_of<DK>(a, sink_place, kh) + wave * kBlocks * 4 * 64 + lane +
+              which * (a.sink_rows * DK / 4);
+        far_step = (int64_t)a.k_heads * (2 * a.sink_rows * DK / 4);
+    }
 #pragma unroll
     for (int i = 4 * block; i < 4 * block + 4; ++i) {
         const f32x4 *p = part + i * 64 + which * kPartFours<DK> / 2;
-        f32x4 sum = *p;
-        for (int k = 1; k < runs; ++k) sum += p[k * kPartFours<DK>];
+        f32x4 sum = {};
+        if (!kWin || runs > 1) {
+            sum = *p;
+            for (int k = 1; k < runs; ++k) sum += p[k * kPartFours<DK>];
+        }
+        // The far queries' sums and, of a tile in one run, its own.
+        if (sinks_too)
+            for (int k = 0; k < sink_runs + (runs == 1); ++k) sum += far[k * far_step + i * 64];
         const int at = 32 * block + c_row(i % 4 * 4, half);
         if (key < s.k_len && at < a.dim)
             *reinterpret_cast<vec4<T> *>(static_cast<T *>(which ? a.dv : a.dk) + at_row + at) =
@@ -486,18 +617,24 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_sum_kernel(AttnArgs a) {
 // the GPU twice over, of eight query tiles at least (7033 packed tokens, 62 tiles
 // on 4 key heads: 528 us uncut, 187 and 27 to add the runs in four).
 struct BwdPlan {
-    int64_t k_items, largest_at, part_at, bytes;
+    int64_t k_items, largest_at, part_at, sink_at, bytes;
     int splits, split_steps;
+    int64_t sink_items;
+    int sink_steps, sink_rows;
 };
 
 constexpr int64_t kBwdRuns = 1024, kBwdRunLeast = 8, kBwdMostSplits = 8;
+constexpr int64_t kSinkSteps = 8;
 
 static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int64_t group,
-                        int64_t dim, int64_t n_seq) {
+                        int64_t dim, int64_t n_seq, int64_t window, int64_t sinks) {
     BwdPlan p{};
     p.k_items = k_tokens / kBwdTile + n_seq + 2;
     const int64_t tiles = (ceil_div(k_tokens, kBwdTile) + n_seq - 1) * k_heads;
-    const int64_t steps = ceil_div(q_tokens, n_seq * kTileRows) * group;
+    int64_t queries = ceil_div(q_tokens, n_seq * kTileRows);
+    if (window > 0 && queries > ceil_div(window + kBwdTile, kTileRows))
+        queries = ceil_div(window + kBwdTile, kTileRows);
+    const int64_t steps = queries * group;
     int64_t splits = kBwdRuns / (tiles > 0 ? tiles : 1);
     if (splits > steps / kBwdRunLeast) splits = steps / kBwdRunLeast;
     splits = splits < 1 ? 1 : splits > kBwdMostSplits ? kBwdMostSplits : splits;
@@ -509,32 +646,42 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     p.bytes = p.part_at;
     const int64_t dk = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
     if (p.splits > 1) p.bytes += p.k_items * k_heads * p.splits * 2 * kBwdTile * dk * 4;
+    p.sink_at = p.bytes;
+    if (sinks > 0) {
+        // Sum over the sequences of SinkItems::all: of key_tiles * (pieces * group + 1),
+        // pieces being at most tokens / (64 sink_steps) + 1 each.
+        p.sink_steps = (int)kSinkSteps;
+        p.sink_rows = (int)(sinks < kBwdTile ? ceil_div(sinks, 32) * 32 : kBwdTile);
+        const int64_t pieces = q_tokens / (kTileRows * p.sink_steps) + n_seq;
+        p.sink_items = ceil_div(sinks, kBwdTile) * (pieces * group + n_seq);
+        p.bytes += p.sink_items * k_heads * 2 * p.sink_rows * dk * 4;
+    }
     return p;
 }
 
-}  // namespace mg
-
-extern "C" {
-
-int64_t mg_attention_backward_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
-                                              int32_t k_heads, int32_t dim, int32_t sequences) {
+static int64_t backward_workspace(int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+                                  int32_t k_heads, int32_t dim, int32_t sequences, int32_t window,
+                                  int32_t sinks) {
     if (q_tokens < 0 || k_tokens < 0 || k_heads < 1 || q_heads < k_heads || sequences < 1) return 0;
-    return mg::bwd_plan(q_tokens, k_tokens, k_heads, q_heads / k_heads, dim, sequences).bytes;
+    AttnArgs a{};
+    a.k_tokens = (int32_t)k_tokens, a.window = window, a.sinks = sinks;
+    hold_window(a);
+    return bwd_plan(q_tokens, k_tokens, k_heads, q_heads / k_heads, dim, sequences, a.window,
+                    a.sinks)
+        .bytes;
 }
 
-int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
-                              int32_t k_heads, int32_t dim, const void *q, int64_t q_token_stride,
-                              int64_t q_head_stride, const void *k, int64_t k_token_stride,
-                              int64_t k_head_stride, const void *v, int64_t v_token_stride,
-                              int64_t v_head_stride, const int32_t *q_offsets,
-                              const int32_t *k_offsets, int32_t sequences, int32_t causal,
-                              float scale, const void *out, const void *out_rest,
-                              const float *lse, const void *dout,
-                              int64_t dout_token_stride, int64_t dout_head_stride, void *dq,
-                              void *dk, void *dv, void *workspace, int64_t workspace_bytes,
-                              mg_stream_t stream) {
-    using namespace mg;
-    const char *who = "mg_attention_backward";
+static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_tokens,
+                                  int64_t k_tokens, int32_t q_heads, int32_t k_heads, int32_t dim,
+                                  const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                                  const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                                  const void *v, int64_t v_token_stride, int64_t v_head_stride,
+                                  const int32_t *q_offsets, const int32_t *k_offsets,
+                                  int32_t sequences, int32_t causal, int32_t window, int32_t sinks,
+                                  float scale, const void *out, const void *out_rest,
+                                  const float *lse, const void *dout, int64_t dout_token_stride,
+                                  int64_t dout_head_stride, void *dq, void *dk, void *dv,
+                                  void *workspace, int64_t workspace_bytes, mg_stream_t stream) {
     MG_REQUIRE(k_heads >= 1 && q_heads >= 1 && q_heads % k_heads == 0,
                "%s: %d query heads are no multiple of %d key heads", who, q_heads, k_heads);
     const int group = q_heads / k_heads;
@@ -550,6 +697,7 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
     a.q_off = q_offsets, a.k_off = k_offsets, a.n_seq = sequences;
     a.q_tokens = (int32_t)q_tokens, a.k_tokens = (int32_t)k_tokens;
     a.k_heads = k_heads, a.group = group, a.dim = dim, a.causal = causal != 0;
+    a.window = window, a.sinks = sinks;
     a.scale = scale, a.scale_log2 = scale_to_log2(scale);
     a.out = const_cast<void *>(out), a.out_rest = const_cast<void *>(out_rest), a.lse = const_cast<float *>(lse);
     a.dq = dq, a.dk = dk, a.dv = dv;
@@ -558,7 +706,9 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
     MG_REQUIRE(q_tokens == 0 || (q && out && lse && dout && dq), "%s: a pointer is NULL", who);
     MG_REQUIRE(k_tokens == 0 || (k && v), "%s: a pointer is NULL", who);
     MG_REQUIRE((dk == nullptr) == (dv == nullptr), "%s: dk and dv go together", who);
-    const BwdPlan p = bwd_plan(q_tokens, k_tokens, k_heads, group, dim, sequences);
+    hold_window(a);
+    const BwdPlan p =
+        bwd_plan(q_tokens, k_tokens, k_heads, group, dim, sequences, a.window, a.sinks);
     MG_REQUIRE(workspace && workspace_bytes >= p.bytes, "%s: workspace of %lld bytes, %lld needed",
                who, (long long)workspace_bytes, (long long)p.bytes);
     char *ws = static_cast<char *>(workspace);
@@ -567,9 +717,11 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
     a.largest_v = a.largest_do + k_heads * norm_places(q_tokens, sequences);
     a.splits = p.splits, a.split_steps = p.split_steps;
     a.part = reinterpret_cast<float *>(ws + p.part_at);
+    a.sink_items = (int32_t)p.sink_items, a.sink_steps = p.sink_steps, a.sink_rows = p.sink_rows;
+    a.sink_part = reinterpret_cast<float *>(ws + p.sink_at);
     hipStream_t st = as_stream(stream);
     const int64_t q_items = (q_tokens * group / kBwdTile + sequences + 2) * k_heads;
-    const int64_t k_items = p.k_items * p.splits * k_heads;
+    const int64_t k_items = (p.k_items * p.splits + p.sink_items) * k_heads;
     const int64_t places =
         k_heads * norm_places(q_tokens > k_tokens ? q_tokens : k_tokens, sequences);
     MG_REQUIRE(grid_fits(q_items, 64 * kBwdWaves) && grid_fits(k_items, 64 * kBwdWaves) &&
@@ -583,29 +735,95 @@ int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens,
     if (q_tokens > 0) {
         TimedScope ts("attention_dq", st);
         attn_form(dtype, dim, [&](auto t, auto d) {
-            attn_dq_kernel<decltype(t), decltype(d)::value>
-                <<<(unsigned)q_items, 64 * kBwdWaves, 0, st>>>(a);
+            using T = decltype(t);
+            constexpr int DK = decltype(d)::value;
+            if (a.window)
+                attn_dq_kernel<T, DK, true><<<(unsigned)q_items, 64 * kBwdWaves, 0, st>>>(a);
+            else
+                attn_dq_kernel<T, DK, false><<<(unsigned)q_items, 64 * kBwdWaves, 0, st>>>(a);
         });
         MG_LAUNCHED("attn_dq_kernel");
     }
     if (k_tokens > 0 && dk) {
         TimedScope ts("attention_dkv", st);
         attn_form(dtype, dim, [&](auto t, auto d) {
-            attn_dkv_kernel<decltype(t), decltype(d)::value>
-                <<<(unsigned)k_items, 64 * kBwdWaves, 0, st>>>(a);
+            using T = decltype(t);
+            constexpr int DK = decltype(d)::value;
+            if (a.window)
+                attn_dkv_kernel<T, DK, true><<<(unsigned)k_items, 64 * kBwdWaves, 0, st>>>(a);
+            else
+                attn_dkv_kernel<T, DK, false><<<(unsigned)k_items, 64 * kBwdWaves, 0, st>>>(a);
         });
         MG_LAUNCHED("attn_dkv_kernel");
     }
-    if (k_tokens > 0 && dk && p.splits > 1) {
+    if (k_tokens > 0 && dk && (p.splits > 1 || a.sinks > 0)) {
         TimedScope ts("attention_sum", st);
         attn_form(dtype, dim, [&](auto t, auto d) {
             constexpr int DK = decltype(d)::value;
             const dim3 grid((unsigned)(p.k_items * k_heads), 2 * DK / 32);
-            attn_sum_kernel<decltype(t), DK><<<grid, 64 * kBwdWaves, 0, st>>>(a);
+            if (a.window)
+                attn_sum_kernel<decltype(t), DK, true><<<grid, 64 * kBwdWaves, 0, st>>>(a);
+            else
+                attn_sum_kernel<decltype(t), DK, false><<<grid, 64 * kBwdWaves, 0, st>>>(a);
         });
         MG_LAUNCHED("attn_sum_kernel");
     }
     return MG_OK;
+}
+
+}  // namespace mg
+
+extern "C" {
+
+int64_t mg_attention_backward_workspace_bytes(int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+                                              int32_t k_heads, int32_t dim, int32_t sequences) {
+    return mg::backward_workspace(q_tokens, k_tokens, q_heads, k_heads, dim, sequences, 0, 0);
+}
+
+int32_t mg_attention_backward(int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads,
+                              int32_t k_heads, int32_t dim, const void *q, int64_t q_token_stride,
+                              int64_t q_head_stride, const void *k, int64_t k_token_stride,
+                              int64_t k_head_stride, const void *v, int64_t v_token_stride,
+                              int64_t v_head_stride, const int32_t *q_offsets,
+                              const int32_t *k_offsets, int32_t sequences, int32_t causal,
+                              float scale, const void *out, const void *out_rest,
+                              const float *lse, const void *dout,
+                              int64_t dout_token_stride, int64_t dout_head_stride, void *dq,
+                              void *dk, void *dv, void *workspace, int64_t workspace_bytes,
+                              mg_stream_t stream) {
+    return mg::attention_backward("mg_attention_backward", dtype, q_tokens, k_tokens, q_heads,
+                                  k_heads, dim, q, q_token_stride, q_head_stride, k,
+                                  k_token_stride, k_head_stride, v, v_token_stride, v_head_stride,
+                                  q_offsets, k_offsets, sequences, causal, 0, 0, scale, out,
+                                  out_rest, lse, dout, dout_token_stride, dout_head_stride, dq, dk,
+                                  dv, workspace, workspace_bytes, stream);
+}
+
+int64_t mg_attention_window_backward_workspace_bytes(int64_t q_tokens, int64_t k_tokens,
+                                                     int32_t q_heads, int32_t k_heads, int32_t dim,
+                                                     int32_t sequences, int32_t window,
+                                                     int32_t sinks) {
+    if (window < 1 || sinks < 0) return 0;
+    return mg::backward_workspace(q_tokens, k_tokens, q_heads, k_heads, dim, sequences, window,
+                                  sinks);
+}
+
+int32_t mg_attention_window_backward(
+    int32_t dtype, int64_t q_tokens, int64_t k_tokens, int32_t q_heads, int32_t k_heads,
+    int32_t dim, const void *q, int64_t q_token_stride, int64_t q_head_stride, const void *k,
+    int64_t k_token_stride, int64_t k_head_stride, const void *v, int64_t v_token_stride,
+    int64_t v_head_stride, const int32_t *q_offsets, const int32_t *k_offsets, int32_t sequences,
+    int32_t window, int32_t sinks, float scale, const void *out, const void *out_rest,
+    const float *lse, const void *dout, int64_t dout_token_stride, int64_t dout_head_stride,
+    void *dq, void *dk, void *dv, void *workspace, int64_t workspace_bytes, mg_stream_t stream) {
+    const char *who = "mg_attention_window_backward";
+    MG_REQUIRE(window >= 1, "%s: a window of %d keys", who, window);
+    return mg::attention_backward(who, dtype, q_tokens, k_tokens, q_heads, k_heads, dim, q,
+                                  q_token_stride, q_head_stride, k, k_token_stride, k_head_stride,
+                                  v, v_token_stride, v_head_stride, q_offsets, k_offsets,
+                                  sequences, 1, window, sinks, scale, out, out_rest, lse, dout,
+                                  dout_token_stride, dout_head_stride, dq, dk, dv, workspace,
+                                  workspace_bytes, stream);
 }
 
 }  // extern "C"

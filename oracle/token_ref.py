@@ -113,11 +113,14 @@ def kept(n, drop, seed, site=0, first=0):
 
 # --------------------------------------------------------------- attention
 
-def sees(nq, nk, causal):
-    """(nq, nk) truth values: query i stands at key i + nk - nq."""
+def sees(nq, nk, causal, window=None, sinks=0):
+    """(nq, nk) truth values: query i stands at key i + nk - nq; with a window it sees
+    the last `window` keys up to there and the first `sinks`."""
     if not causal:
         return np.ones((nq, nk), bool)
-    return np.arange(nk)[None, :] <= np.arange(nq)[:, None] + (nk - nq)
+    key, at = np.arange(nk)[None, :], np.arange(nq)[:, None] + (nk - nq)
+    seen = key <= at
+    return seen if window is None else seen & ((key > at - window) | (key < sinks))
 
 
 def probabilities(q, k, scale, mask):
@@ -129,7 +132,8 @@ def probabilities(q, k, scale, mask):
     return p / np.where(total == 0.0, 1.0, total)
 
 
-def attention(q, k, v, q_offsets, k_offsets, causal, scale, dout=None, unit=0.0):
+def attention(q, k, v, q_offsets, k_offsets, causal, scale, dout=None, unit=0.0, window=None,
+              sinks=0):
     """(o, dq, dk, dv) and, as a second tuple, how far each may be off when o and
     the gradients are rounded to a type of unit roundoff `unit` and p and ds are
     rounded to it for their products, sums being exact: first order, every
@@ -144,7 +148,7 @@ def attention(q, k, v, q_offsets, k_offsets, causal, scale, dout=None, unit=0.0)
     off = [np.zeros(t.shape) for t in (q, q, k, v)]
     for q0, q1, k0, k1 in zip(q_offsets[:-1], q_offsets[1:], k_offsets[:-1], k_offsets[1:]):
         rows, keys = slice(q0, q1), slice(k0, k1)
-        mask = sees(q1 - q0, k1 - k0, causal)
+        mask = sees(q1 - q0, k1 - k0, causal, window, sinks)
         for h in range(q.shape[1]):
             qh, kh, vh = q[rows, h], k[keys, h // group], v[keys, h // group]
             p = probabilities(qh, kh, scale, mask)
