@@ -818,6 +818,29 @@ int32_t mg_attention_window_backward(
     int64_t dout_token_stride, int64_t dout_head_stride, void *dq, void *dk,
     void *dv, void *workspace, int64_t workspace_bytes, mg_stream_t stream);
 
+/* Attention of packed sequences to their own keys (as mg_attention_forward) and, in
+ * the same softmax, to all tokens of a memory that a group of them shares: query
+ * tokens group_offsets[g] .. group_offsets[g + 1] - 1 to shared tokens by
+ * shared_offsets (device, groups + 1 each; both NULL: one group of all). Offsets are
+ * held to the tensors and made to rise. No gradient. */
+int64_t mg_shared_attention_workspace_bytes(int64_t q_tokens, int64_t k_tokens,
+                                            int64_t shared_tokens,
+                                            int32_t q_heads, int32_t k_heads,
+                                            int32_t dim, int32_t sequences,
+                                            int32_t groups);
+int32_t mg_shared_attention(
+    int32_t dtype, int64_t q_tokens, int64_t k_tokens, int64_t shared_tokens,
+    int32_t q_heads, int32_t k_heads, int32_t dim, const void *q,
+    int64_t q_token_stride, int64_t q_head_stride, const void *k,
+    int64_t k_token_stride, int64_t k_head_stride, const void *v,
+    int64_t v_token_stride, int64_t v_head_stride, const void *shared_k,
+    int64_t shared_k_token_stride, int64_t shared_k_head_stride,
+    const void *shared_v, int64_t shared_v_token_stride,
+    int64_t shared_v_head_stride, const int32_t *q_offsets,
+    const int32_t *k_offsets, int32_t sequences, const int32_t *group_offsets,
+    const int32_t *shared_offsets, int32_t groups, int32_t causal, float scale,
+    void *out, void *workspace, int64_t workspace_bytes, mg_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

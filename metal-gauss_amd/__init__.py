@@ -21,7 +21,9 @@ counterpart in the reference):
     rotary, rotary_frequencies
                            rotary positions of queries and keys
     norm_rotary            heads normed and turned in one pass, and its gradients
-    attention              attention over packed sequences and its gradients
+    attention              attention over packed sequences, whole or by a window,
+                           and its gradients
+    shared_attention       attention over memories that several sequences share
     dropout                dropout onto a residual stream, and its gradients
 """
 
@@ -35,7 +37,7 @@ from .norm import layer_norm  # noqa: F401
 from .rotary import rotary, rotary_frequencies  # noqa: F401
 from .norm_rotary import norm_rotary  # noqa: F401
 from .dropout import dropout  # noqa: F401
-from .attention import attention  # noqa: F401
+from .attention import attention, shared_attention  # noqa: F401
 from . import backend, ext  # noqa: F401
 
 __version__ = "0.1.0"

@@ -162,6 +162,12 @@ _SIGNATURES = {
                                             _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp, _i32,
                                             _i32, _i32, _f32, _vp, _vp, _vp, _vp, _i64, _i64, _vp,
                                             _vp, _vp, _vp, _i64, _vp]),
+    "mg_shared_attention_workspace_bytes": (_i64, [_i64, _i64, _i64, _i32, _i32, _i32, _i32,
+                                                   _i32]),
+    "mg_shared_attention": (_i32, [_i32, _i64, _i64, _i64, _i32, _i32, _i32, _vp, _i64, _i64, _vp,
+                                   _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64,
+                                   _vp, _vp, _i32, _vp, _vp, _i32, _i32, _f32, _vp, _vp, _i64,
+                                   _vp]),
 }
 
 EXPORTS = tuple(_SIGNATURES)

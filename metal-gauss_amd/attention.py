@@ -1,5 +1,6 @@
 """Attention over packed sequences on the GPU, forward and backward
-(mg_attention_*).
+(mg_attention_*), and over memories that several sequences share
+(mg_shared_attention).
 
 The reference has no counterpart: this is one of the operators of a network
 that predicts or refines splats, next to ``layer_norm`` and ``rotary``.
@@ -108,6 +109,41 @@ def _check_offsets(off, what, index):
         raise RuntimeError(f"{what} must be on GPU {index}, got device '{off.device}'")
 
 
+def _check_heads(q, k, v, *more):
+    """The head dimension and the GPU of all of them."""
+    dtype, dim, index = q.dtype, q.shape[-1] if q.dim() else 0, q.get_device()
+    for t, what in zip((q, k, v, *more), ("q", "k", "v", "shared_k", "shared_v")):
+        if _lib.type_code(t, what) == 0:
+            raise RuntimeError(f"{what} must be bfloat16 or float16, got {t.dtype}")
+        if t.dim() != 3:
+            raise ValueError(f"{what} must be (tokens, heads, dim), got {tuple(t.shape)}")
+        if t.dtype != dtype or t.shape[2] != dim or t.get_device() != index:
+            raise ValueError(f"{what} must match q's type, device and head dimension; got "
+                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    if k.shape != v.shape:
+        raise ValueError(f"k is {tuple(k.shape)} and v {tuple(v.shape)}; one shape is needed")
+    return dim, index
+
+
+def _check_bounds(q, k, q_offsets, k_offsets, index):
+    """k_offsets, or what stands for them."""
+    if q_offsets is not None:
+        _check_offsets(q_offsets, "q_offsets", index)
+        if k_offsets is None:
+            if k.shape[0] != q.shape[0]:
+                raise ValueError(f"k_offsets is needed: {q.shape[0]} query tokens and "
+                                 f"{k.shape[0]} key tokens")
+            k_offsets = q_offsets
+    if k_offsets is not None and k_offsets is not q_offsets:
+        if q_offsets is None:
+            raise ValueError("k_offsets needs q_offsets")
+        _check_offsets(k_offsets, "k_offsets", index)
+        if k_offsets.shape[0] != q_offsets.shape[0]:
+            raise ValueError(f"q_offsets is {tuple(q_offsets.shape)} and k_offsets "
+                             f"{tuple(k_offsets.shape)}; one number of sequences is needed")
+    return k_offsets
+
+
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
               q_offsets: torch.Tensor | None = None, k_offsets: torch.Tensor | None = None, *,
               causal: bool = False, window: int | None = None, sinks: int = 0,
@@ -142,31 +178,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     call to call; for that, what rounding took from the result is kept, a second
     tensor of its size.
     """
-    dtype, dim, index = q.dtype, q.shape[-1] if q.dim() else 0, q.get_device()
-    for t, what in ((q, "q"), (k, "k"), (v, "v")):
-        if _lib.type_code(t, what) == 0:
-            raise RuntimeError(f"{what} must be bfloat16 or float16, got {t.dtype}")
-        if t.dim() != 3:
-            raise ValueError(f"{what} must be (tokens, heads, dim), got {tuple(t.shape)}")
-        if t.dtype != dtype or t.shape[2] != dim or t.get_device() != index:
-            raise ValueError(f"{what} must match q's type, device and head dimension; got "
-                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
-    if k.shape != v.shape:
-        raise ValueError(f"k is {tuple(k.shape)} and v {tuple(v.shape)}; one shape is needed")
-    if q_offsets is not None:
-        _check_offsets(q_offsets, "q_offsets", index)
-        if k_offsets is None:
-            if k.shape[0] != q.shape[0]:
-                raise ValueError(f"k_offsets is needed: {q.shape[0]} query tokens and "
-                                 f"{k.shape[0]} key tokens")
-            k_offsets = q_offsets
-    if k_offsets is not None and k_offsets is not q_offsets:
-        if q_offsets is None:
-            raise ValueError("k_offsets needs q_offsets")
-        _check_offsets(k_offsets, "k_offsets", index)
-        if k_offsets.shape[0] != q_offsets.shape[0]:
-            raise ValueError(f"q_offsets is {tuple(q_offsets.shape)} and k_offsets "
-                             f"{tuple(k_offsets.shape)}; one number of sequences is needed")
+    dim, index = _check_heads(q, k, v)
+    k_offsets = _check_bounds(q, k, q_offsets, k_offsets, index)
     scale = max(dim, 1) ** -0.5 if scale is None else float(scale)
     if window is not None:
         if not causal:
@@ -181,3 +194,81 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
             or _lib.forward_mode():
         return _Attention.apply(q, k, v, q_offsets, k_offsets, bool(causal), window, scale)
     return _forward(q, k, v, q_offsets, k_offsets, bool(causal), window, scale, False)[0]
+
+
+class _Shared(torch.autograd.Function):
+    """Calls while forward-mode derivatives are taken: autograd refuses a tangent."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return _shared_forward(*args)
+
+    @staticmethod
+    def backward(ctx, dout):
+        raise NotImplementedError("shared_attention has no gradient")
+
+
+def _shared_forward(q, k, v, shared_k, shared_v, q_offsets, k_offsets, group_offsets,
+                    shared_offsets, causal, scale):
+    lib = _lib.load()
+    rows = [_rows(t) for t in (q, k, v, shared_k, shared_v)]     # copies live until the launch
+    Tq, Hq, D = q.shape
+    Tk, Hk, _ = k.shape
+    Ts = shared_k.shape[0]
+    n = 1 if q_offsets is None else q_offsets.numel() - 1
+    groups = 1 if group_offsets is None else group_offsets.numel() - 1
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    need = lib.mg_shared_attention_workspace_bytes(Tq, Tk, Ts, Hq, Hk, D, n, groups)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    at = [None if t is None else t.data_ptr()
+          for t in (q_offsets, k_offsets, group_offsets, shared_offsets)]
+    _lib.launch(lib.mg_shared_attention, q.get_device(), _lib.TYPE_CODES[q.dtype], Tq, Tk, Ts, Hq,
+                Hk, D, *(a for _, args in rows for a in args), at[0], at[1], n, at[2], at[3],
+                groups, causal, scale, out.data_ptr(), ws.data_ptr() if need else None, need)
+    return out
+
+
+def shared_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, shared_k: torch.Tensor,
+                     shared_v: torch.Tensor, q_offsets: torch.Tensor | None = None,
+                     k_offsets: torch.Tensor | None = None,
+                     group_offsets: torch.Tensor | None = None,
+                     shared_offsets: torch.Tensor | None = None, *, causal: bool = False,
+                     scale: float | None = None) -> torch.Tensor:
+    """Attention of packed sequences to their own keys and, in the same softmax, to
+    all of a memory that several sequences share (candidate cameras over one scene):
+    what ``attention`` gives with the memory's keys and values before each sequence's
+    own, while a shared key is read once for all of its group's queries and kept
+    once.
+
+    ``q``, ``k``, ``v``, ``q_offsets`` and ``k_offsets`` are those of ``attention``, and
+    so is ``causal``, which bounds a sequence's own keys alone. ``shared_k`` and
+    ``shared_v`` (their own tokens, k's heads, dim) may lie as k and v.
+    ``group_offsets`` and ``shared_offsets`` (groups + 1, int32, on the GPU) bound each
+    group's query tokens and its memory's tokens; both default to one group of all
+    queries over all of the memory. Queries of no group have no shared keys, those of
+    no sequence no own ones; a query without any gets zeros.
+
+    bfloat16 or float16; scores, softmax and sums are float32 and p is rounded for
+    its product with v, as in ``attention``. For serving: inputs that require a
+    gradient are refused (train with ``attention`` over packed sequences).
+    """
+    dim, index = _check_heads(q, k, v, shared_k, shared_v)
+    if shared_k.shape != shared_v.shape or shared_k.shape[1] != k.shape[1]:
+        raise ValueError(f"shared_k is {tuple(shared_k.shape)} and shared_v "
+                         f"{tuple(shared_v.shape)}; one shape, of k's {k.shape[1]} heads, is "
+                         "needed")
+    k_offsets = _check_bounds(q, k, q_offsets, k_offsets, index)
+    if (group_offsets is None) != (shared_offsets is None):
+        raise ValueError("group_offsets and shared_offsets go together")
+    if group_offsets is not None:
+        _check_offsets(group_offsets, "group_offsets", index)
+        _check_offsets(shared_offsets, "shared_offsets", index)
+        if group_offsets.shape[0] != shared_offsets.shape[0]:
+            raise ValueError(f"group_offsets is {tuple(group_offsets.shape)} and shared_offsets "
+                             f"{tuple(shared_offsets.shape)}; one number of groups is needed")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, shared_k, shared_v)):
+        raise RuntimeError("shared_attention has no gradient, and an input requires one")
+    scale = max(dim, 1) ** -0.5 if scale is None else float(scale)
+    run = _Shared.apply if _lib.forward_mode() else _shared_forward
+    return run(q, k, v, shared_k, shared_v, q_offsets, k_offsets, group_offsets, shared_offsets,
+               bool(causal), scale)

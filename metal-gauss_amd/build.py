@@ -25,7 +25,7 @@ ARCH = "gfx950"
 SOURCES = ["runtime.hip", "adam.hip", "preprocess.hip", "mip.hip", "mcmc.hip", "binning.hip", "sort.hip",
            "rasterize.hip", "ssim.hip", "ply.hip", "norm.hip", "rotary.hip",
            "norm_rotary.hip", "dropout.hip",
-           "attention.hip", "attention_bwd.hip"]
+           "attention.hip", "attention_bwd.hip", "attention_shared.hip"]
 
 # -packed-fp32-ops keeps the compiler from emitting packed fp32 VALU forms;
 # hardware float atomics are requested explicitly (the gradient buffers are

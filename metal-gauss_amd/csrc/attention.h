@@ -54,6 +54,7 @@ struct AttnArgs {
     // afterwards.
     int32_t split_keys, chunk_tiles;
     int32_t span_extra, span_most;       // of the keys an item goes through: span_keys
+    int32_t row_chunks;                  // see Cut
     float2 *part_stats;
     float *part_o;
     // Backward.

@@ -173,3 +173,37 @@ def attention(q, k, v, q_offsets, k_offsets, causal, scale, dout=None, unit=0.0,
     for i in (1, 2, 3):
         off[i] += unit * np.abs(out[i])
     return tuple(out), tuple(off)
+
+
+def shared_attention(q, k, v, shared_k, shared_v, q_offsets, k_offsets, group_offsets,
+                     shared_offsets, causal, scale, unit=0.0):
+    """o and how far it may be off (as `attention`): each query over its group's shared
+    keys and the keys that it sees of its own sequence."""
+    q, k, v, sk, sv = (np.asarray(t, np.float64) for t in (q, k, v, shared_k, shared_v))
+    group = q.shape[1] // k.shape[1]
+    out, off = np.zeros(q.shape), np.zeros(q.shape)
+
+    def bounds(offsets, token):
+        """The sequence that has a token, or -1."""
+        for s in range(len(offsets) - 1):
+            if offsets[s] <= token < offsets[s + 1]:
+                return s
+        return -1
+
+    for t in range(q.shape[0]):
+        s, g = bounds(q_offsets, t), bounds(group_offsets, t)
+        own = np.arange(0)
+        if s >= 0:
+            own = np.arange(k_offsets[s], k_offsets[s + 1])
+            if causal:
+                own = own[:max(0, t - q_offsets[s + 1] + 1 + len(own))]
+        all_shared = np.arange(0) if g < 0 else np.arange(shared_offsets[g], shared_offsets[g + 1])
+        if len(own) + len(all_shared) == 0:
+            continue
+        for h in range(q.shape[1]):
+            kh = np.concatenate([sk[all_shared, h // group], k[own, h // group]])
+            vh = np.concatenate([sv[all_shared, h // group], v[own, h // group]])
+            p = probabilities(q[t:t + 1, h], kh, scale, np.ones((1, len(kh)), bool))[0]
+            out[t, h] = p @ vh
+            off[t, h] = unit * (np.abs(out[t, h]) + p @ np.abs(vh))
+    return out, off
