@@ -717,7 +717,8 @@ int32_t mg_norm_rotary_forward(
  * weights' type), each of which may be NULL. Sums over tokens and heads are
  * formed in a fixed order: equal calls give equal bits. The workspace is needed
  * where a weight's gradient is. */
-int64_t mg_norm_rotary_backward_workspace_bytes(int32_t dim);
+int64_t mg_norm_rotary_backward_workspace_bytes(int32_t q_heads,
+                                                int32_t k_heads, int32_t dim);
 int32_t mg_norm_rotary_backward(
     int64_t tokens, int32_t dtype, const void *q, int64_t q_token_stride,
     int64_t q_head_stride, int32_t q_heads, const void *k,

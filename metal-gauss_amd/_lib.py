@@ -136,7 +136,7 @@ _SIGNATURES = {
     "mg_norm_rotary_forward": (_i32, [_i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32,
                                       _i32, _i32, _vp, _vp, _f32, _vp, _i32, _i32, _vp, _vp,
                                       _i32, _i32, _vp, _vp, _vp]),
-    "mg_norm_rotary_backward_workspace_bytes": (_i64, [_i32]),
+    "mg_norm_rotary_backward_workspace_bytes": (_i64, [_i32, _i32, _i32]),
     "mg_norm_rotary_backward": (_i32, [_i64, _i32, _vp, _i64, _i64, _i32, _vp, _i64, _i64, _i32,
                                        _i32, _i32, _vp, _vp, _f32, _vp, _i32, _i32, _vp, _vp,
                                        _i32, _i32, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _vp,

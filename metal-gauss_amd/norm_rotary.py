@@ -87,7 +87,7 @@ class _NormRotary(torch.autograd.Function):
         if tokens and kept:
             ws, size = None, 0
             if dw[0] is not None or dw[1] is not None:
-                size = lib.mg_norm_rotary_backward_workspace_bytes(dim)
+                size = lib.mg_norm_rotary_backward_workspace_bytes(heads[3], heads[7], dim)
                 ws = torch.empty(size, dtype=torch.uint8, device=dev)
             _lib.launch(lib.mg_norm_rotary_backward, q.get_device(), tokens, code, *heads, dim,
                         _weight_code((q_weight, k_weight), code), *weight_at, ctx.eps,
