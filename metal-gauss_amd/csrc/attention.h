@@ -117,16 +117,13 @@ __device__ __forceinline__ int wave_inclusive_max(int v) {       // v >= 0
 // carried on. Offsets are held to [0, tokens] and made to rise (an offset below
 // one before it counts as that one), so that no value of theirs leads out of the
 // tensors and every token is in one pseudo sequence. For all lanes of a wave.
-__device__ __forceinline__ void seq_bounds(const int32_t *off, int n, int tokens, int s0, int &end,
-                                           int &lo, int &len) {
+__device__ __forceinline__ int seq_offset(const int32_t *off, int n, int tokens, int s0) {
     const int s = s0 + lane_id();
-    int to = tokens;
-    if (off) {
-        if (s <= n) to = clamp_to(off[s], 0, tokens);
-    } else if (s == 0) {
-        to = 0;
-    }
-    to = max(end, wave_inclusive_max(to));
+    if (!off) return s == 0 ? 0 : tokens;
+    return s <= n ? off[s] : tokens;
+}
+__device__ __forceinline__ void seq_bounds(int offset, int tokens, int &end, int &lo, int &len) {
+    const int to = max(end, wave_inclusive_max(clamp_to(offset, 0, tokens)));
     lo = __builtin_amdgcn_update_dpp(end, to, 0x138, 0xf, 0xf, false);   // wave_shr:1
     len = to - lo;
     end = __builtin_amdgcn_readlane(to, 63);
@@ -134,17 +131,25 @@ __device__ __forceinline__ void seq_bounds(const int32_t *off, int n, int tokens
 
 // The sequence that has `item` when a sequence has count(q_len, k_len) items;
 // `before` sums second(q_len, k_len). Every lane of a wave calls with the same
-// item and gets the same answer; where no sequence has the item, found is false.
+// item and gets the same answer; where no sequence has the item, found is false
+// and within the number of all items.
 template <bool kByKeys, typename Count, typename Second>
 __device__ __forceinline__ SeqItem find_item(const AttnArgs &a, int item, Count count,
                                              Second second) {
     SeqItem r{};
     int base = 0, base2 = 0, q_end = 0, k_end = 0;
+    const auto q_at = [&](int s0) { return seq_offset(a.q_off, a.n_seq, a.q_tokens, s0); };
+    const auto k_at = [&](int s0) { return seq_offset(a.k_off, a.n_seq, a.k_tokens, s0); };
+    // Offsets are asked for three steps ahead (128 streams over their own keys: 22 us a
+    // launch without, each step waiting for its own).
+    int q0 = q_at(0), k0 = k_at(0), q1 = q_at(64), k1 = k_at(64), q2 = q_at(128), k2 = k_at(128);
     for (int s0 = 0; s0 < a.n_seq + 2; s0 += 64) {
         const int s = s0 + lane_id();
         int q_lo, q_len, k_lo, k_len;
-        seq_bounds(a.q_off, a.n_seq, a.q_tokens, s0, q_end, q_lo, q_len);
-        seq_bounds(a.k_off, a.n_seq, a.k_tokens, s0, k_end, k_lo, k_len);
+        seq_bounds(q0, a.q_tokens, q_end, q_lo, q_len);
+        seq_bounds(k0, a.k_tokens, k_end, k_lo, k_len);
+        q0 = q1, q1 = q2, k0 = k1, k1 = k2;
+        q2 = q_at(s0 + 192), k2 = k_at(s0 + 192);
         if (s == 0 || s > a.n_seq) (kByKeys ? q_len : k_len) = 0;
         const int n = count(q_len, k_len), n2 = second(q_len, k_len);
         const int upto = wave_inclusive_sum(n), upto2 = wave_inclusive_sum(n2);
@@ -162,6 +167,7 @@ __device__ __forceinline__ SeqItem find_item(const AttnArgs &a, int item, Count 
         base += __builtin_amdgcn_readlane(upto, 63);
         base2 += __builtin_amdgcn_readlane(upto2, 63);
     }
+    r.within = base;
     return r;
 }
 
@@ -246,8 +252,8 @@ __device__ __forceinline__ SeqItem find_longest(const AttnArgs &a, int item, int
     }
     const int seq = lane_id();
     int q_end = 0, k_end = 0, q_lo, q_len, k_lo, k_len;
-    seq_bounds(a.q_off, a.n_seq, a.q_tokens, 0, q_end, q_lo, q_len);
-    seq_bounds(a.k_off, a.n_seq, a.k_tokens, 0, k_end, k_lo, k_len);
+    seq_bounds(seq_offset(a.q_off, a.n_seq, a.q_tokens, 0), a.q_tokens, q_end, q_lo, q_len);
+    seq_bounds(seq_offset(a.k_off, a.n_seq, a.k_tokens, 0), a.k_tokens, k_end, k_lo, k_len);
     if (seq == 0 || seq > a.n_seq) (kByKeys ? q_len : k_len) = 0;
     const int tiles = tiles_of(q_len, k_len);
     const auto with = [&](int w) {                // this lane's sequence's

@@ -205,6 +205,9 @@ struct FwdPlan {
 // one sequence of 2500, 8 heads of 64: 40 aimed at 256, 26 at 512).
 constexpr int64_t kWideSlots = 512, kNarrowSlots = 1536;
 constexpr int64_t kSplitLeast = 768, kChunkLeast = 256;
+// Single tokens with a window have few keys each: shorter chunks (16 tokens of 16
+// heads on 4 of 64, window 2000: 11 us, in chunks of 256 14).
+constexpr int64_t kWindowSplitLeast = 256, kWindowChunkLeast = 128;
 
 static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int group, int dim,
                         int n_seq, int window, int sinks) {
@@ -229,9 +232,11 @@ static FwdPlan fwd_plan(int64_t q_tokens, int64_t k_tokens, int k_heads, int gro
         if (k_tokens > n_seq * most) k_tokens = n_seq * most;
     }
     const int64_t mean_keys = k_tokens / n_seq;
-    if (2 * likely <= slots && mean_keys >= kSplitLeast) {
+    const bool short_chunks = window > 0 && p.waves == kNarrowWaves;
+    if (2 * likely <= slots && mean_keys >= (short_chunks ? kWindowSplitLeast : kSplitLeast)) {
         int64_t keys = ceil_div(ceil_div(mean_keys * likely, slots), tile) * tile;
-        if (keys < kChunkLeast) keys = kChunkLeast;
+        const int64_t least = short_chunks ? kWindowChunkLeast : kChunkLeast;
+        if (keys < least) keys = least;
         p.split_keys = (int)keys;
         // Sum of tiles * (1 + keys / chunk) over the sequences, which have each
         // token once whatever the offsets hold (seq_bounds): the partial results

@@ -202,9 +202,22 @@ __device__ __forceinline__ f32x4 *row_values(const AttnArgs &a, int kh, int64_t 
            (row_group(a, kh, row) * a.row_chunks + chunk) * (32 * DK / 4) + 32 * half + row % 32;
 }
 
-// One work item: false if there is none of this number.
+// The item of a number among those cut into chunks by rows.
+template <int kWaves>
+__device__ __forceinline__ SeqItem find_row_item(const AttnArgs &a, int item) {
+    constexpr int kRows = 32 * kWaves;
+    return find_item<false>(
+        a, item,
+        [&](int ql, int kl) {
+            return (ql * a.group + kRows - 1) / kRows * row_chunks_of<kKeyTile<kWaves>>(a, kl);
+        },
+        [](int, int) { return 0; });
+}
+
+// One work item: false if there is none of this number. By rows, the caller has
+// found it.
 template <typename T, int DK, int kWaves, Cut kCut, bool kWin>
-__device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
+__device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work, SeqItem s = {}) {
     constexpr int kRows = 32 * kWaves, kSteps = DK / 16, kBlocks = DK / 32;
     constexpr bool kInterleave = kWaves == kWideWaves;
     constexpr int kTile = kKeyTile<kWaves>, kParts = kTile / 32;
@@ -217,14 +230,8 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kh = work % a.k_heads, item = work / a.k_heads, G = a.group;
     const auto tiles_of = [&](int ql, int) { return (ql * G + kRows - 1) / kRows; };
-    SeqItem s;
     int tile, chunk = 0, split_keys = 0;
     if constexpr (kCut == kByRow) {
-        s = find_item<false>(
-            a, item,
-            [&](int ql, int kl) { return tiles_of(ql, kl) * row_chunks_of<kTile>(a, kl); },
-            [](int, int) { return 0; });
-        if (!s.found) return false;
         const int chunks = row_chunks_of<kTile>(a, s.k_len);
         split_keys = row_chunk_keys<kTile>(a, s.k_len);
         tile = tiles_of(s.q_len, 0) - 1 - s.within / chunks;
@@ -330,8 +337,9 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work) {
         const bool more = number + kTile < k_to;
         const int next0 = key_at<kWin>(run, number + kTile);
         // The wave's rows see none of these keys.
-        const bool none =
-            key0 >= sees.to(see_last) || (kWin && key0 + kTile <= sees.from(low_first));
+        const bool none = key0 >= sees.to(see_last) ||
+                          (kWin && key0 + kTile <= sees.from(low_first)) ||
+                          (kCut == kByRow && row0 >= s.q_len * G);
         constexpr int kEach = decltype(fill_k)::kLoads;
         if (kInterleave && next0 + kTile <= s.k_len && more && !none) {
             // The next tile's loads one by one between the products: all at once

@@ -12,92 +12,145 @@
 // shared memory they are one sequence of many rows, whose tiles read each key once
 // for 128 rows where a sequence by itself would read it for its own few; over their
 // own keys they are the packed sequences that they are. Both are the work items of
-// attention_fwd.h, in two launches, whose partial results lie by rows, so that the
-// third finds a row's without a search.
+// attention_fwd.h, in one launch, those over the memory first (their own after them
+// in a launch of narrow items: 128 streams of 16 heads on 4 of 128, 30 and 22 us).
+// Partial results lie by rows, so that joining finds a row's without a search.
 #include "attention_fwd.h"
 
 namespace mg {
 
+// Items over the shared memories come first, then those over the sequences' own
+// keys, of which there are `most` in all at most: how many, the device alone knows.
 template <typename T, int DK, int kWaves>
-__global__ __launch_bounds__(64 * kWaves, kWaves == 1 ? 1 : 2) void attn_part_kernel(AttnArgs a) {
-    for (int work = blockIdx.x; attn_fwd_item<T, DK, kWaves, kByRow, false>(a, work);
-         work += gridDim.x)
+__global__ __launch_bounds__(64 * kWaves, kWaves == 1 ? 1 : 2) void attn_part_kernel(
+    AttnArgs shared, AttnArgs alone, int most) {
+    for (int work = blockIdx.x; work < most; work += gridDim.x) {
+        SeqItem s = find_row_item<kWaves>(shared, work / shared.k_heads);
+        const bool of_shared = s.found;
+        if (!of_shared) s = find_row_item<kWaves>(alone, work / alone.k_heads - s.within);
+        if (!s.found) return;
+        attn_fwd_item<T, DK, kWaves, kByRow, false>(of_shared ? shared : alone, work, s);
         tiles_ready();
+    }
+}
+
+// What a lane has joined so far: four columns of a row.
+struct Joined {
+    float top = -INFINITY, sum = 0.f;
+    f32x4 o = {};
+
+    // N chunks' results; those from n on are none.
+    template <int N>
+    __device__ __forceinline__ void add(const float2 (&st)[N], const f32x4 (&x)[N], int n) {
+        float next = top;
+#pragma unroll
+        for (int i = 0; i < N; ++i) next = i < n ? fmaxf(next, st[i].x) : next;
+        const float shrink = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
+        top = next;
+        sum *= shrink;
+        o *= shrink;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float by = st[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(st[i].x - top);
+            // A NaN sum of a chunk without a finite score goes on; a place that no
+            // chunk has filled holds anything.
+            const bool used = i < n && (st[i].x != -INFINITY || st[i].y != 0.f);
+            sum = used ? fmaf(st[i].y, by, sum) : sum;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = used ? fmaf(x[i][k], by, o[k]) : o[k];
+        }
+    }
+};
+
+// Chunks c .. c + N - 1 of a row (past the last, the last's).
+template <int DK, int N>
+__device__ __forceinline__ void ask_chunks(const AttnArgs &a, const float2 *st, const f32x4 *from,
+                                           int c, float2 (&s)[N], f32x4 (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int at = min(c + i, a.row_chunks - 1);
+        s[i] = st[at * 32];
+        x[i] = from[at * (32 * DK / 4)];
+    }
 }
 
 // A wave has four columns of 32 rows in each of its halves: columns 8 j + 4 half ..
-template <typename T, int DK>
+// Stats and values are asked for together, the first chunks of both sets at once.
+// kFirst and kFew are of the numbers of chunks, which are one mostly where rows are
+// many.
+template <typename T, int DK, int kFirst, int kFew>
 __global__ __launch_bounds__(256) void attn_join_parts_kernel(AttnArgs shared, AttnArgs alone) {
-    const AttnArgs *const sets[2] = {&shared, &alone};
     const int lane = lane_id(), half = lane / 32, G = alone.group, kh = blockIdx.y, j = blockIdx.z;
     const int64_t rows = (int64_t)alone.q_tokens * G;
     const int64_t row = ((int64_t)blockIdx.x * 4 + threadIdx.x / 64) * 32 + lane % 32;
     const int at = 8 * j + 4 * half;
     if (row >= rows || at >= alone.dim) return;
-    float top = -INFINITY, sum = 0.f;
-    f32x4 o = {};
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const float2 *st = row_stats(*sets[k], kh, row, 0);
-#pragma unroll 8
-        for (int c = 0; c < sets[k]->row_chunks; ++c) top = fmaxf(top, st[c * 32].x);
+    const float2 *st[2] = {row_stats(shared, kh, row, 0), row_stats(alone, kh, row, 0)};
+    const f32x4 *from[2] = {row_values<DK>(shared, kh, row, 0, half) + 64 * j,
+                            row_values<DK>(alone, kh, row, 0, half) + 64 * j};
+    Joined r;
+    float2 s0[kFirst], s1[kFew];
+    f32x4 x0[kFirst], x1[kFew];
+    ask_chunks<DK>(shared, st[0], from[0], 0, s0, x0);
+    ask_chunks<DK>(alone, st[1], from[1], 0, s1, x1);
+    r.add(s0, x0, shared.row_chunks);
+    r.add(s1, x1, alone.row_chunks);
+    for (int c = kFirst; c < shared.row_chunks; c += kFirst) {
+        ask_chunks<DK>(shared, st[0], from[0], c, s0, x0);
+        r.add(s0, x0, shared.row_chunks - c);
     }
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-        const float2 *st = row_stats(*sets[k], kh, row, 0);
-        const f32x4 *from = row_values<DK>(*sets[k], kh, row, 0, half) + 64 * j;
-#pragma unroll 8
-        for (int c = 0; c < sets[k]->row_chunks; ++c) {
-            const float2 s = st[c * 32];
-            const f32x4 x = from[c * (32 * DK / 4)];
-            const float by = s.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s.x - top);
-            // A NaN sum of a chunk without a finite score goes on; a place that no
-            // chunk has filled holds anything.
-            const bool used = s.x != -INFINITY || s.y != 0.f;
-            sum = fmaf(s.y, by, sum);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) o[i] = used ? fmaf(x[i], by, o[i]) : o[i];
-        }
+    for (int c = kFew; c < alone.row_chunks; c += kFirst) {
+        ask_chunks<DK>(alone, st[1], from[1], c, s0, x0);
+        r.add(s0, x0, alone.row_chunks - c);
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const float inv = r.sum == 0.f ? 0.f : 1.f / r.sum;
     vec4<T> w;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (T)(o[i] * inv);
+    for (int i = 0; i < 4; ++i) w[i] = (T)(r.o[i] * inv);
     const int64_t token = row / G, head = kh * G + row % G;
     *reinterpret_cast<vec4<T> *>(static_cast<T *>(alone.out) +
                                  (token * (alone.k_heads * G) + head) * alone.dim + at) = w;
 }
 
 // -------------------------------------------------------------------- host
-// How one set of items is cut (see fwd_plan, whose limits these are).
+// How one set of items is cut.
 struct PartPlan {
     int waves, split_keys, row_chunks;
     int64_t items;              // of a key head, at most
     int64_t stats_bytes, bytes;
 };
 
-constexpr int64_t kPartWideSlots = 512, kPartNarrowSlots = 1536;
-constexpr int64_t kPartSplitLeast = 768, kPartChunkLeast = 256, kPartMostChunks = 64;
+// Items that run at once.
+static int64_t part_slots(int waves) { return waves == kNarrowWaves ? 1536 : 512; }
+
+constexpr int64_t kPartMostChunks = 64;
+// Keys of a chunk, at least: wide items, narrow ones; and long ones, whose start and
+// partial results cost little beside them.
+constexpr int64_t kPartWideLeast = 256, kPartNarrowLeast = 64, kPartLong = 2048;
+
+// Both sets take the items of one width: wide ones, unless the rows of both fill half
+// of one at most.
+static int part_waves(int64_t rows, int64_t groups, int64_t sequences) {
+    return rows <= 64 * groups && rows <= 64 * sequences ? kNarrowWaves : kWideWaves;
+}
 
 static PartPlan part_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int64_t group,
-                          int dim, int64_t n_seq) {
+                          int dim, int64_t n_seq, int waves) {
     PartPlan p{};
     const int64_t rows = q_tokens * group;
-    p.waves = rows <= 64 * n_seq ? kNarrowWaves : kWideWaves;
-    const int64_t tile_rows = 32 * p.waves;
-    const int64_t slots = p.waves == kNarrowWaves ? kPartNarrowSlots
-                          : n_seq == 1            ? kPartWideSlots
-                                                  : kPartWideSlots / 2;
+    p.waves = waves;
+    const int64_t tile_rows = 32 * p.waves, slots = part_slots(waves);
     const int64_t likely = (ceil_div(rows, tile_rows) + n_seq - 1) * k_heads;
     const int64_t mean_keys = k_tokens / n_seq;
-    p.split_keys = (int)kPartChunkLeast;
-    p.row_chunks = 1;
-    if (2 * likely <= slots && mean_keys >= kPartSplitLeast) {
-        int64_t chunks = slots / likely;
-        if (chunks > ceil_div(mean_keys, kPartChunkLeast))
-            chunks = ceil_div(mean_keys, kPartChunkLeast);
-        p.row_chunks = (int)(chunks < kPartMostChunks ? chunks : kPartMostChunks);
-    }
+    // As many chunks as make items for all slots, of `least` keys at least; and where
+    // chunks stay long, as make several rounds of items, which even out.
+    const int64_t least = waves == kNarrowWaves ? kPartNarrowLeast : kPartWideLeast;
+    int64_t chunks = slots / likely, longer = ceil_div(3 * slots, likely);
+    if (chunks > ceil_div(mean_keys, least)) chunks = ceil_div(mean_keys, least);
+    if (longer > mean_keys / kPartLong) longer = mean_keys / kPartLong;
+    if (chunks < longer) chunks = longer;
+    p.row_chunks = (int)(chunks < 1 ? 1 : chunks < kPartMostChunks ? chunks : kPartMostChunks);
+    p.split_keys = (int)least;
     // The tokens before the first and past the last offset make tiles too, of one
     // chunk each.
     p.items = (rows / tile_rows + n_seq + 2) * p.row_chunks;
@@ -120,8 +173,9 @@ int64_t mg_shared_attention_workspace_bytes(int64_t q_tokens, int64_t k_tokens,
         sequences < 1 || groups < 1)
         return 0;
     const int group = q_heads / k_heads;
-    return mg::part_plan(q_tokens, shared_tokens, k_heads, group, dim, groups).bytes +
-           mg::part_plan(q_tokens, k_tokens, k_heads, group, dim, sequences).bytes;
+    const int waves = mg::part_waves(q_tokens * group, groups, sequences);
+    return mg::part_plan(q_tokens, shared_tokens, k_heads, group, dim, groups, waves).bytes +
+           mg::part_plan(q_tokens, k_tokens, k_heads, group, dim, sequences, waves).bytes;
 }
 
 int32_t mg_shared_attention(
@@ -171,36 +225,38 @@ int32_t mg_shared_attention(
     MG_REQUIRE(q && out && (k_tokens == 0 || (k && v)) &&
                    (shared_tokens == 0 || (shared_k && shared_v)),
                "%s: a pointer is NULL", who);
+    const int waves = part_waves(q_tokens * group, groups, sequences);
     const PartPlan plans[2] = {
-        part_plan(q_tokens, shared_tokens, k_heads, group, dim, groups),
-        part_plan(q_tokens, k_tokens, k_heads, group, dim, sequences)};
-    const int64_t row_blocks = ceil_div(q_tokens * group, 4 * 32);
-    for (const PartPlan &p : plans)
-        MG_REQUIRE(grid_fits(p.items * k_heads, 64 * p.waves) && k_heads < 65536,
-                   "%s: too many work items", who);
+        part_plan(q_tokens, shared_tokens, k_heads, group, dim, groups, waves),
+        part_plan(q_tokens, k_tokens, k_heads, group, dim, sequences, waves)};
+    const int64_t items = (plans[0].items + plans[1].items) * k_heads;
+    MG_REQUIRE(grid_fits(items, 64 * waves) && items < INT32_MAX && k_heads < 65536,
+               "%s: too many work items", who);
     MG_REQUIRE(workspace && workspace_bytes >= plans[0].bytes + plans[1].bytes,
                "%s: workspace of %lld bytes, %lld needed", who, (long long)workspace_bytes,
                (long long)(plans[0].bytes + plans[1].bytes));
-    hipStream_t st = as_stream(stream);
     char *ws = static_cast<char *>(workspace);
     for (int i = 0; i < 2; ++i) {
-        AttnArgs &a = sets[i];
-        const PartPlan &p = plans[i];
-        a.split_keys = p.split_keys, a.row_chunks = p.row_chunks;
-        a.part_stats = reinterpret_cast<float2 *>(ws);
-        a.part_o = reinterpret_cast<float *>(ws + p.stats_bytes);
-        ws += p.bytes;
-        const int64_t items = p.items * k_heads;
-        const int64_t most = 2 * (p.waves == kWideWaves ? kPartWideSlots : kPartNarrowSlots);
+        sets[i].split_keys = plans[i].split_keys, sets[i].row_chunks = plans[i].row_chunks;
+        sets[i].part_stats = reinterpret_cast<float2 *>(ws);
+        sets[i].part_o = reinterpret_cast<float *>(ws + plans[i].stats_bytes);
+        ws += plans[i].bytes;
+    }
+    hipStream_t st = as_stream(stream);
+    {
+        // Items are taken in turn by twice as many workgroups as run at once.
+        const int64_t most = 2 * part_slots(waves);
         const unsigned grid = (unsigned)(items > most ? most : items);
-        TimedScope ts(i == 0 ? "attention_shared" : "attention_alone", st);
+        TimedScope ts("attention_parts", st);
         attn_form(dtype, dim, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int DK = decltype(d)::value;
-            if (p.waves == kWideWaves)
-                attn_part_kernel<T, DK, kWideWaves><<<grid, 64 * kWideWaves, 0, st>>>(a);
+            if (waves == kWideWaves)
+                attn_part_kernel<T, DK, kWideWaves>
+                    <<<grid, 64 * kWideWaves, 0, st>>>(sets[0], sets[1], (int)items);
             else
-                attn_part_kernel<T, DK, kNarrowWaves><<<grid, 64 * kNarrowWaves, 0, st>>>(a);
+                attn_part_kernel<T, DK, kNarrowWaves>
+                    <<<grid, 64 * kNarrowWaves, 0, st>>>(sets[0], sets[1], (int)items);
         });
         MG_LAUNCHED("attn_part_kernel");
     }
@@ -209,8 +265,12 @@ int32_t mg_shared_attention(
         attn_form(dtype, dim, [&](auto t, auto d) {
             using T = decltype(t);
             constexpr int DK = decltype(d)::value;
-            const dim3 grid((unsigned)row_blocks, (unsigned)k_heads, DK / 8);
-            attn_join_parts_kernel<T, DK><<<grid, 256, 0, st>>>(sets[0], sets[1]);
+            const dim3 grid((unsigned)ceil_div(q_tokens * group, 4 * 32), (unsigned)k_heads,
+                            DK / 8);
+            if (plans[0].row_chunks == 1 && plans[1].row_chunks == 1)
+                attn_join_parts_kernel<T, DK, 1, 1><<<grid, 256, 0, st>>>(sets[0], sets[1]);
+            else
+                attn_join_parts_kernel<T, DK, 12, 4><<<grid, 256, 0, st>>>(sets[0], sets[1]);
         });
         MG_LAUNCHED("attn_join_parts_kernel");
     }
