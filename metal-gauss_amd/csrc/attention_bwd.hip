@@ -280,10 +280,11 @@ __device__ __forceinline__ f32x4 *part_of(const AttnArgs &a, int item, int kh, i
 
 // With a window, the queries that see a key tile are few, but those further on all
 // see the sinks. Their sums for the sinks are work items of their own, which go
-// first: one tile of kBwdTile keys, one head and sink_steps query tiles each. Item
-// i keeps them, of sink_rows keys, in place i of sink_part; the sequence's
-// window items, after them, a place each key tile that has sinks (sink_items has them
-// all), where they are not cut into runs.
+// first: one tile of kBwdTile keys, one head and sink_steps query tiles each. Their
+// sums, of sink_rows keys, have a place each in sink_part, and so have those of the
+// window items of key tiles that have sinks; attn_sink_sum_kernel adds them up, in
+// order. A sequence's places follow one another, a key tile's far items' and then
+// its window items'; item i of the far ones has place i.
 struct SinkItems {
     int key_tiles, from, tiles, pieces;    // from: the first query past the window
 
@@ -295,10 +296,9 @@ struct SinkItems {
         if (q_len == 0) key_tiles = 0;
     }
     __device__ __forceinline__ int runs(const AttnArgs &a) const { return pieces * a.group; }
-    // Items, and places, of a sequence.
-    __device__ __forceinline__ int all(const AttnArgs &a) const {
-        return key_tiles * (runs(a) + 1);
-    }
+    // Places of a key tile, and of a sequence.
+    __device__ __forceinline__ int places(const AttnArgs &a) const { return runs(a) + a.splits; }
+    __device__ __forceinline__ int all(const AttnArgs &a) const { return key_tiles * places(a); }
 };
 
 template <int DK>
@@ -357,13 +357,13 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
         const SinkItems of(a, s.q_len, s.k_len);
         sink_runs = of.runs(a);
         if (far) {
-            first_key = s.within / (sink_runs + 1) * kBwdTile;
-            sink_run = s.within % (sink_runs + 1);
-            if (sink_run == sink_runs) return;         // the window item's place
+            first_key = s.within / of.places(a) * kBwdTile;
+            sink_run = s.within % of.places(a);
+            if (sink_run >= sink_runs) return;         // the window items' places
             sink_place = at_item;
             steps_of = {of.from, of.tiles, sink_runs, of.pieces};
         } else {
-            sink_place = s.before + s.within * (sink_runs + 1) + sink_runs;
+            sink_place = s.before + s.within * of.places(a) + sink_runs + split;
         }
     }
     if (!far) {
@@ -499,10 +499,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     lds_reads_done();
     const float down = a.scale * __builtin_amdgcn_exp2f(-power);
     const float down_v = __builtin_amdgcn_exp2f(-kPowerP<T>);
-    // With sinks, the sums of those that queries past the window see too.
-    const bool sinks_too = kWin && sink_runs > 0 && key < a.sinks;
-    if (kWin && (far || (steps_of.runs == 1 && sinks_too))) {
-        if (key >= a.sinks) return;
+    if (kWin && sink_runs > 0 && key < a.sinks) {
         f32x4 *part = sink_part_of<DK>(a, sink_place, kh) + wave * kBlocks * 4 * 64 + lane;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
@@ -519,6 +516,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
             }
         return;
     }
+    if (kWin && far) return;
     if (steps_of.runs > 1) {
         f32x4 *part = part_of<DK>(a, item, kh, split) + wave * kBlocks * 4 * 64 + lane;
 #pragma unroll
@@ -564,52 +562,68 @@ template <typename T, int DK, bool kWin>
 __global__ __launch_bounds__(64 * kBwdWaves) void attn_sum_kernel(AttnArgs a) {
     constexpr int kBlocks = DK / 32;
     const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
-    SeqItem s;
-    if constexpr (kWin)
-        s = find_item<true>(
-            a, item, [&](int, int kl) { return (kl + kBwdTile - 1) / kBwdTile; },
-            [&](int ql, int kl) { return a.sinks > 0 ? SinkItems(a, ql, kl).all(a) : 0; });
-    else
-        s = find_longest<true>(a, item, kBwdTile);
+    const auto key_tiles = [](int, int kl) { return (kl + kBwdTile - 1) / kBwdTile; };
+    const SeqItem s = kWin ? find_item<true>(a, item, key_tiles, [](int, int) { return 0; })
+                           : find_longest<true>(a, item, kBwdTile);
     if (!s.found) return;
     const int first_key = s.within * kBwdTile;
     const int runs = key_steps<kWin>(a, s, first_key).runs;
-    int sink_runs = 0, sink_place = 0;
-    if (kWin && first_key < a.sinks) {
-        sink_runs = SinkItems(a, s.q_len, s.k_len).runs(a);
-        sink_place = s.before + s.within * (sink_runs + 1);
-    }
-    if (runs == 1 && sink_runs == 0) return;
+    if (runs == 1) return;
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / 64);
     const int key = first_key + wave * 32 + lane % 32;
     const int64_t at_row = ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim;
     const f32x4 *part = part_of<DK>(a, item, kh, 0) + wave * kBlocks * 4 * 64 + lane;
     const int which = blockIdx.y % 2, block = blockIdx.y / 2;
-    const bool sinks_too = kWin && sink_runs > 0 && key < a.sinks;
-    if (kWin && runs == 1 && !sinks_too) return;       // written by its only item
-    const f32x4 *far = nullptr;
-    int64_t far_step = 0;
-    if (sinks_too) {
-        far = sink_part_of<DK>(a, sink_place, kh) + wave * kBlocks * 4 * 64 + lane +
-              which * (a.sink_rows * DK / 4);
-        far_step = (int64_t)a.k_heads * (2 * a.sink_rows * DK / 4);
-    }
+    // attn_sink_sum_kernel has these.
+    if (kWin && key < a.sinks && SinkItems(a, s.q_len, s.k_len).runs(a) > 0) return;
 #pragma unroll
     for (int i = 4 * block; i < 4 * block + 4; ++i) {
         const f32x4 *p = part + i * 64 + which * kPartFours<DK> / 2;
-        f32x4 sum = {};
-        if (!kWin || runs > 1) {
-            sum = *p;
-            for (int k = 1; k < runs; ++k) sum += p[k * kPartFours<DK>];
-        }
-        // The far queries' sums and, of a tile in one run, its own.
-        if (sinks_too)
-            for (int k = 0; k < sink_runs + (runs == 1); ++k) sum += far[k * far_step + i * 64];
+        f32x4 sum = *p;
+        for (int k = 1; k < runs; ++k) sum += p[k * kPartFours<DK>];
         const int at = 32 * block + c_row(i % 4 * 4, half);
         if (key < s.k_len && at < a.dim)
             *reinterpret_cast<vec4<T> *>(static_cast<T *>(which ? a.dv : a.dk) + at_row + at) =
                 __builtin_convertvector(sum, vec4<T>);
     }
+}
+
+// The sinks' sums: a workgroup has four columns in each half of a wave, of 32 sinks,
+// of dk or dv, and its waves every kSinkWaves-th place.
+constexpr int kSinkWaves = 16;
+template <typename T, int DK>
+__global__ __launch_bounds__(64 * kSinkWaves) void attn_sink_sum_kernel(AttnArgs a) {
+    constexpr int kBlocks = DK / 32;
+    __shared__ f32x4 s_sum[kSinkWaves][64];
+    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
+    const SeqItem s = find_item<true>(
+        a, item, [&](int ql, int kl) { return SinkItems(a, ql, kl).key_tiles; },
+        [&](int ql, int kl) { return SinkItems(a, ql, kl).all(a); });
+    if (!s.found) return;
+    const SinkItems of(a, s.q_len, s.k_len);
+    if (of.runs(a) == 0) return;                 // the window items have written theirs
+    const int first_key = s.within * kBwdTile;
+    const int places = of.runs(a) + key_steps<true>(a, s, first_key).runs;
+    const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / 64);
+    const int i = blockIdx.y % (kBlocks * 4), rows = blockIdx.y / (kBlocks * 4) / 2 * 32;
+    const int which = blockIdx.y / (kBlocks * 4) % 2;
+    const int key = first_key + rows + lane % 32, at = 32 * (i / 4) + c_row(i % 4 * 4, half);
+    const f32x4 *from = sink_part_of<DK>(a, s.before + s.within * of.places(a), kh) +
+                        (rows / 32 * kBlocks * 4 + i) * 64 + lane +
+                        which * (a.sink_rows * DK / 4);
+    const int64_t step = (int64_t)a.k_heads * (2 * a.sink_rows * DK / 4);
+    f32x4 sum = {};
+    if (key < a.sinks) {
+#pragma unroll 4
+        for (int p = wave; p < places; p += kSinkWaves) sum += from[p * step];
+    }
+    s_sum[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || key >= min(a.sinks, s.k_len) || at >= a.dim) return;
+    for (int w = 1; w < kSinkWaves; ++w) sum += s_sum[w][lane];
+    *reinterpret_cast<vec4<T> *>(static_cast<T *>(which ? a.dv : a.dk) +
+                                 ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim + at) =
+        __builtin_convertvector(sum, vec4<T>);
 }
 
 // Bytes of the backward's scratch: delta, the largest norms, and the runs' sums.
@@ -619,12 +633,15 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_sum_kernel(AttnArgs a) {
 struct BwdPlan {
     int64_t k_items, largest_at, part_at, sink_at, bytes;
     int splits, split_steps;
-    int64_t sink_items;
+    int64_t sink_items, sink_tiles;
     int sink_steps, sink_rows;
 };
 
 constexpr int64_t kBwdRuns = 1024, kBwdRunLeast = 8, kBwdMostSplits = 8;
-constexpr int64_t kSinkSteps = 8;
+// With a window: as many as fill the GPU, as partial results weigh more beside fewer
+// queries (7033 packed tokens, window 475: 118 and 28 us to add them in four runs, 115 and
+// 18 in two). Far items: two rounds of half the GPU's.
+constexpr int64_t kBwdWindowRuns = 512, kSinkItems = 512, kSinkStepsLeast = 4;
 
 static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int64_t group,
                         int64_t dim, int64_t n_seq, int64_t window, int64_t sinks) {
@@ -635,7 +652,7 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     if (window > 0 && queries > ceil_div(window + kBwdTile, kTileRows))
         queries = ceil_div(window + kBwdTile, kTileRows);
     const int64_t steps = queries * group;
-    int64_t splits = kBwdRuns / (tiles > 0 ? tiles : 1);
+    int64_t splits = (window > 0 ? kBwdWindowRuns : kBwdRuns) / (tiles > 0 ? tiles : 1);
     if (splits > steps / kBwdRunLeast) splits = steps / kBwdRunLeast;
     splits = splits < 1 ? 1 : splits > kBwdMostSplits ? kBwdMostSplits : splits;
     p.splits = even_runs((int)splits, (int)group, (int)kBwdMostSplits);
@@ -648,12 +665,16 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     if (p.splits > 1) p.bytes += p.k_items * k_heads * p.splits * 2 * kBwdTile * dk * 4;
     p.sink_at = p.bytes;
     if (sinks > 0) {
-        // Sum over the sequences of SinkItems::all: of key_tiles * (pieces * group + 1),
-        // pieces being at most tokens / (64 sink_steps) + 1 each.
-        p.sink_steps = (int)kSinkSteps;
+        const int64_t key_tiles = ceil_div(sinks, kBwdTile);
+        int64_t most = ceil_div(q_tokens, kTileRows) * group * k_heads * key_tiles / kSinkItems;
+        most = most < kSinkStepsLeast ? kSinkStepsLeast : most;
+        p.sink_steps = (int)(most < 64 ? most : 64);
         p.sink_rows = (int)(sinks < kBwdTile ? ceil_div(sinks, 32) * 32 : kBwdTile);
+        // Sum over the sequences of SinkItems::all: of key_tiles * (pieces * group +
+        // splits), pieces being at most tokens / (64 sink_steps) + 1 each.
         const int64_t pieces = q_tokens / (kTileRows * p.sink_steps) + n_seq;
-        p.sink_items = ceil_div(sinks, kBwdTile) * (pieces * group + n_seq);
+        p.sink_items = key_tiles * (pieces * group + n_seq * p.splits);
+        p.sink_tiles = n_seq * key_tiles;
         p.bytes += p.sink_items * k_heads * 2 * p.sink_rows * dk * 4;
     }
     return p;
@@ -725,6 +746,9 @@ static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_toke
     const int64_t places =
         k_heads * norm_places(q_tokens > k_tokens ? q_tokens : k_tokens, sequences);
     MG_REQUIRE(grid_fits(q_items, 64 * kBwdWaves) && grid_fits(k_items, 64 * kBwdWaves) &&
+                   p.sink_items < INT32_MAX &&
+                   grid_fits(p.sink_tiles * k_heads * (p.sink_rows / 32 * 2 * 128 / 8),
+                             64 * kSinkWaves) &&
                    (dtype != MG_F16 || grid_fits(places, kLargestThreads)),
                "%s: too many work items", who);
     if (dtype == MG_F16) {
@@ -756,7 +780,17 @@ static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_toke
         });
         MG_LAUNCHED("attn_dkv_kernel");
     }
-    if (k_tokens > 0 && dk && (p.splits > 1 || a.sinks > 0)) {
+    if (k_tokens > 0 && dk && a.sinks > 0) {
+        TimedScope ts("attention_sinks", st);
+        attn_form(dtype, dim, [&](auto t, auto d) {
+            constexpr int DK = decltype(d)::value;
+            const dim3 grid((unsigned)(p.sink_tiles * k_heads),
+                            (unsigned)(p.sink_rows / 32 * 2 * DK / 8));
+            attn_sink_sum_kernel<decltype(t), DK><<<grid, 64 * kSinkWaves, 0, st>>>(a);
+        });
+        MG_LAUNCHED("attn_sink_sum_kernel");
+    }
+    if (k_tokens > 0 && dk && p.splits > 1) {
         TimedScope ts("attention_sum", st);
         attn_form(dtype, dim, [&](auto t, auto d) {
             constexpr int DK = decltype(d)::value;
