@@ -112,14 +112,20 @@ def _check_offsets(off, what, index):
 def _check_heads(q, k, v, *more):
     """The head dimension and the GPU of all of them."""
     dtype, dim, index = q.dtype, q.shape[-1] if q.dim() else 0, q.get_device()
-    for t, what in zip((q, k, v, *more), ("q", "k", "v", "shared_k", "shared_v")):
-        if _lib.type_code(t, what) == 0:
-            raise RuntimeError(f"{what} must be bfloat16 or float16, got {t.dtype}")
-        if t.dim() != 3:
-            raise ValueError(f"{what} must be (tokens, heads, dim), got {tuple(t.shape)}")
-        if t.dtype != dtype or t.shape[2] != dim or t.get_device() != index:
-            raise ValueError(f"{what} must match q's type, device and head dimension; got "
-                             f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    others = (k, v, *more)
+    fine = index >= 0 and q.dim() == 3 and (dtype is torch.bfloat16 or dtype is torch.float16)
+    for t in others:
+        fine = fine and t.dtype is dtype and t.get_device() == index and t.dim() == 3 \
+            and t.shape[2] == dim
+    if not fine:
+        for t, what in zip((q, *others), ("q", "k", "v", "shared_k", "shared_v")):
+            if _lib.type_code(t, what) == 0:
+                raise RuntimeError(f"{what} must be bfloat16 or float16, got {t.dtype}")
+            if t.dim() != 3:
+                raise ValueError(f"{what} must be (tokens, heads, dim), got {tuple(t.shape)}")
+            if t.dtype != dtype or t.shape[2] != dim or t.get_device() != index:
+                raise ValueError(f"{what} must match q's type, device and head dimension; got "
+                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
     if k.shape != v.shape:
         raise ValueError(f"k is {tuple(k.shape)} and v {tuple(v.shape)}; one shape is needed")
     return dim, index

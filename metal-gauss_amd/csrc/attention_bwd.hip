@@ -589,8 +589,9 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_sum_kernel(AttnArgs a) {
 }
 
 // The sinks' sums: a workgroup has four columns in each half of a wave, of 32 sinks,
-// of dk or dv, and its waves every kSinkWaves-th place.
-constexpr int kSinkWaves = 16;
+// of dk or dv, and its waves every kSinkWaves-th place (16 waves: 14 us in place of 8
+// for 7033 packed tokens).
+constexpr int kSinkWaves = 4;
 template <typename T, int DK>
 __global__ __launch_bounds__(64 * kSinkWaves) void attn_sink_sum_kernel(AttnArgs a) {
     constexpr int kBlocks = DK / 32;
@@ -614,7 +615,7 @@ __global__ __launch_bounds__(64 * kSinkWaves) void attn_sink_sum_kernel(AttnArgs
     const int64_t step = (int64_t)a.k_heads * (2 * a.sink_rows * DK / 4);
     f32x4 sum = {};
     if (key < a.sinks) {
-#pragma unroll 4
+#pragma unroll 8
         for (int p = wave; p < places; p += kSinkWaves) sum += from[p * step];
     }
     s_sum[wave][lane] = sum;

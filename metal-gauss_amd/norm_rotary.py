@@ -18,15 +18,13 @@ def _args(x, weight):
     """What a C call takes of one tensor's heads."""
     if x is None:
         return (None, 0, 0, 0), None
-    return ((x.data_ptr(), x.stride(0), x.stride(1), x.shape[1]),
-            None if weight is None else weight.data_ptr())
+    tok, head, _ = x.stride()
+    return ((x.data_ptr(), tok, head, x.shape[1]), None if weight is None else weight.data_ptr())
 
 
-def _weight_code(weights, code):
-    for w in weights:
-        if w is not None:
-            return _lib.TYPE_CODES[w.dtype]
-    return code
+def _weight_code(q_weight, k_weight, code):
+    w = k_weight if q_weight is None else q_weight
+    return code if w is None else _lib.TYPE_CODES[w.dtype]
 
 
 def _position_args(positions, frequencies, table, layout):
@@ -36,14 +34,14 @@ def _position_args(positions, frequencies, table, layout):
 
 
 def _forward(q, k, q_weight, k_weight, positions, frequencies, eps, layout, table):
-    lib = _lib.load()
     q, k = _heads(q), None if k is None else _heads(k)
     code = _lib.TYPE_CODES[q.dtype]
+    tokens, _, dim = q.shape
     q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     k_out = None if k is None else torch.empty_like(k, memory_format=torch.contiguous_format)
     (q_at, qw), (k_at, kw) = _args(q, q_weight), _args(k, k_weight)
-    _lib.launch(lib.mg_norm_rotary_forward, q.get_device(), q.shape[0], code, *q_at, *k_at,
-                q.shape[2], _weight_code((q_weight, k_weight), code), qw, kw, eps,
+    _lib.launch(_lib.load().mg_norm_rotary_forward, q.get_device(), tokens, code, *q_at, *k_at,
+                dim, _weight_code(q_weight, k_weight, code), qw, kw, eps,
                 *_position_args(positions, frequencies, table, layout), q_out.data_ptr(),
                 None if k is None else k_out.data_ptr())
     return q_out, k_out
@@ -90,7 +88,7 @@ class _NormRotary(torch.autograd.Function):
                 size = lib.mg_norm_rotary_backward_workspace_bytes(heads[3], heads[7], dim)
                 ws = torch.empty(size, dtype=torch.uint8, device=dev)
             _lib.launch(lib.mg_norm_rotary_backward, q.get_device(), tokens, code, *heads, dim,
-                        _weight_code((q_weight, k_weight), code), *weight_at, ctx.eps,
+                        _weight_code(q_weight, k_weight, code), *weight_at, ctx.eps,
                         *_position_args(positions, frequencies, ctx.table, ctx.layout), *dy_at,
                         *(None if t is None else t.data_ptr() for t in (*dx, *dw)),
                         None if ws is None else ws.data_ptr(), size)
@@ -136,10 +134,11 @@ def norm_rotary(q: torch.Tensor, k: torch.Tensor | None, q_weight: torch.Tensor 
         if q_weight is not None and q_weight.dtype != k_weight.dtype:
             raise ValueError(f"q_weight is {q_weight.dtype} and k_weight {k_weight.dtype}; one "
                              "type is needed")
-    args = (q, k, q_weight, k_weight, positions, frequencies, float(eps), layout, table)
-    if (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4])) \
-            or _lib.forward_mode():
-        out = _NormRotary.apply(*args)
-    else:
-        out = _forward(*args)
+    run = _forward
+    if (torch.is_grad_enabled() and (
+            q.requires_grad or (k is not None and k.requires_grad) or
+            (q_weight is not None and q_weight.requires_grad) or
+            (k_weight is not None and k_weight.requires_grad))) or _lib.forward_mode():
+        run = _NormRotary.apply
+    out = run(q, k, q_weight, k_weight, positions, frequencies, float(eps), layout, table)
     return out if k is not None else out[0]
