@@ -61,38 +61,39 @@ class _NormRotary(torch.autograd.Function):
         # Hooks on saved tensors may give them back in another layout.
         q, k, q_weight, k_weight, positions, frequencies = ctx.saved_tensors
         positions, frequencies = positions.contiguous(), frequencies.contiguous()
-        lib = _lib.load()
-        dev, dtype, code = q.device, q.dtype, _lib.TYPE_CODES[q.dtype]
+        need_q, need_k, need_qw, need_kw = ctx.needs_input_grad[:4]
         tokens, _, dim = q.shape
-        need = ctx.needs_input_grad
-        make = torch.zeros if tokens == 0 else torch.empty
-        heads, weight_at, dy_at, dx, dw, kept = [], [], [], [], [], []
-        for x, w, dy, need_x, need_w in ((q, q_weight, dq_out, need[0], need[2]),
-                                         (k, k_weight, dk_out, need[1], need[3])):
-            if dy is None or not (need_x or need_w):
-                x = w = dy = None
-            else:
-                x, dy = _heads(x), _heads(dy if dy.dtype == dtype else dy.to(dtype))
-                w = None if w is None else w.contiguous()
-                kept.append((x, w, dy))            # copies live until the launch
-            at, weight = _args(x, w)
-            heads += at
-            weight_at.append(weight)
-            dy_at += (None, 0, 0) if dy is None else (dy.data_ptr(), dy.stride(0), dy.stride(1))
-            dx.append(None if x is None or not need_x
-                      else torch.empty(x.shape, dtype=dtype, device=dev))
-            dw.append(None if w is None or not need_w else make(dim, dtype=w.dtype, device=dev))
-        if tokens and kept:
-            ws, size = None, 0
-            if dw[0] is not None or dw[1] is not None:
-                size = lib.mg_norm_rotary_backward_workspace_bytes(heads[3], heads[7], dim)
-                ws = torch.empty(size, dtype=torch.uint8, device=dev)
-            _lib.launch(lib.mg_norm_rotary_backward, q.get_device(), tokens, code, *heads, dim,
-                        _weight_code(q_weight, k_weight, code), *weight_at, ctx.eps,
-                        *_position_args(positions, frequencies, ctx.table, ctx.layout), *dy_at,
-                        *(None if t is None else t.data_ptr() for t in (*dx, *dw)),
+        code = _lib.TYPE_CODES[q.dtype]
+        first = _gradients_of(q, q_weight, dq_out, need_q, need_qw)
+        second = _gradients_of(k, k_weight, dk_out, need_k, need_kw)
+        (_, q_at, qw, dy_q, dq, dqw), (_, k_at, kw, dy_k, dk, dkw) = first, second
+        if tokens and (first[0] or second[0]):
+            lib, ws, size = _lib.load(), None, 0
+            if dqw is not None or dkw is not None:
+                size = lib.mg_norm_rotary_backward_workspace_bytes(q_at[3], k_at[3], dim)
+                ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+            _lib.launch(lib.mg_norm_rotary_backward, q.get_device(), tokens, code, *q_at, *k_at,
+                        dim, _weight_code(q_weight, k_weight, code), qw, kw, ctx.eps,
+                        *_position_args(positions, frequencies, ctx.table, ctx.layout), *dy_q,
+                        *dy_k, *(None if t is None else t.data_ptr() for t in (dq, dk, dqw, dkw)),
                         None if ws is None else ws.data_ptr(), size)
-        return dx[0], dx[1], dw[0], dw[1], None, None, None, None, None
+        return dq, dk, dqw, dkw, None, None, None, None, None
+
+
+def _gradients_of(x, w, dy, need_x, need_w):
+    """One tensor's part of the backward call: what has to live until the launch, what
+    the call takes of its heads, weights and results' gradient, and its gradients."""
+    if dy is None or not (need_x or need_w):
+        return (), (None, 0, 0, 0), None, (None, 0, 0), None, None
+    x, dy = _heads(x), _heads(dy if dy.dtype == x.dtype else dy.to(x.dtype))
+    w = None if w is None else w.contiguous()
+    at, weight = _args(x, w)
+    tok, head, _ = dy.stride()
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
+    dw = None
+    if w is not None and need_w:
+        dw = torch.empty_like(w) if x.shape[0] else torch.zeros_like(w)
+    return (x, w, dy), at, weight, (dy.data_ptr(), tok, head), dx, dw
 
 
 def _check_weight(w, what, dim, index, dtype):
