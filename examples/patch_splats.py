@@ -11,7 +11,13 @@ against that view trains everything through FusedAdam.
 
 With ``causal=True`` a token sees the views before its own and the tokens before
 it, so that a new view can be added to a scene already seen: ``extend`` runs the
-new tokens alone over the keys and values kept of the old ones.
+new tokens alone over the keys and values kept of the old ones, and ``candidates``
+runs several views at once, each by itself, over the one memory that they share.
+
+For the frames of a camera path a network takes ``frames=True``: heads are normed
+and turned by frame, column and row; ``window`` and ``sinks``: a token sees the last
+tokens and the path's first ones alone; and ``drop``: the branches are dropped out
+as they are added to the residual.
 
     python examples/patch_splats.py [--steps 60] [--seed 0]
 
@@ -41,9 +47,11 @@ class Network:
     """Parameters (float32, as FusedAdam keeps them) and the forward pass; matrix
     products and attention run in bfloat16, norms and the residual in float32."""
 
-    def __init__(self, width=128, heads=4, kv_heads=2, blocks=2, seed=0, device="cuda"):
+    def __init__(self, width=128, heads=4, kv_heads=2, blocks=2, seed=0, device="cuda",
+                 frames=False, window=None, sinks=0, drop=0.0):
         g = torch.Generator().manual_seed(seed)
         self.heads, self.kv_heads, self.dim, self.blocks = heads, kv_heads, width // heads, blocks
+        self.window, self.sinks, self.drop = window, sinks, drop
 
         def matrix(rows, cols, gain=1.0):
             return torch.randn(rows, cols, generator=g) * (gain / math.sqrt(cols))
@@ -57,8 +65,16 @@ class Network:
                 p[f"{b}.join"] = matrix(width, width, 0.5)
                 p[f"{b}.up"] = matrix(4 * width, width)
                 p[f"{b}.down"] = matrix(width, 4 * width, 0.5)
+                if frames:
+                    p[f"{b}.q_norm"], p[f"{b}.k_norm"] = torch.ones(self.dim), torch.ones(self.dim)
         self.params = {k: v.to(device).requires_grad_(True) for k, v in p.items()}
-        self.frequencies = mg.rotary_frequencies(self.dim, base=100.0, axes=2, device=device)
+        self.sections = None
+        if frames:                   # a quarter of the pairs for the frame
+            pairs = self.dim // 2
+            self.sections = (pairs // 4, (pairs - pairs // 4) // 2,
+                             pairs - pairs // 4 - (pairs - pairs // 4) // 2)
+        self.frequencies = mg.rotary_frequencies(self.dim, base=100.0, axes=1 if frames else 2,
+                                                 device=device)
 
     def _product(self, x, name):
         return F.linear(x.bfloat16(), self.params[name].bfloat16())
@@ -66,16 +82,30 @@ class Network:
     def _norm(self, x, name):
         return mg.layer_norm(x, self.params[name + ".w"], self.params[name + ".b"])
 
-    def __call__(self, tokens, positions, q_offsets, k_offsets=None, causal=False, memory=None):
-        """tokens (n, patch and ray), positions (n, 2) -> (n, PER_TOKEN, 14).
+    def _turned(self, q, k, positions, block):
+        if self.sections is None:
+            return mg.rotary(q, k, positions, self.frequencies)
+        return mg.norm_rotary(q, k, self.params[f"{block}.q_norm"], self.params[f"{block}.k_norm"],
+                              positions, self.frequencies, sections=self.sections)
+
+    def _add(self, x, branch, seed, site):
+        if seed is None or self.drop == 0.0:
+            return x + branch.float()
+        return mg.dropout(branch, self.drop, seed, residual=x, site=site)
+
+    def __call__(self, tokens, positions, q_offsets, k_offsets=None, causal=False, memory=None,
+                 shared=None, seed=None):
+        """tokens (n, patch and ray), positions (n, 2; of frames 3) -> (n, PER_TOKEN, 14).
 
         ``memory``: per block (keys, values) of the tokens seen before; the new
-        ones' are joined to them, and k_offsets bounds the result."""
+        ones' are joined to them, and k_offsets bounds the result. ``shared``: the
+        same, which all sequences see beside their own. ``seed`` of the step's
+        dropout; None (serving): none."""
         H, Hk, D = self.heads, self.kv_heads, self.dim
         x = self._product(tokens, "embed").float()
         for b in range(self.blocks):
             qkv = self._product(self._norm(x, f"{b}.norm_a"), f"{b}.qkv").view(-1, H + 2 * Hk, D)
-            q, k = mg.rotary(qkv[:, :H], qkv[:, H:H + Hk], positions, self.frequencies)
+            q, k = self._turned(qkv[:, :H], qkv[:, H:H + Hk], positions, b)
             v = qkv[:, H + Hk:]
             if memory is not None:
                 if b < len(memory):
@@ -83,10 +113,14 @@ class Network:
                     memory[b] = (k, v)
                 else:
                     memory.append((k, v))
-            o = mg.attention(q, k, v, q_offsets, k_offsets, causal=causal)
-            x = x + self._product(o.reshape(-1, H * D), f"{b}.join").float()
+            if shared is not None:
+                o = mg.shared_attention(q, k, v, *shared[b], q_offsets, causal=causal)
+            else:
+                o = mg.attention(q, k, v, q_offsets, k_offsets, causal=causal,
+                                 window=self.window, sinks=self.sinks)
+            x = self._add(x, self._product(o.reshape(-1, H * D), f"{b}.join"), seed, 2 * b)
             up = F.gelu(self._product(self._norm(x, f"{b}.norm_b"), f"{b}.up"))
-            x = x + self._product(up, f"{b}.down").float()
+            x = self._add(x, self._product(up, f"{b}.down"), seed, 2 * b + 1)
         out = self._product(self._norm(x, f"{self.blocks}.norm_a"), "out").float()
         return out.view(-1, PER_TOKEN, 14)
 
@@ -165,6 +199,24 @@ def extend(net, scene_tokens, positions, old, device="cuda"):
             memory=memory)
         return net(scene_tokens[old:], positions[old:], offsets_of([n - old], device),
                    offsets_of([n], device), causal=True, memory=memory)
+
+
+def candidates(net, scene_tokens, positions, views, device="cuda"):
+    """The predictions of several views, (tokens, positions) each, of one scene: each
+    view over the scene's memory, read once for all, and none seeing another."""
+    memory, n = [], scene_tokens.shape[0]
+    with torch.no_grad():
+        net(scene_tokens, positions, offsets_of([n], device), causal=True, memory=memory)
+        tokens, at = (torch.cat(t) for t in zip(*views))
+        lengths = [t.shape[0] for t, _ in views]
+        out = net(tokens, at, offsets_of(lengths, device), causal=True, shared=memory)
+    return out.split(lengths)
+
+
+def with_frames(positions, length):
+    """(frame, column, row) of the tokens of frames of `length` tokens each."""
+    frame = torch.arange(positions.shape[0], device=positions.device) // length
+    return torch.cat([frame[:, None].to(positions), positions], 1)
 
 
 def train(steps=60, size=64, views=(2, 4, 3), seed=0, lr=2e-3, device="cuda", log=print):
