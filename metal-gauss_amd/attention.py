@@ -8,6 +8,8 @@ that predicts or refines splats, next to ``layer_norm`` and ``rotary``.
 
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import _lib
@@ -190,10 +192,11 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     if window is not None:
         if not causal:
             raise ValueError("window needs causal=True")
+        window, sinks = operator.index(window), operator.index(sinks)
         if window < 1 or sinks < 0:
             raise ValueError(f"window must be at least 1 and sinks 0, got {window} and {sinks}")
         # More than any tensor has is all of them.
-        window = (min(int(window), 2 ** 31 - 1), min(int(sinks), 2 ** 31 - 1))
+        window = (min(window, 2 ** 31 - 1), min(sinks, 2 ** 31 - 1))
     elif sinks:
         raise ValueError("sinks needs window: without one all first keys are seen")
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)) \

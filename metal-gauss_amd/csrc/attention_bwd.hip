@@ -641,7 +641,9 @@ struct BwdPlan {
 constexpr int64_t kBwdRuns = 1024, kBwdRunLeast = 8, kBwdMostSplits = 8;
 // With a window: as many as fill the GPU, as partial results weigh more beside fewer
 // queries (7033 packed tokens, window 475: 118 and 28 us to add them in four runs, 115 and
-// 18 in two). Far items: two rounds of half the GPU's.
+// 18 in two). As many far items, or pieces of sink_steps = kSinkStepsLeast (in 128 of 8 at
+// least that pass's keys took 171 us for 143): their number bounds the room for their
+// sums.
 constexpr int64_t kBwdWindowRuns = 512, kSinkItems = 512, kSinkStepsLeast = 4;
 
 static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int64_t group,
@@ -665,11 +667,12 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     const int64_t dk = dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 96 ? 96 : 128;
     if (p.splits > 1) p.bytes += p.k_items * k_heads * p.splits * 2 * kBwdTile * dk * 4;
     p.sink_at = p.bytes;
+    p.sink_steps = 1;
     if (sinks > 0) {
         const int64_t key_tiles = ceil_div(sinks, kBwdTile);
         int64_t most = ceil_div(q_tokens, kTileRows) * group * k_heads * key_tiles / kSinkItems;
         most = most < kSinkStepsLeast ? kSinkStepsLeast : most;
-        p.sink_steps = (int)(most < 64 ? most : 64);
+        p.sink_steps = (int)most;
         p.sink_rows = (int)(sinks < kBwdTile ? ceil_div(sinks, 32) * 32 : kBwdTile);
         // Sum over the sequences of SinkItems::all: of key_tiles * (pieces * group +
         // splits), pieces being at most tokens / (64 sink_steps) + 1 each.

@@ -6,6 +6,8 @@ that predicts or refines splats, next to ``layer_norm`` and ``attention``.
 
 from __future__ import annotations
 
+import operator
+
 import torch
 
 from . import _lib
@@ -78,8 +80,11 @@ def dropout(x: torch.Tensor, p: float, seed: int | torch.Tensor, *,
             raise ValueError(f"seed must be one int64, got {seed.dtype} {tuple(seed.shape)}")
         if not seed.is_cuda or seed.get_device() != index:
             raise RuntimeError(f"seed must be on {x.device}, got device '{seed.device}'")
-    elif not 0 <= seed < 2 ** 64:
-        raise ValueError(f"seed must be an integer from 0 to 2^64 - 1, got {seed}")
+    else:
+        seed = operator.index(seed)
+        if not 0 <= seed < 2 ** 64:
+            raise ValueError(f"seed must be an integer from 0 to 2^64 - 1, got {seed}")
+    site = operator.index(site)
     if not 0 <= site < 2 ** 64:
         raise ValueError(f"site must be an integer from 0 to 2^64 - 1, got {site}")
     # Of 65536 draws: all of them for p = 1 alone.
