@@ -134,13 +134,23 @@ static int part_waves(int64_t rows, int64_t groups, int64_t sequences) {
     return rows <= 64 * groups && rows <= 64 * sequences ? kNarrowWaves : kWideWaves;
 }
 
+// Items of a set whose keys are not cut.
+static int64_t part_whole(int64_t rows, int64_t n_seq, int64_t k_heads, int waves) {
+    return (ceil_div(rows, 32 * waves) + n_seq - 1) * k_heads;
+}
+
+// `beside`: the other set's items, which run beside these from the start. Those of the
+// shared memories leave them up to half of the slots (128 streams over 16320 tokens
+// and their own: 54 us and 9 to join with all slots taken by the first, 50 and 6 so).
 static PartPlan part_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int64_t group,
-                          int dim, int64_t n_seq, int waves) {
+                          int dim, int64_t n_seq, int waves, int64_t beside) {
     PartPlan p{};
     const int64_t rows = q_tokens * group;
     p.waves = waves;
-    const int64_t tile_rows = 32 * p.waves, slots = part_slots(waves);
-    const int64_t likely = (ceil_div(rows, tile_rows) + n_seq - 1) * k_heads;
+    const int64_t tile_rows = 32 * p.waves;
+    int64_t slots = part_slots(waves);
+    slots -= beside < slots / 2 ? beside : slots / 2;
+    const int64_t likely = part_whole(rows, n_seq, k_heads, waves);
     const int64_t mean_keys = k_tokens / n_seq;
     // As many chunks as make items for all slots, of `least` keys at least; and where
     // chunks stay long, as make several rounds of items, which even out.
@@ -161,6 +171,19 @@ static PartPlan part_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, i
     return p;
 }
 
+struct PartPlans {
+    PartPlan of[2];             // over the shared memories, and alone
+};
+static PartPlans part_plans(int64_t q_tokens, int64_t k_tokens, int64_t shared_tokens,
+                            int64_t k_heads, int64_t group, int dim, int64_t sequences,
+                            int64_t groups) {
+    const int64_t rows = q_tokens * group;
+    const int waves = part_waves(rows, groups, sequences);
+    return {{part_plan(q_tokens, shared_tokens, k_heads, group, dim, groups, waves,
+                       part_whole(rows, sequences, k_heads, waves)),
+             part_plan(q_tokens, k_tokens, k_heads, group, dim, sequences, waves, 0)}};
+}
+
 }  // namespace mg
 
 extern "C" {
@@ -173,9 +196,9 @@ int64_t mg_shared_attention_workspace_bytes(int64_t q_tokens, int64_t k_tokens,
         sequences < 1 || groups < 1)
         return 0;
     const int group = q_heads / k_heads;
-    const int waves = mg::part_waves(q_tokens * group, groups, sequences);
-    return mg::part_plan(q_tokens, shared_tokens, k_heads, group, dim, groups, waves).bytes +
-           mg::part_plan(q_tokens, k_tokens, k_heads, group, dim, sequences, waves).bytes;
+    const mg::PartPlans p = mg::part_plans(q_tokens, k_tokens, shared_tokens, k_heads, group, dim,
+                                           sequences, groups);
+    return p.of[0].bytes + p.of[1].bytes;
 }
 
 int32_t mg_shared_attention(
@@ -225,10 +248,10 @@ int32_t mg_shared_attention(
     MG_REQUIRE(q && out && (k_tokens == 0 || (k && v)) &&
                    (shared_tokens == 0 || (shared_k && shared_v)),
                "%s: a pointer is NULL", who);
-    const int waves = part_waves(q_tokens * group, groups, sequences);
-    const PartPlan plans[2] = {
-        part_plan(q_tokens, shared_tokens, k_heads, group, dim, groups, waves),
-        part_plan(q_tokens, k_tokens, k_heads, group, dim, sequences, waves)};
+    const PartPlans all =
+        part_plans(q_tokens, k_tokens, shared_tokens, k_heads, group, dim, sequences, groups);
+    const PartPlan(&plans)[2] = all.of;
+    const int waves = plans[0].waves;
     const int64_t items = (plans[0].items + plans[1].items) * k_heads;
     MG_REQUIRE(grid_fits(items, 64 * waves) && items < INT32_MAX && k_heads < 65536,
                "%s: too many work items", who);
