@@ -117,13 +117,16 @@ __device__ __forceinline__ int wave_inclusive_max(int v) {       // v >= 0
 // carried on. Offsets are held to [0, tokens] and made to rise (an offset below
 // one before it counts as that one), so that no value of theirs leads out of the
 // tensors and every token is in one pseudo sequence. For all lanes of a wave.
-__device__ __forceinline__ int seq_offset(const int32_t *off, int n, int tokens, int s0) {
+__device__ __forceinline__ void seq_bounds(const int32_t *off, int n, int tokens, int s0, int &end,
+                                           int &lo, int &len) {
     const int s = s0 + lane_id();
-    if (!off) return s == 0 ? 0 : tokens;
-    return s <= n ? off[s] : tokens;
-}
-__device__ __forceinline__ void seq_bounds(int offset, int tokens, int &end, int &lo, int &len) {
-    const int to = max(end, wave_inclusive_max(clamp_to(offset, 0, tokens)));
+    int to = tokens;
+    if (off) {
+        if (s <= n) to = clamp_to(off[s], 0, tokens);
+    } else if (s == 0) {
+        to = 0;
+    }
+    to = max(end, wave_inclusive_max(to));
     lo = __builtin_amdgcn_update_dpp(end, to, 0x138, 0xf, 0xf, false);   // wave_shr:1
     len = to - lo;
     end = __builtin_amdgcn_readlane(to, 63);
@@ -138,18 +141,11 @@ __device__ __forceinline__ SeqItem find_item(const AttnArgs &a, int item, Count 
                                              Second second) {
     SeqItem r{};
     int base = 0, base2 = 0, q_end = 0, k_end = 0;
-    const auto q_at = [&](int s0) { return seq_offset(a.q_off, a.n_seq, a.q_tokens, s0); };
-    const auto k_at = [&](int s0) { return seq_offset(a.k_off, a.n_seq, a.k_tokens, s0); };
-    // Offsets are asked for three steps ahead (128 streams over their own keys: 22 us a
-    // launch without, each step waiting for its own).
-    int q0 = q_at(0), k0 = k_at(0), q1 = q_at(64), k1 = k_at(64), q2 = q_at(128), k2 = k_at(128);
     for (int s0 = 0; s0 < a.n_seq + 2; s0 += 64) {
         const int s = s0 + lane_id();
         int q_lo, q_len, k_lo, k_len;
-        seq_bounds(q0, a.q_tokens, q_end, q_lo, q_len);
-        seq_bounds(k0, a.k_tokens, k_end, k_lo, k_len);
-        q0 = q1, q1 = q2, k0 = k1, k1 = k2;
-        q2 = q_at(s0 + 192), k2 = k_at(s0 + 192);
+        seq_bounds(a.q_off, a.n_seq, a.q_tokens, s0, q_end, q_lo, q_len);
+        seq_bounds(a.k_off, a.n_seq, a.k_tokens, s0, k_end, k_lo, k_len);
         if (s == 0 || s > a.n_seq) (kByKeys ? q_len : k_len) = 0;
         const int n = count(q_len, k_len), n2 = second(q_len, k_len);
         const int upto = wave_inclusive_sum(n), upto2 = wave_inclusive_sum(n2);
@@ -252,8 +248,8 @@ __device__ __forceinline__ SeqItem find_longest(const AttnArgs &a, int item, int
     }
     const int seq = lane_id();
     int q_end = 0, k_end = 0, q_lo, q_len, k_lo, k_len;
-    seq_bounds(seq_offset(a.q_off, a.n_seq, a.q_tokens, 0), a.q_tokens, q_end, q_lo, q_len);
-    seq_bounds(seq_offset(a.k_off, a.n_seq, a.k_tokens, 0), a.k_tokens, k_end, k_lo, k_len);
+    seq_bounds(a.q_off, a.n_seq, a.q_tokens, 0, q_end, q_lo, q_len);
+    seq_bounds(a.k_off, a.n_seq, a.k_tokens, 0, k_end, k_lo, k_len);
     if (seq == 0 || seq > a.n_seq) (kByKeys ? q_len : k_len) = 0;
     const int tiles = tiles_of(q_len, k_len);
     const auto with = [&](int w) {                // this lane's sequence's
@@ -417,6 +413,57 @@ struct TileLane {
                              (lds_s16x4 *)(tile + column_operand_byte<DK>(column, r, block))));
         };
         return __builtin_shufflevector(read(row0), read(row0 + 8), 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
+
+// ------------------------------------------------------------------- results
+// A wave's 32 rows of results, by way of LDS: a lane of a product has four columns
+// of its row at a time, and stores of those would be 16 bytes a row; from LDS each
+// row goes out whole. (Stored by fours: 16384 tokens of 16 heads of 128 with a window
+// of one key, result and what rounding took from it, 120 us.) Of the tiles'
+// memory, which every wave has done with.
+template <int DK>
+constexpr int kRowPitch = DK * 2 + 16;           // bytes, rows spread over the banks
+template <int DK>
+constexpr int kRowBytes = 32 * kRowPitch<DK>;    // a wave's
+
+template <typename T, int DK>
+struct RowStore {
+    char *lds;                                   // the wave's
+
+    // value(b, e): element e of block b of this lane's row, in T. The row goes to
+    // out + at_row (as lane l % 32 has it) where row_ok.
+    template <typename F>
+    __device__ __forceinline__ void operator()(T *out, int64_t at_row, bool row_ok, int dim,
+                                               F value) const {
+        const int lane = lane_id(), half = lane / 32;
+#pragma unroll
+        for (int b = 0; b < DK / 32; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                vec4<T> w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = value(b, e + i);
+                *reinterpret_cast<vec4<T> *>(lds + lane % 32 * kRowPitch<DK> +
+                                             (32 * b + c_row(e, half)) * 2) = w;
+            }
+        lds_reads_done();
+        constexpr int kLanes = DK <= 32 ? 4 : DK <= 64 ? 8 : 16, kRows = 64 / kLanes;
+        const int chunk = lane % kLanes;
+        const uint64_t to = row_ok ? (uint64_t)(out + at_row) : 0;
+#pragma unroll
+        for (int r = 0; r < 32; r += kRows) {
+            const int row = r + lane / kLanes;
+            // The address that the row's own lane has.
+            const uint32_t lo = __shfl((uint32_t)to, row, 64);
+            const uint32_t hi = __shfl((uint32_t)(to >> 32), row, 64);
+            const uint64_t at = (uint64_t)hi << 32 | lo;
+            const i32x4 w =
+                *reinterpret_cast<const i32x4 *>(lds + row * kRowPitch<DK> + chunk * 16);
+            if (at && chunk * 8 < dim)
+                *(__attribute__((address_space(1))) i32x4 *)(at + chunk * 16) = w;
+        }
+        lds_reads_done();
     }
 };
 

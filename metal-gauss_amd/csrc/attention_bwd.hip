@@ -114,8 +114,11 @@ __device__ __forceinline__ float ds_power(float do_sq, float v_sq) {
 }
 
 // ------------------------------------------------------- the queries' gradient
+// Without a window four waves a SIMD for 64 columns; with one that many keep too few
+// registers (window 777, 64 columns: 60 us, 98).
 template <typename T, int DK, bool kWin>
-__global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kBwdWaves, !kWin && DK == 64 ? 4 : 2) void attn_dq_kernel(
+    AttnArgs a) {
     constexpr int kSteps = DK / 16, kBlocks = DK / 32;
     __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK>];
     const int lane = lane_id(), half = lane / 32;
@@ -238,20 +241,12 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) 
         }
     }
     lds_reads_done();
-    if (!row_ok) return;
+    static_assert(kBwdWaves * kRowBytes<DK> <= (int)sizeof(s_tile), "rows in the tiles' memory");
+    tiles_ready();
+    const RowStore<T, DK> store{&s_tile[0][0][0] + wave * kRowBytes<DK>};
     const float down = a.scale * __builtin_amdgcn_exp2f(-power);
-    T *out = static_cast<T *>(a.dq) +
-             ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int at = 32 * b + c_row(e, half);
-            vec4<T> w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = (T)(dq[b][e + i] * down);
-            if (at < a.dim) *reinterpret_cast<vec4<T> *>(out + at) = w;
-        }
+    store(static_cast<T *>(a.dq), ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim,
+          row_ok, a.dim, [&](int b, int e) { return (T)(dq[b][e] * down); });
 }
 
 // ------------------------------------------- the keys' and values' gradients
@@ -499,7 +494,8 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     lds_reads_done();
     const float down = a.scale * __builtin_amdgcn_exp2f(-power);
     const float down_v = __builtin_amdgcn_exp2f(-kPowerP<T>);
-    if (kWin && sink_runs > 0 && key < a.sinks) {
+    const bool sinks_apart = kWin && sink_runs > 0 && key < a.sinks;
+    if (sinks_apart) {
         f32x4 *part = sink_part_of<DK>(a, sink_place, kh) + wave * kBlocks * 4 * 64 + lane;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
@@ -514,10 +510,10 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
                 part[(b * 4 + e / 4) * 64] = w;
                 part[(b * 4 + e / 4) * 64 + a.sink_rows * DK / 4] = x;
             }
-        return;
     }
     if (kWin && far) return;
     if (steps_of.runs > 1) {
+        if (sinks_apart) return;
         f32x4 *part = part_of<DK>(a, item, kh, split) + wave * kBlocks * 4 * 64 + lane;
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b)
@@ -534,25 +530,15 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
             }
         return;
     }
-    if (!key_ok) return;
+    static_assert(kBwdWaves * kRowBytes<DK> <= (int)sizeof(s_tile), "rows in the tiles' memory");
+    tiles_ready();
+    const RowStore<T, DK> store{&s_tile[0][0][0] + wave * kRowBytes<DK>};
     const int64_t at_row = ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim;
-    T *dkr = static_cast<T *>(a.dk) + at_row, *dvr = static_cast<T *>(a.dv) + at_row;
-#pragma unroll
-    for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int at = 32 * b + c_row(e, half);
-            vec4<T> w, x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                w[i] = (T)(dk[b][e + i] * down);
-                x[i] = (T)(dv[b][e + i] * down_v);
-            }
-            if (at < a.dim) {
-                *reinterpret_cast<vec4<T> *>(dkr + at) = w;
-                *reinterpret_cast<vec4<T> *>(dvr + at) = x;
-            }
-        }
+    const bool here = key_ok && !sinks_apart;
+    store(static_cast<T *>(a.dk), at_row, here, a.dim,
+          [&](int b, int e) { return (T)(dk[b][e] * down); });
+    store(static_cast<T *>(a.dv), at_row, here, a.dim,
+          [&](int b, int e) { return (T)(dv[b][e] * down_v); });
 }
 
 // The sums of the keys' tiles that were cut into runs, in order. A workgroup has

@@ -460,7 +460,22 @@ __device__ __forceinline__ bool attn_fwd_item(const AttnArgs &a, int work, SeqIt
         if (half == 0) a.part_stats[slot] = make_float2(top, sum);
         return true;
     }
-    if (row_ok) store_row_result<T, DK>(a, s.q_lo + token, head, half, 0, top, sum, o);
+    static_assert(kWaves * kRowBytes<DK> <= (int)sizeof(s_tile), "rows in the tiles' memory");
+    tiles_ready();
+    const RowStore<T, DK> store{&s_tile[0][0][0] + wave * kRowBytes<DK>};
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int at_token = s.q_lo + token;
+    const int64_t at_row = ((int64_t)at_token * (a.k_heads * G) + head) * a.dim;
+    store(static_cast<T *>(a.out), at_row, row_ok, a.dim,
+          [&](int b, int e) { return (T)(o[b][e] * inv); });
+    if (a.out_rest)
+        store(static_cast<T *>(a.out_rest), at_row, row_ok, a.dim, [&](int b, int e) {
+            const float f = o[b][e] * inv;
+            return (T)(f - (float)(T)f);
+        });
+    if (a.lse && half == 0 && row_ok)
+        a.lse[(int64_t)head * a.q_tokens + at_token] =
+            sum == 0.f ? INFINITY : top + __builtin_amdgcn_logf(sum);
     return true;
 }
 
