@@ -530,15 +530,25 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
             }
         return;
     }
-    static_assert(kBwdWaves * kRowBytes<DK> <= (int)sizeof(s_tile), "rows in the tiles' memory");
-    tiles_ready();
-    const RowStore<T, DK> store{&s_tile[0][0][0] + wave * kRowBytes<DK>};
+    if (!key_ok || sinks_apart) return;
     const int64_t at_row = ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim;
-    const bool here = key_ok && !sinks_apart;
-    store(static_cast<T *>(a.dk), at_row, here, a.dim,
-          [&](int b, int e) { return (T)(dk[b][e] * down); });
-    store(static_cast<T *>(a.dv), at_row, here, a.dim,
-          [&](int b, int e) { return (T)(dv[b][e] * down_v); });
+    T *dkr = static_cast<T *>(a.dk) + at_row, *dvr = static_cast<T *>(a.dv) + at_row;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int at = 32 * b + c_row(e, half);
+            vec4<T> w, x;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                w[i] = (T)(dk[b][e + i] * down);
+                x[i] = (T)(dv[b][e + i] * down_v);
+            }
+            if (at < a.dim) {
+                *reinterpret_cast<vec4<T> *>(dkr + at) = w;
+                *reinterpret_cast<vec4<T> *>(dvr + at) = x;
+            }
+        }
 }
 
 // The sums of the keys' tiles that were cut into runs, in order. A workgroup has
