@@ -16,9 +16,9 @@
 // in a launch of narrow items: 128 streams of 16 heads on 4 of 128, 30 and 22 us).
 // Partial results lie by rows, so that joining finds a row's without a search.
 //
-// Those streams over 16320 tokens and up to 500 of their own: 47 us and 6 to join (100 MB
-// at 1.9 TB/s, 17 GFLOP: the items' starts weigh); eight streams over 2375: 9 and 6;
-// 1957 tokens of frames over 10000 and 2500, 12 heads of 64: 80 and 10.
+// Those streams over 16320 tokens and up to 500 of their own: 49 us and 6 to join (100 MB
+// at 1.9 TB/s, 17 GFLOP: the items' starts weigh); eight streams over 2375: 10 and 7;
+// 1957 tokens of frames over 10000 and 2500, 12 heads of 64: 85 and 10.
 #include "attention_fwd.h"
 
 namespace mg {
