@@ -468,17 +468,18 @@ __global__ __launch_bounds__(kHeadThreads) void norm_rotary_bwd_kernel(HeadArgs 
                 }
             }
             const float s = rsqrtf(group_sum(ss, p.lanes) * per + p.eps);
-            const float along = group_sum(hx, p.lanes) * per * s * s * s;    // s^2 mean(h u)
+            // By u, never by powers of s, which pass float32's range before dx does.
+            const float along = group_sum(hx, p.lanes) * per * s;            // mean(h u)
             if (r >= n) continue;
 #pragma unroll
             for (int c = 0; c < C; ++c) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float a = h[c].p[i], b = h[c].q[i];
-                    dw[c].p[i] = fmaf(g[c].p[i] * a, s, dw[c].p[i]);
-                    dw[c].q[i] = fmaf(g[c].q[i] * b, s, dw[c].q[i]);
-                    h[c].p[i] = g[c].p[i] * w[c].p[i] * s - a * along;
-                    h[c].q[i] = g[c].q[i] * w[c].q[i] * s - b * along;
+                    const float a = h[c].p[i] * s, b = h[c].q[i] * s;
+                    dw[c].p[i] = fmaf(g[c].p[i], a, dw[c].p[i]);
+                    dw[c].q[i] = fmaf(g[c].q[i], b, dw[c].q[i]);
+                    h[c].p[i] = (g[c].p[i] * w[c].p[i] - a * along) * s;
+                    h[c].q[i] = (g[c].q[i] * w[c].q[i] - b * along) * s;
                 }
                 if (t.out) store_unit<T, V, kHalf>(out + r * p.dim, unit[c], h[c], p.stream);
             }

@@ -135,6 +135,13 @@ def test_norm_rotary_small_and_large_heads(dev, gain):
     check_norm_rotary(dev, "f32", "f32", 6, 2, 2, 64, 64, (32,), "runs", "half", gain=gain)
 
 
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("gain,eps", [(1e14, 1e-6), (1e-14, 0.0)])
+def test_norm_rotary_heads_whose_cubes_pass_the_range(dev, ty, gain, eps):
+    """1 / rms cubed is not in float32's range; the gradients are."""
+    check_norm_rotary(dev, ty, "f32", 6, 2, 2, 64, 64, (32,), "runs", "half", gain=gain, eps=eps)
+
+
 def test_norm_rotary_without_weights(dev):
     check_norm_rotary(dev, "bf16", "f32", 6, 2, 2, 64, 32, (16,), "runs", "interleaved",
                       weights=False)
