@@ -101,6 +101,8 @@ class Network:
         ones' are joined to them, and k_offsets bounds the result. ``shared``: the
         same, which all sequences see beside their own. ``seed`` of the step's
         dropout; None (serving): none."""
+        if shared is not None and self.window is not None:
+            raise ValueError("a shared memory is seen whole: the network's window does not apply")
         H, Hk, D = self.heads, self.kv_heads, self.dim
         x = self._product(tokens, "embed").float()
         for b in range(self.blocks):

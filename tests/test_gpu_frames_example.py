@@ -148,6 +148,13 @@ def test_views_over_a_shared_memory(dev, example):
         assert float((view - alone).abs().max()) < 0.1
 
 
+def test_views_of_a_network_with_a_window_are_refused(dev, example):
+    net = example.Network(seed=3, frames=True, window=20)
+    tokens, positions, _ = path(example, 4, 6)
+    with pytest.raises(ValueError, match="seen whole"):
+        example.candidates(net, tokens[:32], positions[:32], [(tokens[32:], positions[32:])])
+
+
 def test_a_window_over_the_memory(dev, example):
     """New tokens over kept keys and values see what they see in the whole path."""
     net = example.Network(seed=4, frames=True, window=20, sinks=4)
