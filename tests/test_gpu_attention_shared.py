@@ -197,6 +197,18 @@ def test_shared_strided_views(dev):
     assert torch.equal(shared_attention(q, k, v, odd[:, 0], odd[:, 1], causal=True), want)
 
 
+def test_shared_rows_whose_offsets_pass_32_bits(dev):
+    """A memory of 600 keys and values 2^23 elements apart."""
+    from metal_gauss_amd import shared_attention
+
+    g = gen("far rows")
+    far = torch.empty(600, 1 << 23, device=dev, dtype=torch.bfloat16)[:, :256].view(600, 4, 64)
+    far.copy_(torch.randn(600, 4, 64, generator=g))
+    q, k, v = (torch.randn(9, h, 64, generator=g).to(dev, torch.bfloat16) for h in (4, 2, 2))
+    want = shared_attention(q, k, v, far[:, :2].contiguous(), far[:, 2:].contiguous(), causal=True)
+    assert torch.equal(shared_attention(q, k, v, far[:, :2], far[:, 2:], causal=True), want)
+
+
 def test_shared_in_a_graph_and_on_another_stream(dev):
     """Two graphs, replayed in turn with eager work between."""
     from metal_gauss_amd import shared_attention

@@ -244,6 +244,25 @@ def test_window_strided_views(dev):
     assert torch.equal(attention(odd[:, :4], odd[:, 4:6], odd[:, 6:], **kw), want)
 
 
+def test_window_over_rows_whose_offsets_pass_32_bits(dev):
+    """Keys and values 2^23 elements apart, in a memory of 600 of them."""
+    from metal_gauss_amd import attention
+
+    g = gen("far rows")
+    far = torch.empty(600, 1 << 23, device=dev, dtype=torch.bfloat16)[:, :256].view(600, 4, 64)
+    far.copy_(torch.randn(600, 4, 64, generator=g))
+    q = torch.randn(600, 4, 64, generator=g).to(dev, torch.bfloat16)
+    dy = torch.randn(600, 4, 64, generator=g).to(dev, torch.bfloat16)
+    results = []
+    for k, v in ((far[:, :2], far[:, 2:]), (far[:, :2].contiguous(), far[:, 2:].contiguous())):
+        leaves = [t.detach().requires_grad_(True) for t in (q, k, v)]
+        y = attention(*leaves, causal=True, window=130, sinks=5)
+        results.append((y, *torch.autograd.grad(y, leaves, dy)))
+        with torch.no_grad():
+            results[-1] += (attention(q[-1:], k, v, causal=True, window=130, sinks=5),)
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 @pytest.mark.parametrize("grad", [False, True])
 def test_window_in_a_graph_and_on_another_stream(dev, grad):
     from metal_gauss_amd import attention

@@ -202,6 +202,24 @@ def test_norm_rotary_slices_and_strides(dev):
                        norm_rotary(one.contiguous(), None, w, None, pos, freq))
 
 
+def test_norm_rotary_rows_whose_offsets_pass_32_bits(dev):
+    from metal_gauss_amd import norm_rotary, rotary_frequencies
+
+    g = gen("far rows")
+    far = torch.empty(600, 1 << 23, device=dev, dtype=torch.bfloat16)[:, :256].view(600, 4, 64)
+    far.copy_(torch.randn(600, 4, 64, generator=g))
+    far_dy = torch.empty(600, 1 << 23, device=dev, dtype=torch.bfloat16)[:, :128].view(600, 2, 64)
+    far_dy.copy_(torch.randn(600, 2, 64, generator=g))
+    w = torch.rand(64, generator=g).to(dev)
+    pos, freq = torch.arange(600, device=dev), rotary_frequencies(64, device=dev)
+    results = []
+    for x, dy in ((far, far_dy), (far.contiguous(), far_dy.contiguous())):
+        leaves = [t.detach().requires_grad_(True) for t in (x[:, :2], x[:, 2:], w)]
+        y = norm_rotary(leaves[0], leaves[1], leaves[2], leaves[2], pos, freq)
+        results.append((*y, *torch.autograd.grad(y, leaves, (dy, dy))))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
 def test_norm_rotary_gradients_of_some(dev):
     """Of one result, of the weights alone, of the inputs alone."""
     from metal_gauss_amd import norm_rotary, rotary_frequencies
@@ -408,6 +426,17 @@ def test_dropout_many_elements(dev):
     y = dropout(torch.ones(n, device=dev, dtype=torch.bfloat16), 0.5, 77)
     for first in (0, 2 ** 26 + 3, n - 40):
         want = token_ref.kept(40, 32768, 77, first=first)
+        assert np.array_equal((y[first:first + 40] != 0).cpu().numpy(), want)
+
+
+def test_dropout_past_32_bits(dev):
+    """Element numbers of 2^32 and more."""
+    from metal_gauss_amd import dropout
+
+    n = 2 ** 32 + 997
+    y = dropout(torch.ones(1, device=dev, dtype=torch.bfloat16).expand(n), 0.5, 11, site=2)
+    for first in (2 ** 31 - 20, 2 ** 32 - 20, n - 40):
+        want = token_ref.kept(40, 32768, 11, site=2, first=first)
         assert np.array_equal((y[first:first + 40] != 0).cpu().numpy(), want)
 
 
