@@ -67,7 +67,7 @@ struct AttnArgs {
     float *part;
     // With sinks: the first keys' gradients from queries further on than the
     // window, in runs of sink_steps query tiles of one head (attention_bwd.hip).
-    int32_t sink_items, sink_steps, sink_rows;
+    int32_t key_runs, sink_steps, sink_rows;
     float *sink_part;
 };
 

@@ -276,12 +276,13 @@ __device__ __forceinline__ f32x4 *part_of(const AttnArgs &a, int item, int kh, i
 }
 
 // With a window, the queries that see a key tile are few, but those further on all
-// see the sinks. Their sums for the sinks are work items of their own, which go
-// first: one tile of kBwdTile keys, one head and sink_steps query tiles each. Their
+// see the sinks. Their sums for the sinks are work items of their own, which come
+// last, being short ones (first: 147 us in place of 126 for 7033 packed tokens, window
+// 475): one tile of kBwdTile keys, one head and sink_steps query tiles each. Their
 // sums, of sink_rows keys, have a place each in sink_part, and so have those of the
 // window items of key tiles that have sinks; attn_sink_sum_kernel adds them up, in
 // order. A sequence's places follow one another, a key tile's far items' and then
-// its window items'; item i of the far ones has place i.
+// its window items'.
 struct SinkItems {
     int key_tiles, from, tiles, pieces;    // from: the first query past the window
 
@@ -296,6 +297,7 @@ struct SinkItems {
     // Places of a key tile, and of a sequence.
     __device__ __forceinline__ int places(const AttnArgs &a) const { return runs(a) + a.splits; }
     __device__ __forceinline__ int all(const AttnArgs &a) const { return key_tiles * places(a); }
+    __device__ __forceinline__ int items(const AttnArgs &a) const { return key_tiles * runs(a); }
 };
 
 template <int DK>
@@ -336,14 +338,14 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const int kh = blockIdx.x % a.k_heads, at_item = blockIdx.x / a.k_heads;
     // Queries past the window, for the sinks.
-    const bool far = kWin && at_item < a.sink_items;
+    const bool far = kWin && at_item >= a.key_runs;
     const auto sink_count = [&](int ql, int kl) { return SinkItems(a, ql, kl).all(a); };
     const auto key_tiles = [&](int, int kl) { return (kl + kBwdTile - 1) / kBwdTile; };
-    const int after = kWin ? at_item - a.sink_items : at_item;
-    const int item = after / a.splits, split = after % a.splits;
+    const auto far_items = [&](int ql, int kl) { return SinkItems(a, ql, kl).items(a); };
+    const int item = at_item / a.splits, split = at_item % a.splits;
     SeqItem s;
     if constexpr (kWin)
-        s = far ? find_item<true>(a, at_item, sink_count, key_tiles)
+        s = far ? find_item<true>(a, at_item - a.key_runs, far_items, sink_count)
                 : find_item<true>(a, item, key_tiles, sink_count);
     else
         s = find_longest<true>(a, item, kBwdTile);
@@ -354,10 +356,10 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
         const SinkItems of(a, s.q_len, s.k_len);
         sink_runs = of.runs(a);
         if (far) {
-            first_key = s.within / of.places(a) * kBwdTile;
-            sink_run = s.within % of.places(a);
-            if (sink_run >= sink_runs) return;         // the window items' places
-            sink_place = at_item;
+            const int tile = s.within / sink_runs;
+            first_key = tile * kBwdTile;
+            sink_run = s.within % sink_runs;
+            sink_place = s.before + tile * of.places(a) + sink_run;
             steps_of = {of.from, of.tiles, sink_runs, of.pieces};
         } else {
             sink_place = s.before + s.within * of.places(a) + sink_runs + split;
@@ -632,7 +634,7 @@ __global__ __launch_bounds__(64 * kSinkWaves) void attn_sink_sum_kernel(AttnArgs
 struct BwdPlan {
     int64_t k_items, largest_at, part_at, sink_at, bytes;
     int splits, split_steps;
-    int64_t sink_items, sink_tiles;
+    int64_t sink_items, sink_places, sink_tiles;
     int sink_steps, sink_rows;
 };
 
@@ -650,8 +652,15 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     p.k_items = k_tokens / kBwdTile + n_seq + 2;
     const int64_t tiles = (ceil_div(k_tokens, kBwdTile) + n_seq - 1) * k_heads;
     int64_t queries = ceil_div(q_tokens, n_seq * kTileRows);
-    if (window > 0 && queries > ceil_div(window + kBwdTile, kTileRows))
-        queries = ceil_div(window + kBwdTile, kTileRows);
+    // The most that any key tile has, not the average: of unequal sequences the longer
+    // ones are cut, the shorter ones' items have steps for one run and stay whole (12
+    // sequences of 5 to 1461 tokens, 4 heads on 2 of 128: 57 us and 12 to add the runs,
+    // uncut 175; 32 equal ones of 100: 36 and 6, uncut 32).
+    if (window > 0) {
+        const int64_t seen = ceil_div(window + kBwdTile, kTileRows);
+        queries = ceil_div(q_tokens, kTileRows);
+        if (queries > seen) queries = seen;
+    }
     const int64_t steps = queries * group;
     int64_t splits = (window > 0 ? kBwdWindowRuns : kBwdRuns) / (tiles > 0 ? tiles : 1);
     if (splits > steps / kBwdRunLeast) splits = steps / kBwdRunLeast;
@@ -675,9 +684,10 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
         // Sum over the sequences of SinkItems::all: of key_tiles * (pieces * group +
         // splits), pieces being at most tokens / (64 sink_steps) + 1 each.
         const int64_t pieces = q_tokens / (kTileRows * p.sink_steps) + n_seq;
-        p.sink_items = key_tiles * (pieces * group + n_seq * p.splits);
+        p.sink_items = key_tiles * pieces * group;
+        p.sink_places = p.sink_items + key_tiles * n_seq * p.splits;
         p.sink_tiles = n_seq * key_tiles;
-        p.bytes += p.sink_items * k_heads * 2 * p.sink_rows * dk * 4;
+        p.bytes += p.sink_places * k_heads * 2 * p.sink_rows * dk * 4;
     }
     return p;
 }
@@ -740,7 +750,7 @@ static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_toke
     a.largest_v = a.largest_do + k_heads * norm_places(q_tokens, sequences);
     a.splits = p.splits, a.split_steps = p.split_steps;
     a.part = reinterpret_cast<float *>(ws + p.part_at);
-    a.sink_items = (int32_t)p.sink_items, a.sink_steps = p.sink_steps, a.sink_rows = p.sink_rows;
+    a.key_runs = (int32_t)(p.k_items * p.splits), a.sink_steps = p.sink_steps, a.sink_rows = p.sink_rows;
     a.sink_part = reinterpret_cast<float *>(ws + p.sink_at);
     hipStream_t st = as_stream(stream);
     const int64_t q_items = (q_tokens * group / kBwdTile + sequences + 2) * k_heads;
@@ -748,7 +758,7 @@ static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_toke
     const int64_t places =
         k_heads * norm_places(q_tokens > k_tokens ? q_tokens : k_tokens, sequences);
     MG_REQUIRE(grid_fits(q_items, 64 * kBwdWaves) && grid_fits(k_items, 64 * kBwdWaves) &&
-                   p.sink_items < INT32_MAX &&
+                   p.sink_places < INT32_MAX &&
                    grid_fits(p.sink_tiles * k_heads * (p.sink_rows / 32 * 2 * 128 / 8),
                              64 * kSinkWaves) &&
                    (dtype != MG_F16 || grid_fits(places, kLargestThreads)),

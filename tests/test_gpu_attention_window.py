@@ -155,6 +155,16 @@ def test_window_gradients_of_shared_heads_in_runs(dev, heads, kv, sinks):
         check(dev, q, k, v, do, q_lens, k_lens, "bf16", window, sinks)
 
 
+@pytest.mark.parametrize("ty,heads,kv,dim", [("bf16", 4, 2, 64), ("f16", 4, 1, 128)])
+@pytest.mark.parametrize("window,sinks", [(700, 3), (650, 0), (1, 130)])
+def test_window_gradients_of_unequal_sequences(dev, ty, heads, kv, dim, window, sinks):
+    """A long sequence's key tiles are cut into runs, short ones' are not."""
+    lens = [5, 900, 1, 0, 40, 130, 7]
+    n = sum(lens)
+    check(dev, *inputs(("unequal", ty, window), n, n, heads, kv, dim, ty), lens, lens, ty, window,
+          sinks)
+
+
 def test_window_of_all_keys_is_none(dev):
     from metal_gauss_amd import attention
 
