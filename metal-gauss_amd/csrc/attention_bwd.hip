@@ -640,11 +640,12 @@ struct BwdPlan {
 
 constexpr int64_t kBwdRuns = 1024, kBwdRunLeast = 8, kBwdMostSplits = 8;
 // With a window: as many as fill the GPU, as partial results weigh more beside fewer
-// queries (7033 packed tokens, window 475: 118 and 28 us to add them in four runs, 115 and
-// 18 in two). As many far items, or pieces of sink_steps = kSinkStepsLeast (in 128 of 8 at
+// queries (7033 packed tokens, window 475: 132 and 30 us to add them in four runs, 119 and
+// 18 in two), of four query tiles at least (nine sequences of 3 to 1210 tokens, 6 heads
+// on 3 of 128: 42 and 13 us, of eight 77 and 8). As many far items, or pieces of sink_steps = kSinkStepsLeast (in 128 of 8 at
 // least that pass's keys took 171 us for 143): their number bounds the room for their
 // sums.
-constexpr int64_t kBwdWindowRuns = 512, kSinkItems = 512, kSinkStepsLeast = 4;
+constexpr int64_t kBwdWindowRuns = 512, kBwdWindowRunLeast = 4, kSinkItems = 512, kSinkStepsLeast = 4;
 
 static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int64_t group,
                         int64_t dim, int64_t n_seq, int64_t window, int64_t sinks) {
@@ -654,8 +655,8 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     int64_t queries = ceil_div(q_tokens, n_seq * kTileRows);
     // The most that any key tile has, not the average: of unequal sequences the longer
     // ones are cut, the shorter ones' items have steps for one run and stay whole (12
-    // sequences of 5 to 1461 tokens, 4 heads on 2 of 128: 57 us and 12 to add the runs,
-    // uncut 175; 32 equal ones of 100: 36 and 6, uncut 32).
+    // sequences of 5 to 1461 tokens, 4 heads on 2 of 128: 40 us and 12 to add the runs,
+    // uncut 175; 32 equal ones of 100: 35 and 6, uncut 32).
     if (window > 0) {
         const int64_t seen = ceil_div(window + kBwdTile, kTileRows);
         queries = ceil_div(q_tokens, kTileRows);
@@ -663,10 +664,11 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     }
     const int64_t steps = queries * group;
     int64_t splits = (window > 0 ? kBwdWindowRuns : kBwdRuns) / (tiles > 0 ? tiles : 1);
-    if (splits > steps / kBwdRunLeast) splits = steps / kBwdRunLeast;
+    const int64_t least = window > 0 ? kBwdWindowRunLeast : kBwdRunLeast;
+    if (splits > steps / least) splits = steps / least;
     splits = splits < 1 ? 1 : splits > kBwdMostSplits ? kBwdMostSplits : splits;
     p.splits = even_runs((int)splits, (int)group, (int)kBwdMostSplits);
-    p.split_steps = (int)kBwdRunLeast;
+    p.split_steps = (int)least;
     p.largest_at = align256(q_tokens * k_heads * group * 4);
     p.part_at = align256(p.largest_at + k_heads * 4 * (norm_places(q_tokens, n_seq) +
                                                        norm_places(k_tokens, n_seq)));
