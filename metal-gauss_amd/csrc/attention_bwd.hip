@@ -26,7 +26,7 @@
 // 8192 tokens, 16 heads of 128: queries 748 us, keys 1047 (1100 and 1050 TFLOP/s);
 // of 64: 462 and 623 (890 and 880). The queries' kernel is never cut over its keys:
 // 64 queries over 16000 of them, 16 heads on 4 of 128, take 417 us. With a window of 475
-// and 4 sinks 7033 packed tokens (16 heads on 4 of 128) take 90 and 128. As the
+// and 4 sinks 7033 packed tokens (16 heads on 4 of 128) take 92 and 126. As the
 // forward, both need two waves a SIMD to keep products and exponentials going side by
 // side: the keys' kernel with one (256 columns of sums and operands in 472 registers)
 // took 1970.

@@ -11,8 +11,8 @@
 //
 // Memory bounds it: eight draws a block make some 20 vector instructions an element
 // (with the whole 32 bits for each it would be the generator). 65280 x 1024 bfloat16 onto a
-// float32 residual 115 us (5.8 TB/s), and dx from its float32 gradient 72 (5.5). Two and
-// four counters a thread: 117 and 125; 64 x 256 float32: 2.6, the launch.
+// float32 residual 121 us (5.5 TB/s), and dx from its float32 gradient 69 (5.8). Two and
+// four counters a thread: 2 and 9% more; 64 x 256 float32: 2.6, the launch.
 #include "mg_types.h"
 
 namespace mg {

@@ -20,7 +20,7 @@
 // only where it is used.
 //
 // 32640 tokens of 20 heads of 128 bfloat16, a sixth of their rows between them: forward
-// 57 us (5.9 TB/s), backward 95 (5.3) and 4 to join dw; with loads made as they were
+// 57 us (5.9 TB/s), backward 98 (5.1) and 4 to join dw; with loads made as they were
 // needed 77 and 120. 9975 tokens of 32 heads of 64: 18 (4.5 TB/s); 16 tokens: 5.9.
 #include "rotary.h"
 
