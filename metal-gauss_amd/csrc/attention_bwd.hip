@@ -23,8 +23,8 @@
 // sequence packed with it nor tokens of none take digits from it. bfloat16 has
 // float32's range and needs neither.
 //
-// 8192 tokens, 16 heads of 128: queries 748 us, keys 1047 (1100 and 1050 TFLOP/s);
-// of 64: 462 and 623 (890 and 880). The queries' kernel is never cut over its keys:
+// 8192 tokens, 16 heads of 128 bfloat16: queries 800 us, keys 1092 (1030 and 1010 TFLOP/s);
+// of 64: 487 and 635 (850 and 870). The queries' kernel is never cut over its keys:
 // 64 queries over 16000 of them, 16 heads on 4 of 128, take 417 us. With a window of 475
 // and 4 sinks 7033 packed tokens (16 heads on 4 of 128) take 92 and 126. As the
 // forward, both need two waves a SIMD to keep products and exponentials going side by
@@ -116,11 +116,14 @@ __device__ __forceinline__ float ds_power(float do_sq, float v_sq) {
 }
 
 // ------------------------------------------------------- the queries' gradient
-// Without a window four waves a SIMD for 64 columns; with one that many keep too few
-// registers (window 777, 64 columns: 60 us, 98).
+// With a window results leave by whole rows, by way of LDS, as the few keys of an item
+// leave its rows most of the time; without one the stores' code weighs more in the loop
+// than it gains behind it: seven sequences of 7033 tokens, 16 heads on 4 of 128
+// bfloat16, unmasked, 254 us so and 230 by fours (causal 134 and 128; of 64 columns, where it
+// took registers past the 128 of four waves a SIMD, 86 and 82). Of 32 columns it is no
+// slower, float16's 213 and 205.
 template <typename T, int DK, bool kWin>
-__global__ __launch_bounds__(64 * kBwdWaves, !kWin && DK == 64 ? 4 : 2) void attn_dq_kernel(
-    AttnArgs a) {
+__global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dq_kernel(AttnArgs a) {
     constexpr int kSteps = DK / 16, kBlocks = DK / 32;
     __shared__ __align__(16) char s_tile[2][2][kTileBytes<DK>];
     const int lane = lane_id(), half = lane / 32;
@@ -243,12 +246,27 @@ __global__ __launch_bounds__(64 * kBwdWaves, !kWin && DK == 64 ? 4 : 2) void att
         }
     }
     lds_reads_done();
-    static_assert(kBwdWaves * kRowBytes<DK> <= (int)sizeof(s_tile), "rows in the tiles' memory");
-    tiles_ready();
-    const RowStore<T, DK> store{&s_tile[0][0][0] + wave * kRowBytes<DK>};
     const float down = a.scale * __builtin_amdgcn_exp2f(-power);
-    store(static_cast<T *>(a.dq), ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim,
-          row_ok, a.dim, [&](int b, int e) { return (T)(dq[b][e] * down); });
+    const int64_t at_row = ((int64_t)(s.q_lo + token) * (a.k_heads * G) + head) * a.dim;
+    T *out = static_cast<T *>(a.dq);
+    if constexpr (kWin || DK == 32) {
+        static_assert(kBwdWaves * kRowBytes<DK> <= (int)sizeof(s_tile), "rows in the tiles' memory");
+        tiles_ready();
+        const RowStore<T, DK> store{&s_tile[0][0][0] + wave * kRowBytes<DK>};
+        store(out, at_row, row_ok, a.dim, [&](int b, int e) { return (T)(dq[b][e] * down); });
+    } else {
+        if (!row_ok) return;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int at = 32 * b + c_row(e, half);
+                vec4<T> w;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = (T)(dq[b][e + i] * down);
+                if (at < a.dim) *reinterpret_cast<vec4<T> *>(out + at_row + at) = w;
+            }
+    }
 }
 
 // ------------------------------------------- the keys' and values' gradients
