@@ -66,8 +66,8 @@ struct AttnArgs {
     int32_t splits, split_steps;
     float *part;
     // With sinks: the first keys' gradients from queries further on than the
-    // window, in runs of sink_steps query tiles of one head (attention_bwd.hip).
-    int32_t key_runs, sink_steps, sink_rows;
+    // window, in runs of about sink_steps query tiles of one head (sink_cut).
+    int32_t key_runs, sink_steps, sink_near, sink_rows;
     float *sink_part;
 };
 

@@ -294,28 +294,25 @@ __device__ __forceinline__ f32x4 *part_of(const AttnArgs &a, int item, int kh, i
 }
 
 // With a window, the queries that see a key tile are few, but those further on all
-// see the sinks. Their sums for the sinks are work items of their own, which come
-// last, being short ones (first: 147 us in place of 126 for 7033 packed tokens, window
-// 475): one tile of kBwdTile keys, one head and sink_steps query tiles each. Their
-// sums, of sink_rows keys, have a place each in sink_part, and so have those of the
+// see the sinks. Where these are many (sink_cut), their sums for the sinks are work items
+// of their own, which come last, being short ones (first: 147 us in place of 126 for 7033
+// packed tokens, window 475): one tile of kBwdTile keys and a run of query tiles each.
+// Their sums, of sink_rows keys, have a place each in sink_part, and so have those of the
 // window items of key tiles that have sinks; attn_sink_sum_kernel adds them up, in
 // order. A sequence's places follow one another, a key tile's far items' and then
-// its window items'.
-struct SinkItems {
-    int key_tiles, from, tiles, pieces;    // from: the first query past the window
+// its window items'. A sequence with few far queries has its window items go on for them
+// (512 of 64 tokens, 16 heads on 4 of 128, window 16 and 4 sinks, both gradients: 914 us
+// with items and places of their own, so 476).
+static_assert(kSinkTokens == kTileRows && kSinkKeys == kBwdTile, "tiles of the items");
 
-    __device__ __forceinline__ SinkItems(const AttnArgs &a, int q_len, int k_len) {
-        key_tiles = (min(a.sinks, k_len) + kBwdTile - 1) / kBwdTile;
-        from = (int)min((int64_t)q_len, max((int64_t)0, (int64_t)a.window + q_len - k_len));
-        tiles = (q_len - from + kTileRows - 1) / kTileRows;
-        pieces = (tiles + a.sink_steps - 1) / a.sink_steps;
-        if (q_len == 0) key_tiles = 0;
-    }
-    __device__ __forceinline__ int runs(const AttnArgs &a) const { return pieces * a.group; }
-    // Places of a key tile, and of a sequence.
-    __device__ __forceinline__ int places(const AttnArgs &a) const { return runs(a) + a.splits; }
+struct SinkItems : SinkCut {
+    __device__ __forceinline__ SinkItems(const AttnArgs &a, int q_len, int k_len)
+        : SinkCut(sink_cut(q_len, k_len, a.window, a.sinks, a.group, a.sink_steps,
+                           a.sink_near)) {}
+    // Places of a key tile, and of a sequence; items of a sequence.
+    __device__ __forceinline__ int places(const AttnArgs &a) const { return runs + a.splits; }
     __device__ __forceinline__ int all(const AttnArgs &a) const { return key_tiles * places(a); }
-    __device__ __forceinline__ int items(const AttnArgs &a) const { return key_tiles * runs(a); }
+    __device__ __forceinline__ int items() const { return key_tiles * runs; }
 };
 
 template <int DK>
@@ -327,19 +324,22 @@ __device__ __forceinline__ f32x4 *sink_part_of(const AttnArgs &a, int place, int
 // The query tiles that see a key tile (tiles of each of the group's heads, from
 // q_from), and the runs they are cut into: whole heads, or `parts` of each head
 // where there are more runs than heads. Key tiles that run at the same time then
-// read the same heads' queries, which stay in their XCD's L2.
+// read the same heads' queries, which stay in their XCD's L2. `on`: the tile has sinks
+// that no other items have the later queries of.
 struct KeySteps {
     int q_from, tiles, runs, parts;
 };
 
 template <bool kWin>
-__device__ __forceinline__ KeySteps key_steps(const AttnArgs &a, const SeqItem &s, int first_key) {
+__device__ __forceinline__ KeySteps key_steps(const AttnArgs &a, const SeqItem &s, int first_key,
+                                             bool on) {
     const int ahead = s.k_len - s.q_len, G = a.group;
     int from = a.causal ? max(0, first_key - ahead) / kTileRows * kTileRows : 0, to = s.q_len;
     if constexpr (kWin) {
         from = max(0, first_key - ahead);
         const int last = min(first_key + kBwdTile, s.k_len) - 1;
         to = (int)min((int64_t)s.q_len, max((int64_t)0, (int64_t)last + a.window - ahead));
+        if (on) to = s.q_len;
     }
     const int tiles = from < to ? (to - from + kTileRows - 1) / kTileRows : 0;
     int runs = (int)(((int64_t)tiles * G + a.split_steps - 1) / a.split_steps);
@@ -359,7 +359,7 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     const bool far = kWin && at_item >= a.key_runs;
     const auto sink_count = [&](int ql, int kl) { return SinkItems(a, ql, kl).all(a); };
     const auto key_tiles = [&](int, int kl) { return (kl + kBwdTile - 1) / kBwdTile; };
-    const auto far_items = [&](int ql, int kl) { return SinkItems(a, ql, kl).items(a); };
+    const auto far_items = [&](int ql, int kl) { return SinkItems(a, ql, kl).items(); };
     const int item = at_item / a.splits, split = at_item % a.splits;
     SeqItem s;
     if constexpr (kWin)
@@ -370,21 +370,24 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
     if (!s.found) return;
     KeySteps steps_of;
     int first_key = s.within * kBwdTile, sink_run = 0, sink_runs = 0, sink_place = 0;
+    int sinks_to = 0;            // keys below it count as sinks in this item
     if (kWin && a.sinks > 0) {
         const SinkItems of(a, s.q_len, s.k_len);
-        sink_runs = of.runs(a);
+        sink_runs = of.runs;
+        if (far || sink_runs == 0) sinks_to = a.sinks;
         if (far) {
             const int tile = s.within / sink_runs;
             first_key = tile * kBwdTile;
             sink_run = s.within % sink_runs;
             sink_place = s.before + tile * of.places(a) + sink_run;
-            steps_of = {of.from, of.tiles, sink_runs, of.pieces};
+            steps_of = {of.from, of.tiles, sink_runs,
+                        sink_runs > a.group ? sink_runs / a.group : 1};
         } else {
             sink_place = s.before + s.within * of.places(a) + sink_runs + split;
         }
     }
     if (!far) {
-        steps_of = key_steps<kWin>(a, s, first_key);
+        steps_of = key_steps<kWin>(a, s, first_key, first_key < sinks_to);
         if (split >= steps_of.runs) return;
     }
     const int key0 = first_key + wave * 32, key = key0 + lane % 32;
@@ -441,6 +444,17 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
             seq_largest(a, a.largest_v, kh, a.k_tokens, s.seq, s.k_lo, s.k_len));
     const float ds_up = __builtin_amdgcn_exp2f(power - kPowerP<T>);
 
+    // With a window: the queries that see this lane's key, `sees` from sees_from on, of
+    // those that are this item's.
+    int sees_from = 0;
+    uint32_t sees = 0;
+    if constexpr (kWin) {
+        const int past = max(0, key - ahead + a.window);
+        sees_from = far ? past : max(0, key - ahead);
+        const int to = far || key < sinks_to ? s.q_len : min(s.q_len, past);
+        if (key_ok && (!far || key < sinks_to)) sees = max(0, to - sees_from);
+    }
+
     f32x16 dk[kBlocks] = {}, dv[kBlocks] = {};
     const int steps = tiles * heads;
     TileLane<T, DK> lane_at;
@@ -466,8 +480,9 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
             // How far on the tile's rows stand, of the wave's keys.
             const int least = at_row0 + ahead - (key0 + 31);
             const int most = at_row0 + kTileRows - 1 + ahead - key0;
-            if (far ? key0 >= a.sinks || most < a.window : least >= a.window) continue;
-            masked |= far ? key0 + 32 > a.sinks || least < a.window : most >= a.window;
+            if (far ? key0 >= sinks_to || most < a.window : key0 >= sinks_to && least >= a.window)
+                continue;
+            masked |= far ? key0 + 32 > sinks_to || least < a.window : most >= a.window;
         }
 #pragma unroll 1
         for (int b = 0; b < 2; ++b) {
@@ -491,11 +506,14 @@ __global__ __launch_bounds__(64 * kBwdWaves, 2) void attn_dkv_kernel(AttnArgs a)
                     float d = x * ((dp[e] - delta[i]) * ds_up);
                     if (masked) {
                         const int token = at_row0 + r + i;
-                        bool seen = token < s.q_len && key_ok &&
-                                    (!a.causal || key <= token + ahead);
+                        bool seen;
                         if constexpr (kWin) {
-                            const bool within = token + ahead - key < a.window;
-                            seen = seen && (far ? !within && key < a.sinks : within);
+                            // Keeps this a branch: as selects it costs every tile (16320
+                            // tokens, window 1900: 1229 us with the queries', so 1075).
+                            asm volatile("");
+                            seen = (uint32_t)(token - sees_from) < sees;
+                        } else {
+                            seen = token < s.q_len && key_ok && (!a.causal || key <= token + ahead);
                         }
                         x = seen ? x : 0.f;
                         d = seen ? d : 0.f;
@@ -585,15 +603,17 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_sum_kernel(AttnArgs a) {
                            : find_longest<true>(a, item, kBwdTile);
     if (!s.found) return;
     const int first_key = s.within * kBwdTile;
-    const int runs = key_steps<kWin>(a, s, first_key).runs;
+    // attn_sink_sum_kernel has the sinks that have items of their own.
+    const bool sinks_apart =
+        kWin && first_key < a.sinks && SinkItems(a, s.q_len, s.k_len).runs > 0;
+    const int runs = key_steps<kWin>(a, s, first_key, first_key < a.sinks && !sinks_apart).runs;
     if (runs == 1) return;
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / 64);
     const int key = first_key + wave * 32 + lane % 32;
     const int64_t at_row = ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim;
     const f32x4 *part = part_of<DK>(a, item, kh, 0) + wave * kBlocks * 4 * 64 + lane;
     const int which = blockIdx.y % 2, block = blockIdx.y / 2;
-    // attn_sink_sum_kernel has these.
-    if (kWin && key < a.sinks && SinkItems(a, s.q_len, s.k_len).runs(a) > 0) return;
+    if (sinks_apart && key < a.sinks) return;
 #pragma unroll
     for (int i = 4 * block; i < 4 * block + 4; ++i) {
         const f32x4 *p = part + i * 64 + which * kPartFours<DK> / 2;
@@ -620,9 +640,8 @@ __global__ __launch_bounds__(64 * kSinkWaves) void attn_sink_sum_kernel(AttnArgs
         [&](int ql, int kl) { return SinkItems(a, ql, kl).all(a); });
     if (!s.found) return;
     const SinkItems of(a, s.q_len, s.k_len);
-    if (of.runs(a) == 0) return;                 // the window items have written theirs
     const int first_key = s.within * kBwdTile;
-    const int places = of.runs(a) + key_steps<true>(a, s, first_key).runs;
+    const int places = of.runs + key_steps<true>(a, s, first_key, false).runs;
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / 64);
     const int i = blockIdx.y % (kBlocks * 4), rows = blockIdx.y / (kBlocks * 4) / 2 * 32;
     const int which = blockIdx.y / (kBlocks * 4) % 2;
@@ -660,9 +679,9 @@ constexpr int64_t kBwdRuns = 1024, kBwdRunLeast = 8, kBwdMostSplits = 8;
 // With a window: as many as fill the GPU, as partial results weigh more beside fewer
 // queries (7033 packed tokens, window 475: 132 and 30 us to add them in four runs, 119 and
 // 18 in two), of four query tiles at least (nine sequences of 3 to 1210 tokens, 6 heads
-// on 3 of 128: 42 and 13 us, of eight 77 and 8). As many far items, or pieces of sink_steps = kSinkStepsLeast (in 128 of 8 at
-// least that pass's keys took 171 us for 143): their number bounds the room for their
-// sums.
+// on 3 of 128: 42 and 13 us, of eight 77 and 8). As many far items, or runs of
+// sink_steps = kSinkStepsLeast (in 128 of 8 at least that pass's keys took 171 us for
+// 143).
 constexpr int64_t kBwdWindowRuns = 512, kBwdWindowRunLeast = 4, kSinkItems = 512, kSinkStepsLeast = 4;
 
 static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int64_t group,
@@ -696,17 +715,15 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     p.sink_at = p.bytes;
     p.sink_steps = 1;
     if (sinks > 0) {
-        const int64_t key_tiles = ceil_div(sinks, kBwdTile);
-        int64_t most = ceil_div(q_tokens, kTileRows) * group * k_heads * key_tiles / kSinkItems;
-        most = most < kSinkStepsLeast ? kSinkStepsLeast : most;
+        int64_t most = ceil_div(q_tokens, kTileRows) * group * k_heads *
+                       ceil_div(sinks, kBwdTile) / kSinkItems;
+        most = most < kSinkStepsLeast ? kSinkStepsLeast : most < (1 << 30) ? most : 1 << 30;
         p.sink_steps = (int)most;
         p.sink_rows = (int)(sinks < kBwdTile ? ceil_div(sinks, 32) * 32 : kBwdTile);
-        // Sum over the sequences of SinkItems::all: of key_tiles * (pieces * group +
-        // splits), pieces being at most tokens / (64 sink_steps) + 1 each.
-        const int64_t pieces = q_tokens / (kTileRows * p.sink_steps) + n_seq;
-        p.sink_items = key_tiles * pieces * group;
-        p.sink_places = p.sink_items + key_tiles * n_seq * p.splits;
-        p.sink_tiles = n_seq * key_tiles;
+        const SinkRoom room = sink_room(q_tokens, k_tokens, n_seq, window, sinks, group, most);
+        p.sink_items = room.runs;
+        p.sink_tiles = room.key_tiles;
+        p.sink_places = room.runs + room.key_tiles * p.splits;
         p.bytes += p.sink_places * k_heads * 2 * p.sink_rows * dk * 4;
     }
     return p;
@@ -770,7 +787,8 @@ static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_toke
     a.largest_v = a.largest_do + k_heads * norm_places(q_tokens, sequences);
     a.splits = p.splits, a.split_steps = p.split_steps;
     a.part = reinterpret_cast<float *>(ws + p.part_at);
-    a.key_runs = (int32_t)(p.k_items * p.splits), a.sink_steps = p.sink_steps, a.sink_rows = p.sink_rows;
+    a.key_runs = (int32_t)(p.k_items * p.splits), a.sink_steps = p.sink_steps;
+    a.sink_near = (int32_t)sink_near(group, p.sink_steps), a.sink_rows = p.sink_rows;
     a.sink_part = reinterpret_cast<float *>(ws + p.sink_at);
     hipStream_t st = as_stream(stream);
     const int64_t q_items = (q_tokens * group / kBwdTile + sequences + 2) * k_heads;
@@ -812,7 +830,7 @@ static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_toke
         });
         MG_LAUNCHED("attn_dkv_kernel");
     }
-    if (k_tokens > 0 && dk && a.sinks > 0) {
+    if (dk && p.sink_tiles > 0) {
         TimedScope ts("attention_sinks", st);
         attn_form(dtype, dim, [&](auto t, auto d) {
             constexpr int DK = decltype(d)::value;

@@ -98,4 +98,52 @@ constexpr int even_runs(int runs, int group, int most) {
     return even <= most ? even : runs;
 }
 
+// ------------------------------------------------------------------ sinks
+// The keys' gradients of a windowed sequence: the queries past the window of its key 0
+// (tiles of kSinkTokens of them, of each of `group` heads) reach its sinks alone. They
+// are work items of their own, over `key_tiles` tiles of kSinkKeys keys in `runs` runs
+// each: about `steps` tiles of one head a run, a run having whole heads, or each
+// head's being cut into runs / group alike. Where they are one run, or few, the
+// sequence's window items go on for them and it has no runs.
+constexpr int kSinkTokens = 64, kSinkKeys = 128;
+constexpr int64_t sink_near(int64_t group, int64_t steps) {
+    return steps / group > 4 ? steps / group : 4;
+}
+
+struct SinkCut {
+    int from, tiles;             // the first query past the window; tiles from it on
+    int key_tiles, runs;
+};
+// near: sink_near(group, steps). Tokens by `group`, keys and the window are below 2^30.
+constexpr SinkCut sink_cut(int q_len, int k_len, int window, int sinks, int group, int steps,
+                           int near) {
+    const int past = window + q_len - k_len;
+    const int from = past < 0 ? 0 : past < q_len ? past : q_len;
+    const int tiles = (q_len - from + kSinkTokens - 1) / kSinkTokens;
+    if (tiles <= near || sinks == 0) return {from, tiles, 0, 0};
+    const int keys = sinks < k_len ? sinks : k_len;
+    const int runs = (tiles * group + steps - 1) / steps;
+    return {from, tiles, (keys + kSinkKeys - 1) / kSinkKeys,
+            runs > group ? runs / group * group : runs};
+}
+
+// Their sums over all of n_seq sequences, at most, with `sinks` no more than the keys.
+// A sequence with runs has more queries than sink_near tiles, and as many keys past
+// its window.
+struct SinkRoom {
+    int64_t key_tiles, runs;     // runs: over the key tiles
+};
+constexpr SinkRoom sink_room(int64_t q_tokens, int64_t k_tokens, int64_t n_seq, int64_t window,
+                             int64_t sinks, int64_t group, int64_t steps) {
+    const int64_t far = sink_near(group, steps) * kSinkTokens + 1;
+    int64_t with = n_seq;        // sequences that have any
+    if (with > q_tokens / far) with = q_tokens / far;
+    if (with > k_tokens / (window + far)) with = k_tokens / (window + far);
+    if (with == 0) return {0, 0};
+    const int64_t each = (sinks + kSinkKeys - 1) / kSinkKeys;
+    int64_t key_tiles = with * each;
+    if (key_tiles > k_tokens / kSinkKeys + with) key_tiles = k_tokens / kSinkKeys + with;
+    return {key_tiles, each * ((q_tokens / kSinkTokens + with) * group / steps) + key_tiles};
+}
+
 }  // namespace mg

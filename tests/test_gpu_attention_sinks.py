@@ -1,0 +1,53 @@
+"""Gradients of attention's first keys that stay visible, on the GPU, over packs of many
+sequences: those whose window items go on for their sinks, those with items of their
+own, and both in one pack. Against the float64 restatement, by the tolerances of
+test_gpu_attention_window.py."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_attention_window import check, inputs
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("window,sinks", [(1, 1), (3, 130), (9, 33), (475, 1000)])
+@pytest.mark.parametrize("ty,heads,kv,dim", [("bf16", 4, 2, 64), ("f16", 3, 1, 32)])
+def test_many_short_sequences(dev, window, sinks, ty, heads, kv, dim):
+    rng = np.random.default_rng(window)
+    q_lens = [int(x) for x in rng.integers(0, 40, 300)]
+    k_lens = [max(0, n + int(x)) for n, x in zip(q_lens, rng.integers(-5, 25, 300))]
+    q, k, v, do = inputs(("short", window, ty), sum(q_lens), sum(k_lens), heads, kv, dim, ty)
+    check(dev, q, k, v, do, q_lens, k_lens, ty, window, sinks)
+
+
+@pytest.mark.parametrize("ty,heads,kv,dim", [("bf16", 4, 2, 64), ("f16", 5, 1, 128)])
+@pytest.mark.parametrize("sinks", [3, 130, 700])
+@pytest.mark.parametrize("window", [1, 70])
+def test_sequences_about_the_length_of_items_of_their_own(dev, ty, heads, kv, dim, sinks, window):
+    """255 to 257 queries past the window of the first key, one of them alone over a
+    longer memory, and none."""
+    q_lens = [window + 255, window + 256, window + 257, 257, 256, window, 300]
+    k_lens = [window + 255, window + 256, window + 257, window + 600, 900, window, 100]
+    q, k, v, do = inputs(("near", window, sinks, ty), sum(q_lens), sum(k_lens), heads, kv, dim, ty)
+    check(dev, q, k, v, do, q_lens, k_lens, ty, window, sinks)
+
+
+@pytest.mark.parametrize("heads,kv", [(10, 2), (8, 1), (3, 3)])
+def test_runs_of_some_of_the_heads(dev, heads, kv):
+    """Enough tokens for runs of several heads' tiles, even and uneven, beside sequences
+    that have none and one whose heads are cut."""
+    q_lens = [420, 700, 60, 5, 0, 200, 2600, 800] + [510] * 16
+    n = sum(q_lens)
+    q, k, v, do = inputs(("some", heads), n, n, heads, kv, 16, "bf16")
+    check(dev, q, k, v, do, q_lens, q_lens, "bf16", 50, 300)
+
+
+def test_one_sequence_of_sinks_alone(dev):
+    """More sinks than a window leaves out, in items and in place."""
+    for n, window, sinks in ((1500, 1, 1500), (900, 300, 899), (300, 20, 300)):
+        q, k, v, do = inputs(("alone", n), n, n, 4, 2, 64, "f16")
+        check(dev, q, k, v, do, [n], [n], "f16", window, sinks)
