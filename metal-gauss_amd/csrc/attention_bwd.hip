@@ -779,6 +779,14 @@ static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_toke
     hold_window(a);
     const BwdPlan p =
         bwd_plan(q_tokens, k_tokens, k_heads, group, dim, sequences, a.window, a.sinks);
+    const int64_t q_items = (q_tokens * group / kBwdTile + sequences + 2) * k_heads;
+    const int64_t k_items = (p.k_items * p.splits + p.sink_items) * k_heads;
+    const int64_t places =
+        k_heads * norm_places(q_tokens > k_tokens ? q_tokens : k_tokens, sequences);
+    MG_REQUIRE(grid_fits(q_items, 64 * kBwdWaves) && grid_fits(k_items, 64 * kBwdWaves) &&
+                   p.sink_places < INT32_MAX && grid_fits(p.sink_tiles * k_heads, 64 * kSinkWaves) &&
+                   (dtype != MG_F16 || grid_fits(places, kLargestThreads)),
+               "%s: too many work items", who);
     MG_REQUIRE(workspace && workspace_bytes >= p.bytes, "%s: workspace of %lld bytes, %lld needed",
                who, (long long)workspace_bytes, (long long)p.bytes);
     char *ws = static_cast<char *>(workspace);
@@ -791,16 +799,6 @@ static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_toke
     a.sink_near = (int32_t)sink_near(group, p.sink_steps), a.sink_rows = p.sink_rows;
     a.sink_part = reinterpret_cast<float *>(ws + p.sink_at);
     hipStream_t st = as_stream(stream);
-    const int64_t q_items = (q_tokens * group / kBwdTile + sequences + 2) * k_heads;
-    const int64_t k_items = (p.k_items * p.splits + p.sink_items) * k_heads;
-    const int64_t places =
-        k_heads * norm_places(q_tokens > k_tokens ? q_tokens : k_tokens, sequences);
-    MG_REQUIRE(grid_fits(q_items, 64 * kBwdWaves) && grid_fits(k_items, 64 * kBwdWaves) &&
-                   p.sink_places < INT32_MAX &&
-                   grid_fits(p.sink_tiles * k_heads * (p.sink_rows / 32 * 2 * 128 / 8),
-                             64 * kSinkWaves) &&
-                   (dtype != MG_F16 || grid_fits(places, kLargestThreads)),
-               "%s: too many work items", who);
     if (dtype == MG_F16) {
         TimedScope ts("attention_largest", st);
         attn_largest_kernel<f16_t><<<dim3((unsigned)places, 2), kLargestThreads, 0, st>>>(a);

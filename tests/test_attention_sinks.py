@@ -87,3 +87,32 @@ def test_room_of_sinks_does_not_go_by_the_sequences(tokens, heads, kv, dim, sequ
 def test_sequences_within_the_window_take_no_room_for_sinks(sinks):
     """One query past the window is no item of its own."""
     assert backward_room(300, 16, 4, 128, 1, 299, sinks) == backward_room(300, 16, 4, 128, 1, 299, 0)
+
+
+def backward_call(tokens, heads, kv, dim, sequences, window, sinks, dtype=1):
+    """A call whose room is too small: refused before any launch."""
+    from metal_gauss_amd import _lib
+
+    lib = _lib.open_library()
+    rows = (heads * dim, dim), (kv * dim, dim)
+    rc = lib.mg_attention_window_backward(
+        dtype, tokens, tokens, heads, kv, dim, 16, *rows[0], 16, *rows[1], 16, *rows[1], 16, 16,
+        sequences, window, sinks, 1.0, 16, None, 16, 16, *rows[0], 16, 16, 16, 16, 8, None)
+    assert rc == 1
+    return lib.mg_last_error().decode()
+
+
+@pytest.mark.parametrize("tokens,heads,kv,dim,sequences,window,sinks", [
+    (32768, 32, 32, 64, 2048, 475, 130), (32768, 32, 32, 64, 512, 475, 1000),
+    (16320, 32, 32, 32, 1024, 475, 500), (65280, 32, 32, 128, 4096, 1, 130),
+    (90000, 512, 512, 8, 350, 1, 300), (65280, 16, 1, 128, 1, 16, 65279),
+    (262144, 32, 4, 128, 8192, 30, 1000)])
+def test_packs_that_forward_takes_are_taken_backward(tokens, heads, kv, dim, sequences, window,
+                                                     sinks):
+    for dtype in (1, 2):
+        message = backward_call(tokens, heads, kv, dim, sequences, window, sinks, dtype)
+        assert "workspace of 8 bytes" in message
+
+
+def test_more_items_than_a_launch_has_are_refused():
+    assert "too many work items" in backward_call(1 << 25, 2, 2, 64, 1 << 25, 5, 1)

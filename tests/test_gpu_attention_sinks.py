@@ -51,3 +51,30 @@ def test_one_sequence_of_sinks_alone(dev):
     for n, window, sinks in ((1500, 1, 1500), (900, 300, 899), (300, 20, 300)):
         q, k, v, do = inputs(("alone", n), n, n, 4, 2, 64, "f16")
         check(dev, q, k, v, do, [n], [n], "f16", window, sinks)
+
+
+@pytest.mark.parametrize("tokens,sequences,heads,dim,window,sinks", [
+    (32768, 2048, 32, 64, 475, 130), (32768, 512, 32, 64, 475, 1000), (16320, 1024, 32, 32, 475, 500)])
+def test_packs_of_thousands_of_sequences(dev, tokens, sequences, heads, dim, window, sinks):
+    """The first, middle and last sequences of two heads against the restatement."""
+    from metal_gauss_amd import attention
+    from oracle import token_ref
+    from test_gpu_attention_window import UNIT, host
+
+    rng = np.random.default_rng(sequences)
+    at = np.sort(rng.choice(np.arange(1, tokens), sequences - 1, replace=False))
+    off = np.concatenate([[0], at, [tokens]])
+    q, k, v, do = inputs(("thousands", sequences), tokens, tokens, heads, heads, dim, "bf16")
+    leaves = [t.to(dev).requires_grad_(True) for t in (q, k, v)]
+    o = attention(*leaves, torch.tensor(off, dtype=torch.int32, device=dev), causal=True,
+                  window=window, sinks=sinks)
+    got = [o, *torch.autograd.grad(o, leaves, do.to(dev))]
+    for s in (0, 1, sequences // 2, sequences - 2, sequences - 1):
+        lo, hi = int(off[s]), int(off[s + 1])
+        for h in (0, heads - 1):
+            part = [host(t[lo:hi, h:h + 1]) for t in (q, k, v, do)]
+            want, bound = token_ref.attention(*part[:3], [0, hi - lo], [0, hi - lo], True,
+                                              dim ** -0.5, part[3], UNIT["bf16"], window, sinks)
+            for a, w, b in zip(got, want, bound):
+                a = host(a[lo:hi, h:h + 1])
+                assert (np.abs(a - w) <= b * (1.0 + 2.0 ** -14 / UNIT["bf16"]) * 1.05 + 1e-30).all()
