@@ -51,7 +51,7 @@ def _forward(q, k, v, q_offsets, k_offsets, causal, window, scale, keep):
     # With a backward pass ahead, what rounding takes from the result is kept too.
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     rest = torch.empty_like(out) if keep else None
-    lse = torch.empty(Hq, Tq, device=q.device) if keep else None
+    lse = torch.empty(Hq, Tq, dtype=torch.float32, device=q.device) if keep else None
     need = workspace(Tq, Tk, Hq, Hk, D, n, *more)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
     _lib.launch(call, q.get_device(), _lib.TYPE_CODES[q.dtype], Tq, Tk, Hq,

@@ -448,7 +448,7 @@ def _grad_inputs(N, dev, d_uv, d_conic, d_color, d_oe, want_color, want_oe):
                      d_oe.data_ptr() if want_oe else None], k, ())
 
     def dense(t, shape):
-        return torch.zeros(*shape, device=dev) if t is None else t.contiguous()
+        return torch.zeros(*shape, dtype=torch.float32, device=dev) if t is None else t.contiguous()
     keep = (dense(d_uv, (N, 2)), dense(d_conic, (N, 3)),
             dense(d_color, (N, 3)) if want_color else None,
             dense(d_oe, (N,)) if want_oe else None)
@@ -487,12 +487,12 @@ class _PreprocessMetal(torch.autograd.Function):
         else:
             rest = None
         opac = ctx_opac.contiguous()
-        uv = torch.empty(N, 2, device=dev)
-        conic = torch.empty(N, 3, device=dev)
-        depth = torch.empty(N, device=dev)
-        rxy = torch.empty(N, 2, device=dev)
+        uv = torch.empty(N, 2, dtype=torch.float32, device=dev)
+        conic = torch.empty(N, 3, dtype=torch.float32, device=dev)
+        depth = torch.empty(N, dtype=torch.float32, device=dev)
+        rxy = torch.empty(N, 2, dtype=torch.float32, device=dev)
         valid = torch.empty(N, dtype=torch.int32, device=dev)
-        color = torch.empty(N, 3, device=dev) if sh is not None else None
+        color = torch.empty(N, 3, dtype=torch.float32, device=dev) if sh is not None else None
         vm = _lib.host_f32(viewmat)
         cc = _lib.host_f32(cam_center)
         _lib.check(lib.mg_preprocess_forward(
@@ -525,9 +525,9 @@ class _PreprocessMetal(torch.autograd.Function):
         viewmat, fx, fy, cx, cy, W, H, near, far, blur, max_radius, cam_center, deg = ctx.meta
         N = means.shape[0]
         dev = means.device
-        d_means = torch.empty(N, 3, device=dev)
-        d_quats = torch.empty(N, 4, device=dev)
-        d_scales = torch.empty(N, 3, device=dev)
+        d_means = torch.empty(N, 3, dtype=torch.float32, device=dev)
+        d_quats = torch.empty(N, 4, dtype=torch.float32, device=dev)
+        d_scales = torch.empty(N, 3, dtype=torch.float32, device=dev)
         d_sh = d_rest = None
         if ctx.has_sh:
             d_sh = torch.empty_like(sh)
@@ -560,9 +560,9 @@ class _RasterizeMetal(torch.autograd.Function):
         dev = uv.device
         uv, conic, opacity, color = (t.contiguous() for t in (uv, conic, opacity, color))
         N = uv.shape[0]
-        rgb = torch.empty(H, W, 3, device=dev)
-        alpha = torch.empty(H, W, device=dev)
-        T = torch.empty(H, W, device=dev)
+        rgb = torch.empty(H, W, 3, dtype=torch.float32, device=dev)
+        alpha = torch.empty(H, W, dtype=torch.float32, device=dev)
+        T = torch.empty(H, W, dtype=torch.float32, device=dev)
         stop = torch.empty(H, W, dtype=torch.int32, device=dev)
         # Plan + per-chunk pixel states for the chunked backward.
         n_isect = gauss_ids.numel()
@@ -572,8 +572,8 @@ class _RasterizeMetal(torch.autograd.Function):
         # The backward's gradient records, cleared by the forward kernel on
         # the way (the backward then skips its own fill), when a backward can
         # follow.
-        rec = (torch.empty(N, _REC, device=dev) if N and any(ctx.needs_input_grad[:4])
-               else None)
+        rec = (torch.empty(N, _REC, dtype=torch.float32, device=dev)
+               if N and any(ctx.needs_input_grad[:4]) else None)
         # With a backward to come, the forward records each tile's walk
         # length so that the backward can run the longest walks first.
         sched = (torch.empty(lib.mg_rasterize_sched_ints(W, H, tile), dtype=torch.int32,
@@ -616,10 +616,11 @@ class _RasterizeMetal(torch.autograd.Function):
         ctx.rec = None
         sched = ctx.sched
         if rec is None:
-            rec = torch.empty(N, _REC, device=dev)
+            rec = torch.empty(N, _REC, dtype=torch.float32, device=dev)
         if grad_rgb is None and grad_alpha is None:
             return (None,) * 14
-        grad_rgb = torch.zeros(H, W, 3, device=dev) if grad_rgb is None else grad_rgb.contiguous()
+        grad_rgb = (torch.zeros(H, W, 3, dtype=torch.float32, device=dev) if grad_rgb is None
+                    else grad_rgb.contiguous())
         grad_alpha = None if grad_alpha is None else grad_alpha.contiguous()
         _lib.check(lib.mg_rasterize_backward(
             N, uv.data_ptr(), conic.data_ptr(), opacity.data_ptr(), color.data_ptr(),
@@ -676,13 +677,13 @@ class _PreprocessMip(torch.autograd.Function):
             filt = filter_3d.detach().to(torch.float32).contiguous()
             if filt.shape != (N,):
                 raise ValueError(f"filter_3d must be ({N},), got {tuple(filt.shape)}")
-        uv = torch.empty(N, 2, device=dev)
-        conic = torch.empty(N, 3, device=dev)
-        depth = torch.empty(N, device=dev)
-        rxy = torch.empty(N, 2, device=dev)
+        uv = torch.empty(N, 2, dtype=torch.float32, device=dev)
+        conic = torch.empty(N, 3, dtype=torch.float32, device=dev)
+        depth = torch.empty(N, dtype=torch.float32, device=dev)
+        rxy = torch.empty(N, 2, dtype=torch.float32, device=dev)
         valid = torch.empty(N, dtype=torch.int32, device=dev)
-        color = torch.empty(N, 3, device=dev) if sh is not None else None
-        op_eff = torch.empty(N, device=dev)
+        color = torch.empty(N, 3, dtype=torch.float32, device=dev) if sh is not None else None
+        op_eff = torch.empty(N, dtype=torch.float32, device=dev)
         _lib.check(lib.mg_preprocess_forward_mip(
             N, _lib.dev_tensor(means, "means"), _lib.dev_tensor(quats, "quats"),
             _lib.dev_tensor(scales, "scales"),
@@ -741,10 +742,10 @@ class _PreprocessMip(torch.autograd.Function):
                 int(ctx.antialias), ctx.activations, *ctx.reg, p_oe, None, None, None, None,
                 None, None, ctypes.byref(epi), _lib.stream(means)))
             return (None,) * 27
-        d_means = torch.empty(N, 3, device=dev)
-        d_quats = torch.empty(N, 4, device=dev)
-        d_scales = torch.empty(N, 3, device=dev)
-        d_op = torch.empty(N, device=dev)
+        d_means = torch.empty(N, 3, dtype=torch.float32, device=dev)
+        d_quats = torch.empty(N, 4, dtype=torch.float32, device=dev)
+        d_scales = torch.empty(N, 3, dtype=torch.float32, device=dev)
+        d_op = torch.empty(N, dtype=torch.float32, device=dev)
         d_sh = d_rest = None
         if ctx.has_sh:
             d_sh = torch.empty_like(sh)

@@ -63,9 +63,9 @@ def rasterize_forward(uv, conic, opacity, color, gauss_ids, tile_offsets, W, H, 
     W, H, tile, tiles_x = int(W), int(H), int(tile), int(tiles_x)
     _check_tile(tile)
     dev = uv.device
-    rgb = torch.empty(H, W, 3, device=dev)
-    alpha = torch.empty(H, W, device=dev)
-    T = torch.empty(H, W, device=dev)
+    rgb = torch.empty(H, W, 3, dtype=torch.float32, device=dev)
+    alpha = torch.empty(H, W, dtype=torch.float32, device=dev)
+    T = torch.empty(H, W, dtype=torch.float32, device=dev)
     n_contrib = torch.empty(H, W, dtype=torch.int32, device=dev)
     _lib.check(lib.mg_rasterize_forward(
         uv.shape[0], _dev(uv, "input"), _dev(conic, "input"), _dev(opacity, "input"),
@@ -87,7 +87,7 @@ def rasterize_backward(uv, conic, opacity, color, gauss_ids, tile_offsets, final
     _check_tile(tile)
     N = uv.shape[0]
     dev = uv.device
-    rec = torch.empty(N, 10, device=dev)
+    rec = torch.empty(N, 10, dtype=torch.float32, device=dev)
     grad_rgb = grad_rgb.contiguous()
     grad_alpha = grad_alpha.contiguous()
     _lib.check(lib.mg_rasterize_backward(
@@ -97,7 +97,8 @@ def rasterize_backward(uv, conic, opacity, color, gauss_ids, tile_offsets, final
         _dev(n_contrib, "n_contrib", torch.int32), _dev(grad_rgb, "grad_rgb"),
         _dev(grad_alpha, "grad_alpha"), None, None, gauss_ids.numel(), None, 0, W, H, tile,
         tiles_x, rec.data_ptr(), int(bool(want_absgrad)), 0, None, _lib.stream(uv)))
-    d_absuv = rec[:, 9].contiguous() if want_absgrad else torch.zeros(1, device=dev)
+    d_absuv = (rec[:, 9].contiguous() if want_absgrad
+               else torch.zeros(1, dtype=torch.float32, device=dev))
     return [rec[:, 0:2].contiguous(), rec[:, 2:5].contiguous(), rec[:, 5].contiguous(),
             rec[:, 6:9].contiguous(), d_absuv]
 
@@ -129,12 +130,12 @@ def preprocess_forward(means, quats, scales, sh, sh_rest, opacities, viewmat, fx
     fused, sh, rest = _sh_layout(sh, sh_rest)
     means, quats, scales = means.contiguous(), quats.contiguous(), scales.contiguous()
     opacities = opacities.contiguous()
-    uv = torch.empty(N, 2, device=dev)
-    conic = torch.empty(N, 3, device=dev)
-    depth = torch.empty(N, device=dev)
-    rxy = torch.empty(N, 2, device=dev)
+    uv = torch.empty(N, 2, dtype=torch.float32, device=dev)
+    conic = torch.empty(N, 3, dtype=torch.float32, device=dev)
+    depth = torch.empty(N, dtype=torch.float32, device=dev)
+    rxy = torch.empty(N, 2, dtype=torch.float32, device=dev)
     valid = torch.empty(N, dtype=torch.int32, device=dev)
-    color = torch.empty(N, 3, device=dev)
+    color = torch.empty(N, 3, dtype=torch.float32, device=dev)
     vm, cc = _host_pose(viewmat, cam_center)
     _lib.check(lib.mg_preprocess_forward(
         N, _dev(means, "means"), _dev(quats, "quats"), _dev(scales, "scales"), _dev(sh, "sh"),
@@ -156,11 +157,11 @@ def preprocess_backward(means, quats, scales, sh, sh_rest, d_uv, d_conic, d_colo
     N = means.shape[0]
     dev = means.device
     fused, sh, rest = _sh_layout(sh, sh_rest)
-    d_means = torch.empty(N, 3, device=dev)
-    d_quats = torch.empty(N, 4, device=dev)
-    d_scales = torch.empty(N, 3, device=dev)
-    d_sh = torch.empty(N, 16 if fused else 1, 3, device=dev)
-    d_sh_rest = d_sh if fused else torch.empty(N, 15, 3, device=dev)
+    d_means = torch.empty(N, 3, dtype=torch.float32, device=dev)
+    d_quats = torch.empty(N, 4, dtype=torch.float32, device=dev)
+    d_scales = torch.empty(N, 3, dtype=torch.float32, device=dev)
+    d_sh = torch.empty(N, 16 if fused else 1, 3, dtype=torch.float32, device=dev)
+    d_sh_rest = d_sh if fused else torch.empty(N, 15, 3, dtype=torch.float32, device=dev)
     d_uv, d_conic, d_color = d_uv.contiguous(), d_conic.contiguous(), d_color.contiguous()
     vm, cc = _host_pose(viewmat, cam_center)
     _lib.check(lib.mg_preprocess_backward(

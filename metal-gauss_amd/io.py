@@ -223,11 +223,11 @@ def _load_on_gpu(v, names, fields, per_channel, degree, dev, dtype):
     # One host copy out of the memory map (writable, as torch requires), one
     # upload.
     rec = torch.from_numpy(np.array(rec_np, dtype=np.float32, order="C")).to(dev)
-    means = torch.empty(n, 3, device=dev)
-    quats = torch.empty(n, 4, device=dev)
-    scales = torch.empty(n, 3, device=dev)
-    opac = torch.empty(n, device=dev)
-    sh = torch.empty(n, per_channel + 1, 3, device=dev)
+    means = torch.empty(n, 3, dtype=torch.float32, device=dev)
+    quats = torch.empty(n, 4, dtype=torch.float32, device=dev)
+    scales = torch.empty(n, 3, dtype=torch.float32, device=dev)
+    opac = torch.empty(n, dtype=torch.float32, device=dev)
+    sh = torch.empty(n, per_channel + 1, 3, dtype=torch.float32, device=dev)
     _lib.check(lib.mg_ply_decode(n, rec.data_ptr() if n else None, stride,
                                  _lib.i32_array(columns), per_channel, means.data_ptr(),
                                  quats.data_ptr(), scales.data_ptr(), opac.data_ptr(),
@@ -270,7 +270,7 @@ def export_ply(p: dict, path: str, filter_3d=None) -> None:
     if dev.type == "cuda":
         lib = _lib.load()
         cols = [names.index(f) for f in _field_names(per_channel)]
-        rec = torch.empty(n, len(names), device=dev)
+        rec = torch.empty(n, len(names), dtype=torch.float32, device=dev)
         # Every operand on the parameters' device, contiguous float32: the
         # kernel takes raw device pointers.
         c = lambda t: t.detach().to(dev).contiguous().float()  # noqa: E731

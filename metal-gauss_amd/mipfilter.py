@@ -43,7 +43,7 @@ def _view_records(views, near: float, margin: float):
     times the kernels' own."""
     views = list(views)
     if not views:
-        return torch.zeros(0, 20), 0.0
+        return torch.zeros(0, 20, dtype=torch.float32), 0.0
     vm = _host_f64([v.viewmat for v in views], 3, 4)
     K = _host_f64([v.K for v in views], 2, 3)
     shapes = [v.image.shape for v in views]
@@ -76,7 +76,7 @@ def compute_3d_filter(means: torch.Tensor, views, near: float = 0.2,
     N = means.shape[0]
     rec, focal = _view_records(views, near, margin)
     rec = rec.to(means.device)
-    out = torch.empty(N, device=means.device)
+    out = torch.empty(N, dtype=torch.float32, device=means.device)
     scratch = torch.empty(1, dtype=torch.int32, device=means.device)
     _lib.check(lib.mg_compute_3d_filter(
         N, _lib.dev_tensor(means, "means"), rec.shape[0],

@@ -51,7 +51,7 @@ def _forward(x, weight, bias, eps, keep):
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     stats = mean = rstd = None
     if keep:
-        stats = torch.empty(2 * n, device=x.device)
+        stats = torch.empty(2 * n, dtype=torch.float32, device=x.device)
         mean = stats.data_ptr()
         rstd = mean + 4 * n
     _lib.launch(lib.mg_layer_norm_forward, index, n, width, code, rows.data_ptr(), stride, wcode,

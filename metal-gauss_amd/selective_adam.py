@@ -46,7 +46,7 @@ class SelectiveAdam(torch.optim.Optimizer):
             st["exp_avg"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
             st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
             if rowwise:
-                st["steps"] = torch.zeros(p.shape[0], device=p.device)
+                st["steps"] = torch.zeros(p.shape[0], dtype=torch.float32, device=p.device)
             else:
                 st["step"] = 0
         return st

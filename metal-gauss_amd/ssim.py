@@ -48,8 +48,8 @@ class _SSIMFused(torch.autograd.Function):
         if w.numel() != 11:
             raise ValueError(f"SSIM window must have 11 taps, got {w.numel()}")
         H, W = a.shape[0], a.shape[1]
-        partials = torch.empty(9, H, W, device=a.device)
-        mean = torch.empty((), device=a.device)
+        partials = torch.empty(9, H, W, dtype=torch.float32, device=a.device)
+        mean = torch.empty((), dtype=torch.float32, device=a.device)
         ws = torch.empty(lib.mg_ssim_fused_workspace_bytes(H, W), dtype=torch.uint8,
                          device=a.device)
         _lib.check(lib.mg_ssim_fused_forward(
@@ -88,8 +88,8 @@ class _PhotometricLoss(torch.autograd.Function):
         if win.numel() != 11:
             raise ValueError(f"SSIM window must have 11 taps, got {win.numel()}")
         H, W = a.shape[0], a.shape[1]
-        partials = torch.empty(9, H, W, device=a.device)
-        out = torch.empty(3, device=a.device)
+        partials = torch.empty(9, H, W, dtype=torch.float32, device=a.device)
+        out = torch.empty(3, dtype=torch.float32, device=a.device)
         ws = torch.empty(lib.mg_ssim_fused_workspace_bytes(H, W), dtype=torch.uint8,
                          device=a.device)
         _lib.check(lib.mg_photometric_loss_forward(
@@ -149,7 +149,7 @@ def _img_ptrs(*ts):
 
 def stack_blur_h(x, y, w, H, W):
     lib = _lib.load()
-    out = torch.empty(1, 15, H, W, device=x.device)
+    out = torch.empty(1, 15, H, W, dtype=torch.float32, device=x.device)
     px, py, pw = _img_ptrs(x.contiguous(), y.contiguous(), w.contiguous())
     _lib.check(lib.mg_ssim_stack_blur_h(px, py, pw, H, W, out.data_ptr(), _lib.stream(x)))
     return out
@@ -169,7 +169,7 @@ def tail_forward(b, H, W):
     b = b.contiguous()
     if b.numel() != 15 * H * W:
         raise RuntimeError("ssim_tail_forward: expected 15*H*W")
-    out = torch.empty(1, 3, H, W, device=b.device)
+    out = torch.empty(1, 3, H, W, dtype=torch.float32, device=b.device)
     _lib.check(lib.mg_ssim_tail_forward(_lib.dev_tensor(b, "blurred stack"), H, W,
                                         out.data_ptr(), _lib.stream(b)))
     return out
