@@ -628,40 +628,47 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_sum_kernel(AttnArgs a) {
 
 // The sinks' sums: a workgroup has four columns in each half of a wave, of 32 sinks,
 // of dk or dv, and its waves every kSinkWaves-th place (16 waves: 14 us in place of 8
-// for 7033 packed tokens).
+// for 7033 packed tokens). How many key tiles have sums, of `tiles` at most, the device
+// alone knows: as many workgroups as run at once take them in turn (512 sequences of 64
+// tokens that have none: 14 us, with a workgroup for each there might be 74).
 constexpr int kSinkWaves = 4;
+constexpr int64_t kSinkSlots = 2048;
 template <typename T, int DK>
-__global__ __launch_bounds__(64 * kSinkWaves) void attn_sink_sum_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kSinkWaves) void attn_sink_sum_kernel(AttnArgs a, int tiles) {
     constexpr int kBlocks = DK / 32;
     __shared__ f32x4 s_sum[kSinkWaves][64];
-    const int kh = blockIdx.x % a.k_heads, item = blockIdx.x / a.k_heads;
-    const SeqItem s = find_item<true>(
-        a, item, [&](int ql, int kl) { return SinkItems(a, ql, kl).key_tiles; },
-        [&](int ql, int kl) { return SinkItems(a, ql, kl).all(a); });
-    if (!s.found) return;
-    const SinkItems of(a, s.q_len, s.k_len);
-    const int first_key = s.within * kBwdTile;
-    const int places = of.runs + key_steps<true>(a, s, first_key, false).runs;
+    const int kh = blockIdx.x % a.k_heads;
     const int lane = lane_id(), half = lane / 32, wave = uniform(threadIdx.x / 64);
     const int i = blockIdx.y % (kBlocks * 4), rows = blockIdx.y / (kBlocks * 4) / 2 * 32;
     const int which = blockIdx.y / (kBlocks * 4) % 2;
-    const int key = first_key + rows + lane % 32, at = 32 * (i / 4) + c_row(i % 4 * 4, half);
-    const f32x4 *from = sink_part_of<DK>(a, s.before + s.within * of.places(a), kh) +
-                        (rows / 32 * kBlocks * 4 + i) * 64 + lane +
-                        which * (a.sink_rows * DK / 4);
-    const int64_t step = (int64_t)a.k_heads * (2 * a.sink_rows * DK / 4);
-    f32x4 sum = {};
-    if (key < a.sinks) {
+    for (int item = blockIdx.x / a.k_heads; item < tiles; item += gridDim.x / a.k_heads) {
+        const SeqItem s = find_item<true>(
+            a, item, [&](int ql, int kl) { return SinkItems(a, ql, kl).key_tiles; },
+            [&](int ql, int kl) { return SinkItems(a, ql, kl).all(a); });
+        if (!s.found) return;
+        const SinkItems of(a, s.q_len, s.k_len);
+        const int first_key = s.within * kBwdTile;
+        const int places = of.runs + key_steps<true>(a, s, first_key, false).runs;
+        const int key = first_key + rows + lane % 32, at = 32 * (i / 4) + c_row(i % 4 * 4, half);
+        const f32x4 *from = sink_part_of<DK>(a, s.before + s.within * of.places(a), kh) +
+                            (rows / 32 * kBlocks * 4 + i) * 64 + lane +
+                            which * (a.sink_rows * DK / 4);
+        const int64_t step = (int64_t)a.k_heads * (2 * a.sink_rows * DK / 4);
+        f32x4 sum = {};
+        if (key < a.sinks) {
 #pragma unroll 8
-        for (int p = wave; p < places; p += kSinkWaves) sum += from[p * step];
+            for (int p = wave; p < places; p += kSinkWaves) sum += from[p * step];
+        }
+        s_sum[wave][lane] = sum;
+        __syncthreads();
+        if (wave == 0 && key < min(a.sinks, s.k_len) && at < a.dim) {
+            for (int w = 1; w < kSinkWaves; ++w) sum += s_sum[w][lane];
+            *reinterpret_cast<vec4<T> *>(static_cast<T *>(which ? a.dv : a.dk) +
+                                         ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim + at) =
+                __builtin_convertvector(sum, vec4<T>);
+        }
+        __syncthreads();
     }
-    s_sum[wave][lane] = sum;
-    __syncthreads();
-    if (wave != 0 || key >= min(a.sinks, s.k_len) || at >= a.dim) return;
-    for (int w = 1; w < kSinkWaves; ++w) sum += s_sum[w][lane];
-    *reinterpret_cast<vec4<T> *>(static_cast<T *>(which ? a.dv : a.dk) +
-                                 ((int64_t)(s.k_lo + key) * a.k_heads + kh) * a.dim + at) =
-        __builtin_convertvector(sum, vec4<T>);
 }
 
 // Bytes of the backward's scratch: delta, the largest norms, and the runs' sums.
@@ -784,7 +791,7 @@ static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_toke
     const int64_t places =
         k_heads * norm_places(q_tokens > k_tokens ? q_tokens : k_tokens, sequences);
     MG_REQUIRE(grid_fits(q_items, 64 * kBwdWaves) && grid_fits(k_items, 64 * kBwdWaves) &&
-                   p.sink_places < INT32_MAX && grid_fits(p.sink_tiles * k_heads, 64 * kSinkWaves) &&
+                   p.sink_places < INT32_MAX &&
                    (dtype != MG_F16 || grid_fits(places, kLargestThreads)),
                "%s: too many work items", who);
     MG_REQUIRE(workspace && workspace_bytes >= p.bytes, "%s: workspace of %lld bytes, %lld needed",
@@ -832,9 +839,12 @@ static int32_t attention_backward(const char *who, int32_t dtype, int64_t q_toke
         TimedScope ts("attention_sinks", st);
         attn_form(dtype, dim, [&](auto t, auto d) {
             constexpr int DK = decltype(d)::value;
-            const dim3 grid((unsigned)(p.sink_tiles * k_heads),
-                            (unsigned)(p.sink_rows / 32 * 2 * DK / 8));
-            attn_sink_sum_kernel<decltype(t), DK><<<grid, 64 * kSinkWaves, 0, st>>>(a);
+            const int64_t parts = p.sink_rows / 32 * 2 * DK / 8;
+            const int64_t most = ceil_div(kSinkSlots, k_heads * parts);
+            const dim3 grid((unsigned)((p.sink_tiles < most ? p.sink_tiles : most) * k_heads),
+                            (unsigned)parts);
+            attn_sink_sum_kernel<decltype(t), DK>
+                <<<grid, 64 * kSinkWaves, 0, st>>>(a, (int)p.sink_tiles);
         });
         MG_LAUNCHED("attn_sink_sum_kernel");
     }
