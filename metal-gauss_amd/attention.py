@@ -176,8 +176,8 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     its result (the backward pass asks for finite inputs within a sequence).
 
     ``window`` (with ``causal``; 1 or more) leaves a query the last ``window`` of these
-    keys, its own included, and the sequence's first ``sinks``; time and memory go by
-    the keys that are left.
+    keys, its own included, and the sequence's first ``sinks``; time goes by the keys
+    that are left, and scratch memory is bounded by the tokens, not by the sequences.
 
     ``scale`` (default dim ** -0.5) may not be negative.
 

@@ -1,4 +1,4 @@
-// Shared by the attention kernels' two files. Internal header.
+// Shared by the attention kernels' files. Internal header.
 #pragma once
 
 #include "attention_tiles.h"

@@ -26,7 +26,7 @@
 // 8192 tokens, 16 heads of 128 bfloat16: queries 800 us, keys 1092 (1030 and 1010 TFLOP/s);
 // of 64: 487 and 635 (850 and 870). The queries' kernel is never cut over its keys:
 // 64 queries over 16000 of them, 16 heads on 4 of 128, take 417 us. With a window of 475
-// and 4 sinks 7033 packed tokens (16 heads on 4 of 128) take 92 and 126. As the
+// and 4 sinks 7033 packed tokens (16 heads on 4 of 128) take 94 and 106. As the
 // forward, both need two waves a SIMD to keep products and exponentials going side by
 // side: the keys' kernel with one (256 columns of sums and operands in 472 registers)
 // took 1970.
@@ -295,8 +295,8 @@ __device__ __forceinline__ f32x4 *part_of(const AttnArgs &a, int item, int kh, i
 
 // With a window, the queries that see a key tile are few, but those further on all
 // see the sinks. Where these are many (sink_cut), their sums for the sinks are work items
-// of their own, which come last, being short ones (first: 147 us in place of 126 for 7033
-// packed tokens, window 475): one tile of kBwdTile keys and a run of query tiles each.
+// of their own, which come last, being short ones (first, those of 7033 packed tokens,
+// window 475, took 17% longer): one tile of kBwdTile keys and a run of query tiles each.
 // Their sums, of sink_rows keys, have a place each in sink_part, and so have those of the
 // window items of key tiles that have sinks; attn_sink_sum_kernel adds them up, in
 // order. A sequence's places follow one another, a key tile's far items' and then
@@ -627,8 +627,8 @@ __global__ __launch_bounds__(64 * kBwdWaves) void attn_sum_kernel(AttnArgs a) {
 }
 
 // The sinks' sums: a workgroup has four columns in each half of a wave, of 32 sinks,
-// of dk or dv, and its waves every kSinkWaves-th place (16 waves: 14 us in place of 8
-// for 7033 packed tokens). How many key tiles have sums, of `tiles` at most, the device
+// of dk or dv, and its waves every kSinkWaves-th place (16 waves: both gradients
+// of 7033 packed tokens 207 us in place of 196). How many key tiles have sums, of `tiles` at most, the device
 // alone knows: as many workgroups as run at once take them in turn (512 sequences of 64
 // tokens that have none: 14 us, with a workgroup for each there might be 74).
 constexpr int kSinkWaves = 4;
@@ -684,11 +684,10 @@ struct BwdPlan {
 
 constexpr int64_t kBwdRuns = 1024, kBwdRunLeast = 8, kBwdMostSplits = 8;
 // With a window: as many as fill the GPU, as partial results weigh more beside fewer
-// queries (7033 packed tokens, window 475: 132 and 30 us to add them in four runs, 119 and
-// 18 in two), of four query tiles at least (nine sequences of 3 to 1210 tokens, 6 heads
-// on 3 of 128: 42 and 13 us, of eight 77 and 8). As many far items, or runs of
-// sink_steps = kSinkStepsLeast (in 128 of 8 at least that pass's keys took 171 us for
-// 143).
+// queries (both gradients of 7033 packed tokens, window 475, take 196 us, 226 with twice as
+// many and 237 with half), of four query tiles at least (nine sequences of 3 to 1210
+// tokens, 6 heads on 3 of 128: 84 us, of eight 92). As many runs of far items, of
+// sink_steps = kSinkStepsLeast tiles at least (of eight: the nine sequences 105 us).
 constexpr int64_t kBwdWindowRuns = 512, kBwdWindowRunLeast = 4, kSinkItems = 512, kSinkStepsLeast = 4;
 
 static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int64_t group,
@@ -699,8 +698,8 @@ static BwdPlan bwd_plan(int64_t q_tokens, int64_t k_tokens, int64_t k_heads, int
     int64_t queries = ceil_div(q_tokens, n_seq * kTileRows);
     // The most that any key tile has, not the average: of unequal sequences the longer
     // ones are cut, the shorter ones' items have steps for one run and stay whole (12
-    // sequences of 5 to 1461 tokens, 4 heads on 2 of 128: 40 us and 12 to add the runs,
-    // uncut 175; 32 equal ones of 100: 35 and 6, uncut 32).
+    // sequences of 5 to 1461 tokens, 4 heads on 2 of 128: 31 us and 8 to add the runs, by
+    // the average 43 and 6; 32 equal ones of 100: 26 and 4, by the average 23).
     if (window > 0) {
         const int64_t seen = ceil_div(window + kBwdTile, kTileRows);
         queries = ceil_div(q_tokens, kTileRows);

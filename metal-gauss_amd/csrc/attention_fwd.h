@@ -47,8 +47,8 @@ constexpr float kRise = std::is_same<T, f16_t>::value ? 11.f : 0.f;
 // Work items come in two widths. Wide: 128 rows by four waves, tiles of 64
 // keys that all four read. Narrow, where a sequence's rows would leave most of
 // that empty (single tokens): 32 rows by one wave, tiles of 32 keys; memory
-// bounds it, and ten waves (64 columns) or five (128) of a CU each have a
-// tile's loads under way. 16 tokens of 16 heads on 4 of 64 over 75000 keys: 16.5 us
+// bounds it, and of those cut over their keys ten waves a CU (64 columns; with a
+// window eight) or four (128) each have a tile's loads under way. 16 tokens of 16 heads on 4 of 64 over 75000 keys: 16.5 us
 // and 8 to join (tiles of 64 keys: 19, half as many waves), 75 MB of keys and
 // values at 7 TB/s once the loop runs.
 constexpr int kWideWaves = 4, kNarrowWaves = 1;

@@ -15,7 +15,8 @@
 // elements before it forms its cosines, whose chain (position, float64 product,
 // polynomial) is as long as a trip to memory: 10000 tokens of 32 heads of 64
 // bfloat16 16 us (5.1 TB/s; 23 us with the cosines first), 32640 of 20 heads of
-// 128 float32, a quarter of them elsewhere in their rows, 125 us (5.3 TB/s).
+// 128 float32, a quarter of them elsewhere in their rows, 125 us (5.3 TB/s). Pairs dealt to
+// three axes from the table cost 0 to 4% more than equal runs (57 us for 56, 129 for 124).
 #include "rotary.h"
 
 namespace mg {
