@@ -78,3 +78,37 @@ def test_packs_of_thousands_of_sequences(dev, tokens, sequences, heads, dim, win
             for a, w, b in zip(got, want, bound):
                 a = host(a[lo:hi, h:h + 1])
                 assert (np.abs(a - w) <= b * (1.0 + 2.0 ** -14 / UNIT["bf16"]) * 1.05 + 1e-30).all()
+
+
+@pytest.mark.parametrize("sinks", [4, 130])
+def test_items_of_their_own_in_a_graph_and_on_another_stream(dev, sinks):
+    """Replayed with other inputs and other lengths, some sequences gaining items of
+    their own and some losing them, against the eager result."""
+    from metal_gauss_amd import attention
+
+    q, k, v, do = (t.to(dev) for t in inputs(("graph", sinks), 1400, 1400, 4, 2, 64, "bf16"))
+    off = torch.tensor([0, 700, 740, 1400], dtype=torch.int32, device=dev)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+
+    def step():
+        o = attention(*leaves, off, causal=True, window=60, sinks=sinks)
+        return (o.detach(), *torch.autograd.grad(o, leaves, do))
+
+    want = step()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = step()
+    torch.cuda.current_stream().wait_stream(s)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for lens in ([0, 700, 740, 1400], [0, 100, 200, 1400], [0, 300, 620, 940], [0, 0, 1399, 1400]):
+        with torch.no_grad():
+            off.copy_(torch.tensor(lens, dtype=torch.int32))
+            for i, t in enumerate(leaves):
+                t.copy_(inputs(("again", lens[1], i), 1400, 1400, 4, 2, 64, "bf16")[min(i, 1)])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, step()))
